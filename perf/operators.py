@@ -7,7 +7,7 @@ true); `exact` is each operator's definition in 64 bits.
 
 The cache: a K page holds [n_kv][page][head_dim], a V page [n_kv][head_dim][page].  A q8_0 page holds,
 for each head, int8 values in that order and then their fp16 scales, one for 32 values of a head's
-vector (K: [page][head_dim / 32], V: [head_dim / 32][page]).
+vector, [head_dim / 32][page].
 """
 import math
 
@@ -296,7 +296,8 @@ def _values(pool, c, is_v):
     d = by_head[..., P * D:].contiguous().view(torch.float16).float()
     if is_v:
         return (q.reshape(*q.shape[:-1], D // 32, 32, P) * d.reshape(*d.shape[:-1], D // 32, 1, P)).flatten(-3, -2)
-    return (q.reshape(*q.shape[:-1], P, D // 32, 32) * d.reshape(*d.shape[:-1], P, D // 32, 1)).flatten(-2)
+    d = d.reshape(*d.shape[:-1], D // 32, P).transpose(-1, -2)
+    return (q.reshape(*q.shape[:-1], P, D // 32, 32) * d[..., None]).flatten(-2)
 
 
 def _where(s):
@@ -500,7 +501,7 @@ def _exact_attn(c, s):
                 part = [t.view(t.shape[0], c["n_kv"], -1)[pages, h] for t in (s["k"], s["v"])]
                 q8 = [t[:, :P * D].contiguous().view(torch.int8).double() for t in part]
                 sc = [t[:, P * D:].contiguous().view(torch.float16).double() for t in part]
-                k = q8[0].view(-1, D) * sc[0].view(-1, D // 32).repeat_interleave(32, 1)
+                k = q8[0].view(-1, D) * sc[0].view(-1, D // 32, P).transpose(1, 2).reshape(-1, D // 32).repeat_interleave(32, 1)
                 v = q8[1].view(-1, D, P) * sc[1].view(-1, D // 32, P).repeat_interleave(32, 1)
             else:
                 k, v = s["k"][pages, h].double().view(-1, D), s["v"][pages, h].double()
