@@ -1,4 +1,4 @@
-"""ctypes binding of libllapis_moe.so (include/moert_hip.h + include/llapis_moe.h).
+"""ctypes binding of libllapis_moe.so (include/moert_hip.h, include/llapis_moe.h, include/llapis_step.h).
 
 The library is the product: loading fails loudly if it has not been built
 (python -m llapis_amd.build); there is no fallback implementation.
@@ -10,6 +10,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libllapis_moe.so"
 
 # ggml type tags (ggml.h:390-412)
 F32, Q5_0, Q8_0, Q8_1, Q4_K, Q8_K, IQ4_NL, IQ2_S = 0, 6, 8, 9, 12, 15, 20, 22
+F16, BF16 = 1, 30
 ACT_CPU, ACT_Q8_1 = 0, 1
 GELU_TABLE, GELU_TANH = 0, 1
 MM_W_HOT, MM_W_COLD_SRC, MM_W_RAW = 0, 1, 2
@@ -115,6 +116,62 @@ class LlapisResidencyStats(C.Structure):
                                                                            ("host_ms", C.c_double)]
 
 
+# llapis_step.h
+f32 = C.c_float
+KV_MAX_PLANES = 128
+NORM_MAX_OUT = 4
+
+
+class LlapisKvCache(C.Structure):
+    _fields_ = [("type", i32), ("n_kv", i32), ("head_dim", i32), ("page_size", i32), ("n_pages", i32), ("k", vp), ("v", vp),
+                ("k_stride", u64), ("v_stride", u64)]
+
+
+class LlapisKvBatch(C.Structure):
+    _fields_ = [("n_seq", i32), ("n_tokens", i32), ("max_new", i32), ("max_pages", i32), ("table_stride", i64),
+                ("page_table", vp), ("lens", vp), ("new_start", vp)]
+
+
+class LlapisKvQuery(C.Structure):
+    _fields_ = [("type", i32), ("n_head", i32), ("window", i32), ("scale", f32), ("q", vp), ("q_stride", i64), ("out", vp),
+                ("out_stride", i64), ("lse", vp)]
+
+
+class LlapisKvPlanes(C.Structure):
+    _fields_ = [("n_planes", i32), ("n_pages", i32), ("page_size", i32), ("reserved", i32), ("base", vp * KV_MAX_PLANES),
+                ("stride", u64 * KV_MAX_PLANES), ("bytes", u64 * KV_MAX_PLANES)]
+
+
+class LlapisBlockNormArgs(C.Structure):
+    _fields_ = [("type", i32), ("n_tokens", i32), ("d", i32), ("n_out", i32), ("post_norm", i32), ("eps", f32),
+                ("alpha", f32), ("beta", f32), ("h", vp), ("h_stride", i64), ("y", vp), ("y_stride", i64),
+                ("post_weight", vp), ("gate", vp), ("gate_token_stride", i64), ("gate_value_stride", i64),
+                ("h_out", vp), ("h_out_stride", i64), ("weight", vp * NORM_MAX_OUT), ("x", vp * NORM_MAX_OUT),
+                ("x_stride", i64 * NORM_MAX_OUT)]
+
+
+class LlapisVerifyArgs(C.Structure):
+    _fields_ = [("type", i32), ("n_seq", i32), ("max_draft", i32), ("vocab", i32), ("target", vp), ("target_stride", i64),
+                ("draft", vp), ("draft_stride", i64), ("drafts", vp), ("n_draft", vp), ("u", vp), ("u_next", vp),
+                ("tokens", vp), ("accepted", vp)]
+
+
+STEP_SIGNATURES = {
+    "llapis_kv_page_bytes": (u64, [i32, i32, i32, i32]),
+    "llapis_kv_append": (i32, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), i32, vp, i64, vp, i64, vp]),
+    "llapis_kv_attention_workspace_size": (u64, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), i32]),
+    "llapis_kv_attention": (i32, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), C.POINTER(LlapisKvQuery), vp, u64, vp]),
+    "llapis_kv_copy_pages": (i32, [C.POINTER(LlapisKvPlanes), vp, i32, vp]),
+    "llapis_kv_fork": (i32, [C.POINTER(LlapisKvPlanes), vp, i64, i32, vp, i32, vp, i32, vp]),
+    "llapis_kv_page_refs": (i32, [i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp]),
+    "llapis_kv_compact_workspace_size": (u64, [i32]),
+    "llapis_kv_compact": (i32, [C.POINTER(LlapisKvPlanes), vp, i64, i32, vp, i32, vp, vp, vp, vp, u64, vp]),
+    "llapis_block_norm": (i32, [C.POINTER(LlapisBlockNormArgs), vp]),
+    "llapis_verify_drafts_workspace_size": (u64, [i32, i32]),
+    "llapis_verify_drafts": (i32, [C.POINTER(LlapisVerifyArgs), vp, u64, vp]),
+}
+
+
 # moert_store.h
 class MoertStoreInfo(C.Structure):
     _fields_ = [("format_version", C.c_uint32), ("source_uuid", u64), ("arch", C.c_char * 16), ("n_layers", i32),
@@ -151,7 +208,6 @@ def bind(cdll, table):
 
 # moert_policy.h
 REFRESH_PROMPT_END, REFRESH_VISIBLE_INTERVAL, REFRESH_TURN_END, REFRESH_BOUNDARY = 0, 1, 2, 4
-f32 = C.c_float
 
 
 class MoertPolicyConfig(C.Structure):
@@ -217,7 +273,7 @@ POLICY_SIGNATURES = {
 }
 
 
-# every symbol the two public headers declare, with its signature
+# every symbol the public headers declare, with its signature
 SIGNATURES = {
     # moert_hip.h
     "moert_cuda_configure": (None, [C.POINTER(MoertCudaConfig)]),
@@ -293,6 +349,7 @@ SIGNATURES = {
     "llapis_residency_get_stats": (None, [vp, C.POINTER(LlapisResidencyStats)]),
     **POLICY_SIGNATURES,
     **STORE_SIGNATURES,
+    **STEP_SIGNATURES,
 }
 
 STAGES = ("router", "topk", "gate_up", "down", "combine")

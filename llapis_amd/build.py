@@ -20,7 +20,8 @@ LIB = PKG / "libllapis_moe.so"
 ARCH = "gfx950"
 
 HIP_SOURCES = ["mmv.hip", "decode.hip", "prefill.hip", "small_kernels.hip", "transfer.hip", "model_files.hip",
-               "residency.hip", "api.hip"]
+               "residency.hip", "kv_attn_f16.hip", "kv_attn_bf16.hip", "kv_attn_q8.hip", "kv_cache.hip", "step.hip",
+               "api.hip"]
 HOST_SOURCES = ["quantize.cpp", "policy.cpp", "kfit.cpp"]
 
 

@@ -40,6 +40,21 @@ int32_t fail(const std::string & msg) {
     return -1;
 }
 
+}  // namespace
+
+namespace llapis {
+int32_t refuse(const char * msg) noexcept {
+    try {
+        g_err = msg;
+    } catch (...) {
+        g_err.clear();
+    }
+    return -1;
+}
+}  // namespace llapis
+
+namespace {
+
 #define LL_TRY(expr)                                                                 \
     do {                                                                             \
         const hipError_t e_ = (expr);                                                \

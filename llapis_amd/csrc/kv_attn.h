@@ -1,0 +1,719 @@
+// kv_attn.h -- attention of new tokens over the paged cache, the kernel (one
+// instance per cache type, query type, head size and row tiles; kv_attn_*.hip).
+//
+// Work.  A sequence's keys are units of 128; an item is (sequence, kv head,
+// tile of 16 NT query rows: the group's heads of every new token share the kv
+// head, so K and V are read once for all of them).  The items' units lie in one
+// line, of which every workgroup takes an equal run: long and short sequences
+// share the card alike, and no count of splits has to be chosen.  A run that
+// covers an item writes its result; parts of an item go to the workspace as
+// (maximum, sum, unnormalised output) and k_kv_join adds them in order.  The
+// split is a function of the lengths alone.
+//
+// A workgroup's four waves take a unit together.  For its 32 (16) keys a wave forms
+//   S^T = K Q^T     A = K (16 keys x 32 values), B = Q^T from LDS
+// and with the row maxima of all four its P, which goes to LDS; for its quarter
+// of the values' columns and all keys of the unit it then adds
+//   O^T += V^T P^T  A = V^T (16 values x 32 keys), B = P^T
+// (v_mfma_f32_16x16x32).  A lane's column is query row l % 16 in both products,
+// so the running maximum, the sum and the rescaling stay in the lane, and P is
+// written as it is read: K's rows are assigned to the first product such that a
+// lane's scores belong to the keys that are consecutive in its V^T operand.  K
+// and V go from memory to the operands' registers, each once in the workgroup:
+// V is loaded ahead of the unit's first product, the next unit's K behind it.
+//
+// Rounding.  Scores, maxima and sums are fp32.  The products take 16-bit
+// operands: the cache's values are exact in them (q8_0 values are exact in
+// bf16, their scales multiply in fp32), q and p are split into parts whose sum
+// is the fp32 value to 2^-22 (two fp16 parts) or 2^-24 (three bf16 parts); for
+// 16-bit queries two bf16 parts (2^-17) are enough, as out is rounded to 2^-9
+// or 2^-12.  fp16 parts keep their exponent range by powers of two: q's row is
+// scaled to a maximum in [2^13, 2^14), p by 2^15.
+#pragma once
+
+#include <type_traits>
+
+#include "kv.h"
+
+namespace llapis {
+namespace dev {
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+
+enum { KV_F16 = 0, KV_BF16 = 1, KV_Q8 = 2 };
+
+template <bool HALF>
+__device__ __forceinline__ f4v mfma16(u4 a, u4 b, f4v c) {
+    if constexpr (HALF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+}
+
+// eight fp32 values as PARTS 16-bit operands whose sum they are
+template <bool HALF, int PARTS>
+__device__ __forceinline__ void split8(const float (&x)[8], u4 (&out)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if constexpr (HALF) {
+                const h2v h = {(_Float16)a, (_Float16)b};
+                out[p][i] = __builtin_bit_cast(uint32_t, h);
+                if (p + 1 < PARTS) { a -= (float)h[0]; b -= (float)h[1]; }
+            } else {
+                const b2v h = {(__bf16)a, (__bf16)b};
+                const uint32_t w = __builtin_bit_cast(uint32_t, h);
+                out[p][i] = w;
+                if (p + 1 < PARTS) {
+                    a -= __builtin_bit_cast(float, w << 16);
+                    b -= __builtin_bit_cast(float, w & 0xFFFF0000u);
+                }
+            }
+        }
+    }
+}
+
+// eight int8 values as bf16 (exact: at most 8 significant bits)
+__device__ __forceinline__ u4 i8_to_bf16(u2 q) {
+    u4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int w = (int)(q[i >> 1] >> ((i & 1) * 16));
+        const uint32_t a = __builtin_bit_cast(uint32_t, (float)(int8_t)w);
+        const uint32_t b = __builtin_bit_cast(uint32_t, (float)(int8_t)(w >> 8));
+        r[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    }
+    return r;
+}
+
+// the value of lane l ^ 16 / l ^ 32 combined with this lane's
+template <class F>
+__device__ __forceinline__ float over_groups(float x, F f) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = f(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const uint32_t w = __builtin_bit_cast(uint32_t, x);
+    const auto c = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return f(__builtin_bit_cast(float, (uint32_t)c[0]), __builtin_bit_cast(float, (uint32_t)c[1]));
+}
+
+__device__ __forceinline__ void load8(const void * p, int type, int64_t at, float (&x)[8]) {
+    if (type == T_F32) {
+        const f4v * f = (const f4v *)((const float *)p + at);
+        const f4v a = f[0], b = f[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+    } else {
+        const u4 w = *(const u4 *)((const uint16_t *)p + at);
+        if (type == T_F16) {
+            const h8v h = __builtin_bit_cast(h8v, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = __builtin_bit_cast(float, (i & 1) ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        }
+    }
+}
+
+__device__ __forceinline__ void store4(void * p, int type, int64_t at, f4v x) {
+    if (type == T_F32) {
+        *(f4v *)((float *)p + at) = x;
+    } else {
+        u2 w;
+        if (type == T_F16) {
+            const h2v a = {(_Float16)x[0], (_Float16)x[1]}, b = {(_Float16)x[2], (_Float16)x[3]};
+            w = u2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+        } else {
+            const b2v a = {(__bf16)x[0], (__bf16)x[1]}, b = {(__bf16)x[2], (__bf16)x[3]};
+            w = u2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+        }
+        *(u2 *)((uint16_t *)p + at) = w;
+    }
+}
+
+// a sequence's keys as the items see them
+struct SeqUnits {
+    SeqRows r;
+    int k0, kend;          // keys [k0, kend), k0 a multiple of KV_BLOCK
+    int units, tiles;      // of an item; row tiles of a kv head
+};
+
+__device__ __forceinline__ SeqUnits seq_units(const KvSeqs & b, int s, int page_shift, int window, int unit, int group,
+                                               int tile_rows) {
+    SeqUnits u;
+    u.r = seq_rows(b, s);
+    u.kend = min(u.r.len, b.max_pages << page_shift);
+    u.k0 = window > 0 ? min(max(u.r.len - u.r.n - window + 1, 0), u.kend) & ~(KV_BLOCK - 1) : 0;
+    u.units = u.r.n > 0 ? max((u.kend - u.k0 + unit - 1) / unit, 1) : 0;   // a row without keys is written too
+    u.tiles = (u.r.n * group + tile_rows - 1) / tile_rows;
+    return u;
+}
+
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// ... of a sequence that is the same in every lane, held in scalar registers
+__device__ __forceinline__ SeqUnits uniform_units(const SeqUnits & v) {
+    SeqUnits u;
+    u.r.row0 = same(v.r.row0);
+    u.r.n = same(v.r.n);
+    u.r.len = same(v.r.len);
+    u.k0 = same(v.k0);
+    u.kend = same(v.kend);
+    u.units = same(v.units);
+    u.tiles = same(v.tiles);
+    return u;
+}
+
+// run w of n_runs equal ones over `total` units
+__device__ __forceinline__ int run_begin(int w, int n_runs, int total) { return (int)((int64_t)w * total / n_runs); }
+
+// bit i: key `at` + i, i < 8, is in [from, to)
+__device__ __forceinline__ uint32_t seen8(int at, int from, int to) {
+    const uint32_t below = (1u << min(max(to - at, 0), 8)) - 1, before = (1u << min(max(from - at, 0), 8)) - 1;
+    return below & ~before;
+}
+// ones where bits i and i + 1 are set, for a pair of 16-bit values
+__device__ __forceinline__ uint32_t pair_mask(uint32_t bits, int i) {
+    const uint32_t a = (uint32_t)((int)(bits << (31 - i)) >> 31), b = (uint32_t)((int)(bits << (30 - i)) >> 31);
+    return (a & 0xFFFFu) | (b & 0xFFFF0000u);
+}
+
+constexpr float KV_LN2 = 0.69314718055994530942f, KV_LOG2E = 1.44269504088896340736f;
+
+template <int CT, bool F32IO, int HD, int NT>
+struct KvShape {
+    static constexpr bool HALF = CT == KV_F16;
+    static constexpr int PQ = HALF ? (F32IO ? 2 : 1) : (F32IO ? 3 : 2);
+    static constexpr int PP = HALF ? 2 : (F32IO ? 3 : 2);
+    static constexpr int UNIT = kv_unit(HD), KT = UNIT / (16 * KV_WAVES), NB = UNIT / KV_BLOCK;
+    static constexpr int NC = HD / 32, NV = HD / 16, NVW = (NV + KV_WAVES - 1) / KV_WAVES;
+    static constexpr int Q_BYTES = PQ * NT * NC * 1024;
+    static constexpr int P_BYTES = NB * NT * (CT == KV_Q8 ? 2 : PP) * 1024;     // q8_0: fp32, its scales come first
+    static constexpr int LDS = Q_BYTES + P_BYTES;
+};
+
+template <int CT, bool F32IO, int HD, int NT>
+__global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(const KvAttn p) {
+    using Sh = KvShape<CT, F32IO, HD, NT>;
+    constexpr bool HALF = Sh::HALF, Q8 = CT == KV_Q8;
+    constexpr int PQ = Sh::PQ, PP = Sh::PP, NC = Sh::NC, NV = Sh::NV, NVW = Sh::NVW, KT = Sh::KT, NB = Sh::NB;
+    constexpr int UNIT = Sh::UNIT, ROWS = 16 * NT;
+    constexpr int EL = Q8 ? 1 : 2;                                // bytes of a cached value
+    constexpr float P_SHIFT = HALF ? 15.0f : 0.0f;                // log2 of p's scale
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ int s_scan[256 + 1];
+    __shared__ uint32_t s_amax[ROWS];
+    __shared__ float s_top[KV_WAVES][ROWS];
+    uint8_t * const lds_p = lds + Sh::Q_BYTES;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = same(tid >> 6);
+    const int lm = lane & 15, lg = lane >> 4;
+    const int page = 1 << p.page_shift;
+
+    // ---- the line of units: thread t counts sequences [t per, (t + 1) per)
+    const int per = (p.b.n_seq + 255) / 256;
+    {
+        int sum = 0;
+        for (int i = 0; i < per; ++i) {
+            const int s = tid * per + i;
+            if (s < p.b.n_seq) {
+                const SeqUnits u = seq_units(p.b, s, p.page_shift, p.window, UNIT, p.group, ROWS);
+                sum += u.units * u.tiles * p.n_kv;
+            }
+        }
+        s_scan[tid + 1] = sum;
+        if (tid == 0) s_scan[0] = 0;
+        __syncthreads();
+        for (int o = 1; o < 256; o <<= 1) {
+            const int v = tid >= o ? s_scan[tid + 1 - o] : 0;
+            __syncthreads();
+            s_scan[tid + 1] += v;
+            __syncthreads();
+        }
+    }
+    const int total = same(s_scan[256]);
+    const int n_runs = min((int)gridDim.x, total);
+    if (blockIdx.x == 0) {
+        // for the join
+        int at = s_scan[tid];
+        for (int i = 0; i < per; ++i) {
+            const int s = tid * per + i;
+            if (s < p.b.n_seq) {
+                const SeqUnits u = seq_units(p.b, s, p.page_shift, p.window, UNIT, p.group, ROWS);
+                p.base[s] = at;
+                at += u.units * u.tiles * p.n_kv;
+            }
+        }
+        if (tid == 0) p.base[p.b.n_seq] = total;
+    }
+    if ((int)blockIdx.x >= n_runs) return;
+    const int lo = run_begin(blockIdx.x, n_runs, total), hi = run_begin(blockIdx.x + 1, n_runs, total);
+
+    // ---- the sequence of the first unit
+    int seq, seq_at;
+    {
+        int t = 0;
+        for (int step = 128; step; step >>= 1)
+            if (t + step < 256 && s_scan[t + step] <= lo) t += step;
+        t = same(t);
+        seq = t * per;
+        seq_at = same(s_scan[t]);
+    }
+    SeqUnits su = uniform_units(seq_units(p.b, seq, p.page_shift, p.window, UNIT, p.group, ROWS));
+    for (int u = lo; u < hi;) {
+        int n_here;
+        // (the bounds hold if another stream changes the lengths meanwhile)
+        while (u - seq_at >= (n_here = su.units * su.tiles * p.n_kv) && seq + 1 < p.b.n_seq) {
+            seq_at += n_here;
+            ++seq;
+            su = uniform_units(seq_units(p.b, seq, p.page_shift, p.window, UNIT, p.group, ROWS));
+        }
+        if (u - seq_at >= n_here) return;
+        const int item = (u - seq_at) / su.units, u0 = (u - seq_at) - item * su.units;
+        const int n_u = min(su.units - u0, hi - u);
+        const int head = item / su.tiles, tile = item - head * su.tiles;
+        const int n_rows = min(su.r.n * p.group - tile * ROWS, ROWS);
+        const bool whole = n_u == su.units;
+        const int slot = 2 * blockIdx.x + (u0 == 0);
+        u += n_u;
+
+        // ---- Q into LDS as B operands: (part, row tile, 32 values) x lane
+        constexpr int NQ = NT * NC * 64;
+        constexpr int QE = (NQ + 255) / 256;
+        float qx[QE][8];
+        __syncthreads();                                           // the last item's LDS has been read
+        if (HALF && tid < ROWS) s_amax[tid] = 0;
+        if (HALF) __syncthreads();
+#pragma unroll
+        for (int e = 0; e < QE; ++e) {
+            const int i = tid + 256 * e;
+            const int l = i & 63, c = (i >> 6) % NC, nt = (i >> 6) / NC;
+            const int r = 16 * nt + (l & 15);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) qx[e][j] = 0.0f;
+            if (i < NQ && r < n_rows) {
+                const int rr = tile * ROWS + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
+                load8(p.q, F32IO ? (int)T_F32 : p.type, (su.r.row0 + tok) * p.q_stride + hq * HD + 32 * c + 8 * (l >> 4), qx[e]);
+                if (HALF) {
+                    float a = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) a = fmaxf(a, fabsf(qx[e][j]));
+                    atomicMax(&s_amax[r], __builtin_bit_cast(uint32_t, a));
+                }
+            }
+        }
+        if (HALF) __syncthreads();
+#pragma unroll
+        for (int e = 0; e < QE; ++e) {
+            const int i = tid + 256 * e;
+            if (i < NQ) {
+                const int r = 16 * ((i >> 6) / NC) + (i & 15);
+                if (HALF) {
+                    // to [2^13, 2^14): exact, and undone with the scale (frexp's exponent; 0 and non-finite: left)
+                    const float a = __builtin_bit_cast(float, s_amax[r]);
+                    const int ex = a > 0.0f && a < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(a) : 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) qx[e][j] = __builtin_ldexpf(qx[e][j], ex);
+                }
+                u4 part[PQ];
+                split8<HALF, PQ>(qx[e], part);
+#pragma unroll
+                for (int q = 0; q < PQ; ++q) *(u4 *)(lds + ((size_t)q * NQ + i) * 16) = part[q];
+            }
+        }
+        // a lane's query rows: score scale in log2, last visible key, first visible key
+        float q_scale[NT];
+        int t_pos[NT], tok_of[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = 16 * nt + lm, rr = tile * ROWS + r;
+            tok_of[nt] = min(rr / p.group, su.r.n - 1);
+            t_pos[nt] = su.r.len - su.r.n + tok_of[nt];
+            q_scale[nt] = p.scale * KV_LOG2E;
+            if (HALF) {
+                const float a = __builtin_bit_cast(float, s_amax[r]);
+                const int ex = a > 0.0f && a < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(a) : 0;
+                q_scale[nt] = __builtin_ldexpf(q_scale[nt], -ex);
+            }
+        }
+        __syncthreads();
+
+        // ---- the units
+        f4v acc[NT][NVW];
+        float m[NT], l[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt] = -__builtin_inff();
+            l[nt] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < NVW; ++t) acc[nt][t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int key_begin = su.k0 + u0 * UNIT;
+        const int key_end = min(key_begin + n_u * UNIT, su.kend);
+        const int32_t * row = p.b.table + seq * p.b.table_stride;
+        // keys that every row of the sequence sees
+        const int all_to = su.r.len - su.r.n + 1;                            // one past the first new token
+        const int all_from = p.window > 0 ? su.r.len - p.window : 0;         // the last one's first key
+        // places of the wave's keys in the unit: those of its K rows, those of the lane's scores
+        const int w_block = KT == 2 ? wave : wave >> 1, w_half = KT == 2 ? 0 : 4 * (wave & 1);
+        const int k_oct = KV_BLOCK * w_block + 8 * (lm >> 2), s_oct = KV_BLOCK * w_block + 8 * lg;
+        const int page_mask = page - 1;
+        auto page_at = [&](int key) {
+            const int i = key >> p.page_shift;
+            const int pg = row[min(i, p.b.max_pages - 1)];
+            return i < p.b.max_pages ? pg : -1;
+        };
+        auto has_page = [&](int pg) { return (uint32_t)pg < (uint32_t)p.n_pages; };
+        // a head's part of a page, whose int8 values its scales follow
+        const uint64_t part = (uint64_t)head * page * (Q8 ? HD + HD / 16 : 2 * HD);
+        const uint8_t * kbase = p.k + part;
+        const uint8_t * vbase = p.v + part;
+        typedef typename std::conditional<Q8, u2, u4>::type frag;
+        typedef typename std::conditional<KT == 2, u4, u2>::type scales;
+        frag kf[KT][NC], vf[NB][NVW];
+        scales kd[Q8 ? NC : 1];                       // fp16, of the keys whose scores the lane holds
+        int k_pg, s_pg, v_pg[NB];
+        auto load_pages = [&](int at) {
+            k_pg = page_at(at + k_oct);
+            s_pg = Q8 ? page_at(at + s_oct) : 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) v_pg[b] = page_at(at + KV_BLOCK * b + 8 * lg);
+        };
+        auto load_k = [&](int at) {
+            const uint8_t * a = kbase + (uint64_t)(has_page(k_pg) ? k_pg : 0) * p.k_stride +
+                                (((at + k_oct + w_half + (lm & 3)) & page_mask) * HD + 8 * lg) * EL;
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) kf[t][c] = *(const frag *)(a + (4 * t * HD + 32 * c) * EL);
+            if constexpr (Q8) {
+                const uint8_t * d = kbase + (uint64_t)(has_page(s_pg) ? s_pg : 0) * p.k_stride + page * HD +
+                                    ((at + s_oct + w_half) & page_mask) * 2;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) kd[c] = *(const scales *)(d + c * page * 2);
+            }
+        };
+        // the wave's columns of V, from 16 v_tile on (a tile past the last one reads it again)
+        const int v_tile = wave * NVW;
+        if (key_begin < key_end) {
+            load_pages(key_begin);
+            load_k(key_begin);
+        }
+        int lv = lm;
+        for (int key = key_begin; key < key_end; key += UNIT) {
+            asm volatile("" : "+v"(lv));              // V's offsets are formed anew, not held
+            bool full = key + UNIT <= min(all_to, key_end) && key >= all_from;
+            bool s_ok = true;                         // the lane's scores have a page
+            uint32_t ok = 0;                          // bit b: the lane's octet of block b has a page
+            const uint8_t * va[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                va[b] = vbase + (uint64_t)(has_page(v_pg[b]) ? v_pg[b] : 0) * p.v_stride;
+                ok |= (uint32_t)has_page(v_pg[b]) << b;
+            }
+            full = full && __all(ok == (1u << NB) - 1);
+            s_ok = (ok >> w_block) & 1;
+            const int next = key + UNIT;
+            if (next < key_end) load_pages(next);
+            u4 vd[Q8 ? NB : 1][Q8 ? (NVW + 1) / 2 : 1];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int slot = (key + KV_BLOCK * b + 8 * lg) & page_mask;
+#pragma unroll
+                for (int t = 0; t < NVW; ++t) {
+                    const int tile = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
+                    vf[b][t] = *(const frag *)(va[b] + ((16 * tile + lv) * page + slot) * EL);
+                }
+                if constexpr (Q8)
+#pragma unroll
+                    for (int i = 0; i < (NVW + 1) / 2; ++i) {
+                        const int c = min((v_tile >> 1) + i, NC - 1);
+                        vd[b][i] = *(const u4 *)(va[b] + page * HD + (c * page + slot) * 2);
+                    }
+            }
+            // ---- S^T of the wave's keys
+            __builtin_amdgcn_sched_barrier(0);
+            f4v sc[NT][KT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < KT; ++t) sc[nt][t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                u4 a[KT];
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+                    if constexpr (Q8) a[t] = i8_to_bf16(kf[t][c]);
+                    else a[t] = kf[t][c];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    f4v part[KT];
+#pragma unroll
+                    for (int t = 0; t < KT; ++t) part[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int q = 0; q < PQ; ++q) {
+                        const u4 b = *(const u4 *)(lds + ((q * NT + nt) * NC + c) * 1024 + lane * 16);
+#pragma unroll
+                        for (int t = 0; t < KT; ++t)
+                            if constexpr (Q8) part[t] = mfma16<HALF>(a[t], b, part[t]);
+                            else sc[nt][t] = mfma16<HALF>(a[t], b, sc[nt][t]);
+                    }
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int t = 0; t < KT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const h2v d = __builtin_bit_cast(h2v, (uint32_t)kd[c][2 * t + (i >> 1)]);
+                                sc[nt][t][i] = __builtin_fmaf(part[t][i], (float)d[i & 1], sc[nt][t][i]);
+                            }
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (next < key_end) load_k(next);
+            __builtin_amdgcn_sched_barrier(0);
+            // ---- softmax: the lane's keys are key + s_oct + w_half + (0 .. 4 KT - 1)
+            const int s_key = key + s_oct + w_half;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < KT; ++t) sc[nt][t] *= q_scale[nt];
+            if (!full) {
+                const int page_end = s_ok ? key_end : 0;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const int from = p.window > 0 ? t_pos[nt] - p.window + 1 : 0, to = min(t_pos[nt] + 1, page_end);
+#pragma unroll
+                    for (int t = 0; t < KT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = s_key + 4 * t + i;
+                            sc[nt][t][i] = ((at >= from) & (at < to)) ? sc[nt][t][i] : -__builtin_inff();
+                        }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[nt][t][i]);
+                top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
+                if (lg == 0) s_top[wave][16 * nt + lm] = top;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float now = m[nt];
+#pragma unroll
+                for (int w = 0; w < KV_WAVES; ++w) now = fmaxf(now, s_top[w][16 * nt + lm]);
+                const float ref = now == -__builtin_inff() ? 0.0f : now;
+                if (__any(now != m[nt])) {
+                    const float f = __builtin_amdgcn_exp2f(m[nt] - ref);
+                    l[nt] *= f;
+#pragma unroll
+                    for (int t = 0; t < NVW; ++t) acc[nt][t] *= f;
+                    m[nt] = now;
+                }
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4 * KT; ++i) {
+                    x[i] = __builtin_amdgcn_exp2f(sc[nt][i >> 2][i & 3] - (ref - P_SHIFT));
+                    l[nt] += x[i];
+                }
+                if constexpr (Q8) {
+                    uint8_t * w = lds_p + (w_block * NT + nt) * 2048 + lane * 32 + 4 * w_half;
+#pragma unroll
+                    for (int t = 0; t < KT; ++t) *(f4v *)(w + 16 * t) = f4v{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+                } else {
+#pragma unroll
+                    for (int i = 4 * KT; i < 8; ++i) x[i] = 0.0f;
+                    u4 part[PP];
+                    split8<HALF, PP>(x, part);
+#pragma unroll
+                    for (int q = 0; q < PP; ++q) {
+                        uint8_t * w = lds_p + ((w_block * NT + nt) * PP + q) * 1024 + lane * 16;
+                        if constexpr (KT == 2) *(u4 *)w = part[q];
+                        else *(u2 *)(w + 2 * w_half) = u2{part[q][0], part[q][1]};
+                    }
+                }
+            }
+            __syncthreads();
+            // ---- O^T of the wave's columns
+            if constexpr (Q8) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const f4v * x = (const f4v *)(lds_p + (b * NT + nt) * 2048 + lane * 32);
+                        const f4v x0 = x[0], x1 = x[1];
+                        u4 bp[PP];
+#pragma unroll
+                        for (int t = 0; t < NVW; ++t) {
+                            // the scales of the tile's 32 columns; two tiles share them where v_tile is even
+                            if (NVW % 2 || t % 2 == 0) {
+                                const u4 w = NVW % 2 ? (((v_tile + t) >> 1) - (v_tile >> 1) ? vd[b][(t + 1) / 2] : vd[b][t / 2]) : vd[b][t / 2];
+                                const h8v d = __builtin_bit_cast(h8v, w);
+                                float y[8];
+                                // a masked key's p is 0 whatever its scale holds
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const float xi = i < 4 ? x0[i & 3] : x1[i & 3];
+                                    y[i] = xi != 0.0f ? xi * (float)d[i] : 0.0f;
+                                }
+                                split8<HALF, PP>(y, bp);
+                            }
+                            const u4 a = i8_to_bf16(vf[b][t]);
+#pragma unroll
+                            for (int q = 0; q < PP; ++q) acc[nt][t] = mfma16<HALF>(a, bp[q], acc[nt][t]);
+                        }
+                    }
+            } else {
+                // 0 times a masked infinity is no zero: V's values of keys that a row
+                // does not see become 0
+                const int core_to = min(all_to, key_end);
+                if (!full) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t bits = (ok >> b) & 1 ? seen8(key + KV_BLOCK * b + 8 * lg, all_from, core_to) : 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t keep = pair_mask(bits, 2 * i);
+#pragma unroll
+                            for (int t = 0; t < NVW; ++t) vf[b][t][i] &= keep;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int q = 0; q < PP; ++q) {
+                            const u4 bp = *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16);
+#pragma unroll
+                            for (int t = 0; t < NVW; ++t) acc[nt][t] = mfma16<HALF>(vf[b][t], bp, acc[nt][t]);
+                        }
+                // ... and keys that only some of a sequence's tokens see (at its
+                // end, at the window's begin) are added token by token
+                if (!full && su.r.n > 1) {
+#pragma unroll 1
+                    for (int b = 0; b < NB; ++b) {
+                        const int kb = key + KV_BLOCK * b;
+                        const int first = p.window > 0 ? su.r.len - su.r.n - p.window + 1 : 0;
+                        if (!((kb + KV_BLOCK > core_to && kb < key_end) || (kb < all_from && kb + KV_BLOCK > first))) continue;
+                        const int at = kb + 8 * lg, pg = page_at(at);
+                        const uint8_t * a = vbase + (uint64_t)(has_page(pg) ? pg : 0) * p.v_stride + (at & page_mask) * EL;
+                        u4 vz[NVW];
+#pragma unroll
+                        for (int t = 0; t < NVW; ++t) {
+                            const int tile = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
+                            vz[t] = *(const u4 *)(a + (16 * tile + lv) * page * EL);
+                        }
+#pragma unroll 1
+                        for (int tok = 0; tok < su.r.n; ++tok) {
+                            asm volatile("" ::: "memory");    // P stays in LDS
+                            const int pos = su.r.len - su.r.n + tok;
+                            uint32_t bits = seen8(at, p.window > 0 ? pos - p.window + 1 : 0, min(pos + 1, key_end));
+                            bits = has_page(pg) ? bits & ~seen8(at, all_from, core_to) : 0;
+#pragma unroll
+                            for (int t = 0; t < NVW; ++t) {
+                                u4 v;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[i] = vz[t][i] & pair_mask(bits, 2 * i);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    f4v d = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                    for (int q = 0; q < PP; ++q)
+                                        d = mfma16<HALF>(v, *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16), d);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) acc[nt][t][i] += tok_of[nt] == tok ? d[i] : 0.0f;
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- the sums of the four waves, in their order; maxima are the same in all
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) l[nt] = over_groups(l[nt], [](float a, float b) { return a + b; });
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            if (lg == 0) s_top[wave][16 * nt + lm] = l[nt];
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = 16 * nt + lm;
+            if (r >= n_rows) continue;
+            const float sum = (s_top[0][r] + s_top[1][r]) + (s_top[2][r] + s_top[3][r]);
+            if (whole) {
+                const int rr = tile * ROWS + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
+                const int64_t out_row = su.r.row0 + tok;
+                const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                for (int t = 0; t < NVW; ++t)
+                    if (v_tile + t < NV)
+                        store4(p.out, F32IO ? (int)T_F32 : p.type,
+                               out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
+                if (p.lse && wave == 0 && lg == 0)
+                    p.lse[out_row * (p.group * p.n_kv) + hq] =
+                        sum == 0.0f ? -__builtin_inff() : (m[nt] + (__builtin_amdgcn_logf(sum) - P_SHIFT)) * KV_LN2;
+            } else {
+                float * a = p.acc + ((int64_t)slot * ROWS + r) * HD;
+#pragma unroll
+                for (int t = 0; t < NVW; ++t)
+                    if (v_tile + t < NV) *(f4v *)(a + 16 * (v_tile + t) + 4 * lg) = acc[nt][t];
+                if (wave == 0 && lg == 0) {
+                    p.ml[((int64_t)slot * ROWS + r) * 2] = m[nt];
+                    p.ml[((int64_t)slot * ROWS + r) * 2 + 1] = sum;
+                }
+            }
+        }
+    }
+}
+
+template <int CT, bool F32IO, int HD, int NT>
+hipError_t launch_kv_attn_one(const KvAttn & p, int grid, hipStream_t s) {
+    constexpr int lds = KvShape<CT, F32IO, HD, NT>::LDS;
+    hipLaunchKernelGGL((k_kv_attn<CT, F32IO, HD, NT>), dim3(grid), dim3(256), lds, s, p);
+    return hipGetLastError();
+}
+
+template <int CT, bool F32IO, int NT>
+hipError_t launch_kv_attn_hd(const KvAttn & p, int head_dim, int grid, hipStream_t s) {
+    switch (head_dim) {
+        case 64: return launch_kv_attn_one<CT, F32IO, 64, NT>(p, grid, s);
+        case 96: return launch_kv_attn_one<CT, F32IO, 96, NT>(p, grid, s);
+        case 128: return launch_kv_attn_one<CT, F32IO, 128, NT>(p, grid, s);
+        case 192: return launch_kv_attn_one<CT, F32IO, 192, NT>(p, grid, s);
+        case 256: return launch_kv_attn_one<CT, F32IO, 256, NT>(p, grid, s);
+        case 512: return launch_kv_attn_one<CT, F32IO, 512, NT>(p, grid, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <int CT>
+hipError_t launch_kv_attn_type(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s) {
+    if (p.type == T_F32)
+        return nt == 1 ? launch_kv_attn_hd<CT, true, 1>(p, head_dim, grid, s) : launch_kv_attn_hd<CT, true, 2>(p, head_dim, grid, s);
+    return nt == 1 ? launch_kv_attn_hd<CT, false, 1>(p, head_dim, grid, s) : launch_kv_attn_hd<CT, false, 2>(p, head_dim, grid, s);
+}
+
+}  // namespace dev
+}  // namespace llapis

@@ -1,0 +1,10 @@
+// kv_attn_bf16.hip -- kv_attn.h's kernel for this cache type.
+#include "kv_attn.h"
+
+namespace llapis {
+
+hipError_t launch_kv_attn_bf16(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s) {
+    return dev::launch_kv_attn_type<dev::KV_BF16>(p, head_dim, nt, grid, s);
+}
+
+}  // namespace llapis
