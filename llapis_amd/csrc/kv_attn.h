@@ -213,13 +213,15 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
     constexpr float P_SHIFT = HALF ? 15.0f : 0.0f;                // log2 of p's scale
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int s_scan[256 + 1];
-    __shared__ uint32_t s_amax[ROWS];
+    __shared__ int s_part[KV_WAVES];
+    __shared__ int s_exp[ROWS];
     __shared__ float s_top[KV_WAVES][ROWS];
     uint8_t * const lds_p = lds + Sh::Q_BYTES;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = same(tid >> 6);
     const int lm = lane & 15, lg = lane >> 4;
-    const int page = 1 << p.page_shift;
+    const int page = 1 << p.page_shift, page_mask = page - 1;
+    auto units_at = [&](int s) { return seq_units(p.b, s, p.page_shift, p.window, UNIT, p.group, ROWS); };
 
     // ---- the line of units: thread t counts sequences [t per, (t + 1) per)
     const int per = (p.b.n_seq + 255) / 256;
@@ -228,19 +230,20 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
         for (int i = 0; i < per; ++i) {
             const int s = tid * per + i;
             if (s < p.b.n_seq) {
-                const SeqUnits u = seq_units(p.b, s, p.page_shift, p.window, UNIT, p.group, ROWS);
+                const SeqUnits u = units_at(s);
                 sum += u.units * u.tiles * p.n_kv;
             }
         }
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 63) s_part[wave] = sum;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) sum += s_part[w];
         s_scan[tid + 1] = sum;
         if (tid == 0) s_scan[0] = 0;
         __syncthreads();
-        for (int o = 1; o < 256; o <<= 1) {
-            const int v = tid >= o ? s_scan[tid + 1 - o] : 0;
-            __syncthreads();
-            s_scan[tid + 1] += v;
-            __syncthreads();
-        }
     }
     const int total = same(s_scan[256]);
     const int n_runs = min((int)gridDim.x, total);
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
         for (int i = 0; i < per; ++i) {
             const int s = tid * per + i;
             if (s < p.b.n_seq) {
-                const SeqUnits u = seq_units(p.b, s, p.page_shift, p.window, UNIT, p.group, ROWS);
+                const SeqUnits u = units_at(s);
                 p.base[s] = at;
                 at += u.units * u.tiles * p.n_kv;
             }
@@ -260,94 +263,154 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
     if ((int)blockIdx.x >= n_runs) return;
     const int lo = run_begin(blockIdx.x, n_runs, total), hi = run_begin(blockIdx.x + 1, n_runs, total);
 
-    // ---- the sequence of the first unit
-    int seq, seq_at;
+    // ---- the sequence of the first unit, and from there on piece by piece
+    int at_seq, at_unit;                              // a sequence and its first unit
     {
         int t = 0;
         for (int step = 128; step; step >>= 1)
             if (t + step < 256 && s_scan[t + step] <= lo) t += step;
         t = same(t);
-        seq = t * per;
-        seq_at = same(s_scan[t]);
+        at_seq = t * per;
+        at_unit = same(s_scan[t]);
     }
-    SeqUnits su = uniform_units(seq_units(p.b, seq, p.page_shift, p.window, UNIT, p.group, ROWS));
-    for (int u = lo; u < hi;) {
+    struct Piece {
+        SeqUnits su;
+        int seq, head, tile, u0, n_u, key_begin, key_end;
+        const int32_t * row;                          // of the page table
+        uint64_t part;                                // a head's part of a page, which its scales follow
+    };
+    SeqUnits at_su = uniform_units(units_at(at_seq));
+    // the piece from unit u on; false where another stream has changed the lengths meanwhile
+    auto piece_at = [&](int u, Piece & c) {
         int n_here;
-        // (the bounds hold if another stream changes the lengths meanwhile)
-        while (u - seq_at >= (n_here = su.units * su.tiles * p.n_kv) && seq + 1 < p.b.n_seq) {
-            seq_at += n_here;
-            ++seq;
-            su = uniform_units(seq_units(p.b, seq, p.page_shift, p.window, UNIT, p.group, ROWS));
+        while (u - at_unit >= (n_here = at_su.units * at_su.tiles * p.n_kv)) {
+            if (at_seq + 1 >= p.b.n_seq) return false;
+            at_unit += n_here;
+            ++at_seq;
+            at_su = uniform_units(units_at(at_seq));
         }
-        if (u - seq_at >= n_here) return;
-        const int item = (u - seq_at) / su.units, u0 = (u - seq_at) - item * su.units;
-        const int n_u = min(su.units - u0, hi - u);
-        const int head = item / su.tiles, tile = item - head * su.tiles;
-        const int n_rows = min(su.r.n * p.group - tile * ROWS, ROWS);
-        const bool whole = n_u == su.units;
-        const int slot = 2 * blockIdx.x + (u0 == 0);
-        u += n_u;
+        c.su = at_su;
+        c.seq = at_seq;
+        const int item = (u - at_unit) / at_su.units;
+        c.u0 = u - at_unit - item * at_su.units;
+        c.n_u = min(at_su.units - c.u0, hi - u);
+        c.head = item / at_su.tiles;
+        c.tile = item - c.head * at_su.tiles;
+        c.key_begin = at_su.k0 + c.u0 * UNIT;
+        c.key_end = min(c.key_begin + c.n_u * UNIT, at_su.kend);
+        c.row = p.b.table + at_seq * p.b.table_stride;
+        c.part = (uint64_t)c.head * page * (Q8 ? HD + HD / 16 : 2 * HD);
+        return true;
+    };
 
-        // ---- Q into LDS as B operands: (part, row tile, 32 values) x lane
-        constexpr int NQ = NT * NC * 64;
-        constexpr int QE = (NQ + 255) / 256;
-        float qx[QE][8];
-        __syncthreads();                                           // the last item's LDS has been read
-        if (HALF && tid < ROWS) s_amax[tid] = 0;
-        if (HALF) __syncthreads();
+    // ---- loads of a unit's K, ahead of its use
+    // places of the wave's keys in a unit: those of its K rows, those of the lane's scores
+    const int w_block = KT == 2 ? wave : wave >> 1, w_half = KT == 2 ? 0 : 4 * (wave & 1);
+    const int k_oct = KV_BLOCK * w_block + 8 * (lm >> 2), s_oct = KV_BLOCK * w_block + 8 * lg;
+    typedef typename std::conditional<Q8, u2, u4>::type frag;
+    typedef typename std::conditional<KT == 2, u4, u2>::type scales;
+    frag kf[KT][NC], vf[NB][NVW];
+    scales kd[Q8 ? NC : 1];                           // fp16, of the keys whose scores the lane holds
+    int k_pg = 0, s_pg = 0, v_pg[NB];
+    auto has_page = [&](int pg) { return (uint32_t)pg < (uint32_t)p.n_pages; };
+    auto page_at = [&](const int32_t * row, int key) {
+        const int i = key >> p.page_shift;
+        const int pg = row[min(i, p.b.max_pages - 1)];
+        return i < p.b.max_pages ? pg : -1;
+    };
+    auto load_pages = [&](const int32_t * row, int at) {
+        k_pg = page_at(row, at + k_oct);
+        s_pg = Q8 ? page_at(row, at + s_oct) : 0;
 #pragma unroll
-        for (int e = 0; e < QE; ++e) {
-            const int i = tid + 256 * e;
-            const int l = i & 63, c = (i >> 6) % NC, nt = (i >> 6) / NC;
-            const int r = 16 * nt + (l & 15);
+        for (int b = 0; b < NB; ++b) v_pg[b] = page_at(row, at + KV_BLOCK * b + 8 * lg);
+    };
+    auto load_k = [&](uint64_t part, int at) {
+        const uint8_t * a = p.k + part + (uint64_t)(has_page(k_pg) ? k_pg : 0) * p.k_stride +
+                            (((at + k_oct + w_half + (lm & 3)) & page_mask) * HD + 8 * lg) * EL;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) qx[e][j] = 0.0f;
-            if (i < NQ && r < n_rows) {
-                const int rr = tile * ROWS + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
-                load8(p.q, F32IO ? (int)T_F32 : p.type, (su.r.row0 + tok) * p.q_stride + hq * HD + 32 * c + 8 * (l >> 4), qx[e]);
-                if (HALF) {
-                    float a = 0.0f;
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) a = fmaxf(a, fabsf(qx[e][j]));
-                    atomicMax(&s_amax[r], __builtin_bit_cast(uint32_t, a));
+            for (int c = 0; c < NC; ++c) kf[t][c] = *(const frag *)(a + (4 * t * HD + 32 * c) * EL);
+        if constexpr (Q8) {
+            const uint8_t * d = p.k + part + (uint64_t)(has_page(s_pg) ? s_pg : 0) * p.k_stride + page * HD +
+                                ((at + s_oct + w_half) & page_mask) * 2;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) kd[c] = *(const scales *)(d + c * page * 2);
+        }
+    };
+    // the wave's columns of V, from 16 v_tile on (a tile past the last one reads it again)
+    const int v_tile = wave * NVW;
+
+    Piece cur, then;
+    if (!piece_at(lo, cur)) return;
+    if (cur.key_begin < cur.key_end) {
+        load_pages(cur.row, cur.key_begin);
+        load_k(cur.part, cur.key_begin);
+    }
+    for (int u = lo;;) {
+        const SeqUnits & su = cur.su;
+        const int head = cur.head, tile = cur.tile, key_end = cur.key_end;
+        const int n_rows = min(su.r.n * p.group - tile * ROWS, ROWS);
+        const bool whole = cur.n_u == su.units;
+        const int slot = 2 * blockIdx.x + (cur.u0 == 0);
+        u += cur.n_u;
+
+        // ---- Q into LDS as B operands, (part, row tile, 32 values) x lane: 16
+        // threads a row
+        constexpr int QE = (HD / 8 + 15) / 16;
+        __syncthreads();                                           // the last piece's LDS has been read
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = 16 * nt + (tid >> 4), rr = tile * ROWS + r, tok = rr / p.group;
+            const int64_t from = (su.r.row0 + tok) * p.q_stride + (int64_t)(head * p.group + rr - tok * p.group) * HD;
+            float qx[QE][8];
+            float amax = 0.0f;
+#pragma unroll
+            for (int e = 0; e < QE; ++e) {
+                const int o = (tid & 15) + 16 * e;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) qx[e][j] = 0.0f;
+                if (r < n_rows && o < HD / 8) load8(p.q, F32IO ? (int)T_F32 : p.type, from + 8 * o, qx[e]);
+                if (HALF)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[e][j]));
+            }
+            int ex = 0;
+            if (HALF) {
+                // the row's largest to [2^13, 2^14): exact, and undone with the scale (0 and non-finite: left)
+#pragma unroll
+                for (int o = 8; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+                ex = amax > 0.0f && amax < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(amax) : 0;
+                if ((tid & 15) == 0) s_exp[r] = ex;
+            }
+#pragma unroll
+            for (int e = 0; e < QE; ++e) {
+                const int o = (tid & 15) + 16 * e;
+                if (o < HD / 8) {
+                    if (HALF)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) qx[e][j] = __builtin_ldexpf(qx[e][j], ex);
+                    u4 part[PQ];
+                    split8<HALF, PQ>(qx[e], part);
+#pragma unroll
+                    for (int q = 0; q < PQ; ++q)
+                        *(u4 *)(lds + ((q * NT + nt) * NC + (o >> 2)) * 1024 + ((o & 3) * 16 + (tid >> 4)) * 16) = part[q];
                 }
             }
         }
-        if (HALF) __syncthreads();
-#pragma unroll
-        for (int e = 0; e < QE; ++e) {
-            const int i = tid + 256 * e;
-            if (i < NQ) {
-                const int r = 16 * ((i >> 6) / NC) + (i & 15);
-                if (HALF) {
-                    // to [2^13, 2^14): exact, and undone with the scale (frexp's exponent; 0 and non-finite: left)
-                    const float a = __builtin_bit_cast(float, s_amax[r]);
-                    const int ex = a > 0.0f && a < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(a) : 0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) qx[e][j] = __builtin_ldexpf(qx[e][j], ex);
-                }
-                u4 part[PQ];
-                split8<HALF, PQ>(qx[e], part);
-#pragma unroll
-                for (int q = 0; q < PQ; ++q) *(u4 *)(lds + ((size_t)q * NQ + i) * 16) = part[q];
-            }
-        }
-        // a lane's query rows: score scale in log2, last visible key, first visible key
+        // the next piece, whose first K is loaded during this one's last unit
+        const bool more = u < hi && piece_at(u, then);
+        __syncthreads();
+        // a lane's query rows: score scale in log2, position
         float q_scale[NT];
         int t_pos[NT], tok_of[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = 16 * nt + lm, rr = tile * ROWS + r;
-            tok_of[nt] = min(rr / p.group, su.r.n - 1);
+            tok_of[nt] = min((tile * ROWS + 16 * nt + lm) / p.group, su.r.n - 1);
             t_pos[nt] = su.r.len - su.r.n + tok_of[nt];
             q_scale[nt] = p.scale * KV_LOG2E;
-            if (HALF) {
-                const float a = __builtin_bit_cast(float, s_amax[r]);
-                const int ex = a > 0.0f && a < __builtin_inff() ? 14 - __builtin_amdgcn_frexp_expf(a) : 0;
-                q_scale[nt] = __builtin_ldexpf(q_scale[nt], -ex);
-            }
+            if (HALF) q_scale[nt] = __builtin_ldexpf(q_scale[nt], -s_exp[16 * nt + lm]);
         }
-        __syncthreads();
 
         // ---- the units
         f4v acc[NT][NVW];
@@ -359,59 +422,17 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
 #pragma unroll
             for (int t = 0; t < NVW; ++t) acc[nt][t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        const int key_begin = su.k0 + u0 * UNIT;
-        const int key_end = min(key_begin + n_u * UNIT, su.kend);
-        const int32_t * row = p.b.table + seq * p.b.table_stride;
         // keys that every row of the sequence sees
         const int all_to = su.r.len - su.r.n + 1;                            // one past the first new token
         const int all_from = p.window > 0 ? su.r.len - p.window : 0;         // the last one's first key
-        // places of the wave's keys in the unit: those of its K rows, those of the lane's scores
-        const int w_block = KT == 2 ? wave : wave >> 1, w_half = KT == 2 ? 0 : 4 * (wave & 1);
-        const int k_oct = KV_BLOCK * w_block + 8 * (lm >> 2), s_oct = KV_BLOCK * w_block + 8 * lg;
-        const int page_mask = page - 1;
-        auto page_at = [&](int key) {
-            const int i = key >> p.page_shift;
-            const int pg = row[min(i, p.b.max_pages - 1)];
-            return i < p.b.max_pages ? pg : -1;
-        };
-        auto has_page = [&](int pg) { return (uint32_t)pg < (uint32_t)p.n_pages; };
-        // a head's part of a page, whose int8 values its scales follow
-        const uint64_t part = (uint64_t)head * page * (Q8 ? HD + HD / 16 : 2 * HD);
-        const uint8_t * kbase = p.k + part;
-        const uint8_t * vbase = p.v + part;
-        typedef typename std::conditional<Q8, u2, u4>::type frag;
-        typedef typename std::conditional<KT == 2, u4, u2>::type scales;
-        frag kf[KT][NC], vf[NB][NVW];
-        scales kd[Q8 ? NC : 1];                       // fp16, of the keys whose scores the lane holds
-        int k_pg, s_pg, v_pg[NB];
-        auto load_pages = [&](int at) {
-            k_pg = page_at(at + k_oct);
-            s_pg = Q8 ? page_at(at + s_oct) : 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) v_pg[b] = page_at(at + KV_BLOCK * b + 8 * lg);
-        };
-        auto load_k = [&](int at) {
-            const uint8_t * a = kbase + (uint64_t)(has_page(k_pg) ? k_pg : 0) * p.k_stride +
-                                (((at + k_oct + w_half + (lm & 3)) & page_mask) * HD + 8 * lg) * EL;
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) kf[t][c] = *(const frag *)(a + (4 * t * HD + 32 * c) * EL);
-            if constexpr (Q8) {
-                const uint8_t * d = kbase + (uint64_t)(has_page(s_pg) ? s_pg : 0) * p.k_stride + page * HD +
-                                    ((at + s_oct + w_half) & page_mask) * 2;
-#pragma unroll
-                for (int c = 0; c < NC; ++c) kd[c] = *(const scales *)(d + c * page * 2);
-            }
-        };
-        // the wave's columns of V, from 16 v_tile on (a tile past the last one reads it again)
-        const int v_tile = wave * NVW;
-        if (key_begin < key_end) {
-            load_pages(key_begin);
-            load_k(key_begin);
+        const uint8_t * vbase = p.v + cur.part;
+        const bool then_keys = more && then.key_begin < then.key_end;
+        if (cur.key_begin >= key_end && then_keys) {
+            load_pages(then.row, then.key_begin);
+            load_k(then.part, then.key_begin);
         }
         int lv = lm;
-        for (int key = key_begin; key < key_end; key += UNIT) {
+        for (int key = cur.key_begin; key < key_end; key += UNIT) {
             asm volatile("" : "+v"(lv));              // V's offsets are formed anew, not held
             bool full = key + UNIT <= min(all_to, key_end) && key >= all_from;
             bool s_ok = true;                         // the lane's scores have a page
@@ -424,8 +445,9 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
             }
             full = full && __all(ok == (1u << NB) - 1);
             s_ok = (ok >> w_block) & 1;
-            const int next = key + UNIT;
-            if (next < key_end) load_pages(next);
+            const bool last = key + UNIT >= key_end, ahead = !last || then_keys;
+            const int next = last ? then.key_begin : key + UNIT;
+            if (ahead) load_pages(last ? then.row : cur.row, next);
             u4 vd[Q8 ? NB : 1][Q8 ? (NVW + 1) / 2 : 1];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -481,7 +503,7 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (next < key_end) load_k(next);
+            if (ahead) load_k(last ? then.part : cur.part, next);
             __builtin_amdgcn_sched_barrier(0);
             // ---- softmax: the lane's keys are key + s_oct + w_half + (0 .. 4 KT - 1)
             const int s_key = key + s_oct + w_half;
@@ -614,7 +636,7 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                         const int kb = key + KV_BLOCK * b;
                         const int first = p.window > 0 ? su.r.len - su.r.n - p.window + 1 : 0;
                         if (!((kb + KV_BLOCK > core_to && kb < key_end) || (kb < all_from && kb + KV_BLOCK > first))) continue;
-                        const int at = kb + 8 * lg, pg = page_at(at);
+                        const int at = kb + 8 * lg, pg = page_at(cur.row, at);
                         const uint8_t * a = vbase + (uint64_t)(has_page(pg) ? pg : 0) * p.v_stride + (at & page_mask) * EL;
                         u4 vz[NVW];
 #pragma unroll
@@ -685,6 +707,8 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 }
             }
         }
+        if (!more) return;
+        cur = then;
     }
 }
 

@@ -10,80 +10,91 @@ namespace dev {
 
 // ---------------------------------------------------------------- join
 //
-// One workgroup a query row whose item several workgroups of k_kv_attn shared:
-// with M the largest maximum, out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i
-// over the parts in order of their keys.  Wave w takes parts w, w + 8, ..., so
-// that as many loads are in flight; the waves' sums are added in order.
-constexpr int JOIN_WAVES = 8;
-
-template <int V>
-__global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv_join(const KvAttn p, int head_dim, int tile_rows, float p_shift) {
-    __shared__ float s_w[1024];
-    __shared__ float s_red[JOIN_WAVES];
-    __shared__ float s_acc[JOIN_WAVES][64 * V];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n_head = p.n_kv * p.group;
-    const int seq = blockIdx.x, tok = blockIdx.y / n_head, hq = blockIdx.y - tok * n_head;
-    const int head = hq / p.group;
+// The parts of an item that several workgroups of k_kv_attn shared: with M the
+// largest maximum, out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i.  A
+// workgroup takes 1024 / PG values of an item's tile, four a thread; its PG
+// groups of threads take every PG-th part, each under a running maximum of its
+// own, and are added in their order.  A part is read once, its maximum and sum
+// with its values, so that the loads of several parts are in flight.
+template <int PG>
+__global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, int tile_rows, int tiles, float p_shift) {
+    constexpr int TPG = 256 / PG;
+    __shared__ f4v s_acc[PG][TPG];
+    __shared__ float s_m[PG][TPG], s_l[PG][TPG];
+    const int tid = threadIdx.x, g = tid / TPG, e = tid - g * TPG;
+    const int seq = blockIdx.x / (p.n_kv * tiles), rest = blockIdx.x - seq * p.n_kv * tiles;
+    const int total = p.base[p.b.n_seq], base = p.base[seq];
     const SeqUnits su = seq_units(p.b, seq, p.page_shift, p.window, p.unit, p.group, tile_rows);
-    if (tok >= su.r.n) return;
-    const int rr = tok * p.group + hq - head * p.group, tile = rr / tile_rows, r = rr - tile * tile_rows;
-    const int total = p.base[p.b.n_seq], first = p.base[seq] + (head * su.tiles + tile) * su.units;
+    const int head = rest / tiles, tile = rest - head * tiles;
+    const int n_rows = min(su.r.n * p.group - tile * tile_rows, tile_rows);
+    const int at = (blockIdx.y * TPG + e) * 4, r = at / head_dim, d = at - r * head_dim;
+    if ((int)(blockIdx.y * TPG * 4) >= n_rows * head_dim) return;      // also: no such item
+    const int first = base + (head * su.tiles + tile) * su.units;
     const int64_t n_runs = min(p.grid, total);
     const int w0 = (int)(((int64_t)(first + 1) * n_runs - 1) / total);
     const int w1 = (int)(((int64_t)(first + su.units) * n_runs - 1) / total);
-    if (w0 == w1) return;                                   // written by k_kv_attn
-    const int n = w1 - w0 + 1;                              // <= grid <= 1024
-    auto slot = [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0)) * tile_rows + r; };
-    float top = -__builtin_inff();
-    for (int i = tid; i < n; i += 64 * JOIN_WAVES) {
-        const float m = p.ml[slot(i) * 2];
-        s_w[i] = m;
-        top = fmaxf(top, m);
-    }
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if (lane == 0) s_red[wave] = top;
-    __syncthreads();
-    for (int w = 0; w < JOIN_WAVES; ++w) top = fmaxf(top, s_red[w]);
-    const float ref = top == -__builtin_inff() ? 0.0f : top;
-    __syncthreads();
-    float sum = 0.0f;
-    for (int i = tid; i < n; i += 64 * JOIN_WAVES) {
-        const float f = __builtin_amdgcn_exp2f(s_w[i] - ref);
-        s_w[i] = f;
-        sum += f * p.ml[slot(i) * 2 + 1];
-    }
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) s_red[wave] = sum;
-    __syncthreads();
-    sum = 0.0f;
-    for (int w = 0; w < JOIN_WAVES; ++w) sum += s_red[w];
-    float a[V];
+    if (w0 == w1) return;                                              // written by k_kv_attn
+    const bool live = r < n_rows;
+    f4v a = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -__builtin_inff(), l = 0.0f;
+    constexpr int UN = 8;
+    for (int i0 = g; i0 <= w1 - w0; i0 += PG * UN) {
+        f4v x[UN];
+        float xm[UN], xl[UN];
 #pragma unroll
-    for (int j = 0; j < V; ++j) a[j] = 0.0f;
-#pragma unroll 4
-    for (int i = wave; i < n; i += JOIN_WAVES) {
-        const float * src = p.acc + slot(i) * head_dim;
-        const float f = s_w[i];
+        for (int j = 0; j < UN; ++j) {
+            const int i = i0 + PG * j;
+            x[j] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            xm[j] = -__builtin_inff();
+            xl[j] = 0.0f;
+            if (live && i <= w1 - w0) {
+                const int64_t row = (int64_t)(2 * (w0 + i) + (i == 0)) * tile_rows + r;
+                x[j] = *(const f4v *)(p.acc + row * head_dim + d);
+                xm[j] = p.ml[2 * row];
+                xl[j] = p.ml[2 * row + 1];
+            }
+        }
+        float top = m;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (lane + 64 * j < head_dim) a[j] += f * src[lane + 64 * j];
+        for (int j = 0; j < UN; ++j) top = fmaxf(top, xm[j]);
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        a *= f;
+        l *= f;
+        m = top;
+#pragma unroll
+        for (int j = 0; j < UN; ++j) {
+            const float w = __builtin_amdgcn_exp2f(xm[j] - ref);
+            a += w * x[j];
+            l += w * xl[j];
+        }
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) s_acc[wave][lane + 64 * j] = a[j];
-    __syncthreads();
+    if (PG > 1) {
+        s_acc[g][e] = a;
+        s_m[g][e] = m;
+        s_l[g][e] = l;
+        __syncthreads();
+        if (g > 0) return;
+        float top = m;
+        for (int i = 1; i < PG; ++i) top = fmaxf(top, s_m[i][e]);
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        a *= f;
+        l *= f;
+        m = top;
+        for (int i = 1; i < PG; ++i) {
+            const float w = __builtin_amdgcn_exp2f(s_m[i][e] - ref);
+            a += w * s_acc[i][e];
+            l += w * s_l[i][e];
+        }
+    }
+    if (!live) return;
+    const int rr = tile * tile_rows + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
     const int64_t row = su.r.row0 + tok;
-    for (int d = tid; d < head_dim; d += 64 * JOIN_WAVES) {
-        float o = 0.0f;
-        for (int w = 0; w < JOIN_WAVES; ++w) o += s_acc[w][d];
-        o = sum == 0.0f ? 0.0f : o / sum;
-        const int64_t at = row * p.out_stride + (int64_t)hq * head_dim + d;
-        if (p.type == T_F32) ((float *)p.out)[at] = o;
-        else if (p.type == T_F16) ((_Float16 *)p.out)[at] = (_Float16)o;
-        else ((__bf16 *)p.out)[at] = (__bf16)o;
-    }
-    if (p.lse && tid == 0)
-        p.lse[row * n_head + hq] = sum == 0.0f ? -__builtin_inff() : (top + (__builtin_amdgcn_logf(sum) - p_shift)) * KV_LN2;
+    const float inv = 1.0f / l;
+    store4(p.out, p.type, row * p.out_stride + (int64_t)hq * head_dim + d, l == 0.0f ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : a * inv);
+    if (p.lse && d == 0)
+        p.lse[row * (p.n_kv * p.group) + hq] = l == 0.0f ? -__builtin_inff() : (m + (__builtin_amdgcn_logf(l) - p_shift)) * KV_LN2;
 }
 
 // -------------------------------------------------------------- append
@@ -572,7 +583,6 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
         return refuse_as(who, "q and out must be 16-byte aligned, rows too");
     if (sq.n_tokens > 1 && (q->q_stride < width || q->out_stride < width)) return refuse_as(who, "rows shorter than n_head * head_dim");
     if (!workspace || !aligned16(workspace) || ws_bytes < a.bytes()) return refuse_as(who, "workspace too small or not 16-byte aligned");
-    if ((int64_t)sq.max_new * q->n_head > 65535) return refuse_as(who, "more than 65535 query rows a sequence");
     KvAttn p{};
     p.b = sq;
     p.k = (const uint8_t *)c->k;
@@ -602,12 +612,17 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     else if (c->type == T_BF16) KV_TRY(launch_kv_attn_bf16(p, c->head_dim, a.nt, a.grid, s));
     else KV_TRY(launch_kv_attn_q8(p, c->head_dim, a.nt, a.grid, s));
     if ((int64_t)b->max_pages * c->page_size <= p.unit) return 0;      // every item is one unit
-    const dim3 grid(sq.n_seq, sq.max_new * q->n_head), wg(64 * JOIN_WAVES);
+    // parts of an item, as many as the bounds suggest; workgroups by an item's rows
+    const int rows = q->n_head / c->n_kv * sq.max_new, tiles = (rows + a.rows - 1) / a.rows;
+    const int64_t items = (int64_t)sq.n_seq * c->n_kv * tiles;
+    const int parts = (int)(a.grid / items);
+    const int pg = parts < 4 ? 1 : parts < 16 ? 4 : 16;
+    const int per = 1024 / pg;
+    const dim3 grid((unsigned)items, (std::min(rows, a.rows) * c->head_dim + per - 1) / per), wg(256);
     const float shift = c->type == T_F16 ? 15.0f : 0.0f;
-    if (c->head_dim <= 64) hipLaunchKernelGGL(k_kv_join<1>, grid, wg, 0, s, p, c->head_dim, a.rows, shift);
-    else if (c->head_dim <= 128) hipLaunchKernelGGL(k_kv_join<2>, grid, wg, 0, s, p, c->head_dim, a.rows, shift);
-    else if (c->head_dim <= 256) hipLaunchKernelGGL(k_kv_join<4>, grid, wg, 0, s, p, c->head_dim, a.rows, shift);
-    else hipLaunchKernelGGL(k_kv_join<8>, grid, wg, 0, s, p, c->head_dim, a.rows, shift);
+    if (pg == 1) hipLaunchKernelGGL(k_kv_join<1>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
+    else if (pg == 4) hipLaunchKernelGGL(k_kv_join<4>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
+    else hipLaunchKernelGGL(k_kv_join<16>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
     KV_TRY(hipGetLastError());
     return 0;
 }
