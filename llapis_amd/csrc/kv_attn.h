@@ -23,12 +23,15 @@
 // V is loaded ahead of the unit's first product, the next unit's K behind it.
 //
 // Rounding.  Scores, maxima and sums are fp32.  The products take 16-bit
-// operands: the cache's values are exact in them (q8_0 values are exact in
-// bf16, their scales multiply in fp32), q and p are split into parts whose sum
-// is the fp32 value to 2^-22 (two fp16 parts) or 2^-24 (three bf16 parts); for
-// 16-bit queries two bf16 parts (2^-17) are enough, as out is rounded to 2^-9
-// or 2^-12.  fp16 parts keep their exponent range by powers of two: q's row is
-// scaled to a maximum in [2^13, 2^14), p by 2^15.
+// operands: the cache's values are exact in them; q and p are split into parts
+// whose sum is the fp32 value to 2^-22 (two fp16 parts) or 2^-24 (three bf16
+// parts).  16-bit queries are exact in one fp16 or two bf16 parts, and their p in
+// two bf16 parts (2^-17) is far below out's rounding.  fp16 parts keep their
+// exponent range by powers of two: q's row is scaled to a maximum in [2^13,
+// 2^14), p by 2^15.  q8_0: K's int8 values are exact in fp16 and its scales
+// multiply the fp32 sums of their 32 values; V's values are int8 times scale in
+// two fp16 parts, which is exact (18 bits), or for bf16 results in the first
+// part alone (2^-12, an eighth of out's rounding).
 #pragma once
 
 #include <type_traits>
@@ -82,17 +85,30 @@ __device__ __forceinline__ void split8(const float (&x)[8], u4 (&out)[PARTS]) {
     }
 }
 
-// eight int8 values as bf16 (exact: at most 8 significant bits)
-__device__ __forceinline__ u4 i8_to_bf16(u2 q) {
+// eight int8 values as fp16: 1024 + (q + 128) by its bits, less 1152
+__device__ __forceinline__ u4 i8_to_half(u2 q) {
     u4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int w = (int)(q[i >> 1] >> ((i & 1) * 16));
-        const uint32_t a = __builtin_bit_cast(uint32_t, (float)(int8_t)w);
-        const uint32_t b = __builtin_bit_cast(uint32_t, (float)(int8_t)(w >> 8));
-        r[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t w = q[i] ^ 0x80808080u;
+        const h2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+        const h2v a = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + off;
+        const h2v b = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + off;
+        r[2 * i] = __builtin_bit_cast(uint32_t, a);
+        r[2 * i + 1] = __builtin_bit_cast(uint32_t, b);
     }
     return r;
+}
+
+// int8 values (as fp16) times their scales: the product's rounding and what it leaves
+__device__ __forceinline__ void times_scale(u4 q, u4 d, u4 & hi, u4 & lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const h2v a = __builtin_bit_cast(h2v, (uint32_t)q[i]), b = __builtin_bit_cast(h2v, (uint32_t)d[i]);
+        const h2v p = a * b;
+        hi[i] = __builtin_bit_cast(uint32_t, p);
+        lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(a, b, -p));
+    }
 }
 
 // the value of lane l ^ 16 / l ^ 32 combined with this lane's
@@ -191,24 +207,26 @@ __device__ __forceinline__ uint32_t pair_mask(uint32_t bits, int i) {
 
 constexpr float KV_LN2 = 0.69314718055994530942f, KV_LOG2E = 1.44269504088896340736f;
 
-template <int CT, bool F32IO, int HD, int NT>
+// WIDE: fp32 results (q8_0: fp32 and fp16 ones)
+template <int CT, bool WIDE, int HD, int NT>
 struct KvShape {
-    static constexpr bool HALF = CT == KV_F16;
-    static constexpr int PQ = HALF ? (F32IO ? 2 : 1) : (F32IO ? 3 : 2);
-    static constexpr int PP = HALF ? 2 : (F32IO ? 3 : 2);
+    static constexpr bool HALF = CT != KV_BF16;
+    static constexpr int PQ = HALF ? (WIDE ? 2 : 1) : (WIDE ? 3 : 2);
+    static constexpr int PP = HALF ? 2 : (WIDE ? 3 : 2);
     static constexpr int UNIT = kv_unit(HD), KT = UNIT / (16 * KV_WAVES), NB = UNIT / KV_BLOCK;
     static constexpr int NC = HD / 32, NV = HD / 16, NVW = (NV + KV_WAVES - 1) / KV_WAVES;
     static constexpr int Q_BYTES = PQ * NT * NC * 1024;
-    static constexpr int P_BYTES = NB * NT * (CT == KV_Q8 ? 2 : PP) * 1024;     // q8_0: fp32, its scales come first
+    static constexpr int P_BYTES = NB * NT * PP * 1024;
     static constexpr int LDS = Q_BYTES + P_BYTES;
 };
 
-template <int CT, bool F32IO, int HD, int NT>
+template <int CT, bool WIDE, int HD, int NT>
 __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(const KvAttn p) {
-    using Sh = KvShape<CT, F32IO, HD, NT>;
+    using Sh = KvShape<CT, WIDE, HD, NT>;
     constexpr bool HALF = Sh::HALF, Q8 = CT == KV_Q8;
     constexpr int PQ = Sh::PQ, PP = Sh::PP, NC = Sh::NC, NV = Sh::NV, NVW = Sh::NVW, KT = Sh::KT, NB = Sh::NB;
     constexpr int UNIT = Sh::UNIT, ROWS = 16 * NT;
+    constexpr int V_TOP = HD > 256 ? NB / 2 : NB;                 // blocks of V loaded ahead of a unit's first product
     constexpr int EL = Q8 ? 1 : 2;                                // bytes of a cached value
     constexpr float P_SHIFT = HALF ? 15.0f : 0.0f;                // log2 of p's scale
     extern __shared__ __align__(16) uint8_t lds[];
@@ -370,7 +388,7 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 const int o = (tid & 15) + 16 * e;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) qx[e][j] = 0.0f;
-                if (r < n_rows && o < HD / 8) load8(p.q, F32IO ? (int)T_F32 : p.type, from + 8 * o, qx[e]);
+                if (r < n_rows && o < HD / 8) load8(p.q, WIDE && !Q8 ? (int)T_F32 : p.type, from + 8 * o, qx[e]);
                 if (HALF)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[e][j]));
@@ -448,14 +466,14 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
             const bool last = key + UNIT >= key_end, ahead = !last || then_keys;
             const int next = last ? then.key_begin : key + UNIT;
             if (ahead) load_pages(last ? then.row : cur.row, next);
+            // the scales of a tile's 32 columns; two tiles share them where v_tile is even
             u4 vd[Q8 ? NB : 1][Q8 ? (NVW + 1) / 2 : 1];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
+            auto load_v = [&](int b) {
                 const int slot = (key + KV_BLOCK * b + 8 * lg) & page_mask;
 #pragma unroll
                 for (int t = 0; t < NVW; ++t) {
-                    const int tile = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
-                    vf[b][t] = *(const frag *)(va[b] + ((16 * tile + lv) * page + slot) * EL);
+                    const int vt = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
+                    vf[b][t] = *(const frag *)(va[b] + ((16 * vt + lv) * page + slot) * EL);
                 }
                 if constexpr (Q8)
 #pragma unroll
@@ -463,7 +481,9 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                         const int c = min((v_tile >> 1) + i, NC - 1);
                         vd[b][i] = *(const u4 *)(va[b] + page * HD + (c * page + slot) * 2);
                     }
-            }
+            };
+#pragma unroll
+            for (int b = 0; b < V_TOP; ++b) load_v(b);
             // ---- S^T of the wave's keys
             __builtin_amdgcn_sched_barrier(0);
             f4v sc[NT][KT];
@@ -476,8 +496,13 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 u4 a[KT];
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
-                    if constexpr (Q8) a[t] = i8_to_bf16(kf[t][c]);
-                    else a[t] = kf[t][c];
+                    if constexpr (Q8) {
+                        // no part of the conversion moves up to the load, to wait for it there
+                        asm volatile("" : "+v"(kf[t][c]));
+                        a[t] = i8_to_half(kf[t][c]);
+                    } else {
+                        a[t] = kf[t][c];
+                    }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     f4v part[KT];
@@ -503,7 +528,12 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (ahead) load_k(last ? then.part : cur.part, next);
+            if constexpr (V_TOP < NB) {
+#pragma unroll
+                for (int b = V_TOP; b < NB; ++b) load_v(b);
+            } else if (ahead) {
+                load_k(last ? then.part : cur.part, next);
+            }
             __builtin_amdgcn_sched_barrier(0);
             // ---- softmax: the lane's keys are key + s_oct + w_half + (0 .. 4 KT - 1)
             const int s_key = key + s_oct + w_half;
@@ -555,71 +585,54 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                     x[i] = __builtin_amdgcn_exp2f(sc[nt][i >> 2][i & 3] - (ref - P_SHIFT));
                     l[nt] += x[i];
                 }
-                if constexpr (Q8) {
-                    uint8_t * w = lds_p + (w_block * NT + nt) * 2048 + lane * 32 + 4 * w_half;
 #pragma unroll
-                    for (int t = 0; t < KT; ++t) *(f4v *)(w + 16 * t) = f4v{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
-                } else {
+                for (int i = 4 * KT; i < 8; ++i) x[i] = 0.0f;
+                u4 part[PP];
+                split8<HALF, PP>(x, part);
 #pragma unroll
-                    for (int i = 4 * KT; i < 8; ++i) x[i] = 0.0f;
-                    u4 part[PP];
-                    split8<HALF, PP>(x, part);
-#pragma unroll
-                    for (int q = 0; q < PP; ++q) {
-                        uint8_t * w = lds_p + ((w_block * NT + nt) * PP + q) * 1024 + lane * 16;
-                        if constexpr (KT == 2) *(u4 *)w = part[q];
-                        else *(u2 *)(w + 2 * w_half) = u2{part[q][0], part[q][1]};
-                    }
+                for (int q = 0; q < PP; ++q) {
+                    uint8_t * w = lds_p + ((w_block * NT + nt) * PP + q) * 1024 + lane * 16;
+                    if constexpr (KT == 2) *(u4 *)w = part[q];
+                    else *(u2 *)(w + 2 * w_half) = u2{part[q][0], part[q][1]};
                 }
             }
             __syncthreads();
             // ---- O^T of the wave's columns
-            if constexpr (Q8) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const f4v * x = (const f4v *)(lds_p + (b * NT + nt) * 2048 + lane * 32);
-                        const f4v x0 = x[0], x1 = x[1];
-                        u4 bp[PP];
-#pragma unroll
-                        for (int t = 0; t < NVW; ++t) {
-                            // the scales of the tile's 32 columns; two tiles share them where v_tile is even
-                            if (NVW % 2 || t % 2 == 0) {
-                                const u4 w = NVW % 2 ? (((v_tile + t) >> 1) - (v_tile >> 1) ? vd[b][(t + 1) / 2] : vd[b][t / 2]) : vd[b][t / 2];
-                                const h8v d = __builtin_bit_cast(h8v, w);
-                                float y[8];
-                                // a masked key's p is 0 whatever its scale holds
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const float xi = i < 4 ? x0[i & 3] : x1[i & 3];
-                                    y[i] = xi != 0.0f ? xi * (float)d[i] : 0.0f;
-                                }
-                                split8<HALF, PP>(y, bp);
-                            }
-                            const u4 a = i8_to_bf16(vf[b][t]);
-#pragma unroll
-                            for (int q = 0; q < PP; ++q) acc[nt][t] = mfma16<HALF>(a, bp[q], acc[nt][t]);
-                        }
-                    }
-            } else {
-                // 0 times a masked infinity is no zero: V's values of keys that a row
-                // does not see become 0
-                const int core_to = min(all_to, key_end);
+            // 0 times a masked infinity is no zero: what is not seen by every row
+            // becomes 0 in V, for q8_0 in its scales
+            const int core_to = min(all_to, key_end);
+            auto add_block = [&](int b) {
                 if (!full) {
+                    const uint32_t bits = (ok >> b) & 1 ? seen8(key + KV_BLOCK * b + 8 * lg, all_from, core_to) : 0;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const uint32_t bits = (ok >> b) & 1 ? seen8(key + KV_BLOCK * b + 8 * lg, all_from, core_to) : 0;
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t keep = pair_mask(bits, 2 * i);
+                        if constexpr (Q8) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t keep = pair_mask(bits, 2 * i);
+                            for (int c = 0; c < (NVW + 1) / 2; ++c) vd[b][c][i] &= keep;
+                        } else {
 #pragma unroll
                             for (int t = 0; t < NVW; ++t) vf[b][t][i] &= keep;
                         }
                     }
                 }
+                if constexpr (Q8) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+                    for (int t = 0; t < NVW; ++t) {
+                        asm volatile("" : "+v"(vf[b][t]));        // not converted where it is loaded
+                        const u4 d = NVW % 2 == 0 || !(v_tile & 1) ? vd[b][t / 2] : vd[b][(t + 1) / 2 < (NVW + 1) / 2 ? (t + 1) / 2 : t / 2];
+                        u4 hi, lo;
+                        times_scale(i8_to_half(vf[b][t]), d, hi, lo);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int q = 0; q < PP; ++q) {
+                                const u4 bp = *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16);
+                                acc[nt][t] = mfma16<HALF>(hi, bp, acc[nt][t]);
+                                if (WIDE && q == 0) acc[nt][t] = mfma16<HALF>(lo, bp, acc[nt][t]);
+                            }
+                    }
+                } else {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -628,42 +641,60 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
 #pragma unroll
                             for (int t = 0; t < NVW; ++t) acc[nt][t] = mfma16<HALF>(vf[b][t], bp, acc[nt][t]);
                         }
-                // ... and keys that only some of a sequence's tokens see (at its
-                // end, at the window's begin) are added token by token
-                if (!full && su.r.n > 1) {
+                }
+            };
+#pragma unroll
+            for (int b = 0; b < V_TOP; ++b) add_block(b);
+            if constexpr (V_TOP < NB) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (ahead) load_k(last ? then.part : cur.part, next);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int b = V_TOP; b < NB; ++b) add_block(b);
+            }
+            // keys that only some of a sequence's tokens see (at its end, at the
+            // window's begin) are added token by token
+            if (!full && su.r.n > 1) {
 #pragma unroll 1
-                    for (int b = 0; b < NB; ++b) {
-                        const int kb = key + KV_BLOCK * b;
-                        const int first = p.window > 0 ? su.r.len - su.r.n - p.window + 1 : 0;
-                        if (!((kb + KV_BLOCK > core_to && kb < key_end) || (kb < all_from && kb + KV_BLOCK > first))) continue;
-                        const int at = kb + 8 * lg, pg = page_at(cur.row, at);
-                        const uint8_t * a = vbase + (uint64_t)(has_page(pg) ? pg : 0) * p.v_stride + (at & page_mask) * EL;
-                        u4 vz[NVW];
+                for (int b = 0; b < NB; ++b) {
+                    const int kb = key + KV_BLOCK * b;
+                    const int first = p.window > 0 ? su.r.len - su.r.n - p.window + 1 : 0;
+                    if (!((kb + KV_BLOCK > core_to && kb < key_end) || (kb < all_from && kb + KV_BLOCK > first))) continue;
+                    const int at = kb + 8 * lg, pg = page_at(cur.row, at), slot = at & page_mask;
+                    const uint8_t * a = vbase + (uint64_t)(has_page(pg) ? pg : 0) * p.v_stride;
+                    frag vz[NVW];
+                    u4 dz[Q8 ? NVW : 1];
+#pragma unroll
+                    for (int t = 0; t < NVW; ++t) {
+                        const int vt = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
+                        vz[t] = *(const frag *)(a + ((16 * vt + lv) * page + slot) * EL);
+                        if constexpr (Q8) dz[t] = *(const u4 *)(a + page * HD + ((vt >> 1) * page + slot) * 2);
+                    }
+#pragma unroll 1
+                    for (int tok = 0; tok < su.r.n; ++tok) {
+                        asm volatile("" ::: "memory");        // P stays in LDS
+                        const int pos = su.r.len - su.r.n + tok;
+                        uint32_t bits = seen8(at, p.window > 0 ? pos - p.window + 1 : 0, min(pos + 1, key_end));
+                        bits = has_page(pg) ? bits & ~seen8(at, all_from, core_to) : 0;
+                        u4 keep;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) keep[i] = pair_mask(bits, 2 * i);
 #pragma unroll
                         for (int t = 0; t < NVW; ++t) {
-                            const int tile = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
-                            vz[t] = *(const u4 *)(a + (16 * tile + lv) * page * EL);
-                        }
-#pragma unroll 1
-                        for (int tok = 0; tok < su.r.n; ++tok) {
-                            asm volatile("" ::: "memory");    // P stays in LDS
-                            const int pos = su.r.len - su.r.n + tok;
-                            uint32_t bits = seen8(at, p.window > 0 ? pos - p.window + 1 : 0, min(pos + 1, key_end));
-                            bits = has_page(pg) ? bits & ~seen8(at, all_from, core_to) : 0;
+                            u4 hi, lo;
+                            if constexpr (Q8) times_scale(i8_to_half(vz[t]), dz[t] & keep, hi, lo);
+                            else hi = vz[t] & keep;
 #pragma unroll
-                            for (int t = 0; t < NVW; ++t) {
-                                u4 v;
+                            for (int nt = 0; nt < NT; ++nt) {
+                                f4v d = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) v[i] = vz[t][i] & pair_mask(bits, 2 * i);
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    f4v d = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                                    for (int q = 0; q < PP; ++q)
-                                        d = mfma16<HALF>(v, *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16), d);
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) acc[nt][t][i] += tok_of[nt] == tok ? d[i] : 0.0f;
+                                for (int q = 0; q < PP; ++q) {
+                                    const u4 bp = *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16);
+                                    d = mfma16<HALF>(hi, bp, d);
+                                    if (Q8 && WIDE && q == 0) d = mfma16<HALF>(lo, bp, d);
                                 }
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) acc[nt][t][i] += tok_of[nt] == tok ? d[i] : 0.0f;
                             }
                         }
                     }
@@ -691,7 +722,7 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
 #pragma unroll
                 for (int t = 0; t < NVW; ++t)
                     if (v_tile + t < NV)
-                        store4(p.out, F32IO ? (int)T_F32 : p.type,
+                        store4(p.out, WIDE && !Q8 ? (int)T_F32 : p.type,
                                out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
                 if (p.lse && wave == 0 && lg == 0)
                     p.lse[out_row * (p.group * p.n_kv) + hq] =
@@ -712,29 +743,29 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
     }
 }
 
-template <int CT, bool F32IO, int HD, int NT>
+template <int CT, bool WIDE, int HD, int NT>
 hipError_t launch_kv_attn_one(const KvAttn & p, int grid, hipStream_t s) {
-    constexpr int lds = KvShape<CT, F32IO, HD, NT>::LDS;
-    hipLaunchKernelGGL((k_kv_attn<CT, F32IO, HD, NT>), dim3(grid), dim3(256), lds, s, p);
+    constexpr int lds = KvShape<CT, WIDE, HD, NT>::LDS;
+    hipLaunchKernelGGL((k_kv_attn<CT, WIDE, HD, NT>), dim3(grid), dim3(256), lds, s, p);
     return hipGetLastError();
 }
 
-template <int CT, bool F32IO, int NT>
+template <int CT, bool WIDE, int NT>
 hipError_t launch_kv_attn_hd(const KvAttn & p, int head_dim, int grid, hipStream_t s) {
     switch (head_dim) {
-        case 64: return launch_kv_attn_one<CT, F32IO, 64, NT>(p, grid, s);
-        case 96: return launch_kv_attn_one<CT, F32IO, 96, NT>(p, grid, s);
-        case 128: return launch_kv_attn_one<CT, F32IO, 128, NT>(p, grid, s);
-        case 192: return launch_kv_attn_one<CT, F32IO, 192, NT>(p, grid, s);
-        case 256: return launch_kv_attn_one<CT, F32IO, 256, NT>(p, grid, s);
-        case 512: return launch_kv_attn_one<CT, F32IO, 512, NT>(p, grid, s);
+        case 64: return launch_kv_attn_one<CT, WIDE, 64, NT>(p, grid, s);
+        case 96: return launch_kv_attn_one<CT, WIDE, 96, NT>(p, grid, s);
+        case 128: return launch_kv_attn_one<CT, WIDE, 128, NT>(p, grid, s);
+        case 192: return launch_kv_attn_one<CT, WIDE, 192, NT>(p, grid, s);
+        case 256: return launch_kv_attn_one<CT, WIDE, 256, NT>(p, grid, s);
+        case 512: return launch_kv_attn_one<CT, WIDE, 512, NT>(p, grid, s);
     }
     return hipErrorInvalidValue;
 }
 
 template <int CT>
 hipError_t launch_kv_attn_type(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s) {
-    if (p.type == T_F32)
+    if (p.type == T_F32 || (CT == KV_Q8 && p.type == T_F16))
         return nt == 1 ? launch_kv_attn_hd<CT, true, 1>(p, head_dim, grid, s) : launch_kv_attn_hd<CT, true, 2>(p, head_dim, grid, s);
     return nt == 1 ? launch_kv_attn_hd<CT, false, 1>(p, head_dim, grid, s) : launch_kv_attn_hd<CT, false, 2>(p, head_dim, grid, s);
 }

@@ -619,7 +619,7 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     const int pg = parts < 4 ? 1 : parts < 16 ? 4 : 16;
     const int per = 1024 / pg;
     const dim3 grid((unsigned)items, (std::min(rows, a.rows) * c->head_dim + per - 1) / per), wg(256);
-    const float shift = c->type == T_F16 ? 15.0f : 0.0f;
+    const float shift = c->type == T_BF16 ? 0.0f : 15.0f;
     if (pg == 1) hipLaunchKernelGGL(k_kv_join<1>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
     else if (pg == 4) hipLaunchKernelGGL(k_kv_join<4>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
     else hipLaunchKernelGGL(k_kv_join<16>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
