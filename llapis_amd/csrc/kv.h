@@ -52,11 +52,11 @@ struct KvAttn {
 // tiles of 16 query rows a workgroup holds at once: 1 or 2
 inline int kv_tiles(int rows) { return rows <= 16 ? 1 : 2; }
 // workgroups of the kernel that a CU's registers and LDS hold
-constexpr int kv_wgs(bool q8, int head_dim, int nt) {
-    return head_dim > 256 ? (nt == 1 ? 2 : 1) : q8 || nt == 2 ? 2 : head_dim == 64 ? 4 : 3;
+constexpr int kv_wgs(int head_dim, int nt) {
+    return head_dim > 256 ? (nt == 1 ? 2 : 1) : nt == 2 ? 2 : head_dim == 64 ? 4 : 3;
 }
 // workgroups that share the work out
-inline int kv_grid(int type, int head_dim, int nt) { return 256 * kv_wgs(type == LLAPIS_T_Q8_0, head_dim, nt); }
+inline int kv_grid(int head_dim, int nt) { return 256 * kv_wgs(head_dim, nt); }
 
 // llapis_last_error() gets the message; returns -1
 int32_t refuse(const char * msg) noexcept;

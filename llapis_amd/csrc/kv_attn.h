@@ -28,10 +28,14 @@
 // parts).  16-bit queries are exact in one fp16 or two bf16 parts, and their p in
 // two bf16 parts (2^-17) is far below out's rounding.  fp16 parts keep their
 // exponent range by powers of two: q's row is scaled to a maximum in [2^13,
-// 2^14), p by 2^15.  q8_0: K's int8 values are exact in fp16 and its scales
-// multiply the fp32 sums of their 32 values; V's values are int8 times scale in
-// two fp16 parts, which is exact (18 bits), or for bf16 results in the first
-// part alone (2^-12, an eighth of out's rounding).
+// 2^14), p by 2^15.  q8_0: an
+// int8 value times its scale is exact in two fp16 parts (18 bits; magnitudes
+// above 65504 become infinite, as an F16 cache's would), of which V's second is
+// left out for bf16 results (2^-12, an eighth of out's rounding).
+//
+// q8_0's loads are 16 bytes a lane too: of a K row the lane's 16 values go to two
+// products, and of a V column 16 keys, so that the products' order of values and
+// of keys is another (Q and P are laid out to it).
 #pragma once
 
 #include <type_traits>
@@ -221,12 +225,12 @@ struct KvShape {
 };
 
 template <int CT, bool WIDE, int HD, int NT>
-__global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(const KvAttn p) {
+__global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p) {
     using Sh = KvShape<CT, WIDE, HD, NT>;
     constexpr bool HALF = Sh::HALF, Q8 = CT == KV_Q8;
     constexpr int PQ = Sh::PQ, PP = Sh::PP, NC = Sh::NC, NV = Sh::NV, NVW = Sh::NVW, KT = Sh::KT, NB = Sh::NB;
     constexpr int UNIT = Sh::UNIT, ROWS = 16 * NT;
-    constexpr int V_TOP = HD > 256 ? NB / 2 : NB;                 // blocks of V loaded ahead of a unit's first product
+    constexpr int V_TOP = Q8 ? UNIT / 64 : HD > 256 ? NB / 2 : NB;    // V's loads ahead of a unit's first product
     constexpr int EL = Q8 ? 1 : 2;                                // bytes of a cached value
     constexpr float P_SHIFT = HALF ? 15.0f : 0.0f;                // log2 of p's scale
     extern __shared__ __align__(16) uint8_t lds[];
@@ -325,35 +329,48 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
     // places of the wave's keys in a unit: those of its K rows, those of the lane's scores
     const int w_block = KT == 2 ? wave : wave >> 1, w_half = KT == 2 ? 0 : 4 * (wave & 1);
     const int k_oct = KV_BLOCK * w_block + 8 * (lm >> 2), s_oct = KV_BLOCK * w_block + 8 * lg;
-    typedef typename std::conditional<Q8, u2, u4>::type frag;
-    typedef typename std::conditional<KT == 2, u4, u2>::type scales;
-    frag kf[KT][NC], vf[NB][NVW];
-    scales kd[Q8 ? NC : 1];                           // fp16, of the keys whose scores the lane holds
-    int k_pg = 0, s_pg = 0, v_pg[NB];
+    constexpr int NP = Q8 ? NC / 2 : 0, ODD = Q8 ? NC % 2 : 0;    // q8_0: pairs of 32 values, a last one
+    constexpr int NKF = Q8 ? NP + ODD : NC;                       // K's loads of a row
+    constexpr int NVL = Q8 ? UNIT / 64 : NB;                      // V's loads of a column
+    constexpr int NVD = (NVW + 1) / 2;                            // 32-column blocks of a wave's V tiles
+    u4 kf[KT][NKF], vf[NVL][NVW];
+    uint32_t kd[KT][Q8 ? NKF : 1];                    // fp16 scales of the lane's K row
+    int k_pg = 0, s_pg = 0, v_pg[NVL];
     auto has_page = [&](int pg) { return (uint32_t)pg < (uint32_t)p.n_pages; };
     auto page_at = [&](const int32_t * row, int key) {
         const int i = key >> p.page_shift;
         const int pg = row[min(i, p.b.max_pages - 1)];
         return i < p.b.max_pages ? pg : -1;
     };
+    // places of a lane's V keys in a unit: 8 of each block, q8_0: 16 of each load, whose halves are blocks
+    auto v_place = [&](int b) { return Q8 ? 64 * (b >> 1) + 16 * lg + 8 * (b & 1) : KV_BLOCK * b + 8 * lg; };
     auto load_pages = [&](const int32_t * row, int at) {
         k_pg = page_at(row, at + k_oct);
         s_pg = Q8 ? page_at(row, at + s_oct) : 0;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) v_pg[b] = page_at(row, at + KV_BLOCK * b + 8 * lg);
+        for (int i = 0; i < NVL; ++i) v_pg[i] = page_at(row, at + v_place(Q8 ? 2 * i : i));
     };
     auto load_k = [&](uint64_t part, int at) {
-        const uint8_t * a = p.k + part + (uint64_t)(has_page(k_pg) ? k_pg : 0) * p.k_stride +
-                            (((at + k_oct + w_half + (lm & 3)) & page_mask) * HD + 8 * lg) * EL;
+        const uint8_t * pg = p.k + part + (uint64_t)(has_page(k_pg) ? k_pg : 0) * p.k_stride;
+        const int slot = (at + k_oct + w_half + (lm & 3)) & page_mask;
+        const uint8_t * a = pg + (slot * HD + (Q8 ? 16 : 8) * lg) * EL;
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int t = 0; t < KT; ++t) {
+            if constexpr (Q8) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) kf[t][c] = *(const frag *)(a + (4 * t * HD + 32 * c) * EL);
-        if constexpr (Q8) {
-            const uint8_t * d = p.k + part + (uint64_t)(has_page(s_pg) ? s_pg : 0) * p.k_stride + page * HD +
-                                ((at + s_oct + w_half) & page_mask) * 2;
+                for (int c = 0; c < NP; ++c) kf[t][c] = *(const u4 *)(a + 4 * t * HD + 64 * c);
+                if constexpr (ODD != 0) {
+                    const u2 w = *(const u2 *)(a - 8 * lg + 4 * t * HD + 64 * NP);
+                    kf[t][NP] = u4{w[0], w[1], 0, 0};
+                }
+                const uint16_t * d = (const uint16_t *)(pg + page * HD) + slot + 4 * t;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) kd[c] = *(const scales *)(d + c * page * 2);
+                for (int c = 0; c < NP; ++c) kd[t][c] = d[(2 * c + (lg >> 1)) * page];
+                if constexpr (ODD != 0) kd[t][NP] = d[2 * NP * page];
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) kf[t][c] = *(const u4 *)(a + (4 * t * HD + 32 * c) * EL);
+            }
         }
     };
     // the wave's columns of V, from 16 v_tile on (a tile past the last one reads it again)
@@ -377,7 +394,7 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
         // threads a row
         constexpr int QE = (HD / 8 + 15) / 16;
         __syncthreads();                                           // the last piece's LDS has been read
-#pragma unroll
+#pragma unroll 1
         for (int nt = 0; nt < NT; ++nt) {
             const int r = 16 * nt + (tid >> 4), rr = tile * ROWS + r, tok = rr / p.group;
             const int64_t from = (su.r.row0 + tok) * p.q_stride + (int64_t)(head * p.group + rr - tok * p.group) * HD;
@@ -410,9 +427,11 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                         for (int j = 0; j < 8; ++j) qx[e][j] = __builtin_ldexpf(qx[e][j], ex);
                     u4 part[PQ];
                     split8<HALF, PQ>(qx[e], part);
+                    // the product and lane group that eight values go to
+                    const int c = o < 8 * NP ? 2 * (o >> 3) + (o & 1) : o >> 2, g = o < 8 * NP ? (o >> 1) & 3 : o & 3;
 #pragma unroll
                     for (int q = 0; q < PQ; ++q)
-                        *(u4 *)(lds + ((q * NT + nt) * NC + (o >> 2)) * 1024 + ((o & 3) * 16 + (tid >> 4)) * 16) = part[q];
+                        *(u4 *)(lds + ((q * NT + nt) * NC + c) * 1024 + (g * 16 + (tid >> 4)) * 16) = part[q];
                 }
             }
         }
@@ -453,37 +472,37 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
         for (int key = cur.key_begin; key < key_end; key += UNIT) {
             asm volatile("" : "+v"(lv));              // V's offsets are formed anew, not held
             bool full = key + UNIT <= min(all_to, key_end) && key >= all_from;
-            bool s_ok = true;                         // the lane's scores have a page
-            uint32_t ok = 0;                          // bit b: the lane's octet of block b has a page
-            const uint8_t * va[NB];
+            uint32_t ok = 0;                          // bit i: the keys of the lane's load i have a page
+            const uint8_t * va[NVL];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                va[b] = vbase + (uint64_t)(has_page(v_pg[b]) ? v_pg[b] : 0) * p.v_stride;
-                ok |= (uint32_t)has_page(v_pg[b]) << b;
+            for (int i = 0; i < NVL; ++i) {
+                va[i] = vbase + (uint64_t)(has_page(v_pg[i]) ? v_pg[i] : 0) * p.v_stride;
+                ok |= (uint32_t)has_page(v_pg[i]) << i;
             }
-            full = full && __all(ok == (1u << NB) - 1);
-            s_ok = (ok >> w_block) & 1;
+            full = full && __all(ok == (1u << NVL) - 1);
+            const bool s_ok = Q8 ? has_page(s_pg) : (ok >> w_block) & 1;      // the lane's scores have a page
             const bool last = key + UNIT >= key_end, ahead = !last || then_keys;
             const int next = last ? then.key_begin : key + UNIT;
             if (ahead) load_pages(last ? then.row : cur.row, next);
-            // the scales of a tile's 32 columns; two tiles share them where v_tile is even
-            u4 vd[Q8 ? NB : 1][Q8 ? (NVW + 1) / 2 : 1];
-            auto load_v = [&](int b) {
-                const int slot = (key + KV_BLOCK * b + 8 * lg) & page_mask;
+            // the scales of a block's 32 columns, which two tiles share where v_tile is even
+            u4 vd[Q8 ? NB : 1][Q8 ? NVD : 1];
+            auto load_v = [&](int i) {
+                const int slot = (key + v_place(Q8 ? 2 * i : i)) & page_mask;
 #pragma unroll
                 for (int t = 0; t < NVW; ++t) {
                     const int vt = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
-                    vf[b][t] = *(const frag *)(va[b] + ((16 * vt + lv) * page + slot) * EL);
+                    vf[i][t] = *(const u4 *)(va[i] + ((16 * vt + lv) * page + slot) * EL);
                 }
                 if constexpr (Q8)
 #pragma unroll
-                    for (int i = 0; i < (NVW + 1) / 2; ++i) {
-                        const int c = min((v_tile >> 1) + i, NC - 1);
-                        vd[b][i] = *(const u4 *)(va[b] + page * HD + (c * page + slot) * 2);
+                    for (int c = 0; c < NVD; ++c) {
+                        const u4 * d = (const u4 *)(va[i] + page * HD + (min((v_tile >> 1) + c, NC - 1) * page + slot) * 2);
+                        vd[2 * i][c] = d[0];
+                        vd[2 * i + 1][c] = d[1];
                     }
             };
 #pragma unroll
-            for (int b = 0; b < V_TOP; ++b) load_v(b);
+            for (int i = 0; i < V_TOP; ++i) load_v(i);
             // ---- S^T of the wave's keys
             __builtin_amdgcn_sched_barrier(0);
             f4v sc[NT][KT];
@@ -493,44 +512,34 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 for (int t = 0; t < KT; ++t) sc[nt][t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                u4 a[KT];
+                u4 a[KT], a_lo[KT];
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
                     if constexpr (Q8) {
+                        const int f = c < 2 * NP ? c >> 1 : NP, h = c < 2 * NP ? c & 1 : 0;
                         // no part of the conversion moves up to the load, to wait for it there
-                        asm volatile("" : "+v"(kf[t][c]));
-                        a[t] = i8_to_half(kf[t][c]);
+                        if (h == 0) asm volatile("" : "+v"(kf[t][f]), "+v"(kd[t][f]));
+                        const uint32_t d = kd[t][f] | kd[t][f] << 16;
+                        times_scale(i8_to_half(u2{kf[t][f][2 * h], kf[t][f][2 * h + 1]}), u4{d, d, d, d}, a[t], a_lo[t]);
                     } else {
                         a[t] = kf[t][c];
                     }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    f4v part[KT];
-#pragma unroll
-                    for (int t = 0; t < KT; ++t) part[t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int q = 0; q < PQ; ++q) {
                         const u4 b = *(const u4 *)(lds + ((q * NT + nt) * NC + c) * 1024 + lane * 16);
 #pragma unroll
-                        for (int t = 0; t < KT; ++t)
-                            if constexpr (Q8) part[t] = mfma16<HALF>(a[t], b, part[t]);
-                            else sc[nt][t] = mfma16<HALF>(a[t], b, sc[nt][t]);
+                        for (int t = 0; t < KT; ++t) {
+                            sc[nt][t] = mfma16<HALF>(a[t], b, sc[nt][t]);
+                            if (Q8 && q == 0) sc[nt][t] = mfma16<HALF>(a_lo[t], b, sc[nt][t]);
+                        }
                     }
-                    if constexpr (Q8) {
-#pragma unroll
-                        for (int t = 0; t < KT; ++t)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const h2v d = __builtin_bit_cast(h2v, (uint32_t)kd[c][2 * t + (i >> 1)]);
-                                sc[nt][t][i] = __builtin_fmaf(part[t][i], (float)d[i & 1], sc[nt][t][i]);
-                            }
-                    }
-                }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (V_TOP < NB) {
+            if constexpr (V_TOP < NVL) {
 #pragma unroll
-                for (int b = V_TOP; b < NB; ++b) load_v(b);
+                for (int i = V_TOP; i < NVL; ++i) load_v(i);
             } else if (ahead) {
                 load_k(last ? then.part : cur.part, next);
             }
@@ -591,7 +600,9 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 split8<HALF, PP>(x, part);
 #pragma unroll
                 for (int q = 0; q < PP; ++q) {
-                    uint8_t * w = lds_p + ((w_block * NT + nt) * PP + q) * 1024 + lane * 16;
+                    const int b = Q8 ? 2 * (w_block >> 1) + (lg & 1) : w_block;
+                    const int l = Q8 ? (2 * (w_block & 1) + (lg >> 1)) * 16 + lm : lane;
+                    uint8_t * w = lds_p + ((b * NT + nt) * PP + q) * 1024 + l * 16;
                     if constexpr (KT == 2) *(u4 *)w = part[q];
                     else *(u2 *)(w + 2 * w_half) = u2{part[q][0], part[q][1]};
                 }
@@ -602,14 +613,15 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
             // becomes 0 in V, for q8_0 in its scales
             const int core_to = min(all_to, key_end);
             auto add_block = [&](int b) {
+                if (HD > 256) __builtin_amdgcn_sched_barrier(0);
                 if (!full) {
-                    const uint32_t bits = (ok >> b) & 1 ? seen8(key + KV_BLOCK * b + 8 * lg, all_from, core_to) : 0;
+                    const uint32_t bits = (ok >> (Q8 ? b >> 1 : b)) & 1 ? seen8(key + v_place(b), all_from, core_to) : 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t keep = pair_mask(bits, 2 * i);
                         if constexpr (Q8) {
 #pragma unroll
-                            for (int c = 0; c < (NVW + 1) / 2; ++c) vd[b][c][i] &= keep;
+                            for (int c = 0; c < NVD; ++c) vd[b][c][i] &= keep;
                         } else {
 #pragma unroll
                             for (int t = 0; t < NVW; ++t) vf[b][t][i] &= keep;
@@ -619,10 +631,11 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                 if constexpr (Q8) {
 #pragma unroll
                     for (int t = 0; t < NVW; ++t) {
-                        asm volatile("" : "+v"(vf[b][t]));        // not converted where it is loaded
-                        const u4 d = NVW % 2 == 0 || !(v_tile & 1) ? vd[b][t / 2] : vd[b][(t + 1) / 2 < (NVW + 1) / 2 ? (t + 1) / 2 : t / 2];
+                        if (b % 2 == 0) asm volatile("" : "+v"(vf[b / 2][t]));      // not converted where it is loaded
+                        const u4 d = vd[b][NVW % 2 == 0 ? t / 2 : 0], d1 = vd[b][NVD - 1];
+                        const bool next = NVW % 2 && ((v_tile + t) >> 1) != v_tile >> 1;
                         u4 hi, lo;
-                        times_scale(i8_to_half(vf[b][t]), d, hi, lo);
+                        times_scale(i8_to_half(u2{vf[b / 2][t][2 * (b % 2)], vf[b / 2][t][2 * (b % 2) + 1]}), next ? d1 : d, hi, lo);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -643,25 +656,29 @@ __global__ __launch_bounds__(256, kv_wgs(CT == KV_Q8, HD, NT)) void k_kv_attn(co
                         }
                 }
             };
+            constexpr int B_TOP = Q8 ? 2 * V_TOP : V_TOP;
 #pragma unroll
-            for (int b = 0; b < V_TOP; ++b) add_block(b);
-            if constexpr (V_TOP < NB) {
+            for (int b = 0; b < B_TOP; ++b) add_block(b);
+            if constexpr (V_TOP < NVL) {
                 __builtin_amdgcn_sched_barrier(0);
                 if (ahead) load_k(last ? then.part : cur.part, next);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int b = V_TOP; b < NB; ++b) add_block(b);
+                for (int b = B_TOP; b < NB; ++b) add_block(b);
             }
             // keys that only some of a sequence's tokens see (at its end, at the
             // window's begin) are added token by token
             if (!full && su.r.n > 1) {
 #pragma unroll 1
                 for (int b = 0; b < NB; ++b) {
-                    const int kb = key + KV_BLOCK * b;
+                    // the block's keys lie in [kb, kb + span)
+                    constexpr int span = Q8 ? 64 : KV_BLOCK;
+                    const int kb = key + span * (Q8 ? b >> 1 : b);
                     const int first = p.window > 0 ? su.r.len - su.r.n - p.window + 1 : 0;
-                    if (!((kb + KV_BLOCK > core_to && kb < key_end) || (kb < all_from && kb + KV_BLOCK > first))) continue;
-                    const int at = kb + 8 * lg, pg = page_at(cur.row, at), slot = at & page_mask;
+                    if (!((kb + span > core_to && kb < key_end) || (kb < all_from && kb + span > first))) continue;
+                    const int at = key + v_place(b), pg = page_at(cur.row, at), slot = at & page_mask;
                     const uint8_t * a = vbase + (uint64_t)(has_page(pg) ? pg : 0) * p.v_stride;
+                    typedef typename std::conditional<Q8, u2, u4>::type frag;
                     frag vz[NVW];
                     u4 dz[Q8 ? NVW : 1];
 #pragma unroll

@@ -470,7 +470,7 @@ const char * plan_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     const int64_t units = ((int64_t)b->max_pages * c->page_size + unit - 1) / unit + 1;
     const int64_t all = units * c->n_kv * ((rows + a.rows - 1) / a.rows) * b->n_seq;
     if (all >= (int64_t)1 << 31) return "the batch has 2^31 units of work or more";
-    a.grid = (int)std::min<int64_t>(kv_grid(c->type, c->head_dim, a.nt), all);
+    a.grid = (int)std::min<int64_t>(kv_grid(c->head_dim, a.nt), all);
     a.base_bytes = ((uint64_t)(b->n_seq + 1) * 4 + 255) / 256 * 256;
     a.ml_bytes = (uint64_t)a.grid * 2 * a.rows * 2 * 4;
     a.acc_bytes = (uint64_t)a.grid * 2 * a.rows * c->head_dim * 4;
