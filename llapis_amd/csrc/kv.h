@@ -21,11 +21,11 @@ struct KvSeqs {
 };
 
 constexpr int KV_BLOCK = 32;         // keys of one P V matrix instruction
-constexpr int KV_WAVES = 4;
-// keys of a unit, what the work is shared out in and a workgroup takes at a
-// time: 32 a wave, 16 where a wave's part of K and V would not leave room for
-// more workgroups' registers
-constexpr int kv_unit(int head_dim) { return KV_WAVES * (head_dim > 128 ? 16 : 32); }
+// waves of a workgroup, and keys of a unit, what the work is shared out in and a
+// workgroup takes at a time: 32 a wave, 16 where a wave's part of K and V would
+// not leave registers for more waves
+constexpr int kv_waves(int head_dim) { return head_dim > 256 ? 8 : 4; }
+constexpr int kv_unit(int head_dim) { return kv_waves(head_dim) * (head_dim > 128 ? 16 : 32); }
 constexpr int KV_MAX_NEW = 16;
 
 struct KvAttn {
@@ -44,26 +44,23 @@ struct KvAttn {
     int64_t out_stride;
     float * lse;
     int32_t * base;                  // [n_seq + 1] first unit of each sequence, [n_seq] their number
-    int grid;                        // workgroups of the attention kernel
-    float * ml;                      // [2 grid][rows of a tile][2] running maximum and sum of a partial result
-    float * acc;                     // [2 grid][rows of a tile][head_dim]
+    int nt;                          // 16-row tiles of a workgroup
+    int runs, tiles;                 // runs (a multiple of 8) of `tiles` workgroups, one for each 16 nt query rows
+    float * ml;                      // [runs][tiles][2 parts][16 nt rows][2] running maximum and sum of a partial result
+    float * acc;                     // [runs][tiles][2 parts][16 nt rows][head_dim]
 };
 
-// tiles of 16 query rows a workgroup holds at once: 1 or 2
+// tiles of 16 query rows a workgroup holds
 inline int kv_tiles(int rows) { return rows <= 16 ? 1 : 2; }
 // workgroups of the kernel that a CU's registers and LDS hold
-constexpr int kv_wgs(int head_dim, int nt) {
-    return head_dim > 256 ? (nt == 1 ? 2 : 1) : nt == 2 ? 2 : head_dim == 64 ? 4 : 3;
-}
-// workgroups that share the work out
-inline int kv_grid(int head_dim, int nt) { return 256 * kv_wgs(head_dim, nt); }
+constexpr int kv_wgs(int head_dim, int nt) { return head_dim > 256 ? 1 : nt == 2 ? 2 : head_dim == 64 ? 4 : 3; }
 
 // llapis_last_error() gets the message; returns -1
 int32_t refuse(const char * msg) noexcept;
 
-hipError_t launch_kv_attn_f16(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s);
-hipError_t launch_kv_attn_bf16(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s);
-hipError_t launch_kv_attn_q8(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s);
+hipError_t launch_kv_attn_f16(const KvAttn & p, int head_dim, hipStream_t s);
+hipError_t launch_kv_attn_bf16(const KvAttn & p, int head_dim, hipStream_t s);
+hipError_t launch_kv_attn_q8(const KvAttn & p, int head_dim, hipStream_t s);
 
 #if defined(__HIPCC__)
 

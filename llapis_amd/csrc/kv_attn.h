@@ -1,18 +1,21 @@
 // kv_attn.h -- attention of new tokens over the paged cache, the kernel (one
 // instance per cache type, query type, head size and row tiles; kv_attn_*.hip).
 //
-// Work.  A sequence's keys are units of 128; an item is (sequence, kv head,
-// tile of 16 NT query rows: the group's heads of every new token share the kv
-// head, so K and V are read once for all of them).  The items' units lie in one
-// line, of which every workgroup takes an equal run: long and short sequences
-// share the card alike, and no count of splits has to be chosen.  A run that
-// covers an item writes its result; parts of an item go to the workspace as
-// (maximum, sum, unnormalised output) and k_kv_join adds them in order.  The
-// split is a function of the lengths alone.
+// Work.  A sequence's keys are units of 128 or 64; an item is (sequence, kv
+// head).  The items' units lie in one line, of which every run of workgroups
+// takes an equal part: long and short sequences share the card alike, and no
+// count of splits has to be chosen.  A workgroup holds the kv head's query heads
+// of every new token, up to 32 rows, and reads K and V once for all of them; more
+// rows are tiles of 32 in workgroups of the same run, eight apart and so on one
+// XCD, where they walk the same keys at the same time.  (Tiles of 16 in two
+// workgroups instead of 32 in one measured 3.6 against 5.3 TB/s at head size 128:
+// they do not stay close enough for the L2.)  A run that covers an item writes
+// its result; parts of an item go to the workspace as (maximum, sum, unnormalised
+// output) and k_kv_join adds them.  The split is a function of the lengths alone.
 //
-// A workgroup's four waves take a unit together.  For its 32 (16) keys a wave forms
+// A workgroup's waves take a unit together.  For its 32 (16) keys a wave forms
 //   S^T = K Q^T     A = K (16 keys x 32 values), B = Q^T from LDS
-// and with the row maxima of all four its P, which goes to LDS; for its quarter
+// and with the row maxima of all waves its P, which goes to LDS; for its share
 // of the values' columns and all keys of the unit it then adds
 //   O^T += V^T P^T  A = V^T (16 values x 32 keys), B = P^T
 // (v_mfma_f32_16x16x32).  A lane's column is query row l % 16 in both products,
@@ -162,21 +165,19 @@ __device__ __forceinline__ void store4(void * p, int type, int64_t at, f4v x) {
     }
 }
 
-// a sequence's keys as the items see them
+// a sequence's keys as its items see them
 struct SeqUnits {
     SeqRows r;
     int k0, kend;          // keys [k0, kend), k0 a multiple of KV_BLOCK
-    int units, tiles;      // of an item; row tiles of a kv head
+    int units;             // of an item
 };
 
-__device__ __forceinline__ SeqUnits seq_units(const KvSeqs & b, int s, int page_shift, int window, int unit, int group,
-                                               int tile_rows) {
+__device__ __forceinline__ SeqUnits seq_units(const KvSeqs & b, int s, int page_shift, int window, int unit) {
     SeqUnits u;
     u.r = seq_rows(b, s);
     u.kend = min(u.r.len, b.max_pages << page_shift);
     u.k0 = window > 0 ? min(max(u.r.len - u.r.n - window + 1, 0), u.kend) & ~(KV_BLOCK - 1) : 0;
     u.units = u.r.n > 0 ? max((u.kend - u.k0 + unit - 1) / unit, 1) : 0;   // a row without keys is written too
-    u.tiles = (u.r.n * group + tile_rows - 1) / tile_rows;
     return u;
 }
 
@@ -191,7 +192,6 @@ __device__ __forceinline__ SeqUnits uniform_units(const SeqUnits & v) {
     u.k0 = same(v.k0);
     u.kend = same(v.kend);
     u.units = same(v.units);
-    u.tiles = same(v.tiles);
     return u;
 }
 
@@ -217,44 +217,43 @@ struct KvShape {
     static constexpr bool HALF = CT != KV_BF16;
     static constexpr int PQ = HALF ? (WIDE ? 2 : 1) : (WIDE ? 3 : 2);
     static constexpr int PP = HALF ? 2 : (WIDE ? 3 : 2);
-    static constexpr int UNIT = kv_unit(HD), KT = UNIT / (16 * KV_WAVES), NB = UNIT / KV_BLOCK;
-    static constexpr int NC = HD / 32, NV = HD / 16, NVW = (NV + KV_WAVES - 1) / KV_WAVES;
+    static constexpr int WAVES = kv_waves(HD), UNIT = kv_unit(HD), KT = UNIT / (16 * WAVES), NB = UNIT / KV_BLOCK;
+    static constexpr int NC = HD / 32, NV = HD / 16, NVW = (NV + WAVES - 1) / WAVES;
     static constexpr int Q_BYTES = PQ * NT * NC * 1024;
     static constexpr int P_BYTES = NB * NT * PP * 1024;
     static constexpr int LDS = Q_BYTES + P_BYTES;
 };
 
 template <int CT, bool WIDE, int HD, int NT>
-__global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p) {
+__global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 4) void k_kv_attn(const KvAttn p) {
     using Sh = KvShape<CT, WIDE, HD, NT>;
     constexpr bool HALF = Sh::HALF, Q8 = CT == KV_Q8;
     constexpr int PQ = Sh::PQ, PP = Sh::PP, NC = Sh::NC, NV = Sh::NV, NVW = Sh::NVW, KT = Sh::KT, NB = Sh::NB;
-    constexpr int UNIT = Sh::UNIT, ROWS = 16 * NT;
-    constexpr int V_TOP = Q8 ? UNIT / 64 : HD > 256 ? NB / 2 : NB;    // V's loads ahead of a unit's first product
+    constexpr int UNIT = Sh::UNIT, ROWS = 16 * NT, WAVES = Sh::WAVES, WGT = 64 * WAVES;
     constexpr int EL = Q8 ? 1 : 2;                                // bytes of a cached value
     constexpr float P_SHIFT = HALF ? 15.0f : 0.0f;                // log2 of p's scale
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ int s_scan[256 + 1];
-    __shared__ int s_part[KV_WAVES];
+    __shared__ int s_scan[WGT + 1];
+    __shared__ int s_part[WAVES];
     __shared__ int s_exp[ROWS];
-    __shared__ float s_top[KV_WAVES][ROWS];
+    __shared__ float s_top[WAVES][ROWS];
     uint8_t * const lds_p = lds + Sh::Q_BYTES;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = same(tid >> 6);
     const int lm = lane & 15, lg = lane >> 4;
     const int page = 1 << p.page_shift, page_mask = page - 1;
-    auto units_at = [&](int s) { return seq_units(p.b, s, p.page_shift, p.window, UNIT, p.group, ROWS); };
+    const int type = WIDE && !Q8 ? (int)T_F32 : p.type;
+    // run and tile: a run's tiles are eight workgroups apart, on one XCD
+    const int octet = blockIdx.x >> 3, tile = octet % p.tiles, run = octet / p.tiles * 8 + (blockIdx.x & 7);
+    auto units_at = [&](int s) { return seq_units(p.b, s, p.page_shift, p.window, UNIT); };
 
     // ---- the line of units: thread t counts sequences [t per, (t + 1) per)
-    const int per = (p.b.n_seq + 255) / 256;
+    const int per = (p.b.n_seq + WGT - 1) / WGT;
     {
         int sum = 0;
         for (int i = 0; i < per; ++i) {
             const int s = tid * per + i;
-            if (s < p.b.n_seq) {
-                const SeqUnits u = units_at(s);
-                sum += u.units * u.tiles * p.n_kv;
-            }
+            if (s < p.b.n_seq) sum += units_at(s).units * p.n_kv;
         }
         for (int o = 1; o < 64; o <<= 1) {
             const int v = __shfl_up(sum, o, 64);
@@ -267,62 +266,68 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
         if (tid == 0) s_scan[0] = 0;
         __syncthreads();
     }
-    const int total = same(s_scan[256]);
-    const int n_runs = min((int)gridDim.x, total);
+    const int total = same(s_scan[WGT]);
+    const int n_runs = min(p.runs, total);
     if (blockIdx.x == 0) {
         // for the join
         int at = s_scan[tid];
         for (int i = 0; i < per; ++i) {
             const int s = tid * per + i;
             if (s < p.b.n_seq) {
-                const SeqUnits u = units_at(s);
                 p.base[s] = at;
-                at += u.units * u.tiles * p.n_kv;
+                at += units_at(s).units * p.n_kv;
             }
         }
         if (tid == 0) p.base[p.b.n_seq] = total;
     }
-    if ((int)blockIdx.x >= n_runs) return;
-    const int lo = run_begin(blockIdx.x, n_runs, total), hi = run_begin(blockIdx.x + 1, n_runs, total);
+    if (run >= n_runs) return;
+    const int lo = run_begin(run, n_runs, total), hi = run_begin(run + 1, n_runs, total);
 
     // ---- the sequence of the first unit, and from there on piece by piece
     int at_seq, at_unit;                              // a sequence and its first unit
     {
         int t = 0;
-        for (int step = 128; step; step >>= 1)
-            if (t + step < 256 && s_scan[t + step] <= lo) t += step;
+        for (int step = WGT / 2; step; step >>= 1)
+            if (t + step < WGT && s_scan[t + step] <= lo) t += step;
         t = same(t);
         at_seq = t * per;
         at_unit = same(s_scan[t]);
     }
     struct Piece {
         SeqUnits su;
-        int seq, head, tile, u0, n_u, key_begin, key_end;
+        int head, u0, n_u, key_begin, key_end;
         const int32_t * row;                          // of the page table
         uint64_t part;                                // a head's part of a page, which its scales follow
     };
     SeqUnits at_su = uniform_units(units_at(at_seq));
-    // the piece from unit u on; false where another stream has changed the lengths meanwhile
-    auto piece_at = [&](int u, Piece & c) {
-        int n_here;
-        while (u - at_unit >= (n_here = at_su.units * at_su.tiles * p.n_kv)) {
-            if (at_seq + 1 >= p.b.n_seq) return false;
-            at_unit += n_here;
-            ++at_seq;
-            at_su = uniform_units(units_at(at_seq));
+    int u = lo;
+    // the next piece with rows of this tile; false at the run's end (and where
+    // another stream has changed the lengths meanwhile)
+    auto next_piece = [&](Piece & c) {
+        while (u < hi) {
+            int n_here;
+            while (u - at_unit >= (n_here = at_su.units * p.n_kv)) {
+                if (at_seq + 1 >= p.b.n_seq) return false;
+                at_unit += n_here;
+                ++at_seq;
+                at_su = uniform_units(units_at(at_seq));
+            }
+            if (tile * ROWS >= at_su.r.n * p.group) {
+                u = at_unit + n_here;                 // this sequence has fewer rows
+                continue;
+            }
+            c.su = at_su;
+            c.head = (u - at_unit) / at_su.units;
+            c.u0 = u - at_unit - c.head * at_su.units;
+            c.n_u = min(at_su.units - c.u0, hi - u);
+            c.key_begin = at_su.k0 + c.u0 * UNIT;
+            c.key_end = min(c.key_begin + c.n_u * UNIT, at_su.kend);
+            c.row = p.b.table + at_seq * p.b.table_stride;
+            c.part = (uint64_t)c.head * page * (Q8 ? HD + HD / 16 : 2 * HD);
+            u += c.n_u;
+            return true;
         }
-        c.su = at_su;
-        c.seq = at_seq;
-        const int item = (u - at_unit) / at_su.units;
-        c.u0 = u - at_unit - item * at_su.units;
-        c.n_u = min(at_su.units - c.u0, hi - u);
-        c.head = item / at_su.tiles;
-        c.tile = item - c.head * at_su.tiles;
-        c.key_begin = at_su.k0 + c.u0 * UNIT;
-        c.key_end = min(c.key_begin + c.n_u * UNIT, at_su.kend);
-        c.row = p.b.table + at_seq * p.b.table_stride;
-        c.part = (uint64_t)c.head * page * (Q8 ? HD + HD / 16 : 2 * HD);
-        return true;
+        return false;
     };
 
     // ---- loads of a unit's K, ahead of its use
@@ -377,26 +382,24 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
     const int v_tile = wave * NVW;
 
     Piece cur, then;
-    if (!piece_at(lo, cur)) return;
+    if (!next_piece(cur)) return;
     if (cur.key_begin < cur.key_end) {
         load_pages(cur.row, cur.key_begin);
         load_k(cur.part, cur.key_begin);
     }
-    for (int u = lo;;) {
+    for (;;) {
         const SeqUnits & su = cur.su;
-        const int head = cur.head, tile = cur.tile, key_end = cur.key_end;
+        const int head = cur.head, key_end = cur.key_end;
         const int n_rows = min(su.r.n * p.group - tile * ROWS, ROWS);
         const bool whole = cur.n_u == su.units;
-        const int slot = 2 * blockIdx.x + (cur.u0 == 0);
-        u += cur.n_u;
+        const int64_t slot = ((int64_t)run * p.tiles + tile) * 2 + (cur.u0 == 0);
 
-        // ---- Q into LDS as B operands, (part, row tile, 32 values) x lane: 16
-        // threads a row
-        constexpr int QE = (HD / 8 + 15) / 16;
+        // ---- Q into LDS as B operands, (part, 32 values) x lane: 16 threads a row
         __syncthreads();                                           // the last piece's LDS has been read
+        constexpr int QE = (HD / 8 + 15) / 16;
 #pragma unroll 1
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = 16 * nt + (tid >> 4), rr = tile * ROWS + r, tok = rr / p.group;
+        for (int r = tid >> 4; r < ROWS; r += WGT / 16) {
+            const int rr = tile * ROWS + r, tok = rr / p.group;
             const int64_t from = (su.r.row0 + tok) * p.q_stride + (int64_t)(head * p.group + rr - tok * p.group) * HD;
             float qx[QE][8];
             float amax = 0.0f;
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                 const int o = (tid & 15) + 16 * e;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) qx[e][j] = 0.0f;
-                if (r < n_rows && o < HD / 8) load8(p.q, WIDE && !Q8 ? (int)T_F32 : p.type, from + 8 * o, qx[e]);
+                if (r < n_rows && o < HD / 8) load8(p.q, type, from + 8 * o, qx[e]);
                 if (HALF)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[e][j]));
@@ -430,17 +433,16 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                     // the product and lane group that eight values go to
                     const int c = o < 8 * NP ? 2 * (o >> 3) + (o & 1) : o >> 2, g = o < 8 * NP ? (o >> 1) & 3 : o & 3;
 #pragma unroll
-                    for (int q = 0; q < PQ; ++q)
-                        *(u4 *)(lds + ((q * NT + nt) * NC + c) * 1024 + (g * 16 + (tid >> 4)) * 16) = part[q];
+                    for (int q = 0; q < PQ; ++q) *(u4 *)(lds + ((q * NT + (r >> 4)) * NC + c) * 1024 + (g * 16 + (r & 15)) * 16) = part[q];
                 }
             }
         }
         // the next piece, whose first K is loaded during this one's last unit
-        const bool more = u < hi && piece_at(u, then);
+        const bool more = next_piece(then);
         __syncthreads();
-        // a lane's query rows: score scale in log2, position
-        float q_scale[NT];
+        // the lane's query rows: token, position, score scale in log2
         int t_pos[NT], tok_of[NT];
+        float q_scale[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             tok_of[nt] = min((tile * ROWS + 16 * nt + lm) / p.group, su.r.n - 1);
@@ -490,7 +492,7 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                 const int slot = (key + v_place(Q8 ? 2 * i : i)) & page_mask;
 #pragma unroll
                 for (int t = 0; t < NVW; ++t) {
-                    const int vt = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
+                    const int vt = NV % WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
                     vf[i][t] = *(const u4 *)(va[i] + ((16 * vt + lv) * page + slot) * EL);
                 }
                 if constexpr (Q8)
@@ -502,7 +504,7 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                     }
             };
 #pragma unroll
-            for (int i = 0; i < V_TOP; ++i) load_v(i);
+            for (int i = 0; i < NVL; ++i) load_v(i);
             // ---- S^T of the wave's keys
             __builtin_amdgcn_sched_barrier(0);
             f4v sc[NT][KT];
@@ -537,35 +539,23 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (V_TOP < NVL) {
-#pragma unroll
-                for (int i = V_TOP; i < NVL; ++i) load_v(i);
-            } else if (ahead) {
-                load_k(last ? then.part : cur.part, next);
-            }
+            if (ahead) load_k(last ? then.part : cur.part, next);
             __builtin_amdgcn_sched_barrier(0);
             // ---- softmax: the lane's keys are key + s_oct + w_half + (0 .. 4 KT - 1)
-            const int s_key = key + s_oct + w_half;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int t = 0; t < KT; ++t) sc[nt][t] *= q_scale[nt];
-            if (!full) {
-                const int page_end = s_ok ? key_end : 0;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int from = p.window > 0 ? t_pos[nt] - p.window + 1 : 0, to = min(t_pos[nt] + 1, page_end);
+                if (!full) {
+                    const int from = p.window > 0 ? t_pos[nt] - p.window + 1 : 0, to = min(t_pos[nt] + 1, s_ok ? key_end : 0);
 #pragma unroll
                     for (int t = 0; t < KT; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int at = s_key + 4 * t + i;
+                            const int at = key + s_oct + w_half + 4 * t + i;
                             sc[nt][t][i] = ((at >= from) & (at < to)) ? sc[nt][t][i] : -__builtin_inff();
                         }
                 }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
                 float top = -__builtin_inff();
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
@@ -579,7 +569,7 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
             for (int nt = 0; nt < NT; ++nt) {
                 float now = m[nt];
 #pragma unroll
-                for (int w = 0; w < KV_WAVES; ++w) now = fmaxf(now, s_top[w][16 * nt + lm]);
+                for (int w = 0; w < WAVES; ++w) now = fmaxf(now, s_top[w][16 * nt + lm]);
                 const float ref = now == -__builtin_inff() ? 0.0f : now;
                 if (__any(now != m[nt])) {
                     const float f = __builtin_amdgcn_exp2f(m[nt] - ref);
@@ -598,11 +588,11 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                 for (int i = 4 * KT; i < 8; ++i) x[i] = 0.0f;
                 u4 part[PP];
                 split8<HALF, PP>(x, part);
+                const int b = Q8 ? 2 * (w_block >> 1) + (lg & 1) : w_block;
+                const int at = Q8 ? (2 * (w_block & 1) + (lg >> 1)) * 16 + lm : lane;
 #pragma unroll
                 for (int q = 0; q < PP; ++q) {
-                    const int b = Q8 ? 2 * (w_block >> 1) + (lg & 1) : w_block;
-                    const int l = Q8 ? (2 * (w_block & 1) + (lg >> 1)) * 16 + lm : lane;
-                    uint8_t * w = lds_p + ((b * NT + nt) * PP + q) * 1024 + l * 16;
+                    uint8_t * w = lds_p + ((b * NT + nt) * PP + q) * 1024 + at * 16;
                     if constexpr (KT == 2) *(u4 *)w = part[q];
                     else *(u2 *)(w + 2 * w_half) = u2{part[q][0], part[q][1]};
                 }
@@ -613,7 +603,6 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
             // becomes 0 in V, for q8_0 in its scales
             const int core_to = min(all_to, key_end);
             auto add_block = [&](int b) {
-                if (HD > 256) __builtin_amdgcn_sched_barrier(0);
                 if (!full) {
                     const uint32_t bits = (ok >> (Q8 ? b >> 1 : b)) & 1 ? seen8(key + v_place(b), all_from, core_to) : 0;
 #pragma unroll
@@ -628,44 +617,34 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                         }
                     }
                 }
-                if constexpr (Q8) {
+                u4 bp[NT][PP];
 #pragma unroll
-                    for (int t = 0; t < NVW; ++t) {
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int q = 0; q < PP; ++q)
+                        bp[nt][q] = *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16);
+#pragma unroll
+                for (int t = 0; t < NVW; ++t) {
+                    u4 hi, lo;
+                    if constexpr (Q8) {
                         if (b % 2 == 0) asm volatile("" : "+v"(vf[b / 2][t]));      // not converted where it is loaded
                         const u4 d = vd[b][NVW % 2 == 0 ? t / 2 : 0], d1 = vd[b][NVD - 1];
-                        const bool next = NVW % 2 && ((v_tile + t) >> 1) != v_tile >> 1;
-                        u4 hi, lo;
-                        times_scale(i8_to_half(u2{vf[b / 2][t][2 * (b % 2)], vf[b / 2][t][2 * (b % 2) + 1]}), next ? d1 : d, hi, lo);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int q = 0; q < PP; ++q) {
-                                const u4 bp = *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16);
-                                acc[nt][t] = mfma16<HALF>(hi, bp, acc[nt][t]);
-                                if (WIDE && q == 0) acc[nt][t] = mfma16<HALF>(lo, bp, acc[nt][t]);
-                            }
+                        const bool next_block = NVW % 2 && ((v_tile + t) >> 1) != v_tile >> 1;
+                        times_scale(i8_to_half(u2{vf[b / 2][t][2 * (b % 2)], vf[b / 2][t][2 * (b % 2) + 1]}),
+                                    next_block ? d1 : d, hi, lo);
+                    } else {
+                        hi = vf[b][t];
                     }
-                } else {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                        for (int q = 0; q < PP; ++q) {
-                            const u4 bp = *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16);
-#pragma unroll
-                            for (int t = 0; t < NVW; ++t) acc[nt][t] = mfma16<HALF>(vf[b][t], bp, acc[nt][t]);
-                        }
+                        for (int q = 0; q < PP; ++q) acc[nt][t] = mfma16<HALF>(hi, bp[nt][q], acc[nt][t]);
+                        if (Q8 && WIDE) acc[nt][t] = mfma16<HALF>(lo, bp[nt][0], acc[nt][t]);
+                    }
                 }
             };
-            constexpr int B_TOP = Q8 ? 2 * V_TOP : V_TOP;
 #pragma unroll
-            for (int b = 0; b < B_TOP; ++b) add_block(b);
-            if constexpr (V_TOP < NVL) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (ahead) load_k(last ? then.part : cur.part, next);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int b = B_TOP; b < NB; ++b) add_block(b);
-            }
+            for (int b = 0; b < NB; ++b) add_block(b);
             // keys that only some of a sequence's tokens see (at its end, at the
             // window's begin) are added token by token
             if (!full && su.r.n > 1) {
@@ -683,7 +662,7 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
                     u4 dz[Q8 ? NVW : 1];
 #pragma unroll
                     for (int t = 0; t < NVW; ++t) {
-                        const int vt = NV % KV_WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
+                        const int vt = NV % WAVES ? min(v_tile + t, NV - 1) : v_tile + t;
                         vz[t] = *(const frag *)(a + ((16 * vt + lv) * page + slot) * EL);
                         if constexpr (Q8) dz[t] = *(const u4 *)(a + page * HD + ((vt >> 1) * page + slot) * 2);
                     }
@@ -719,7 +698,7 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
             }
         }
 
-        // ---- the sums of the four waves, in their order; maxima are the same in all
+        // ---- the sums of the waves, in their order; maxima are the same in all
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) l[nt] = over_groups(l[nt], [](float a, float b) { return a + b; });
         __syncthreads();
@@ -731,7 +710,9 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
         for (int nt = 0; nt < NT; ++nt) {
             const int r = 16 * nt + lm;
             if (r >= n_rows) continue;
-            const float sum = (s_top[0][r] + s_top[1][r]) + (s_top[2][r] + s_top[3][r]);
+            float sum = s_top[0][r];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) sum += s_top[w][r];
             if (whole) {
                 const int rr = tile * ROWS + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
                 const int64_t out_row = su.r.row0 + tok;
@@ -739,19 +720,18 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
 #pragma unroll
                 for (int t = 0; t < NVW; ++t)
                     if (v_tile + t < NV)
-                        store4(p.out, WIDE && !Q8 ? (int)T_F32 : p.type,
-                               out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
+                        store4(p.out, type, out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
                 if (p.lse && wave == 0 && lg == 0)
                     p.lse[out_row * (p.group * p.n_kv) + hq] =
                         sum == 0.0f ? -__builtin_inff() : (m[nt] + (__builtin_amdgcn_logf(sum) - P_SHIFT)) * KV_LN2;
             } else {
-                float * a = p.acc + ((int64_t)slot * ROWS + r) * HD;
+                float * a = p.acc + (slot * ROWS + r) * HD;
 #pragma unroll
                 for (int t = 0; t < NVW; ++t)
                     if (v_tile + t < NV) *(f4v *)(a + 16 * (v_tile + t) + 4 * lg) = acc[nt][t];
                 if (wave == 0 && lg == 0) {
-                    p.ml[((int64_t)slot * ROWS + r) * 2] = m[nt];
-                    p.ml[((int64_t)slot * ROWS + r) * 2 + 1] = sum;
+                    p.ml[(slot * ROWS + r) * 2] = m[nt];
+                    p.ml[(slot * ROWS + r) * 2 + 1] = sum;
                 }
             }
         }
@@ -761,30 +741,30 @@ __global__ __launch_bounds__(256, kv_wgs(HD, NT)) void k_kv_attn(const KvAttn p)
 }
 
 template <int CT, bool WIDE, int HD, int NT>
-hipError_t launch_kv_attn_one(const KvAttn & p, int grid, hipStream_t s) {
-    constexpr int lds = KvShape<CT, WIDE, HD, NT>::LDS;
-    hipLaunchKernelGGL((k_kv_attn<CT, WIDE, HD, NT>), dim3(grid), dim3(256), lds, s, p);
+hipError_t launch_kv_attn_one(const KvAttn & p, hipStream_t s) {
+    hipLaunchKernelGGL((k_kv_attn<CT, WIDE, HD, NT>), dim3(p.runs * p.tiles), dim3(64 * kv_waves(HD)),
+                       (KvShape<CT, WIDE, HD, NT>::LDS), s, p);
     return hipGetLastError();
 }
 
 template <int CT, bool WIDE, int NT>
-hipError_t launch_kv_attn_hd(const KvAttn & p, int head_dim, int grid, hipStream_t s) {
+hipError_t launch_kv_attn_hd(const KvAttn & p, int head_dim, hipStream_t s) {
     switch (head_dim) {
-        case 64: return launch_kv_attn_one<CT, WIDE, 64, NT>(p, grid, s);
-        case 96: return launch_kv_attn_one<CT, WIDE, 96, NT>(p, grid, s);
-        case 128: return launch_kv_attn_one<CT, WIDE, 128, NT>(p, grid, s);
-        case 192: return launch_kv_attn_one<CT, WIDE, 192, NT>(p, grid, s);
-        case 256: return launch_kv_attn_one<CT, WIDE, 256, NT>(p, grid, s);
-        case 512: return launch_kv_attn_one<CT, WIDE, 512, NT>(p, grid, s);
+        case 64: return launch_kv_attn_one<CT, WIDE, 64, NT>(p, s);
+        case 96: return launch_kv_attn_one<CT, WIDE, 96, NT>(p, s);
+        case 128: return launch_kv_attn_one<CT, WIDE, 128, NT>(p, s);
+        case 192: return launch_kv_attn_one<CT, WIDE, 192, NT>(p, s);
+        case 256: return launch_kv_attn_one<CT, WIDE, 256, NT>(p, s);
+        case 512: return launch_kv_attn_one<CT, WIDE, 512, NT>(p, s);
     }
     return hipErrorInvalidValue;
 }
 
 template <int CT>
-hipError_t launch_kv_attn_type(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s) {
+hipError_t launch_kv_attn_type(const KvAttn & p, int head_dim, hipStream_t s) {
     if (p.type == T_F32 || (CT == KV_Q8 && p.type == T_F16))
-        return nt == 1 ? launch_kv_attn_hd<CT, true, 1>(p, head_dim, grid, s) : launch_kv_attn_hd<CT, true, 2>(p, head_dim, grid, s);
-    return nt == 1 ? launch_kv_attn_hd<CT, false, 1>(p, head_dim, grid, s) : launch_kv_attn_hd<CT, false, 2>(p, head_dim, grid, s);
+        return p.nt == 1 ? launch_kv_attn_hd<CT, true, 1>(p, head_dim, s) : launch_kv_attn_hd<CT, true, 2>(p, head_dim, s);
+    return p.nt == 1 ? launch_kv_attn_hd<CT, false, 1>(p, head_dim, s) : launch_kv_attn_hd<CT, false, 2>(p, head_dim, s);
 }
 
 }  // namespace dev

@@ -3,8 +3,8 @@
 
 namespace llapis {
 
-hipError_t launch_kv_attn_bf16(const KvAttn & p, int head_dim, int nt, int grid, hipStream_t s) {
-    return dev::launch_kv_attn_type<dev::KV_BF16>(p, head_dim, nt, grid, s);
+hipError_t launch_kv_attn_bf16(const KvAttn & p, int head_dim, hipStream_t s) {
+    return dev::launch_kv_attn_type<dev::KV_BF16>(p, head_dim, s);
 }
 
 }  // namespace llapis

@@ -17,20 +17,20 @@ namespace dev {
 // own, and are added in their order.  A part is read once, its maximum and sum
 // with its values, so that the loads of several parts are in flight.
 template <int PG>
-__global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, int tile_rows, int tiles, float p_shift) {
+__global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, float p_shift) {
     constexpr int TPG = 256 / PG;
     __shared__ f4v s_acc[PG][TPG];
     __shared__ float s_m[PG][TPG], s_l[PG][TPG];
-    const int tid = threadIdx.x, g = tid / TPG, e = tid - g * TPG;
-    const int seq = blockIdx.x / (p.n_kv * tiles), rest = blockIdx.x - seq * p.n_kv * tiles;
+    const int tid = threadIdx.x, g = tid / TPG, e = tid - g * TPG, tile_rows = 16 * p.nt;
+    const int seq = blockIdx.x / (p.n_kv * p.tiles), rest = blockIdx.x - seq * p.n_kv * p.tiles;
     const int total = p.base[p.b.n_seq], base = p.base[seq];
-    const SeqUnits su = seq_units(p.b, seq, p.page_shift, p.window, p.unit, p.group, tile_rows);
-    const int head = rest / tiles, tile = rest - head * tiles;
+    const SeqUnits su = seq_units(p.b, seq, p.page_shift, p.window, p.unit);
+    const int head = rest / p.tiles, tile = rest - head * p.tiles;
     const int n_rows = min(su.r.n * p.group - tile * tile_rows, tile_rows);
     const int at = (blockIdx.y * TPG + e) * 4, r = at / head_dim, d = at - r * head_dim;
     if ((int)(blockIdx.y * TPG * 4) >= n_rows * head_dim) return;      // also: no such item
-    const int first = base + (head * su.tiles + tile) * su.units;
-    const int64_t n_runs = min(p.grid, total);
+    const int first = base + head * su.units;
+    const int64_t n_runs = min(p.runs, total);
     const int w0 = (int)(((int64_t)(first + 1) * n_runs - 1) / total);
     const int w1 = (int)(((int64_t)(first + su.units) * n_runs - 1) / total);
     if (w0 == w1) return;                                              // written by k_kv_attn
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, i
             xm[j] = -__builtin_inff();
             xl[j] = 0.0f;
             if (live && i <= w1 - w0) {
-                const int64_t row = (int64_t)(2 * (w0 + i) + (i == 0)) * tile_rows + r;
+                const int64_t row = (((int64_t)(w0 + i) * p.tiles + tile) * 2 + (i == 0)) * tile_rows + r;
                 x[j] = *(const f4v *)(p.acc + row * head_dim + d);
                 xm[j] = p.ml[2 * row];
                 xl[j] = p.ml[2 * row + 1];
@@ -452,9 +452,9 @@ KvSeqs seqs_of(const llapis_kv_batch * b) {
     return {b->page_table, b->lens, b->new_start, b->table_stride, b->n_seq, b->n_tokens, b->new_start ? b->max_new : 1, b->max_pages};
 }
 
-// sizes of an attention call; grid 0: nothing to do
+// sizes of an attention call
 struct AttnPlan {
-    int nt, rows, grid;
+    int nt, runs, tiles;
     uint64_t base_bytes, ml_bytes, acc_bytes;
     uint64_t bytes() const { return base_bytes + ml_bytes + acc_bytes; }
 };
@@ -465,15 +465,18 @@ const char * plan_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     if (max_new > KV_MAX_NEW) return "more than 16 new tokens a sequence";
     const int rows = n_head / c->n_kv * std::max(max_new, 1);
     a.nt = kv_tiles(rows);
-    a.rows = 16 * a.nt;
+    a.tiles = (rows + 16 * a.nt - 1) / (16 * a.nt);
     const int unit = kv_unit(c->head_dim);
     const int64_t units = ((int64_t)b->max_pages * c->page_size + unit - 1) / unit + 1;
-    const int64_t all = units * c->n_kv * ((rows + a.rows - 1) / a.rows) * b->n_seq;
+    const int64_t all = units * c->n_kv * b->n_seq;
     if (all >= (int64_t)1 << 31) return "the batch has 2^31 units of work or more";
-    a.grid = (int)std::min<int64_t>(kv_grid(c->head_dim, a.nt), all);
+    // as many workgroups as the card holds at once
+    const int64_t most = std::max(256 * kv_wgs(c->head_dim, a.nt) / a.tiles, 8);
+    a.runs = (int)((std::min(most, all) + 7) / 8 * 8);
+    const uint64_t parts = (uint64_t)a.runs * a.tiles * 2;
     a.base_bytes = ((uint64_t)(b->n_seq + 1) * 4 + 255) / 256 * 256;
-    a.ml_bytes = (uint64_t)a.grid * 2 * a.rows * 2 * 4;
-    a.acc_bytes = (uint64_t)a.grid * 2 * a.rows * c->head_dim * 4;
+    a.ml_bytes = parts * 16 * a.nt * 2 * 4;
+    a.acc_bytes = parts * 16 * a.nt * c->head_dim * 4;
     return nullptr;
 }
 
@@ -583,6 +586,7 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
         return refuse_as(who, "q and out must be 16-byte aligned, rows too");
     if (sq.n_tokens > 1 && (q->q_stride < width || q->out_stride < width)) return refuse_as(who, "rows shorter than n_head * head_dim");
     if (!workspace || !aligned16(workspace) || ws_bytes < a.bytes()) return refuse_as(who, "workspace too small or not 16-byte aligned");
+    if ((int64_t)sq.n_seq * c->n_kv * a.tiles >= (int64_t)1 << 31) return refuse_as(who, "2^31 items or more");
     KvAttn p{};
     p.b = sq;
     p.k = (const uint8_t *)c->k;
@@ -606,23 +610,23 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     p.base = (int32_t *)ws;
     p.ml = (float *)(ws + a.base_bytes);
     p.acc = (float *)(ws + a.base_bytes + a.ml_bytes);
-    p.grid = a.grid;
+    p.nt = a.nt;
+    p.runs = a.runs;
+    p.tiles = a.tiles;
     hipStream_t s = (hipStream_t)stream;
-    if (c->type == T_F16) KV_TRY(launch_kv_attn_f16(p, c->head_dim, a.nt, a.grid, s));
-    else if (c->type == T_BF16) KV_TRY(launch_kv_attn_bf16(p, c->head_dim, a.nt, a.grid, s));
-    else KV_TRY(launch_kv_attn_q8(p, c->head_dim, a.nt, a.grid, s));
+    if (c->type == T_F16) KV_TRY(launch_kv_attn_f16(p, c->head_dim, s));
+    else if (c->type == T_BF16) KV_TRY(launch_kv_attn_bf16(p, c->head_dim, s));
+    else KV_TRY(launch_kv_attn_q8(p, c->head_dim, s));
     if ((int64_t)b->max_pages * c->page_size <= p.unit) return 0;      // every item is one unit
     // parts of an item, as many as the bounds suggest; workgroups by an item's rows
-    const int rows = q->n_head / c->n_kv * sq.max_new, tiles = (rows + a.rows - 1) / a.rows;
-    const int64_t items = (int64_t)sq.n_seq * c->n_kv * tiles;
-    const int parts = (int)(a.grid / items);
-    const int pg = parts < 4 ? 1 : parts < 16 ? 4 : 16;
-    const int per = 1024 / pg;
-    const dim3 grid((unsigned)items, (std::min(rows, a.rows) * c->head_dim + per - 1) / per), wg(256);
+    const int64_t items = (int64_t)sq.n_seq * c->n_kv;
+    const int parts = (int)(a.runs / items), pg = parts < 4 ? 1 : parts < 16 ? 4 : 16, per = 1024 / pg;
+    const int rows = std::min(q->n_head / c->n_kv * sq.max_new, 16 * a.nt);
+    const dim3 grid((unsigned)(items * a.tiles), (rows * c->head_dim + per - 1) / per), wg(256);
     const float shift = c->type == T_BF16 ? 0.0f : 15.0f;
-    if (pg == 1) hipLaunchKernelGGL(k_kv_join<1>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
-    else if (pg == 4) hipLaunchKernelGGL(k_kv_join<4>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
-    else hipLaunchKernelGGL(k_kv_join<16>, grid, wg, 0, s, p, c->head_dim, a.rows, tiles, shift);
+    if (pg == 1) hipLaunchKernelGGL(k_kv_join<1>, grid, wg, 0, s, p, c->head_dim, shift);
+    else if (pg == 4) hipLaunchKernelGGL(k_kv_join<4>, grid, wg, 0, s, p, c->head_dim, shift);
+    else hipLaunchKernelGGL(k_kv_join<16>, grid, wg, 0, s, p, c->head_dim, shift);
     KV_TRY(hipGetLastError());
     return 0;
 }
