@@ -195,8 +195,25 @@ __device__ __forceinline__ SeqUnits uniform_units(const SeqUnits & v) {
     return u;
 }
 
-// run w of n_runs equal ones over `total` units
-__device__ __forceinline__ int run_begin(int w, int n_runs, int total) { return (int)((int64_t)w * total / n_runs); }
+// The line that runs share out, in halves of a unit: an item has one half more
+// than its units, for what a piece costs beside them (its queries, its first
+// loads, its results).
+__device__ __forceinline__ int item_steps(int units) { return units > 0 ? 2 * units + 1 : 0; }
+// Runs over `total` steps: the first total % n take one more.
+struct Runs {
+    int q, more;
+    __device__ __forceinline__ Runs(int total, int n) : q(total / n), more(total - total / n * n) {}
+    __device__ __forceinline__ int begin(int run) const { return run * q + min(run, more); }
+    __device__ __forceinline__ int owner(int step) const {
+        const int head = more * (q + 1);
+        return step < head ? step / (q + 1) : more + (step - head) / q;
+    }
+};
+// Of an item's steps, counted from its first, unit k is the run's that has step
+// 2 k + 1; the last step is no unit's.  Runs have two steps at least, so that each
+// run between an item's first and last has a unit of it.
+__device__ __forceinline__ int units_before(int step) { return step >> 1; }
+__device__ __forceinline__ int runs_of(int most, int total) { return min(most, total >> 1); }
 
 // bit i: key `at` + i, i < 8, is in [from, to)
 __device__ __forceinline__ uint32_t seen8(int at, int from, int to) {
@@ -233,7 +250,7 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
     constexpr int EL = Q8 ? 1 : 2;                                // bytes of a cached value
     constexpr float P_SHIFT = HALF ? 15.0f : 0.0f;                // log2 of p's scale
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ int s_scan[WGT + 1];
+    __shared__ struct { int seq, step; SeqUnits su; } s_first;
     __shared__ int s_part[WAVES];
     __shared__ int s_exp[ROWS];
     __shared__ float s_top[WAVES][ROWS];
@@ -247,84 +264,91 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
     const int octet = blockIdx.x >> 3, tile = octet % p.tiles, run = octet / p.tiles * 8 + (blockIdx.x & 7);
     auto units_at = [&](int s) { return seq_units(p.b, s, p.page_shift, p.window, UNIT); };
 
-    // ---- the line of units: thread t counts sequences [t per, (t + 1) per)
+    // ---- the line: thread t counts sequences [t per, (t + 1) per)
     const int per = (p.b.n_seq + WGT - 1) / WGT;
-    {
-        int sum = 0;
-        for (int i = 0; i < per; ++i) {
-            const int s = tid * per + i;
-            if (s < p.b.n_seq) sum += units_at(s).units * p.n_kv;
-        }
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += v;
-        }
-        if (lane == 63) s_part[wave] = sum;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) sum += s_part[w];
-        s_scan[tid + 1] = sum;
-        if (tid == 0) s_scan[0] = 0;
-        __syncthreads();
+    int sum = 0;
+    for (int i = 0; i < per; ++i) {
+        const int s = tid * per + i;
+        if (s < p.b.n_seq) sum += item_steps(units_at(s).units) * p.n_kv;
     }
-    const int total = same(s_scan[WGT]);
-    const int n_runs = min(p.runs, total);
+    const int own = sum;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 63) s_part[wave] = sum;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) sum += s_part[w];
+        total += s_part[w];
+    }
+    total = same(total);
+    const int n_runs = runs_of(p.runs, total);
     if (blockIdx.x == 0) {
         // for the join
-        int at = s_scan[tid];
+        int at = sum - own;
         for (int i = 0; i < per; ++i) {
             const int s = tid * per + i;
             if (s < p.b.n_seq) {
                 p.base[s] = at;
-                at += units_at(s).units * p.n_kv;
+                at += item_steps(units_at(s).units) * p.n_kv;
             }
         }
         if (tid == 0) p.base[p.b.n_seq] = total;
     }
     if (run >= n_runs) return;
-    const int lo = run_begin(run, n_runs, total), hi = run_begin(run + 1, n_runs, total);
+    const Runs runs(total, n_runs);
+    const int lo = runs.begin(run), hi = runs.begin(run + 1);
 
-    // ---- the sequence of the first unit, and from there on piece by piece
-    int at_seq, at_unit;                              // a sequence and its first unit
-    {
-        int t = 0;
-        for (int step = WGT / 2; step; step >>= 1)
-            if (t + step < WGT && s_scan[t + step] <= lo) t += step;
-        t = same(t);
-        at_seq = t * per;
-        at_unit = same(s_scan[t]);
+    // ---- the sequence of the first step, which one thread has counted, and from
+    // there on piece by piece
+    if (sum - own <= lo && lo < sum) {
+        int s = tid * per, at = sum - own;
+        SeqUnits v = units_at(s);
+        for (int n; lo - at >= (n = item_steps(v.units) * p.n_kv) && s + 1 < p.b.n_seq; v = units_at(++s)) at += n;
+        s_first.seq = s;
+        s_first.step = at;
+        s_first.su = v;
     }
+    __syncthreads();
+    int at_seq = same(s_first.seq), at_step = same(s_first.step);      // a sequence and its first step
+    SeqUnits at_su = uniform_units(s_first.su);
     struct Piece {
         SeqUnits su;
         int head, u0, n_u, key_begin, key_end;
         const int32_t * row;                          // of the page table
         uint64_t part;                                // a head's part of a page, which its scales follow
     };
-    SeqUnits at_su = uniform_units(units_at(at_seq));
-    int u = lo;
+    int step = lo;
     // the next piece with rows of this tile; false at the run's end (and where
     // another stream has changed the lengths meanwhile)
     auto next_piece = [&](Piece & c) {
-        while (u < hi) {
+        while (step < hi) {
             int n_here;
-            while (u - at_unit >= (n_here = at_su.units * p.n_kv)) {
+            while (step - at_step >= (n_here = item_steps(at_su.units) * p.n_kv)) {
                 if (at_seq + 1 >= p.b.n_seq) return false;
-                at_unit += n_here;
+                at_step += n_here;
                 ++at_seq;
                 at_su = uniform_units(units_at(at_seq));
             }
             if (tile * ROWS >= at_su.r.n * p.group) {
-                u = at_unit + n_here;                 // this sequence has fewer rows
+                step = at_step + n_here;              // this sequence has fewer rows
                 continue;
             }
+            const int steps = item_steps(at_su.units), head = (step - at_step) / steps, first = at_step + head * steps;
+            const int u0 = units_before(step - first), u1 = units_before(min(hi - first, steps));
+            step = min(hi, first + steps);
+            if (u1 <= u0) continue;
             c.su = at_su;
-            c.head = (u - at_unit) / at_su.units;
-            c.u0 = u - at_unit - c.head * at_su.units;
-            c.n_u = min(at_su.units - c.u0, hi - u);
-            c.key_begin = at_su.k0 + c.u0 * UNIT;
+            c.head = head;
+            c.u0 = u0;
+            c.n_u = u1 - u0;
+            c.key_begin = at_su.k0 + u0 * UNIT;
             c.key_end = min(c.key_begin + c.n_u * UNIT, at_su.kend);
             c.row = p.b.table + at_seq * p.b.table_stride;
-            c.part = (uint64_t)c.head * page * (Q8 ? HD + HD / 16 : 2 * HD);
-            u += c.n_u;
+            c.part = (uint64_t)head * page * (Q8 ? HD + HD / 16 : 2 * HD);
             return true;
         }
         return false;

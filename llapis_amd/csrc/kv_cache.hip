@@ -29,10 +29,10 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, f
     const int n_rows = min(su.r.n * p.group - tile * tile_rows, tile_rows);
     const int at = (blockIdx.y * TPG + e) * 4, r = at / head_dim, d = at - r * head_dim;
     if ((int)(blockIdx.y * TPG * 4) >= n_rows * head_dim) return;      // also: no such item
-    const int first = base + head * su.units;
-    const int64_t n_runs = min(p.runs, total);
-    const int w0 = (int)(((int64_t)(first + 1) * n_runs - 1) / total);
-    const int w1 = (int)(((int64_t)(first + su.units) * n_runs - 1) / total);
+    // the runs of the item's first and last unit
+    const Runs runs(total, runs_of(p.runs, total));
+    const int first = base + head * item_steps(su.units);
+    const int w0 = runs.owner(first + 1), w1 = runs.owner(first + 2 * su.units - 1);
     if (w0 == w1) return;                                              // written by k_kv_attn
     const bool live = r < n_rows;
     f4v a = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -469,7 +469,7 @@ const char * plan_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     const int unit = kv_unit(c->head_dim);
     const int64_t units = ((int64_t)b->max_pages * c->page_size + unit - 1) / unit + 1;
     const int64_t all = units * c->n_kv * b->n_seq;
-    if (all >= (int64_t)1 << 31) return "the batch has 2^31 units of work or more";
+    if (all >= (int64_t)1 << 29) return "the batch has 2^29 units of work or more";
     // as many workgroups as the card holds at once
     const int64_t most = std::max(256 * kv_wgs(c->head_dim, a.nt) / a.tiles, 8);
     a.runs = (int)((std::min(most, all) + 7) / 8 * 8);
