@@ -99,11 +99,12 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, f
 
 // -------------------------------------------------------------- append
 //
-// One workgroup for 32 consecutive positions (from a multiple of 32) of one
-// sequence and kv head.  K: a thread converts eight values of a row, written as
-// they lie.  V: a thread converts a column's eight consecutive positions, which
-// are one 16-byte store in the transposed page; at the ends of a run the
-// positions that the call brings are stored one by one.
+// Two workgroups, K's and V's, for 32 consecutive positions (from a multiple of
+// 32) of one sequence and kv head.  K: a thread converts eight values of a row,
+// written as they lie.  V: a thread converts a column's eight consecutive
+// positions, which are one 16-byte store in the transposed page; at the ends of a
+// run the positions that the call brings are stored one by one.  A thread asks for
+// all its values before it converts the first.
 constexpr int APP_POS = 32;
 
 struct KvAppend {
@@ -131,10 +132,11 @@ __device__ __forceinline__ Q8Scale q8_scale(float amax) {
 }
 __device__ __forceinline__ int q8_value(float x, float id) { return (int)__builtin_rintf(x * id) & 0xFF; }
 
-template <int CT>
+// HDT: the head size, 0 for one that is not a multiple of 64
+template <int CT, int HDT>
 __global__ __launch_bounds__(256) void k_kv_append(const KvAppend p) {
     constexpr int EL = CT == KV_Q8 ? 1 : 2;
-    const int seq = blockIdx.x, head = blockIdx.z, tid = threadIdx.x;
+    const int seq = blockIdx.x, head = blockIdx.z >> 1, tid = threadIdx.x;
     const SeqRows r = seq_rows(p.b, seq);
     const int p0 = r.len - r.n;                                   // may be negative: such tokens have no place
     const int cap = p.b.max_pages << p.page_shift;
@@ -142,90 +144,126 @@ __global__ __launch_bounds__(256) void k_kv_append(const KvAppend p) {
     const int base = (max(p0, 0) & ~(APP_POS - 1)) + APP_POS * blockIdx.y;
     const int from = max(p0, base), to = min(min(r.len, base + APP_POS), cap);
     if (from >= to) return;
-    const int HD = p.head_dim, page = 1 << p.page_shift, mask = page - 1;
+    const int HD = HDT ? HDT : p.head_dim, page = 1 << p.page_shift, mask = page - 1;
     const int32_t * row = p.b.table + seq * p.b.table_stride;
     const uint64_t part = (uint64_t)head * page * (CT == KV_Q8 ? HD + HD / 16 : 2 * HD);
-    const int chunks = HD / 8;
-    // K: (position, eight values)
-    for (int i = tid; i < APP_POS * chunks; i += 256) {
-        const int at = base + i / chunks, c = i % chunks;
-        const bool live = at >= from && at < to;
-        const int pg = live ? row[at >> p.page_shift] : -1;
-        const bool there = (uint32_t)pg < (uint32_t)p.n_pages;
-        float x[8] = {};
-        if (there) load8(p.xk, p.x_type, (int64_t)(r.row0 + at - p0) * p.xk_stride + head * HD + 8 * c, x);
-        uint8_t * dst = p.k + (uint64_t)(there ? pg : 0) * p.k_stride + part;
-        if constexpr (CT == KV_Q8) {
-            float amax = 0.0f;
+    const int items = APP_POS / 8 * HD;                           // of eight values
+    constexpr int UN = HDT ? (HDT / 64 < 4 ? HDT / 64 : 4) : 1;   // of a thread at a time
+    if (blockIdx.z & 1) {
+        // V: (eight positions, column)
+        for (int i0 = tid; i0 < items; i0 += 256 * UN) {
+            float x[UN][8];
+            int pg[UN];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
-            amax = fmaxf(amax, __shfl_xor(amax, 1, 64));          // four threads hold a block of 32
-            amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
-            if (there) {
-                const Q8Scale s = q8_scale(amax);
-                u2 w = {0, 0};
+            for (int e = 0; e < UN; ++e) {
+                const int i = i0 + 256 * e, oct = base + 8 * (i / HD), c = i % HD;
+                const int lo = max(from, oct), hi = min(to, oct + 8);
+                pg[e] = lo < hi ? row[oct >> p.page_shift] : -1;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)q8_value(x[j], s.id) << (8 * (j & 3));
-                *(u2 *)(dst + (at & mask) * HD + 8 * c) = w;
-                if (c % 4 == 0) *(uint16_t *)(dst + page * HD + ((c / 4) * page + (at & mask)) * 2) = s.d;
+                for (int j = 0; j < 8; ++j)
+                    x[e][j] = oct + j >= lo && oct + j < hi
+                                  ? load1(p.xv, p.x_type, (int64_t)(r.row0 + oct + j - p0) * p.xv_stride + head * HD + c) : 0.0f;
             }
-        } else if (there) {
-            u4 w[1];
-            split8<CT == KV_F16, 1>(x, w);
-            *(u4 *)(dst + ((at & mask) * HD + 8 * c) * EL) = w[0];
+#pragma unroll
+            for (int e = 0; e < UN; ++e) {
+                const int i = i0 + 256 * e, oct = base + 8 * (i / HD), c = i % HD;
+                const int lo = max(from, oct), hi = min(to, oct + 8);
+                if ((uint32_t)pg[e] >= (uint32_t)p.n_pages) continue;         // the same in the 32 threads of a block of columns
+                uint8_t * dst = p.v + (uint64_t)pg[e] * p.v_stride + part;
+                uint8_t * at = dst + (c * page + (oct & mask)) * EL;
+                if constexpr (CT == KV_Q8) {
+                    u2 w = {0, 0};
+                    uint16_t d[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float amax = fabsf(x[e][j]);
+#pragma unroll
+                        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+                        const Q8Scale s = q8_scale(amax);
+                        w[j >> 2] |= (uint32_t)q8_value(x[e][j], s.id) << (8 * (j & 3));
+                        d[j] = s.d;
+                    }
+                    uint16_t * sc = (uint16_t *)(dst + page * HD) + (c / 32) * page + (oct & mask);
+                    if (hi - lo == 8) {
+                        *(u2 *)at = w;
+                        if (c % 32 == 0)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) sc[j] = d[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (oct + j >= lo && oct + j < hi) {
+                                at[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+                                if (c % 32 == 0) sc[j] = d[j];
+                            }
+                    }
+                } else {
+                    u4 w[1];
+                    split8<CT == KV_F16, 1>(x[e], w);
+                    if (hi - lo == 8) {
+                        *(u4 *)at = w[0];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (oct + j >= lo && oct + j < hi) ((uint16_t *)at)[j] = (uint16_t)(w[0][j >> 1] >> (16 * (j & 1)));
+                    }
+                }
+            }
+        }
+        return;
+    }
+    // K: (position, eight values)
+    const int chunks = HD / 8;
+    for (int i0 = tid; i0 < items; i0 += 256 * UN) {
+        float x[UN][8];
+        int pg[UN];
+#pragma unroll
+        for (int e = 0; e < UN; ++e) {
+            const int i = i0 + 256 * e, at = base + i / chunks, c = i % chunks;
+            const bool live = at >= from && at < to;
+            pg[e] = live ? row[at >> p.page_shift] : -1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[e][j] = 0.0f;
+            if (live) load8(p.xk, p.x_type, (int64_t)(r.row0 + at - p0) * p.xk_stride + head * HD + 8 * c, x[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < UN; ++e) {
+            const int i = i0 + 256 * e, at = base + i / chunks, c = i % chunks;
+            const bool there = (uint32_t)pg[e] < (uint32_t)p.n_pages;
+            uint8_t * dst = p.k + (uint64_t)(there ? pg[e] : 0) * p.k_stride + part;
+            if constexpr (CT == KV_Q8) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[e][j]));
+                amax = fmaxf(amax, __shfl_xor(amax, 1, 64));      // four threads hold a block of 32
+                amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
+                if (there) {
+                    const Q8Scale s = q8_scale(amax);
+                    u2 w = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)q8_value(x[e][j], s.id) << (8 * (j & 3));
+                    *(u2 *)(dst + (at & mask) * HD + 8 * c) = w;
+                    if (c % 4 == 0) *(uint16_t *)(dst + page * HD + ((c / 4) * page + (at & mask)) * 2) = s.d;
+                }
+            } else if (there) {
+                u4 w[1];
+                split8<CT == KV_F16, 1>(x[e], w);
+                *(u4 *)(dst + ((at & mask) * HD + 8 * c) * EL) = w[0];
+            }
         }
     }
-    // V: (eight positions, column)
-    for (int i = tid; i < APP_POS / 8 * HD; i += 256) {
-        const int oct = base + 8 * (i / HD), c = i % HD;
-        const int lo = max(from, oct), hi = min(to, oct + 8);
-        if (lo >= hi) continue;                                   // the same in the 32 threads of a block of columns
-        const int pg = row[oct >> p.page_shift];
-        if ((uint32_t)pg >= (uint32_t)p.n_pages) continue;
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            x[j] = oct + j >= lo && oct + j < hi
-                       ? load1(p.xv, p.x_type, (int64_t)(r.row0 + oct + j - p0) * p.xv_stride + head * HD + c) : 0.0f;
-        uint8_t * dst = p.v + (uint64_t)pg * p.v_stride + part;
-        uint8_t * at = dst + (c * page + (oct & mask)) * EL;
-        if constexpr (CT == KV_Q8) {
-            u2 w = {0, 0};
-            uint16_t d[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float amax = fabsf(x[j]);
-#pragma unroll
-                for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-                const Q8Scale s = q8_scale(amax);
-                w[j >> 2] |= (uint32_t)q8_value(x[j], s.id) << (8 * (j & 3));
-                d[j] = s.d;
-            }
-            uint16_t * sc = (uint16_t *)(dst + page * HD) + (c / 32) * page + (oct & mask);
-            if (hi - lo == 8) {
-                *(u2 *)at = w;
-                if (c % 32 == 0)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sc[j] = d[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (oct + j >= lo && oct + j < hi) {
-                        at[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-                        if (c % 32 == 0) sc[j] = d[j];
-                    }
-            }
-        } else {
-            u4 w[1];
-            split8<CT == KV_F16, 1>(x, w);
-            if (hi - lo == 8) {
-                *(u4 *)at = w[0];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (oct + j >= lo && oct + j < hi) ((uint16_t *)at)[j] = (uint16_t)(w[0][j >> 1] >> (16 * (j & 1)));
-            }
-        }
+}
+
+template <int CT>
+void launch_append(const KvAppend & p, dim3 grid, hipStream_t s) {
+    const dim3 wg(256);
+    switch (p.head_dim) {
+        case 64: hipLaunchKernelGGL((k_kv_append<CT, 64>), grid, wg, 0, s, p); break;
+        case 128: hipLaunchKernelGGL((k_kv_append<CT, 128>), grid, wg, 0, s, p); break;
+        case 192: hipLaunchKernelGGL((k_kv_append<CT, 192>), grid, wg, 0, s, p); break;
+        case 256: hipLaunchKernelGGL((k_kv_append<CT, 256>), grid, wg, 0, s, p); break;
+        case 512: hipLaunchKernelGGL((k_kv_append<CT, 512>), grid, wg, 0, s, p); break;
+        default: hipLaunchKernelGGL((k_kv_append<CT, 0>), grid, wg, 0, s, p);
     }
 }
 
@@ -347,9 +385,8 @@ __global__ __launch_bounds__(SCAN_WG) void k_kv_free(const int32_t * refs, int n
 
 // The moves of a compaction: place[p] = where page p goes (-1: nowhere), the
 // pairs (from, to), and their number.
-__global__ __launch_bounds__(SCAN_WG) void k_kv_plan(const int32_t * refs, int n_pages, int32_t * place, int32_t * from,
-                                                     int32_t * to, int32_t * n_moves, int32_t * n_live, int32_t * refs_out) {
-    __shared__ int s_part[SCAN_WG / 64];
+__device__ __forceinline__ void plan_moves(const int * refs, int n_pages, int32_t * place, int32_t * from, int32_t * to,
+                                           int32_t * n_moves, int32_t * n_live, int32_t * refs_out, int * s_part) {
     int live = 0, total;
     for (int p0 = threadIdx.x; p0 < n_pages; p0 += SCAN_WG) live += refs[p0] > 0;
     (void)block_scan(live, s_part, total);
@@ -379,6 +416,45 @@ __global__ __launch_bounds__(SCAN_WG) void k_kv_plan(const int32_t * refs, int n
     if (threadIdx.x == 0) {
         *n_moves = n_from;
         *n_live = live;
+    }
+}
+
+__global__ __launch_bounds__(SCAN_WG) void k_kv_plan(const int32_t * refs, int n_pages, int32_t * place, int32_t * from,
+                                                     int32_t * to, int32_t * n_moves, int32_t * n_live, int32_t * refs_out) {
+    __shared__ int s_part[SCAN_WG / 64];
+    plan_moves(refs, n_pages, place, from, to, n_moves, n_live, refs_out, s_part);
+}
+
+// All of the above for a pool and a table that one workgroup goes through in the
+// time of a few launches: the counts are in LDS.
+constexpr int SMALL_PAGES = 8192, SMALL_ENTRIES = 65536;
+
+__global__ __launch_bounds__(SCAN_WG) void k_kv_plan_small(const int32_t * table, int64_t table_stride, int max_pages,
+                                                           const int32_t * lens, int n_seq, int page_size, int n_pages,
+                                                           int32_t * place, int32_t * from, int32_t * to, int32_t * n_moves,
+                                                           int32_t * n_live, int32_t * refs_out, int32_t * table_out) {
+    __shared__ int s_part[SCAN_WG / 64];
+    __shared__ int s_refs[SMALL_PAGES];
+    for (int i = threadIdx.x; i < n_pages; i += SCAN_WG) s_refs[i] = 0;
+    __syncthreads();
+    // a wave a row at a time
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int seq = wave; seq < n_seq; seq += SCAN_WG / 64) {
+        const int n = held_pages(lens[seq], page_size, max_pages);
+        for (int i = lane; i < n; i += 64) {
+            const int pg = table[seq * table_stride + i];
+            if (in_pool(pg, n_pages)) atomicAdd(&s_refs[pg], 1);
+        }
+    }
+    __syncthreads();
+    plan_moves(s_refs, n_pages, place, from, to, n_moves, n_live, refs_out, s_part);
+    __syncthreads();
+    for (int seq = wave; seq < n_seq; seq += SCAN_WG / 64) {
+        const int n = held_pages(lens[seq], page_size, max_pages);
+        for (int i = lane; i < max_pages; i += 64) {
+            const int pg = i < n ? table[seq * table_stride + i] : -1;
+            table_out[seq * table_stride + i] = in_pool(pg, n_pages) ? place[pg] : -1;
+        }
     }
 }
 
@@ -551,11 +627,11 @@ int32_t llapis_kv_append(const llapis_kv_cache * c, const llapis_kv_batch * b, i
     if (tiles > 65535) return refuse_as(who, "more than 65535 * 32 new tokens of a sequence");
     KvAppend p{q, (uint8_t *)c->k, (uint8_t *)c->v, c->k_stride, c->v_stride, c->n_pages, log2_of(c->page_size), c->n_kv,
                c->head_dim, x_type, k, v, k_stride, v_stride};
-    const dim3 grid(q.n_seq, (unsigned)tiles, c->n_kv);
+    const dim3 grid(q.n_seq, (unsigned)tiles, 2 * c->n_kv);
     hipStream_t s = (hipStream_t)stream;
-    if (c->type == T_F16) hipLaunchKernelGGL(k_kv_append<KV_F16>, grid, dim3(256), 0, s, p);
-    else if (c->type == T_BF16) hipLaunchKernelGGL(k_kv_append<KV_BF16>, grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL(k_kv_append<KV_Q8>, grid, dim3(256), 0, s, p);
+    if (c->type == T_F16) launch_append<KV_F16>(p, grid, s);
+    else if (c->type == T_BF16) launch_append<KV_BF16>(p, grid, s);
+    else launch_append<KV_Q8>(p, grid, s);
     KV_TRY(hipGetLastError());
     return 0;
 }
@@ -692,12 +768,18 @@ int32_t llapis_kv_compact(const llapis_kv_planes * p, const int32_t * page_table
     const int n = p->n_pages;
     int32_t * counts = (int32_t *)workspace, * place = counts + n, * from = place + n, * to = from + n, * n_moves = to + n;
     hipStream_t s = (hipStream_t)stream;
-    KV_TRY(launch_refs(page_table, table_stride, max_pages, lens, n_seq, p->page_size, n, counts, s));
-    hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(SCAN_WG), 0, s, counts, n, place, from, to, n_moves, n_live, refs);
+    if (n <= SMALL_PAGES && (int64_t)n_seq * max_pages <= SMALL_ENTRIES) {
+        hipLaunchKernelGGL(k_kv_plan_small, dim3(1), dim3(SCAN_WG), 0, s, page_table, table_stride, max_pages, lens, n_seq,
+                           p->page_size, n, place, from, to, n_moves, n_live, refs, table_out);
+    } else {
+        KV_TRY(launch_refs(page_table, table_stride, max_pages, lens, n_seq, p->page_size, n, counts, s));
+        hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(SCAN_WG), 0, s, counts, n, place, from, to, n_moves, n_live, refs);
+        KV_TRY(hipGetLastError());
+        if (n_seq > 0)
+            hipLaunchKernelGGL(k_kv_remap, table_grid(n_seq, max_pages), dim3(256), 0, s, page_table, table_stride, max_pages,
+                               lens, p->page_size, n, place, table_out);
+    }
     KV_TRY(hipGetLastError());
-    if (n_seq > 0)
-        hipLaunchKernelGGL(k_kv_remap, table_grid(n_seq, max_pages), dim3(256), 0, s, page_table, table_stride, max_pages, lens,
-                           p->page_size, n, place, table_out);
     // at most half of the pool moves
     const int64_t all = (int64_t)(n / 2) * p->n_planes * chunks;
     if (all > 0)

@@ -12,19 +12,25 @@ namespace dev {
 typedef float f4 __attribute__((ext_vector_type(4)));
 template <class T> struct Four { typedef T v __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
 
+// values i .. i + 3 of a row of n, zeros past its end
 template <class T>
-__device__ __forceinline__ f4 get4(const T * p, int i, int n) {
-    f4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ typename Four<T>::v raw4(const T * p, int i, int n) {
+    typename Four<T>::v r = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
     if (i + 4 <= n) {
-        const typename Four<T>::v w = *(const typename Four<T>::v *)(p + i);
-        r = f4{(float)w[0], (float)w[1], (float)w[2], (float)w[3]};
+        r = *(const typename Four<T>::v *)(p + i);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (i + j < n) r[j] = (float)p[i + j];
+            if (i + j < n) r[j] = p[i + j];
     }
     return r;
 }
+
+template <class T>
+__device__ __forceinline__ f4 wide4(typename Four<T>::v w) { return f4{(float)w[0], (float)w[1], (float)w[2], (float)w[3]}; }
+
+template <class T>
+__device__ __forceinline__ f4 get4(const T * p, int i, int n) { return wide4<T>(raw4(p, i, n)); }
 
 template <class T>
 __device__ __forceinline__ void put4(T * p, int i, int n, f4 x) {
@@ -42,9 +48,11 @@ __device__ __forceinline__ void put4(T * p, int i, int n, f4 x) {
 
 // --------------------------------------------------------------- norms
 //
-// One workgroup a token.  Every load is issued before the first sum; a thread
-// holds 4 NCH values, which are read and written once.  The squares are summed
-// per thread in order, then over the wave, then over the waves in order.
+// A workgroup takes tokens blockIdx, blockIdx + grid, ...; a thread holds 4 NCH
+// values of a token, which are read and written once, and its share of the
+// weights, which it reads once for all its tokens.  The next token's values are
+// asked for before this one's sums.  The squares are summed per thread in order,
+// then over the wave, then over the waves in order.
 
 __device__ __forceinline__ float block_sum(float x, float * s_part) {
     for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, 64);
@@ -56,81 +64,109 @@ __device__ __forceinline__ float block_sum(float x, float * s_part) {
     return s;
 }
 
-template <class T, int NCH>
-__global__ __launch_bounds__(1024) void k_block_norm(const llapis_block_norm_args a) {
-    __shared__ float s_part[2][16];
-    const int d = a.d, n = blockDim.x;
-    const int64_t t = blockIdx.x;
-    const T * hp = (const T *)a.h + t * a.h_stride;
-    f4 h[NCH], u[NCH];
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) h[c] = get4(hp, 4 * (threadIdx.x + c * n), d);
-    if (a.y) {
-        const T * yp = (const T *)a.y + t * a.y_stride;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) u[c] = get4(yp, 4 * (threadIdx.x + c * n), d);
-        if (a.post_norm) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NCH; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(u[c][j], u[c][j], ss);
-            const float inv = 1.0f / __fsqrt_rn(block_sum(ss, s_part[0]) / (float)d + a.eps);
-#pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                u[c] *= inv;
-                if (a.post_weight) u[c] *= get4(a.post_weight, 4 * (threadIdx.x + c * n), d);
-            }
-        }
-        if (a.gate) {
-            const T * gp = (const T *)a.gate + t * a.gate_token_stride;
-            const float g = a.gate_value_stride ? 0.0f : (float)gp[0];
-#pragma unroll
-            for (int c = 0; c < NCH; ++c)
-                u[c] *= a.gate_value_stride ? get4(gp, 4 * (threadIdx.x + c * n), d) : f4{g, g, g, g};
-        }
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) h[c] = a.alpha * h[c] + a.beta * u[c];
-    } else {
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) h[c] = a.alpha * h[c];
-    }
-    if (a.h_out) {
-        T * op = (T *)a.h_out + t * a.h_out_stride;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) put4(op, 4 * (threadIdx.x + c * n), d, h[c]);
-    }
-    if (a.n_out == 0) return;
+template <int NCH>
+__device__ __forceinline__ float squares(const f4 (&x)[NCH]) {
     float ss = 0.0f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(h[c][j], h[c][j], ss);
-    const float inv = 1.0f / __fsqrt_rn(block_sum(ss, s_part[1]) / (float)d + a.eps);
+        for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(x[c][j], x[c][j], ss);
+    return ss;
+}
+
+// a token's values, as they lie until they are used
+template <class T, int NCH>
+struct NormRow {
+    typename Four<T>::v h[NCH], y[NCH], g[NCH];
+    float g1;
+    __device__ __forceinline__ void load(const llapis_block_norm_args & a, int64_t t) {
+        const int n = blockDim.x;
 #pragma unroll
-    for (int o = 0; o < LLAPIS_NORM_MAX_OUT; ++o)
-        if (o < a.n_out) {
-            T * xp = (T *)a.x[o] + t * a.x_stride[o];
+        for (int c = 0; c < NCH; ++c) h[c] = raw4((const T *)a.h + t * a.h_stride, 4 * (threadIdx.x + c * n), a.d);
+        if (!a.y) return;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                const int i = 4 * (threadIdx.x + c * n);
-                f4 x = h[c] * inv;
-                if (a.weight[o]) x *= get4(a.weight[o], i, d);
-                put4(xp, i, d, x);
-            }
+        for (int c = 0; c < NCH; ++c) y[c] = raw4((const T *)a.y + t * a.y_stride, 4 * (threadIdx.x + c * n), a.d);
+        if (!a.gate) return;
+        const T * gp = (const T *)a.gate + t * a.gate_token_stride;
+        if (a.gate_value_stride) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) g[c] = raw4(gp, 4 * (threadIdx.x + c * n), a.d);
+        } else {
+            g1 = (float)gp[0];
         }
+    }
+};
+
+// NO: outputs that weights are held for, n_out at most
+template <class T, int NCH, int NO, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_block_norm(const llapis_block_norm_args a) {
+    __shared__ float s_part[2][2][16];
+    const int d = a.d, n = blockDim.x;
+    NormRow<T, NCH> row, next;
+    row.load(a, blockIdx.x);
+    // (4096 threads' worth of values and weights is more than the registers
+    // hold: the weights are then read where they are used)
+    constexpr bool HOLD = THREADS * NCH <= 2048;
+    const float * wp = a.y && a.post_norm ? a.post_weight : nullptr;
+    auto weight = [&](const float * w, int c) { return w ? get4(w, 4 * (threadIdx.x + c * n), d) : f4{1.0f, 1.0f, 1.0f, 1.0f}; };
+    f4 w_post[HOLD ? NCH : 1], w_pre[NO][HOLD ? NCH : 1];
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) w_post[c] = weight(wp, c);
+#pragma unroll
+        for (int o = 0; o < NO; ++o)
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) w_pre[o][c] = weight(o < a.n_out ? a.weight[o] : nullptr, c);
+    }
+    int turn = 0;                                       // the sums' places are used in turn: one barrier a sum
+    for (int64_t t = blockIdx.x; t < a.n_tokens; t += gridDim.x, turn ^= 1) {
+        const bool more = t + gridDim.x < a.n_tokens;
+        if (HOLD && more) next.load(a, t + gridDim.x);
+        f4 h[NCH];
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) h[c] = a.alpha * wide4<T>(row.h[c]);
+        if (a.y) {
+            f4 u[NCH];
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) u[c] = wide4<T>(row.y[c]);
+            if (a.post_norm) {
+                const float inv = 1.0f / __fsqrt_rn(block_sum(squares<NCH>(u), s_part[turn][0]) / (float)d + a.eps);
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) u[c] = u[c] * inv * (HOLD ? w_post[HOLD ? c : 0] : weight(wp, c));
+            }
+            if (a.gate)
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) u[c] *= a.gate_value_stride ? wide4<T>(row.g[c]) : f4{row.g1, row.g1, row.g1, row.g1};
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) h[c] += a.beta * u[c];
+        }
+        if (a.h_out)
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) put4((T *)a.h_out + t * a.h_out_stride, 4 * (threadIdx.x + c * n), d, h[c]);
+        if (a.n_out > 0) {
+            const float inv = 1.0f / __fsqrt_rn(block_sum(squares<NCH>(h), s_part[turn][1]) / (float)d + a.eps);
+#pragma unroll
+            for (int o = 0; o < NO; ++o)
+                if (o < a.n_out)
+#pragma unroll
+                    for (int c = 0; c < NCH; ++c)
+                        put4((T *)a.x[o] + t * a.x_stride[o], 4 * (threadIdx.x + c * n), d, h[c] * inv * (HOLD ? w_pre[o][HOLD ? c : 0] : weight(a.weight[o], c)));
+        }
+        if (HOLD && more) row = next;
+        if (!HOLD && more) row.load(a, t + gridDim.x);
+    }
 }
 
 // -------------------------------------------------------- verification
 //
 // k_verify_sum: every workgroup finds the number of taken drafts anew (a few
-// loads) and sums a run of VER_RUN values of the row the next token comes from,
-// r and, for drafts that all were refused to no rest, p.  k_verify_pick: one
-// workgroup a sequence adds the runs in order, finds the run where the sum
-// passes u_next of the whole, and in it the token.
+// loads) and sums 8 segments of 1024 values of the row the next token comes from:
+// r, and p for the case that r is 0 everywhere.  k_verify_pick: one workgroup a
+// sequence adds the segments in order, finds the one where the sum passes u_next
+// of the whole, and in it the token.
 
-constexpr int VER_PER = 32;                     // consecutive values of a thread
-constexpr int VER_RUN = 256 * VER_PER;
+constexpr int VER_SEG = 1024;                   // values of a segment: 16 a lane, four a thread of the pick
+constexpr int VER_RUN = 8 * VER_SEG;            // values of a workgroup, two segments a wave
 
 template <class T>
 __device__ __forceinline__ double prob(const T * p, int64_t i) {
@@ -138,25 +174,28 @@ __device__ __forceinline__ double prob(const T * p, int64_t i) {
     return x > 0.0f && x < __builtin_inff() ? (double)x : 0.0;
 }
 
-struct Verdict { int a, n, draft; };            // taken, drafted, the refused draft (or -1)
+// taken, whether one was refused, and it; from the first kernel to the second
+struct Verdict { int a, refused, draft, pad; };
 
 template <class T>
 __device__ __forceinline__ Verdict verdict(const llapis_verify_args & v, int seq) {
     const int lane = threadIdx.x & 63;
     const int n = v.n_draft ? min(max(v.n_draft[seq], 0), v.max_draft) : v.max_draft;
     bool ok = false;
-    if (lane < n) {
+    int x = -1;
+    if (lane < v.max_draft) {
         const int64_t i = (int64_t)seq * v.max_draft + lane;
-        const int x = v.drafts[i];
-        if (x >= 0 && x < v.vocab) {
+        x = v.drafts[i];
+        const float u = v.u[i];
+        if (lane < n && x >= 0 && x < v.vocab) {
             const double p = prob((const T *)v.target + ((int64_t)seq * (v.max_draft + 1) + lane) * v.target_stride, x);
             const double q = v.draft ? prob((const T *)v.draft + i * v.draft_stride, x) : 1.0;
-            ok = (double)v.u[i] * q < p;
+            ok = (double)u * q < p;
         }
     }
     const uint64_t no = ~__ballot(ok);
     const int a = min(no ? (int)__builtin_ctzll(no) : 64, n);
-    return {a, n, a < n ? v.drafts[(int64_t)seq * v.max_draft + a] : -1};
+    return {a, a < n, a < n ? __shfl(x, a, 64) : -1, 0};
 }
 
 // the row the next token comes from, and what is taken off it
@@ -167,10 +206,10 @@ struct Row {
     int draft;                                  // without q: the place that 1 is taken off
     __device__ __forceinline__ Row(const llapis_verify_args & v, int seq, const Verdict & w) {
         p = (const T *)v.target + ((int64_t)seq * (v.max_draft + 1) + w.a) * v.target_stride;
-        q = w.a < w.n && v.draft ? (const T *)v.draft + ((int64_t)seq * v.max_draft + w.a) * v.draft_stride : nullptr;
-        draft = w.a < w.n && !v.draft ? w.draft : -1;
+        q = w.refused && v.draft ? (const T *)v.draft + ((int64_t)seq * v.max_draft + w.a) * v.draft_stride : nullptr;
+        draft = w.refused && !v.draft ? w.draft : -1;
     }
-    // VER_PER / 8 or fewer values from i on: r, and p
+    // four values from i on: r, and p
     __device__ __forceinline__ void four(int i, int n, double (&r)[4], double (&whole)[4]) const {
         const f4 x = get4(p, i, n);
         const f4 y = q ? get4(q, i, n) : f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -184,144 +223,144 @@ struct Row {
     }
 };
 
-__device__ __forceinline__ double wave_sum(double x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
-}
+struct Sums { double r, p; };
+
+// segments of a sequence, a whole number of workgroups
+__host__ __device__ __forceinline__ int verify_segments(int vocab) { return (vocab + VER_RUN - 1) / VER_RUN * 8; }
 
 template <class T>
-__global__ __launch_bounds__(256) void k_verify_sum(const llapis_verify_args v, double * sums) {
-    __shared__ double s_part[4][2];
+__global__ __launch_bounds__(256) void k_verify_sum(const llapis_verify_args v, Sums * sums, Verdict * verdicts) {
     const int seq = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Row<T> row(v, seq, verdict<T>(v, seq));
-    const int at = blockIdx.x * VER_RUN;
-    double s = 0.0, w = 0.0;
-#pragma unroll
-    for (int c = 0; c < VER_PER / 4; ++c) {
-        double r[4], p[4];
-        row.four(at + 4 * (threadIdx.x + 256 * c), v.vocab, r, p);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s += r[j];
-            w += p[j];
-        }
-    }
-    s = wave_sum(s);
-    w = wave_sum(w);
-    if (lane == 0) {
-        s_part[wave][0] = s;
-        s_part[wave][1] = w;
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const int k = threadIdx.x;
-        sums[((int64_t)seq * gridDim.x + blockIdx.x) * 2 + k] =
-            (s_part[0][k] + s_part[1][k]) + (s_part[2][k] + s_part[3][k]);
-    }
-}
-
-// exclusive sum over the workgroup's 256 threads in order, and the whole
-__device__ __forceinline__ double scan256(double x, double * s_part, double & total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double v = x;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    __syncthreads();
-    if (lane == 63) s_part[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-    total = 0.0;
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += s_part[w];
-        total += s_part[w];
-    }
-    const double prev = __shfl_up(v, 1, 64);
-    return before + (lane ? prev : 0.0);
-}
-
-template <class T>
-__global__ __launch_bounds__(256) void k_verify_pick(const llapis_verify_args v, const double * sums, int n_runs) {
-    __shared__ double s_part[4];
-    __shared__ int s_run, s_tok, s_last;
-    __shared__ double s_before;
-    const int seq = blockIdx.x, tid = threadIdx.x;
     const Verdict w = verdict<T>(v, seq);
     const Row<T> row(v, seq, w);
-    const double * mine = sums + (int64_t)seq * n_runs * 2;
-    // the sum of r, or of p where r is 0
-    double part[2] = {0.0, 0.0};
-    for (int i = tid; i < n_runs; i += 256) {
-        part[0] += mine[2 * i];
-        part[1] += mine[2 * i + 1];
-    }
-    double rest, whole;
-    (void)scan256(part[0], s_part, rest);
-    (void)scan256(part[1], s_part, whole);
-    const int k = rest > 0.0 && w.a < w.n ? 0 : 1;
-    const double goal = (double)v.u_next[seq] * (k ? whole : rest);
-    if (tid == 0) {
-        s_run = -1;
-        s_tok = s_last = -1;
-        s_before = 0.0;
-    }
-    __syncthreads();
-    // the run in which the sum passes the goal; without one (rounding, u_next
-    // of 1 and more) the last run that has anything
-    double before = 0.0;
-    for (int i0 = 0; i0 < n_runs; i0 += 256) {
-        const double x = i0 + tid < n_runs ? mine[2 * (i0 + tid) + k] : 0.0;
-        double all;
-        const double at = before + scan256(x, s_part, all);
-        const bool passes = x > 0.0 && at + x > goal;
-        const int here = passes ? i0 + tid : 0x7FFFFFFF;
-        // first passing run of the workgroup, last one with a positive sum
-        if (x > 0.0) atomicMax(&s_last, i0 + tid);
-        __syncthreads();
-        if (passes) atomicMin((unsigned int *)&s_run, (unsigned int)here);      // -1 is the largest unsigned
-        __syncthreads();
-        if (s_run == i0 + tid || (s_run < 0 && s_last == i0 + tid)) s_before = at;
-        before += all;
-        __syncthreads();
-        if (s_run >= 0) break;
-    }
-    const bool found = s_run >= 0;
-    const int run = found ? s_run : s_last;
-    __syncthreads();
-    if (run >= 0) {
-        if (tid == 0) s_last = -1;
-        const int at = run * VER_RUN + tid * VER_PER;
-        double x[VER_PER], sum = 0.0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) verdicts[seq] = w;
+    Sums s[2] = {{0.0, 0.0}, {0.0, 0.0}};
 #pragma unroll
-        for (int c = 0; c < VER_PER / 4; ++c) {
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
             double r[4], p[4];
-            row.four(at + 4 * c, v.vocab, r, p);
+            row.four(blockIdx.x * VER_RUN + (2 * wave + g) * VER_SEG + 256 * c + 4 * lane, v.vocab, r, p);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                x[4 * c + j] = k ? p[j] : r[j];
-                sum += x[4 * c + j];
+                s[g].r += r[j];
+                s[g].p += p[j];
             }
         }
-        double all;
-        double cum = s_before + scan256(sum, s_part, all);
-        int tok = 0x7FFFFFFF, last = -1;
+    for (int o = 32; o; o >>= 1)
 #pragma unroll
-        for (int j = 0; j < VER_PER; ++j) {
-            cum += x[j];
-            if (x[j] > 0.0) {
-                last = at + j;
-                if (found && cum > goal && tok == 0x7FFFFFFF) tok = at + j;
-            }
+        for (int g = 0; g < 2; ++g) {
+            s[g].r += __shfl_xor(s[g].r, o, 64);
+            s[g].p += __shfl_xor(s[g].p, o, 64);
         }
-        if (last >= 0) atomicMax(&s_last, last);
-        if (tok != 0x7FFFFFFF) atomicMin((unsigned int *)&s_tok, (unsigned int)tok);
+    if (lane < 2) sums[(int64_t)seq * (8 * gridDim.x) + blockIdx.x * 8 + 2 * wave + lane] = lane ? s[1] : s[0];
+}
+
+// exclusive sums over the workgroup's 256 threads in order, and the whole
+__device__ __forceinline__ Sums scan256(Sums x, Sums * s_part, Sums & total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Sums v = x;
+    for (int o = 1; o < 64; o <<= 1) {
+        const double r = __shfl_up(v.r, o, 64), p = __shfl_up(v.p, o, 64);
+        if (lane >= o) {
+            v.r += r;
+            v.p += p;
+        }
+    }
+    if (lane == 63) s_part[wave] = v;
+    __syncthreads();
+    Sums before = {0.0, 0.0};
+    total = {0.0, 0.0};
+    for (int w = 0; w < 4; ++w) {
+        const Sums y = s_part[w];
+        if (w < wave) {
+            before.r += y.r;
+            before.p += y.p;
+        }
+        total.r += y.r;
+        total.p += y.p;
+    }
+    const double r = __shfl_up(v.r, 1, 64), p = __shfl_up(v.p, 1, 64);
+    return {before.r + (lane ? r : 0.0), before.p + (lane ? p : 0.0)};
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void k_verify_pick(const llapis_verify_args v, const Sums * sums, const Verdict * verdicts) {
+    __shared__ Sums s_part[2][4];
+    __shared__ unsigned int s_first, s_tok;               // the smallest found
+    __shared__ int s_last, s_last_tok;                    // the largest with anything
+    __shared__ int s_seg;
+    __shared__ double s_before;
+    const int seq = blockIdx.x, tid = threadIdx.x;
+    const int n_seg = verify_segments(v.vocab), per = (n_seg + 255) / 256;
+    const Verdict w = verdicts[seq];
+    const float u = v.u_next[seq];
+    const Sums * mine = sums + (int64_t)seq * n_seg;
+    const int drafted = tid < w.a ? v.drafts[(int64_t)seq * v.max_draft + tid] : -1;
+    if (tid == 0) {
+        s_first = s_tok = 0xFFFFFFFFu;
+        s_last = s_last_tok = -1;
+        s_seg = -1;
+    }
+    // a thread's segments are consecutive
+    Sums x = {0.0, 0.0}, total;
+    for (int i = tid * per; i < min((tid + 1) * per, n_seg); ++i) {
+        x.r += mine[i].r;
+        x.p += mine[i].p;
+    }
+    const Sums before = scan256(x, s_part[0], total);     // its barrier: the places above are set
+    const bool rest = w.refused && total.r > 0.0;
+    const double goal = (double)u * (rest ? total.r : total.p), part = rest ? x.r : x.p;
+    const double at = rest ? before.r : before.p;
+    // the thread in whose segments the sum passes the goal; without one
+    // (rounding, u_next of 1 and more) the last that has anything
+    if (part > 0.0) {
+        atomicMax(&s_last, tid);
+        if (at + part > goal) atomicMin(&s_first, (unsigned int)tid);
     }
     __syncthreads();
-    const int next = s_tok >= 0 ? s_tok : run >= 0 ? s_last : -1;
-    for (int i = tid; i <= v.max_draft; i += 256)
-        v.tokens[(int64_t)seq * (v.max_draft + 1) + i] =
-            i < w.a ? v.drafts[(int64_t)seq * v.max_draft + i] : i == w.a ? next : -1;
+    const bool found = s_first != 0xFFFFFFFFu;
+    if (tid == (found ? (int)s_first : s_last)) {
+        // ... and the segment
+        double cum = at;
+        int seg = -1;
+        for (int i = tid * per; i < min((tid + 1) * per, n_seg); ++i) {
+            const double y = rest ? mine[i].r : mine[i].p;
+            if (!(y > 0.0)) continue;
+            s_before = cum;
+            seg = i;
+            cum += y;
+            if (found && cum > goal) break;
+        }
+        s_seg = seg;
+    }
+    __syncthreads();
+    const int seg = s_seg;
+    if (seg >= 0) {
+        const Row<T> row(v, seq, w);
+        double r[4], p[4];
+        const int i0 = seg * VER_SEG + 4 * tid;
+        row.four(i0, v.vocab, r, p);
+        Sums y = {0.0, 0.0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!rest) r[j] = p[j];
+            y.r += r[j];
+        }
+        double cum = s_before + scan256(y, s_part[1], total).r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            cum += r[j];
+            if (r[j] > 0.0) {
+                atomicMax(&s_last_tok, i0 + j);
+                if (found && cum > goal) atomicMin(&s_tok, (unsigned int)(i0 + j));
+            }
+        }
+    }
+    __syncthreads();
+    const int next = s_tok != 0xFFFFFFFFu ? (int)s_tok : s_last_tok;
+    if (tid <= v.max_draft)
+        v.tokens[(int64_t)seq * (v.max_draft + 1) + tid] = tid < w.a ? drafted : tid == w.a ? next : -1;
     if (tid == 0) v.accepted[seq] = w.a;
 }
 
@@ -343,32 +382,51 @@ int32_t refuse_as(const char * who, const char * why) noexcept {
     return refuse(msg);
 }
 
+template <class T, int NO>
+void launch_norm_chunks(const llapis_block_norm_args & a, int nch, int threads, int grid, hipStream_t s) {
+    const dim3 g(grid), wg(threads);
+    if (nch == 1) {
+        if (threads <= 256) hipLaunchKernelGGL((k_block_norm<T, 1, NO, 256>), g, wg, 0, s, a);
+        else hipLaunchKernelGGL((k_block_norm<T, 1, NO, 1024>), g, wg, 0, s, a);
+    } else if (nch == 2) {
+        if (threads <= 256) hipLaunchKernelGGL((k_block_norm<T, 2, NO, 256>), g, wg, 0, s, a);
+        else hipLaunchKernelGGL((k_block_norm<T, 2, NO, 1024>), g, wg, 0, s, a);
+    } else if (threads <= 256) {
+        if (nch == 3) hipLaunchKernelGGL((k_block_norm<T, 3, NO, 256>), g, wg, 0, s, a);
+        else hipLaunchKernelGGL((k_block_norm<T, 4, NO, 256>), g, wg, 0, s, a);
+    } else {
+        hipLaunchKernelGGL((k_block_norm<T, 4, NO, 1024>), g, wg, 0, s, a);
+    }
+}
+
 template <class T>
 hipError_t launch_norm(const llapis_block_norm_args & a, hipStream_t s) {
-    // few tokens: as many threads as a token has use for; many: fewer, with
-    // more values each
+    // few tokens: as many threads as a token has use for; many: fewer, with more
+    // values each, and as many workgroups as the card holds, each for as many tokens
     const int quads = (a.d + 3) / 4;
-    int threads = a.n_tokens <= 512 ? 1024 : 256;
+    int threads = a.n_tokens > 512 ? 256 : 1024;
     while (threads > 64 && threads / 2 >= quads) threads /= 2;
     while (threads < 1024 && (quads + threads - 1) / threads > 4) threads *= 2;
     const int nch = (quads + threads - 1) / threads;
-    const dim3 grid(a.n_tokens), wg(threads);
-    if (nch <= 1) hipLaunchKernelGGL((k_block_norm<T, 1>), grid, wg, 0, s, a);
-    else if (nch <= 2) hipLaunchKernelGGL((k_block_norm<T, 2>), grid, wg, 0, s, a);
-    else if (nch <= 3) hipLaunchKernelGGL((k_block_norm<T, 3>), grid, wg, 0, s, a);
-    else hipLaunchKernelGGL((k_block_norm<T, 4>), grid, wg, 0, s, a);
+    const int held = 256 * 1024 / threads;
+    const int each = (a.n_tokens + held - 1) / held, grid = (a.n_tokens + each - 1) / each;
+    if (a.n_out <= 1) launch_norm_chunks<T, 1>(a, nch, threads, grid, s);
+    else if (a.n_out == 2) launch_norm_chunks<T, 2>(a, nch, threads, grid, s);
+    else launch_norm_chunks<T, 4>(a, nch, threads, grid, s);
     return hipGetLastError();
 }
 
-int verify_runs(int vocab) { return (vocab + VER_RUN - 1) / VER_RUN; }
+// a sequence's sums, then its verdict
+uint64_t verify_sums_bytes(int n_seq, int vocab) { return (uint64_t)n_seq * verify_segments(vocab) * sizeof(Sums); }
 
 template <class T>
-hipError_t launch_verify(const llapis_verify_args & v, double * sums, hipStream_t s) {
-    const int runs = verify_runs(v.vocab);
-    hipLaunchKernelGGL((k_verify_sum<T>), dim3(runs, v.n_seq), dim3(256), 0, s, v, sums);
+hipError_t launch_verify(const llapis_verify_args & v, void * ws, hipStream_t s) {
+    Sums * sums = (Sums *)ws;
+    Verdict * verdicts = (Verdict *)((uint8_t *)ws + verify_sums_bytes(v.n_seq, v.vocab));
+    hipLaunchKernelGGL((k_verify_sum<T>), dim3(verify_segments(v.vocab) / 8, v.n_seq), dim3(256), 0, s, v, sums, verdicts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_verify_pick<T>), dim3(v.n_seq), dim3(256), 0, s, v, sums, runs);
+    hipLaunchKernelGGL((k_verify_pick<T>), dim3(v.n_seq), dim3(256), 0, s, v, sums, verdicts);
     return hipGetLastError();
 }
 
@@ -404,7 +462,7 @@ int32_t llapis_block_norm(const llapis_block_norm_args * a, void * stream) {
 }
 
 uint64_t llapis_verify_drafts_workspace_size(int32_t n_seq, int32_t vocab) {
-    return n_seq <= 0 || vocab <= 0 ? 0 : (uint64_t)n_seq * verify_runs(vocab) * 16;
+    return n_seq <= 0 || vocab <= 0 ? 0 : verify_sums_bytes(n_seq, vocab) + (uint64_t)n_seq * sizeof(Verdict);
 }
 
 int32_t llapis_verify_drafts(const llapis_verify_args * a, void * workspace, uint64_t ws_bytes, void * stream) {
@@ -419,11 +477,10 @@ int32_t llapis_verify_drafts(const llapis_verify_args * a, void * workspace, uin
     if (a->target_stride < a->vocab || (a->draft && a->draft_stride < a->vocab)) return refuse_as(who, "rows shorter than vocab");
     if (!workspace || ((uintptr_t)workspace & 7) || ws_bytes < llapis_verify_drafts_workspace_size(a->n_seq, a->vocab))
         return refuse_as(who, "workspace too small or not 8-byte aligned");
-    double * sums = (double *)workspace;
     hipStream_t s = (hipStream_t)stream;
-    if (a->type == T_F32) ST_TRY(launch_verify<float>(*a, sums, s));
-    else if (a->type == T_F16) ST_TRY(launch_verify<_Float16>(*a, sums, s));
-    else ST_TRY(launch_verify<__bf16>(*a, sums, s));
+    if (a->type == T_F32) ST_TRY(launch_verify<float>(*a, workspace, s));
+    else if (a->type == T_F16) ST_TRY(launch_verify<_Float16>(*a, workspace, s));
+    else ST_TRY(launch_verify<__bf16>(*a, workspace, s));
     return 0;
 }
 

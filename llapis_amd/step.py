@@ -22,9 +22,14 @@ from .moe import _torch
 KV_MAX_NEW = 16
 
 
+_tags = {}
+
+
 def _tag(dtype):
     torch = _torch()
-    tag = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
+    if not _tags:
+        _tags.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    tag = _tags.get(dtype)
     if tag is None:
         raise ValueError(f"need float32, float16 or bfloat16 values, got {dtype}")
     return tag
@@ -36,8 +41,8 @@ def _need(ok, what):
 
 
 def _is(t, dtype, shape, dev, what):
-    _need(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.device == dev and t.is_contiguous(),
-          f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
+    if t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
 
 
 def _ptr(t):
@@ -48,11 +53,13 @@ def _call(name, dev, *args):
     """The entry point on the current stream of `dev`, which becomes the current device for it."""
     torch = _torch()
     fn = getattr(lib(), name)
+    # (the raw handle: torch.cuda.current_stream builds an object around it, 2 us a call)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if dev.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), name)
+        check(fn(*args, stream), name)
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), name)
+            check(fn(*args, stream), name)
 
 
 def _on_gpu(t, what):
@@ -136,11 +143,11 @@ class KvCache:
                    torch.empty(n_pages, n_kv, head_dim, page_size, dtype=dt, device=device))
 
     def _rows(self, t, batch, n_heads, what):
-        D = self.head_dim
-        _need(t.dim() == 3 and t.shape[0] >= batch.n_tokens and t.shape[1] == n_heads and t.shape[2] == D
-              and t.stride(2) == 1 and (n_heads == 1 or t.stride(1) == D) and t.device == self.device,
-              f"{what} must be [{batch.n_tokens} or more, {n_heads}, {D}] on {self.device}, rows of consecutive values")
-        return t.stride(0)
+        D, shape, stride = self.head_dim, t.shape, t.stride()
+        if (len(shape) != 3 or shape[0] < batch.n_tokens or shape[1] != n_heads or shape[2] != D or stride[2] != 1
+                or (n_heads > 1 and stride[1] != D) or t.device != self.device):
+            raise ValueError(f"{what} must be [{batch.n_tokens} or more, {n_heads}, {D}] on {self.device}, rows of consecutive values")
+        return stride[0]
 
     def append(self, batch, k, v):
         """Write the new tokens' keys and values (k, v [n_tokens, n_kv, head_dim],
@@ -172,8 +179,9 @@ class KvCache:
         os_ = self._rows(out, batch, n_head, "out")
         _need(out.dtype == q.dtype, "out must be of q's type")
         if lse is not None:
-            _need(lse.dtype == torch.float32 and lse.device == self.device and lse.is_contiguous() and lse.dim() == 2
-                  and lse.shape[0] >= batch.n_tokens and lse.shape[1] == n_head,
+            shape = lse.shape
+            _need(lse.dtype == torch.float32 and lse.device == self.device and lse.is_contiguous() and len(shape) == 2
+                  and shape[0] >= batch.n_tokens and shape[1] == n_head,
                   "lse must be a contiguous float32 [n_tokens, n_head]")
         if workspace is None:
             workspace = self.attention_workspace(batch, n_head)
@@ -208,11 +216,12 @@ class KvPages:
 
     def _table(self, page_table, lens):
         torch = _torch()
-        _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.stride(1) == 1
-              and page_table.shape[1] > 0 and page_table.device == self.device,
-              f"page_table must be int32 [n_seq, max_pages] on {self.device}, rows of consecutive entries")
-        _is(lens, torch.int32, (page_table.shape[0],), self.device, "lens")
-        return page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), page_table.shape[1]
+        shape, stride = page_table.shape, page_table.stride()
+        if (page_table.dtype != torch.int32 or len(shape) != 2 or stride[1] != 1 or shape[1] == 0
+                or page_table.device != self.device):
+            raise ValueError(f"page_table must be int32 [n_seq, max_pages] on {self.device}, rows of consecutive entries")
+        _is(lens, torch.int32, (shape[0],), self.device, "lens")
+        return page_table.data_ptr(), max(stride[0], shape[1]), shape[1]
 
     def copy(self, pairs):
         """Copy page pairs[i, 0] to page pairs[i, 1] (int32 [n, 2] on the GPU) in every layer."""
@@ -284,38 +293,41 @@ def block_norm(h, y=None, post_weight=None, post_norm=True, gate=None, alpha=1.0
     [1, 1]; weights float32 [d] or None each (at most 4), post_weight too.  h_out
     may be h; out: the x_j's tensors."""
     torch = _torch()
-    _need(h.dim() == 2 and h.stride(1) == 1, "h must be [T, d], rows of consecutive values")
-    dev, (T, d) = _on_gpu(h, "h"), h.shape
-    row = lambda t, what: _need(t.shape == h.shape and t.dtype == h.dtype and t.device == dev and t.stride(1) == 1,
-                                f"{what} must be shaped and typed as h, rows of consecutive values")
-    a = L.LlapisBlockNormArgs(_tag(h.dtype), T, d, len(weights), int(post_norm), eps, alpha, beta, h.data_ptr(), h.stride(0))
-    if y is not None:
-        row(y, "y")
-        a.y, a.y_stride = y.data_ptr(), y.stride(0)
+    shape, dtype, dev = h.shape, h.dtype, _on_gpu(h, "h")
+    _need(len(shape) == 2 and h.stride(1) == 1, "h must be [T, d], rows of consecutive values")
+    T, d = shape
+
+    def row(t, what):
+        stride = t.stride()
+        if t.shape != shape or t.dtype != dtype or t.device != dev or stride[1] != 1:
+            raise ValueError(f"{what} must be shaped and typed as h, rows of consecutive values")
+        return t.data_ptr(), stride[0]
+
+    n_out = len(weights)
+    _need(n_out <= L.NORM_MAX_OUT, "at most 4 outputs")
+    y_row = (None, 0) if y is None else row(y, "y")
     if post_weight is not None:
         _is(post_weight, torch.float32, (d,), dev, "post_weight")
-        a.post_weight = post_weight.data_ptr()
+    gate_at = (None, 0, 0)
     if gate is not None:
-        _need(gate.dim() == 2 and gate.shape[0] in (1, T) and gate.shape[1] in (1, d) and gate.dtype == h.dtype
-              and gate.device == dev and (gate.shape[1] == 1 or gate.stride(1) == 1),
-              "gate must be [T or 1, d or 1] of h's type, rows of consecutive values")
-        a.gate = gate.data_ptr()
-        a.gate_token_stride = gate.stride(0) if gate.shape[0] > 1 else 0
-        a.gate_value_stride = 1 if gate.shape[1] > 1 else 0
-    _need(len(weights) <= L.NORM_MAX_OUT, "at most 4 outputs")
+        gs, stride = gate.shape, gate.stride()
+        _need(len(gs) == 2 and gs[0] in (1, T) and gs[1] in (1, d) and gate.dtype == dtype and gate.device == dev
+              and (gs[1] == 1 or stride[1] == 1), "gate must be [T or 1, d or 1] of h's type, rows of consecutive values")
+        gate_at = gate.data_ptr(), stride[0] if gs[0] > 1 else 0, 1 if gs[1] > 1 else 0
     if h_out is None:
-        h_out = torch.empty(T, d, dtype=h.dtype, device=dev)
-    row(h_out, "h_out")
-    a.h_out, a.h_out_stride = h_out.data_ptr(), h_out.stride(0)
+        h_out = torch.empty(T, d, dtype=dtype, device=dev)
     if out is None:
-        out = [torch.empty(T, d, dtype=h.dtype, device=dev) for _ in weights]
-    _need(len(out) == len(weights), "out needs a tensor for each of weights")
-    for i, (w, x) in enumerate(zip(weights, out)):
-        row(x, "out")
+        out = [torch.empty(T, d, dtype=dtype, device=dev) for _ in weights]
+    _need(len(out) == n_out, "out needs a tensor for each of weights")
+    a = L.LlapisBlockNormArgs(_tag(dtype), T, d, n_out, int(post_norm), eps, alpha, beta, h.data_ptr(), h.stride(0), *y_row,
+                              _ptr(post_weight), *gate_at, *row(h_out, "h_out"))
+    w_at, x_at, x_stride = a.weight, a.x, a.x_stride
+    for i, x in enumerate(out):
+        w = weights[i]
         if w is not None:
             _is(w, torch.float32, (d,), dev, "weights")
-            a.weight[i] = w.data_ptr()
-        a.x[i], a.x_stride[i] = x.data_ptr(), x.stride(0)
+            w_at[i] = w.data_ptr()
+        x_at[i], x_stride[i] = row(x, "out")
     _call("llapis_block_norm", dev, C.byref(a))
     return h_out, out
 
@@ -334,21 +346,20 @@ def verify_drafts(target, draft, drafts, u, u_next, n_draft=None, tokens=None, a
     probabilities, drafts [n_seq, n] int32, u [n_seq, n] and u_next [n_seq]
     float32 in [0, 1), n_draft [n_seq] int32 where sequences have fewer drafts."""
     torch = _torch()
-    _need(target.dim() == 3 and target.shape[1] > 0, "target must be [n_seq, drafts + 1, vocab]")
-    dev = _on_gpu(target, "target")
-    S, n, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    shape, dtype, dev = target.shape, target.dtype, _on_gpu(target, "target")
+    _need(len(shape) == 3 and shape[1] > 0, "target must be [n_seq, drafts + 1, vocab]")
+    S, n, V = shape[0], shape[1] - 1, shape[2]
 
     def rows(t, k, what):
-        _need(tuple(t.shape) == (S, k, V) and t.dtype == target.dtype and t.device == dev and t.stride(2) == 1
-              and (S == 1 or k == 1 or t.stride(0) == k * t.stride(1)),
-              f"{what} must be [{S}, {k}, {V}] of target's type, rows evenly spaced")
+        stride = t.stride()
+        if (t.shape != (S, k, V) or t.dtype != dtype or t.device != dev or stride[2] != 1
+                or (S > 1 and k > 1 and stride[0] != k * stride[1])):
+            raise ValueError(f"{what} must be [{S}, {k}, {V}] of target's type, rows evenly spaced")
         # a sequence's rows follow each other; with one row each, the sequences' do
-        return (t.stride(1) if k > 1 else t.stride(0)) if S * k > 1 else V
+        return t.data_ptr(), (stride[1] if k > 1 else stride[0]) if S * k > 1 else V
 
-    a = L.LlapisVerifyArgs(_tag(target.dtype), S, n, V, target.data_ptr(), rows(target, n + 1, "target"))
-    if draft is not None and n > 0:
-        a.draft_stride = rows(draft, n, "draft")
-        a.draft = draft.data_ptr()
+    target_rows = rows(target, n + 1, "target")
+    draft_rows = rows(draft, n, "draft") if draft is not None and n > 0 else (None, 0)
     _is(drafts, torch.int32, (S, n), dev, "drafts")
     _is(u, torch.float32, (S, n), dev, "u")
     _is(u_next, torch.float32, (S,), dev, "u_next")
@@ -362,7 +373,7 @@ def verify_drafts(target, draft, drafts, u, u_next, n_draft=None, tokens=None, a
     _is(accepted, torch.int32, (S,), dev, "accepted")
     if workspace is None:
         workspace = verify_workspace(S, V, dev)
-    a.drafts, a.n_draft, a.u, a.u_next = drafts.data_ptr(), _ptr(n_draft), u.data_ptr(), u_next.data_ptr()
-    a.tokens, a.accepted = tokens.data_ptr(), accepted.data_ptr()
+    a = L.LlapisVerifyArgs(_tag(dtype), S, n, V, *target_rows, *draft_rows, drafts.data_ptr(), _ptr(n_draft), u.data_ptr(),
+                           u_next.data_ptr(), tokens.data_ptr(), accepted.data_ptr())
     _call("llapis_verify_drafts", dev, C.byref(a), workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return tokens, accepted
