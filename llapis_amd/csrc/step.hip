@@ -12,11 +12,15 @@ namespace dev {
 typedef float f4 __attribute__((ext_vector_type(4)));
 template <class T> struct Four { typedef T v __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
 
-// values i .. i + 3 of a row of n, zeros past its end
-template <class T>
+// values i .. i + 3 of a row of n, zeros past its end.  WHOLE: n is a multiple of
+// 4 (and not 0); no branch then parts one load from the next
+template <bool WHOLE, class T>
 __device__ __forceinline__ typename Four<T>::v raw4(const T * p, int i, int n) {
     typename Four<T>::v r = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
-    if (i + 4 <= n) {
+    if constexpr (WHOLE) {
+        const typename Four<T>::v w = *(const typename Four<T>::v *)(p + min(i, n - 4));
+        r = i < n ? w : r;
+    } else if (i + 4 <= n) {
         r = *(const typename Four<T>::v *)(p + i);
     } else {
 #pragma unroll
@@ -29,8 +33,8 @@ __device__ __forceinline__ typename Four<T>::v raw4(const T * p, int i, int n) {
 template <class T>
 __device__ __forceinline__ f4 wide4(typename Four<T>::v w) { return f4{(float)w[0], (float)w[1], (float)w[2], (float)w[3]}; }
 
-template <class T>
-__device__ __forceinline__ f4 get4(const T * p, int i, int n) { return wide4<T>(raw4(p, i, n)); }
+template <bool WHOLE, class T>
+__device__ __forceinline__ f4 get4(const T * p, int i, int n) { return wide4<T>(raw4<WHOLE>(p, i, n)); }
 
 template <class T>
 __device__ __forceinline__ void put4(T * p, int i, int n, f4 x) {
@@ -79,21 +83,26 @@ template <class T, int NCH>
 struct NormRow {
     typename Four<T>::v h[NCH], y[NCH], g[NCH];
     float g1;
-    __device__ __forceinline__ void load(const llapis_block_norm_args & a, int64_t t) {
+    template <bool WHOLE>
+    __device__ __forceinline__ void read(const llapis_block_norm_args & a, int64_t t) {
         const int n = blockDim.x;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) h[c] = raw4((const T *)a.h + t * a.h_stride, 4 * (threadIdx.x + c * n), a.d);
+        for (int c = 0; c < NCH; ++c) h[c] = raw4<WHOLE>((const T *)a.h + t * a.h_stride, 4 * (threadIdx.x + c * n), a.d);
         if (!a.y) return;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) y[c] = raw4((const T *)a.y + t * a.y_stride, 4 * (threadIdx.x + c * n), a.d);
+        for (int c = 0; c < NCH; ++c) y[c] = raw4<WHOLE>((const T *)a.y + t * a.y_stride, 4 * (threadIdx.x + c * n), a.d);
         if (!a.gate) return;
         const T * gp = (const T *)a.gate + t * a.gate_token_stride;
         if (a.gate_value_stride) {
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) g[c] = raw4(gp, 4 * (threadIdx.x + c * n), a.d);
+            for (int c = 0; c < NCH; ++c) g[c] = raw4<WHOLE>(gp, 4 * (threadIdx.x + c * n), a.d);
         } else {
             g1 = (float)gp[0];
         }
+    }
+    __device__ __forceinline__ void load(const llapis_block_norm_args & a, int64_t t) {
+        if (a.d % 4 == 0) read<true>(a, t);
+        else read<false>(a, t);
     }
 };
 
@@ -108,7 +117,10 @@ __global__ __launch_bounds__(THREADS) void k_block_norm(const llapis_block_norm_
     // hold: the weights are then read where they are used)
     constexpr bool HOLD = THREADS * NCH <= 2048;
     const float * wp = a.y && a.post_norm ? a.post_weight : nullptr;
-    auto weight = [&](const float * w, int c) { return w ? get4(w, 4 * (threadIdx.x + c * n), d) : f4{1.0f, 1.0f, 1.0f, 1.0f}; };
+    auto weight = [&](const float * w, int c) {
+        const int i = 4 * (threadIdx.x + c * n);
+        return !w ? f4{1.0f, 1.0f, 1.0f, 1.0f} : d % 4 == 0 ? get4<true>(w, i, d) : get4<false>(w, i, d);
+    };
     f4 w_post[HOLD ? NCH : 1], w_pre[NO][HOLD ? NCH : 1];
     if constexpr (HOLD) {
 #pragma unroll
@@ -160,13 +172,14 @@ __global__ __launch_bounds__(THREADS) void k_block_norm(const llapis_block_norm_
 // -------------------------------------------------------- verification
 //
 // k_verify_sum: every workgroup finds the number of taken drafts anew (a few
-// loads) and sums 8 segments of 1024 values of the row the next token comes from:
-// r, and p for the case that r is 0 everywhere.  k_verify_pick: one workgroup a
+// loads) and sums 4 segments of 1024 values of the row the next token comes from,
+// r, and p for the case that r is 0 everywhere.  (16 loads of 16 bytes a lane in two
+// batches, or in one at three waves a SIMD, took twice the time of one batch of 8.)  k_verify_pick: one workgroup a
 // sequence adds the segments in order, finds the one where the sum passes u_next
 // of the whole, and in it the token.
 
 constexpr int VER_SEG = 1024;                   // values of a segment: 16 a lane, four a thread of the pick
-constexpr int VER_RUN = 8 * VER_SEG;            // values of a workgroup, two segments a wave
+constexpr int VER_RUN = 4 * VER_SEG;            // values of a workgroup, a segment a wave
 
 template <class T>
 __device__ __forceinline__ double prob(const T * p, int64_t i) {
@@ -198,62 +211,80 @@ __device__ __forceinline__ Verdict verdict(const llapis_verify_args & v, int seq
     return {a, a < n, a < n ? __shfl(x, a, 64) : -1, 0};
 }
 
-// the row the next token comes from, and what is taken off it
+// the row the next token comes from, and what is taken off it: the draft's row
+// (less), without one 1 at the place `draft`
 template <class T>
 struct Row {
     const T * p;
-    const T * q;                                // or null
-    int draft;                                  // without q: the place that 1 is taken off
+    const T * q;
+    bool less;
+    int draft;
     __device__ __forceinline__ Row(const llapis_verify_args & v, int seq, const Verdict & w) {
         p = (const T *)v.target + ((int64_t)seq * (v.max_draft + 1) + w.a) * v.target_stride;
-        q = w.refused && v.draft ? (const T *)v.draft + ((int64_t)seq * v.max_draft + w.a) * v.draft_stride : nullptr;
+        q = (const T *)v.draft + ((int64_t)seq * v.max_draft + w.a) * v.draft_stride;
+        less = w.refused && v.draft;
         draft = w.refused && !v.draft ? w.draft : -1;
     }
-    // four values from i on: r, and p
-    __device__ __forceinline__ void four(int i, int n, double (&r)[4], double (&whole)[4]) const {
-        const f4 x = get4(p, i, n);
-        const f4 y = q ? get4(q, i, n) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+    // N times four values, from i + 0, i + step, ...
+    template <int N>
+    __device__ __forceinline__ void read(const T * row, int i, int step, int n, f4 (&x)[N]) const {
+        if (n % 4 == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            whole[j] = x[j] > 0.0f && x[j] < __builtin_inff() ? (double)x[j] : 0.0;
-            double off = y[j] > 0.0f && y[j] < __builtin_inff() ? (double)y[j] : 0.0;
-            if (i + j == draft) off = 1.0;
-            r[j] = whole[j] > off ? whole[j] - off : 0.0;
+            for (int c = 0; c < N; ++c) x[c] = get4<true>(row, i + c * step, n);
+        } else {
+#pragma unroll
+            for (int c = 0; c < N; ++c) x[c] = get4<false>(row, i + c * step, n);
         }
     }
+    // f(c, j, r, p) of each value j of each four c
+    template <int N, class F>
+    __device__ __forceinline__ void values(int i, int step, int n, F f) const {
+        f4 x[N], y[N];
+        read<N>(p, i, step, n, x);
+        if (less) {
+            read<N>(q, i, step, n, y);
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double w = (double)some(x[c][j]);
+                    f(c, j, fmax(w - (double)some(y[c][j]), 0.0), w);
+                }
+        } else {
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double w = (double)some(x[c][j]);
+                    f(c, j, i + c * step + j == draft ? fmax(w - 1.0, 0.0) : w, w);
+                }
+        }
+    }
+    // what is not positive and finite counts as 0
+    static __device__ __forceinline__ float some(float x) { return x > 0.0f && x < __builtin_inff() ? x : 0.0f; }
 };
 
 struct Sums { double r, p; };
 
 // segments of a sequence, a whole number of workgroups
-__host__ __device__ __forceinline__ int verify_segments(int vocab) { return (vocab + VER_RUN - 1) / VER_RUN * 8; }
+__host__ __device__ __forceinline__ int verify_segments(int vocab) { return (vocab + VER_RUN - 1) / VER_RUN * 4; }
 
 template <class T>
-__global__ __launch_bounds__(256) void k_verify_sum(const llapis_verify_args v, Sums * sums, Verdict * verdicts) {
+__global__ __launch_bounds__(256, 4) void k_verify_sum(const llapis_verify_args v, Sums * sums, Verdict * verdicts) {
     const int seq = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Verdict w = verdict<T>(v, seq);
     const Row<T> row(v, seq, w);
     if (blockIdx.x == 0 && threadIdx.x == 0) verdicts[seq] = w;
-    Sums s[2] = {{0.0, 0.0}, {0.0, 0.0}};
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            double r[4], p[4];
-            row.four(blockIdx.x * VER_RUN + (2 * wave + g) * VER_SEG + 256 * c + 4 * lane, v.vocab, r, p);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[g].r += r[j];
-                s[g].p += p[j];
-            }
-        }
-    for (int o = 32; o; o >>= 1)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            s[g].r += __shfl_xor(s[g].r, o, 64);
-            s[g].p += __shfl_xor(s[g].p, o, 64);
-        }
-    if (lane < 2) sums[(int64_t)seq * (8 * gridDim.x) + blockIdx.x * 8 + 2 * wave + lane] = lane ? s[1] : s[0];
+    Sums s = {0.0, 0.0};
+    row.template values<4>(blockIdx.x * VER_RUN + wave * VER_SEG + 4 * lane, 256, v.vocab, [&](int, int, double r, double p) {
+        s.r += r;
+        s.p += p;
+    });
+    for (int o = 32; o; o >>= 1) {
+        s.r += __shfl_xor(s.r, o, 64);
+        s.p += __shfl_xor(s.p, o, 64);
+    }
+    if (lane == 0) sums[((int64_t)seq * gridDim.x + blockIdx.x) * 4 + wave] = s;
 }
 
 // exclusive sums over the workgroup's 256 threads in order, and the whole
@@ -287,40 +318,46 @@ __device__ __forceinline__ Sums scan256(Sums x, Sums * s_part, Sums & total) {
 template <class T>
 __global__ __launch_bounds__(256) void k_verify_pick(const llapis_verify_args v, const Sums * sums, const Verdict * verdicts) {
     __shared__ Sums s_part[2][4];
-    __shared__ unsigned int s_first, s_tok;               // the smallest found
-    __shared__ int s_last, s_last_tok;                    // the largest with anything
+    // of each wave: the first thread whose sum passes the goal, the last that has
+    // anything; then the tokens
+    __shared__ int s_first[2][4], s_last[2][4];
     __shared__ int s_seg;
     __shared__ double s_before;
-    const int seq = blockIdx.x, tid = threadIdx.x;
+    const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n_seg = verify_segments(v.vocab), per = (n_seg + 255) / 256;
     const Verdict w = verdicts[seq];
     const float u = v.u_next[seq];
     const Sums * mine = sums + (int64_t)seq * n_seg;
     const int drafted = tid < w.a ? v.drafts[(int64_t)seq * v.max_draft + tid] : -1;
-    if (tid == 0) {
-        s_first = s_tok = 0xFFFFFFFFu;
-        s_last = s_last_tok = -1;
-        s_seg = -1;
-    }
+    if (tid == 0) s_seg = -1;
+    auto vote = [&](int k, bool any, bool passes, int mark) {
+        const uint64_t a = __ballot(any), p = __ballot(passes);
+        const int first = __shfl(mark, p ? __builtin_ctzll(p) : 0, 64);
+        const int last = __shfl(mark, a ? 63 - __builtin_clzll(a) : 0, 64);
+        if (lane == 0) {
+            s_first[k][wave] = p ? first : 0x7FFFFFFF;
+            s_last[k][wave] = a ? last : -1;
+        }
+    };
+    auto first_of = [&](int k) { return min(min(s_first[k][0], s_first[k][1]), min(s_first[k][2], s_first[k][3])); };
+    auto last_of = [&](int k) { return max(max(s_last[k][0], s_last[k][1]), max(s_last[k][2], s_last[k][3])); };
     // a thread's segments are consecutive
     Sums x = {0.0, 0.0}, total;
     for (int i = tid * per; i < min((tid + 1) * per, n_seg); ++i) {
         x.r += mine[i].r;
         x.p += mine[i].p;
     }
-    const Sums before = scan256(x, s_part[0], total);     // its barrier: the places above are set
+    const Sums before = scan256(x, s_part[0], total);
     const bool rest = w.refused && total.r > 0.0;
     const double goal = (double)u * (rest ? total.r : total.p), part = rest ? x.r : x.p;
     const double at = rest ? before.r : before.p;
     // the thread in whose segments the sum passes the goal; without one
     // (rounding, u_next of 1 and more) the last that has anything
-    if (part > 0.0) {
-        atomicMax(&s_last, tid);
-        if (at + part > goal) atomicMin(&s_first, (unsigned int)tid);
-    }
+    vote(0, part > 0.0, part > 0.0 && at + part > goal, tid);
     __syncthreads();
-    const bool found = s_first != 0xFFFFFFFFu;
-    if (tid == (found ? (int)s_first : s_last)) {
+    const int first = first_of(0);
+    const bool found = first != 0x7FFFFFFF;
+    if (tid == (found ? first : last_of(0))) {
         // ... and the segment
         double cum = at;
         int seg = -1;
@@ -335,30 +372,33 @@ __global__ __launch_bounds__(256) void k_verify_pick(const llapis_verify_args v,
         s_seg = seg;
     }
     __syncthreads();
+    int next = -1;
     const int seg = s_seg;
     if (seg >= 0) {
         const Row<T> row(v, seq, w);
-        double r[4], p[4];
+        double r[4];
         const int i0 = seg * VER_SEG + 4 * tid;
-        row.four(i0, v.vocab, r, p);
         Sums y = {0.0, 0.0};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!rest) r[j] = p[j];
+        row.template values<1>(i0, 0, v.vocab, [&](int, int j, double a, double p) {
+            r[j] = rest ? a : p;
             y.r += r[j];
-        }
+        });
         double cum = s_before + scan256(y, s_part[1], total).r;
+        int tok = -1, last = -1;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             cum += r[j];
             if (r[j] > 0.0) {
-                atomicMax(&s_last_tok, i0 + j);
-                if (found && cum > goal) atomicMin(&s_tok, (unsigned int)(i0 + j));
+                last = i0 + j;
+                if (tok < 0 && found && cum > goal) tok = i0 + j;
             }
         }
+        // a thread that passes marks its token, the others their last
+        vote(1, last >= 0, tok >= 0, tok >= 0 ? tok : last);
+        __syncthreads();
+        const int f = first_of(1);
+        next = f != 0x7FFFFFFF ? f : last_of(1);
     }
-    __syncthreads();
-    const int next = s_tok != 0xFFFFFFFFu ? (int)s_tok : s_last_tok;
     if (tid <= v.max_draft)
         v.tokens[(int64_t)seq * (v.max_draft + 1) + tid] = tid < w.a ? drafted : tid == w.a ? next : -1;
     if (tid == 0) v.accepted[seq] = w.a;
@@ -423,7 +463,7 @@ template <class T>
 hipError_t launch_verify(const llapis_verify_args & v, void * ws, hipStream_t s) {
     Sums * sums = (Sums *)ws;
     Verdict * verdicts = (Verdict *)((uint8_t *)ws + verify_sums_bytes(v.n_seq, v.vocab));
-    hipLaunchKernelGGL((k_verify_sum<T>), dim3(verify_segments(v.vocab) / 8, v.n_seq), dim3(256), 0, s, v, sums, verdicts);
+    hipLaunchKernelGGL((k_verify_sum<T>), dim3(verify_segments(v.vocab) / 4, v.n_seq), dim3(256), 0, s, v, sums, verdicts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((k_verify_pick<T>), dim3(v.n_seq), dim3(256), 0, s, v, sums, verdicts);
