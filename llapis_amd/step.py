@@ -17,18 +17,25 @@ import ctypes as C
 
 from . import _lib as L
 from ._lib import BF16, F16, F32, Q8_0, check, lib
-from .moe import _torch
 
 KV_MAX_NEW = 16
 
 
+_module = None
 _tags = {}
 
 
-def _tag(dtype):
-    torch = _torch()
-    if not _tags:
+def _torch():
+    """torch, imported at the first call (an import statement costs every call 0.3 us)."""
+    global _module
+    if _module is None:
+        import torch
         _tags.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _module = torch
+    return _module
+
+
+def _tag(dtype):
     tag = _tags.get(dtype)
     if tag is None:
         raise ValueError(f"need float32, float16 or bfloat16 values, got {dtype}")
@@ -51,14 +58,13 @@ def _ptr(t):
 
 def _call(name, dev, *args):
     """The entry point on the current stream of `dev`, which becomes the current device for it."""
-    torch = _torch()
-    fn = getattr(lib(), name)
+    fn, index, gpu = getattr(lib(), name), dev.index, _module._C
     # (the raw handle: torch.cuda.current_stream builds an object around it, 2 us a call)
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if dev.index == torch.cuda.current_device():
+    stream = gpu._cuda_getCurrentRawStream(index)
+    if index == gpu._cuda_getDevice():
         check(fn(*args, stream), name)
     else:
-        with torch.cuda.device(dev):
+        with _module.cuda.device(dev):
             check(fn(*args, stream), name)
 
 
