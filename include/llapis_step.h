@@ -36,7 +36,9 @@ enum { LLAPIS_T_F16 = 1, LLAPIS_T_BF16 = 30 };
  * in that order and after them their fp16 scales [head_dim / 32][page_size]
  * (K's and V's alike), one for 32 consecutive values of a token's vector:
  * ggml's q8_0 blocks with the planes apart (d = amax / 127 rounded to fp16,
- * q = x times the fp32 reciprocal of the unrounded d, rounded to nearest even).
+ * q = x times the fp32 reciprocal of the unrounded d, rounded to nearest even; a
+ * block with a NaN has a NaN scale).  Attention reads magnitudes above 65504 as
+ * infinite, as an F16 cache holds them.
  * Page p is at base + p * stride bytes; strides are multiples of 16 and at
  * least llapis_kv_page_bytes (pages of several layers may interleave). */
 typedef struct llapis_kv_cache {
@@ -83,7 +85,8 @@ int32_t llapis_kv_append(const llapis_kv_cache * c, const llapis_kv_batch * b, i
  *   lse = ln sum_i e^(s_i)
  * A row that sees no key gets out 0 and lse -infinity, whatever the masked
  * places hold.  q, out: [n_tokens][n_head][head_dim] of `type`, rows q_stride /
- * out_stride values apart, 16-byte aligned; lse [n_tokens][n_head] or NULL.
+ * out_stride values apart, 16-byte aligned, out apart from q; lse [n_tokens]
+ * [n_head] or NULL.
  * Scores, sums and the running maximum are fp32; F32 queries are multiplied
  * as exact sums of 16-bit parts. */
 typedef struct llapis_kv_query {
@@ -168,7 +171,8 @@ int32_t  llapis_kv_compact(const llapis_kv_planes * p, const int32_t * page_tabl
  *   x_j = h' / rms(h') * weight_j      j < n_out
  * with rms(z) = sqrt(mean z^2 + eps) over a token's d values, sums in fp32;
  * each output is rounded once (x_j is computed from the unrounded h').
- * Activations are of `type`, weights fp32; y NULL leaves the second term out. */
+ * Activations are of `type`, weights fp32; y NULL leaves the second term out.
+ * h_out and the x_j may lie on h or y row for row; other overlaps are not allowed. */
 #define LLAPIS_NORM_MAX_OUT 4
 typedef struct llapis_block_norm_args {
     int32_t type;                  /* LLAPIS_T_F32, LLAPIS_T_F16 or LLAPIS_T_BF16 */

@@ -130,6 +130,11 @@ __device__ __forceinline__ Q8Scale q8_scale(float amax) {
     const float d = __fdiv_rn(amax, 127.0f);
     return {d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f, __builtin_bit_cast(uint16_t, (_Float16)d)};
 }
+// the larger magnitude, NaN if one is: the block's scale then says so
+__device__ __forceinline__ float larger(float a, float b) {
+    b = fabsf(b);
+    return a != a || b != b ? __builtin_nanf("") : fmaxf(a, b);
+}
 __device__ __forceinline__ int q8_value(float x, float id) { return (int)__builtin_rintf(x * id) & 0xFF; }
 
 // HDT: the head size, 0 for one that is not a multiple of 64
@@ -178,7 +183,7 @@ __global__ __launch_bounds__(256) void k_kv_append(const KvAppend p) {
                     for (int j = 0; j < 8; ++j) {
                         float amax = fabsf(x[e][j]);
 #pragma unroll
-                        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+                        for (int o = 16; o; o >>= 1) amax = larger(amax, __shfl_xor(amax, o, 64));
                         const Q8Scale s = q8_scale(amax);
                         w[j >> 2] |= (uint32_t)q8_value(x[e][j], s.id) << (8 * (j & 3));
                         d[j] = s.d;
@@ -234,9 +239,9 @@ __global__ __launch_bounds__(256) void k_kv_append(const KvAppend p) {
             if constexpr (CT == KV_Q8) {
                 float amax = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[e][j]));
-                amax = fmaxf(amax, __shfl_xor(amax, 1, 64));      // four threads hold a block of 32
-                amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
+                for (int j = 0; j < 8; ++j) amax = larger(amax, x[e][j]);
+                amax = larger(amax, __shfl_xor(amax, 1, 64));     // four threads hold a block of 32
+                amax = larger(amax, __shfl_xor(amax, 2, 64));
                 if (there) {
                     const Q8Scale s = q8_scale(amax);
                     u2 w = {0, 0};
@@ -658,6 +663,7 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     if (sq.n_seq == 0 || sq.n_tokens == 0 || sq.max_new == 0) return 0;
     const int es = el_bytes(q->type), width = q->n_head * c->head_dim;
     if (!q->q || !q->out) return refuse_as(who, "null q or out");
+    if (q->q == q->out) return refuse_as(who, "out may not be q: its rows are read by several workgroups");
     if (!aligned16(q->q) || !aligned16(q->out) || (q->q_stride * es) % 16 || (q->out_stride * es) % 16)
         return refuse_as(who, "q and out must be 16-byte aligned, rows too");
     if (sq.n_tokens > 1 && (q->q_stride < width || q->out_stride < width)) return refuse_as(who, "rows shorter than n_head * head_dim");

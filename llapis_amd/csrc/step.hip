@@ -490,7 +490,7 @@ int32_t llapis_block_norm(const llapis_block_norm_args * a, void * stream) {
     for (int i = 0; i < a->n_out; ++i)
         if (!a->x[i]) return refuse_as(who, "null output");
     if (a->n_tokens > 1) {
-        bool shorter = (a->y && a->y_stride < 0) || a->h_stride < 0 || (a->h_out && a->h_out_stride < a->d);
+        bool shorter = a->h_out && a->h_out_stride < a->d;
         for (int i = 0; i < a->n_out; ++i) shorter |= a->x_stride[i] < a->d;
         if (shorter) return refuse_as(who, "output rows overlap");
     }

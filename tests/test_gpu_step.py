@@ -157,6 +157,20 @@ def test_append_one_each(gpu):
     assert torch.equal(c.k, want) and torch.equal(c.v.transpose(2, 3), wv)
 
 
+def test_append_q8_non_finite(gpu):
+    """A NaN or an infinity among a block's 32 values makes that block NaN, and no other."""
+    D, H, P = 96, 1, 16
+    c = la.KvCache.empty(2, P, H, D, la.Q8_0, gpu)
+    k, v = torch.randn(12, H, D), torch.randn(12, H, D)
+    k[3, 0, 40], k[5, 0, 95], v[2, 0, 0], v[9, 0, 33] = float("nan"), float("inf"), -float("inf"), float("nan")
+    c.append(la.KvBatch(i32([[1]], gpu), i32([12], gpu), i32([0, 12], gpu), n_tokens=12, max_new=12), k.to(gpu), v.to(gpu))
+    for x, is_v in ((k, False), (v, True)):
+        got = ref.unpack(c, 1, is_v)[0, :12]
+        bad = ~torch.isfinite(x[:, 0].reshape(12, 3, 32)).all(-1)
+        assert torch.equal(torch.isnan(got.reshape(12, 3, 32)).all(-1), bad)
+        assert torch.isfinite(got.reshape(12, 3, 32)[~bad]).all()
+
+
 # ----------------------------------------------------------- attention
 
 SHAPES = [(64, 16), (96, 32), (128, 64), (192, 128), (256, 256), (512, 64)]
@@ -668,3 +682,169 @@ def test_verify_draws_the_target(gpu):
     seen = torch.bincount(tokens[:, 0].cpu().long(), minlength=V).double()
     want = S * p1.double()
     assert float(((seen - want) ** 2 / want).sum()) < 50
+
+
+# ------------------------------------------------------------ together
+
+class Step:
+    """A decode / verify step of a two-layer sandwich-normed model as a user
+    runs it: the norms and the residual stream between attention and the MoE
+    layer, the cache of every layer behind one page table, and the verification of
+    the step's drafts against the model's own probabilities."""
+    EPS = 1e-6
+
+    def __init__(self, gpu, spec, n_seq, width, page):
+        from helpers import layer
+        D, self.H, self.G, self.hd = spec.d_model, 2, 4, 64
+        g = torch.Generator().manual_seed(77)
+        mat = lambda *s: (torch.randn(*s, generator=g) / math.sqrt(s[0])).to(gpu)
+        w = lambda: (1 + 0.1 * torch.randn(D, generator=g)).to(gpu)
+        nh = self.H * self.G
+        self.layers = [dict(qkv=mat(D, (nh + 2 * self.H) * self.hd), o=mat(nh * self.hd, D), attn_in=w(), attn_out=w(), moe_in=w(),
+                            router_in=w(), moe_out=w(), scale=0.9 + 0.1 * i,
+                            moe=la.DeviceLayer(layer(spec, 40 + i, [1, 4, 6, 9, 12], scales=True), gpu),
+                            cache=la.KvCache.empty(n_seq * width + 4, page, self.H, self.hd, la.F16, gpu)) for i in range(2)]
+        self.final, self.head = w(), mat(D, 300)
+        self.pages = la.KvPages([l["cache"] for l in self.layers])
+
+    def run(self, h, batch, record=None):
+        """Probabilities [T, vocab] of the new tokens' embeddings h [T, D]."""
+        T, nh = h.shape[0], self.H * self.G
+        note = record if record is not None else lambda *a: None
+        h, (x,) = la.block_norm(h, weights=[self.layers[0]["attn_in"]], eps=self.EPS)
+        for i, l in enumerate(self.layers):
+            qkv = (x @ l["qkv"]).view(T, nh + 2 * self.H, self.hd)
+            q, k, v = qkv[:, :nh], qkv[:, nh:nh + self.H], qkv[:, nh + self.H:]
+            l["cache"].append(batch, k, v)
+            a = l["cache"].attention(batch, q, window=40 if i else 0)
+            note("attention", i, q, k, v, a)
+            y = a.reshape(T, -1) @ l["o"]
+            h2, xs = la.block_norm(h, y, post_weight=l["attn_out"], weights=[l["moe_in"], l["router_in"]], eps=self.EPS)
+            note("norm", h, y, l["attn_out"], 1.0, [l["moe_in"], l["router_in"]], h2, xs)
+            m, _, _ = l["moe"].forward(xs[0], x_router=xs[1])
+            then = self.layers[1]["attn_in"] if i == 0 else self.final
+            h3, (x,) = la.block_norm(h2, m, post_weight=l["moe_out"], alpha=l["scale"], beta=l["scale"], weights=[then], eps=self.EPS)
+            note("norm", h2, m, l["moe_out"], l["scale"], [then], h3, [x])
+            h = h3
+        return torch.softmax(x @ self.head, -1)
+
+
+def test_decode_steps_together(gpu):
+    """Prompts appended, a verify step of four tokens a sequence, one sequence
+    forked and another freed, the pool compacted, and single-token steps: every
+    stage of every step against its 64-bit form on the stage's own inputs, and a
+    captured step's replays bit for bit against eager ones."""
+    from helpers import SMALL
+    n_seq, width, page = 4, 8, 16
+    m = Step(gpu, SMALL, n_seq, width, page)
+    g = torch.Generator().manual_seed(78)
+    emb = torch.randn(300, SMALL.d_model, generator=g).to(gpu)
+    history = [[(torch.zeros(0, m.H, m.hd),) * 2 for _ in range(n_seq)] for _ in m.layers]      # of each layer and sequence, fp16
+
+    def check(starts, lens):
+        def record(kind, *a):
+            if kind == "norm":
+                h, y, post, scale, weights, h2, xs = a
+                up = lambda t: t.cpu()
+                want_h, want_x = ref.block_norm(up(h), up(y), up(post), True, None, scale, scale, [up(w) for w in weights], m.EPS)
+                u = ref.block_norm(0 * up(h), up(y), up(post), True, None, scale, scale, (), m.EPS)[0]
+                mag = scale * up(h).double().abs() + u.abs()
+                for x, want, w in zip(xs, want_x, weights):
+                    bh, bx = norm_bound(want_h, want, mag, up(w), la.F32, scale, scale, h.shape[1])
+                    assert ((up(x).double() - want).abs() <= bx).all()
+                assert ((up(h2).double() - want_h).abs() <= bh).all()
+                return
+            i, q, k, v, out = a
+            q, k, v, out = (t.cpu() for t in (q, k, v, out))
+            for s in range(n_seq):
+                rows = slice(starts[s], starts[s + 1])
+                hk, hv = history[i][s]
+                history[i][s] = (torch.cat([hk, k[rows].half().float()]), torch.cat([hv, v[rows].half().float()]))
+            cache = m.layers[i]["cache"]
+            want, _, tol = ref.attention(cache, table.tolist(), lens, starts, q, m.hd ** -0.5, 40 if i else 0)
+            assert ((out.double() - want).abs() <= tol).all()
+            for s in range(n_seq):                   # and the cache holds what was appended, where the table says
+                ck, cv, there = ref.sequence(cache, table.tolist()[s], lens[s])
+                assert there.all() and torch.equal(ck.transpose(0, 1).float(), history[i][s][0])
+                assert torch.equal(cv.transpose(0, 1).float(), history[i][s][1])
+        return record
+
+    order = torch.randperm(n_seq * width + 4, generator=g).tolist()
+    table = i32([[order.pop() for _ in range(width)] for _ in range(n_seq)], gpu)
+    spare = order.pop()
+
+    def step(new, tokens, lens):
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        b = la.KvBatch(table, i32(lens, gpu), i32(starts, gpu), n_tokens=starts[-1], max_new=max(new))
+        return m.run(emb[tokens], b, check(starts, lens)), starts
+
+    # prompts of ragged lengths, 16 tokens a call
+    lens, prompt = [0] * n_seq, [50, 17, 0, 33]
+    while any(a < b for a, b in zip(lens, prompt)):
+        new = [min(16, b - a) for a, b in zip(lens, prompt)]
+        lens = [a + n for a, n in zip(lens, new)]
+        step(new, torch.randint(0, 300, (sum(new),), generator=g), lens)
+    # a verify step: the last token and three drafts of each living sequence
+    new = [4, 4, 0, 4]
+    lens = [a + n for a, n in zip(lens, new)]
+    tok = torch.randint(0, 300, (12,), generator=g).to(torch.int32)
+    p, _ = step(new, tok.long(), lens)
+    u, un = torch.rand(3, 3, generator=g), torch.rand(3, generator=g)
+    drafts = tok.reshape(3, 4)[:, 1:].contiguous()
+    target = p.reshape(3, 4, 300)
+    got, taken = la.verify_drafts(target, None, drafts.to(gpu), u.to(gpu), un.to(gpu))
+    want, want_taken = ref.verify(target.cpu(), None, drafts, u, un, None)
+    assert got.tolist() == want and taken.tolist() == want_taken
+    # refused drafts leave the cache by their length alone
+    for s, a in zip((0, 1, 3), want_taken):
+        lens[s] -= 3 - a
+        for i in range(2):
+            history[i][s] = tuple(t[:lens[s]] for t in history[i][s])
+    # sequence 0 is forked into row 2, sequence 1 ends, and the pool is compacted
+    ln = i32(lens, gpu)
+    m.pages.fork(table, ln, i32([[0, 2, spare]], gpu))
+    lens[2] = lens[0]
+    lens[1] = 0
+    ln[1] = 0
+    for i in range(2):
+        history[i][2], history[i][1] = history[i][0], history[i][1]
+        history[i][1] = (torch.zeros(0, m.H, m.hd),) * 2
+    refs, _, n_free = m.pages.refs(table, ln)
+    _, after, n_live = m.pages.compact(table, ln, table_out=table)
+    used = int(n_live)
+    assert used + int(n_free) == m.pages.n_pages and int(refs.sum()) == int(after.sum()) == sum(-(-n // page) for n in lens)
+    assert ln.tolist() == lens
+    # room to grow: the free pages lie behind the live ones
+    free = iter(range(used, m.pages.n_pages))
+    rows = table.tolist()
+    for s in range(n_seq):
+        for i in range(-(-lens[s] // page), width):
+            rows[s][i] = next(free, -1)
+    # the fork's partly filled last page is its own
+    if lens[0] % page:
+        assert rows[0][lens[0] // page] != rows[2][lens[0] // page]
+    table.copy_(i32(rows, gpu))
+    # single-token steps; lengths that the table holds
+    for _ in range(3):
+        new = [1, 0, 1, 1]
+        lens = [a + n for a, n in zip(lens, new)]
+        step(new, torch.randint(0, 300, (3,), generator=g), lens)
+    # the step as a graph: every replay against the eager step
+    ln, st = i32(lens, gpu), i32([0, 1, 1, 2, 3], gpu)
+    b = la.KvBatch(table, ln, st, n_tokens=3, max_new=1)
+    x = emb[:3].clone()
+    eager = m.run(x, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.run(x, b)
+    for k in range(3):
+        x.copy_(emb[10 * k:10 * k + 3])
+        ln.add_(torch.tensor([1, 0, 1, 1], dtype=torch.int32, device=gpu))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, m.run(x, b))
+    assert torch.isfinite(eager).all()

@@ -49,7 +49,7 @@ def batch(**kw):
 
 
 def query(**kw):
-    a = dict(type=la.F32, n_head=4, window=0, scale=0.125, q=P, q_stride=256, out=P, out_stride=256, lse=None)
+    a = dict(type=la.F32, n_head=4, window=0, scale=0.125, q=P, q_stride=256, out=2 * P, out_stride=256, lse=None)
     a.update(kw)
     return _lib.LlapisKvQuery(**a)
 
@@ -82,7 +82,7 @@ def test_batch_refusals(bad):
 
 @pytest.mark.parametrize("bad", [dict(type=la.Q8_0), dict(n_head=3), dict(n_head=0), dict(n_head=2048), dict(window=-1),
                                  dict(scale=float("nan")), dict(q=None), dict(out=None), dict(q=P + 4),
-                                 dict(q_stride=258), dict(out_stride=250)], ids=str)
+                                 dict(q_stride=258), dict(out_stride=250), dict(out=P)], ids=str)
 def test_query_refusals(bad):
     c, b, q = cache(), batch(n_seq=2, n_tokens=2), query(**bad)
     refused(la.lib().llapis_kv_attention(C.byref(c), C.byref(b), C.byref(q), P, 1 << 40, None), "llapis_kv_attention")
