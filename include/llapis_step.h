@@ -55,8 +55,8 @@ uint64_t llapis_kv_page_bytes(int32_t type, int32_t n_kv, int32_t head_dim, int3
  * them, on the pages page_table[s * table_stride + i] (token t: entry
  * t / page_size).  Its new tokens are rows new_start[s] .. new_start[s + 1] - 1
  * of the step's activations, the last of its tokens in order (new_start NULL:
- * row s alone).  All three arrays are read on the device when the call runs; a
- * sequence may have no token or no new one.  The host gives the bounds:
+ * row s alone).  All three arrays are read on the device when the call runs, and
+ * stay as they are until it has; a sequence may have no token or no new one.  The host gives the bounds:
  * n_tokens rows, max_new new tokens of a sequence, max_pages table entries a
  * row.  What lies beyond them is not touched: rows past n_tokens, new tokens
  * past max_new of a sequence, keys past max_pages * page_size.  A table entry
@@ -108,7 +108,8 @@ int32_t  llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * 
  *
  * Operations on whole pages, the same in every plane: a plane is one layer's
  * K or V pool, pages of `bytes` bytes (a multiple of 16) `stride` apart.  More
- * planes than LLAPIS_KV_MAX_PLANES take several calls. */
+ * planes than LLAPIS_KV_MAX_PLANES take several calls.  n_pages and max_pages are
+ * 2^30 at most. */
 #define LLAPIS_KV_MAX_PLANES 128
 typedef struct llapis_kv_planes {
     int32_t n_planes, n_pages, page_size;
@@ -209,7 +210,8 @@ int32_t llapis_block_norm(const llapis_block_norm_args * a, void * stream);
  * finite count as 0, a draft outside the vocabulary is not taken; n_draft is
  * clamped to 0 .. max_draft.  tokens [n_seq][max_draft + 1] receives the taken
  * drafts, the next token and -1 behind it, accepted [n_seq] the number a.  The
- * next token is -1 where the target row has no positive value. */
+ * next token is -1 where the target row has no positive value.  n_seq is 65535
+ * at most, max_draft 63, vocab 2^30 (the workspace size of more is 0). */
 typedef struct llapis_verify_args {
     int32_t type;                  /* LLAPIS_T_F32, LLAPIS_T_F16 or LLAPIS_T_BF16 */
     int32_t n_seq, max_draft, vocab;

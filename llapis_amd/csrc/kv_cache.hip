@@ -274,6 +274,8 @@ void launch_append(const KvAppend & p, dim3 grid, hipStream_t s) {
 
 // --------------------------------------------------------------- pages
 
+// counts that loops run up to leave room for their steps in 32 bits
+constexpr int KV_MAX_COUNT = 1 << 30;
 constexpr int PG_CHUNK = 16384;                                   // bytes a workgroup copies at a time
 
 // bytes [at, at + PG_CHUNK) of a page of `plane`, from one page to another:
@@ -565,7 +567,7 @@ const char * plan_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
 const char * check_planes(const llapis_kv_planes * p, int & chunks) {
     if (!p) return "null planes";
     if (p->n_planes <= 0 || p->n_planes > LLAPIS_KV_MAX_PLANES) return "need 0 < n_planes <= 128";
-    if (p->n_pages <= 0 || p->page_size <= 0) return "need n_pages > 0 and page_size > 0";
+    if (p->n_pages <= 0 || p->n_pages > KV_MAX_COUNT || p->page_size <= 0) return "need 0 < n_pages <= 2^30 and page_size > 0";
     uint64_t most = 0;
     for (int i = 0; i < p->n_planes; ++i) {
         if (!p->base[i] || !aligned16(p->base[i]) || p->stride[i] % 16 || p->bytes[i] % 16 || !p->bytes[i] ||
@@ -580,7 +582,7 @@ const char * check_planes(const llapis_kv_planes * p, int & chunks) {
 
 const char * check_table(const void * table, int64_t stride, int max_pages, const void * lens, int n_seq) {
     if (n_seq < 0) return "negative n_seq";
-    if (max_pages <= 0 || stride < max_pages) return "need 0 < max_pages <= table_stride";
+    if (max_pages <= 0 || max_pages > KV_MAX_COUNT || stride < max_pages) return "need 0 < max_pages <= table_stride, max_pages <= 2^30";
     if (n_seq > 0 && (!table || !lens)) return "null page table or lengths";
     return nullptr;
 }
@@ -746,7 +748,7 @@ int32_t llapis_kv_page_refs(int32_t n_pages, int32_t page_size, const int32_t * 
                             int32_t max_pages, const int32_t * lens, int32_t n_seq, int32_t * refs, int32_t * free_pages,
                             int32_t * n_free, void * stream) {
     const char * bad = check_table(page_table, table_stride, max_pages, lens, n_seq);
-    if (!bad && (n_pages <= 0 || page_size <= 0)) bad = "need n_pages > 0 and page_size > 0";
+    if (!bad && (n_pages <= 0 || n_pages > KV_MAX_COUNT || page_size <= 0)) bad = "need 0 < n_pages <= 2^30 and page_size > 0";
     if (!bad && !refs) bad = "null refs";
     if (bad) return refuse_as("llapis_kv_page_refs", bad);
     hipStream_t s = (hipStream_t)stream;
@@ -758,7 +760,7 @@ int32_t llapis_kv_page_refs(int32_t n_pages, int32_t page_size, const int32_t * 
     return 0;
 }
 
-uint64_t llapis_kv_compact_workspace_size(int32_t n_pages) { return n_pages > 0 ? ((uint64_t)n_pages * 4 + 1) * 4 : 0; }
+uint64_t llapis_kv_compact_workspace_size(int32_t n_pages) { return n_pages > 0 && n_pages <= KV_MAX_COUNT ? ((uint64_t)n_pages * 4 + 1) * 4 : 0; }
 
 int32_t llapis_kv_compact(const llapis_kv_planes * p, const int32_t * page_table, int64_t table_stride, int32_t max_pages,
                           const int32_t * lens, int32_t n_seq, int32_t * table_out, int32_t * refs, int32_t * n_live,

@@ -449,12 +449,14 @@ hipError_t launch_norm(const llapis_block_norm_args & a, hipStream_t s) {
     while (threads < 1024 && (quads + threads - 1) / threads > 4) threads *= 2;
     const int nch = (quads + threads - 1) / threads;
     const int held = 256 * 1024 / threads;
-    const int each = (a.n_tokens + held - 1) / held, grid = (a.n_tokens + each - 1) / each;
+    const int each = (a.n_tokens - 1) / held + 1, grid = (a.n_tokens - 1) / each + 1;
     if (a.n_out <= 1) launch_norm_chunks<T, 1>(a, nch, threads, grid, s);
     else if (a.n_out == 2) launch_norm_chunks<T, 2>(a, nch, threads, grid, s);
     else launch_norm_chunks<T, 4>(a, nch, threads, grid, s);
     return hipGetLastError();
 }
+
+constexpr int VER_MAX_SEQ = 65535, VER_MAX_VOCAB = 1 << 30;
 
 // a sequence's sums, then its verdict
 uint64_t verify_sums_bytes(int n_seq, int vocab) { return (uint64_t)n_seq * verify_segments(vocab) * sizeof(Sums); }
@@ -502,14 +504,14 @@ int32_t llapis_block_norm(const llapis_block_norm_args * a, void * stream) {
 }
 
 uint64_t llapis_verify_drafts_workspace_size(int32_t n_seq, int32_t vocab) {
-    return n_seq <= 0 || vocab <= 0 ? 0 : verify_sums_bytes(n_seq, vocab) + (uint64_t)n_seq * sizeof(Verdict);
+    return n_seq <= 0 || n_seq > VER_MAX_SEQ || vocab <= 0 || vocab > VER_MAX_VOCAB ? 0 : verify_sums_bytes(n_seq, vocab) + (uint64_t)n_seq * sizeof(Verdict);
 }
 
 int32_t llapis_verify_drafts(const llapis_verify_args * a, void * workspace, uint64_t ws_bytes, void * stream) {
     const char * who = "llapis_verify_drafts";
     if (!a) return refuse_as(who, "null arguments");
     if (a->type != T_F32 && a->type != T_F16 && a->type != T_BF16) return refuse_as(who, "need type F32, F16 or BF16");
-    if (a->n_seq < 0 || a->n_seq > 65535 || a->max_draft < 0 || a->max_draft > 63 || a->vocab <= 0 || a->vocab > 1 << 30)
+    if (a->n_seq < 0 || a->n_seq > VER_MAX_SEQ || a->max_draft < 0 || a->max_draft > 63 || a->vocab <= 0 || a->vocab > VER_MAX_VOCAB)
         return refuse_as(who, "need 0 <= n_seq <= 65535, 0 <= max_draft <= 63, 0 < vocab <= 2^30");
     if (a->n_seq == 0) return 0;
     if (!a->target || !a->u_next || !a->tokens || !a->accepted || (a->max_draft > 0 && (!a->drafts || !a->u)))

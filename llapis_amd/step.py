@@ -52,6 +52,13 @@ def _is(t, dtype, shape, dev, what):
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
 
 
+def _count(*values):
+    """Sizes as the library takes them: a larger one would wrap around in 32 bits."""
+    for x in values:
+        if not 0 <= x < 1 << 31:
+            raise ValueError(f"a size of {x} is negative or 2^31 and more")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -94,6 +101,7 @@ class KvBatch:
         else:
             _need(max_new == 1 and n_tokens in (None, n), "without new_start every sequence has one new token")
             n_tokens = n
+        _count(n, n_tokens, max_new, page_table.shape[1])
         self.page_table, self.lens, self.new_start = page_table, lens, new_start
         self.n_seq, self.n_tokens, self.max_new, self.max_pages = n, n_tokens, max_new, page_table.shape[1]
         self.struct = L.LlapisKvBatch(n, n_tokens, max_new, self.max_pages, max(page_table.stride(0), self.max_pages),
@@ -125,6 +133,7 @@ class KvCache:
             need = int(lib().llapis_kv_page_bytes(tag, H, D, P))
             _need(k.shape[1] == need and v.shape == k.shape and k.stride(1) == 1 and v.stride(1) == 1,
                   f"a page must be {need} contiguous bytes")
+        _count(n_pages, H, P, D)
         es = k.element_size()
         self.k, self.v, self.type = k, v, tag
         self.n_pages, self.n_kv, self.page_size, self.head_dim = n_pages, H, P, D
@@ -175,7 +184,8 @@ class KvCache:
         cache they have been appended to -> out, shaped and typed as q.  scale:
         head_dim ** -0.5 by default; window > 0: each token sees that many keys at
         most, itself the last; lse [rows, n_head] float32 receives the logarithm
-        of the softmax sums.  Rows of no sequence are left as they are."""
+        of the softmax sums.  Rows of no sequence are left as they are (in an
+        out made here: as the allocation holds them)."""
         torch = _torch()
         _need(q.dim() == 3 and batch.device == self.device, "q must be [n_tokens, n_head, head_dim], the batch on its device")
         n_head = q.shape[1]
@@ -191,6 +201,7 @@ class KvCache:
                   "lse must be a contiguous float32 [n_tokens, n_head]")
         if workspace is None:
             workspace = self.attention_workspace(batch, n_head)
+        _count(window)
         _need(workspace.device == self.device and workspace.is_contiguous(), "the workspace must be contiguous and on the cache's device")
         a = L.LlapisKvQuery(_tag(q.dtype), n_head, window, self.head_dim ** -0.5 if scale is None else scale,
                             q.data_ptr(), qs, out.data_ptr(), os_, _ptr(lse))
@@ -227,11 +238,13 @@ class KvPages:
                 or page_table.device != self.device):
             raise ValueError(f"page_table must be int32 [n_seq, max_pages] on {self.device}, rows of consecutive entries")
         _is(lens, torch.int32, (shape[0],), self.device, "lens")
+        _count(*shape)
         return page_table.data_ptr(), max(stride[0], shape[1]), shape[1]
 
     def copy(self, pairs):
         """Copy page pairs[i, 0] to page pairs[i, 1] (int32 [n, 2] on the GPU) in every layer."""
         _is(pairs, _torch().int32, (pairs.shape[0], 2), self.device, "pairs")
+        _count(pairs.shape[0])
         for s in self.structs:
             _call("llapis_kv_copy_pages", self.device, C.byref(s), pairs.data_ptr(), pairs.shape[0])
 
@@ -241,6 +254,7 @@ class KvPages:
         partly filled last one.  Updates page_table and lens."""
         table, stride, width = self._table(page_table, lens)
         _is(forks, _torch().int32, (forks.shape[0], 3), self.device, "forks")
+        _count(forks.shape[0])
         for s in self.structs:
             _call("llapis_kv_fork", self.device, C.byref(s), table, stride, width, lens.data_ptr(), page_table.shape[0],
                   forks.data_ptr(), forks.shape[0])
@@ -302,6 +316,7 @@ def block_norm(h, y=None, post_weight=None, post_norm=True, gate=None, alpha=1.0
     shape, dtype, dev = h.shape, h.dtype, _on_gpu(h, "h")
     _need(len(shape) == 2 and h.stride(1) == 1, "h must be [T, d], rows of consecutive values")
     T, d = shape
+    _count(T, d)
 
     def row(t, what):
         stride = t.stride()
@@ -355,6 +370,7 @@ def verify_drafts(target, draft, drafts, u, u_next, n_draft=None, tokens=None, a
     shape, dtype, dev = target.shape, target.dtype, _on_gpu(target, "target")
     _need(len(shape) == 3 and shape[1] > 0, "target must be [n_seq, drafts + 1, vocab]")
     S, n, V = shape[0], shape[1] - 1, shape[2]
+    _count(S, n, V)
 
     def rows(t, k, what):
         stride = t.stride()

@@ -848,3 +848,32 @@ def test_decode_steps_together(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out, m.run(x, b))
     assert torch.isfinite(eager).all()
+
+
+# ------------------------------------------------------------ the largest
+def test_sizes_past_32_bits_are_refused(gpu):
+    """The library's sizes have 32 bits: what is larger would wrap around to a size that fits."""
+    c = la.KvCache.empty(4, 16, 2, 64, la.F16, gpu)
+    table, lens = i32([[0, 1]], gpu), i32([5], gpu)
+    with pytest.raises(ValueError, match="2\\^31"):
+        c.attention(la.KvBatch(table, lens), torch.zeros(1, 4, 64, device=gpu), window=(1 << 32) + 1)
+    for n_tokens, max_new in (((1 << 32) + 1, 1), (1, (1 << 32) + 1), (-1, 1), (1, -1)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            la.KvBatch(table, lens, i32([0, 1], gpu), n_tokens, max_new)
+    with pytest.raises(ValueError, match="2\\^31"):
+        la.block_norm(torch.zeros(1, 1, device=gpu).expand((1 << 32) + 1, 1))
+    with pytest.raises(ValueError, match="2\\^31"):
+        la.verify_drafts(torch.zeros(1, 1, 1, device=gpu).expand(1, 1, (1 << 32) + 1), None, torch.zeros(1, 0, dtype=torch.int32, device=gpu),
+                         torch.zeros(1, 0, device=gpu), torch.zeros(1, device=gpu))
+
+
+def test_block_norm_most_tokens(gpu):
+    """2^31 - 1 tokens: no count wraps around on the way to the launch, and each token is written."""
+    T = (1 << 31) - 1
+    h = torch.tensor([[3.0]], device=gpu, dtype=torch.float16).expand(T, 1)
+    out = torch.zeros(T, 1, dtype=torch.float16, device=gpu)
+    w = torch.tensor([4.0], device=gpu)
+    h_out, _ = la.block_norm(h, weights=[w], eps=7.0, out=[out])         # 3, 3 / sqrt(9 + 7) * 4 = 3
+    for x in (h_out, out):
+        for at in range(0, T, 1 << 29):
+            assert bool((x[at:at + (1 << 29)] == 3.0).all())

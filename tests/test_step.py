@@ -214,3 +214,17 @@ def test_python_refuses_host_tensors():
         la.block_norm(torch.zeros(2, 64))
     with pytest.raises(ValueError, match="GPU"):
         la.verify_drafts(torch.zeros(1, 2, 10), None, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 1), torch.zeros(1))
+
+
+def test_largest_counts():
+    """Counts that loops would run past 32 bits with are refused, and have no workspace."""
+    lib, big = la.lib(), (1 << 30) + 1
+    refused(lib.llapis_kv_page_refs(big, 16, P, 4, 4, P, 2, P, P, P, None), "n_pages")
+    refused(lib.llapis_kv_page_refs(4, 16, P, big, big, P, 2, P, P, P, None), "max_pages")
+    refused(lib.llapis_kv_fork(C.byref(planes()), P, big, big, P, 2, P, 1, None), "max_pages")
+    refused(lib.llapis_kv_copy_pages(C.byref(planes(n_pages=big)), P, 1, None), "n_pages")
+    assert lib.llapis_kv_compact_workspace_size(big) == 0
+    assert lib.llapis_kv_compact_workspace_size(1 << 30) == ((4 << 30) + 1) * 4
+    assert lib.llapis_verify_drafts_workspace_size(1, big) == 0 == lib.llapis_verify_drafts_workspace_size(1 << 16, 10)
+    assert lib.llapis_verify_drafts_workspace_size(1, (1 << 31) - 1) == 0
+    assert lib.llapis_verify_drafts_workspace_size(1, 1 << 30) > 0
