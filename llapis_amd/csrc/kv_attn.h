@@ -39,6 +39,21 @@
 // q8_0's loads are 16 bytes a lane too: of a K row the lane's 16 values go to two
 // products, and of a V column 16 keys, so that the products' order of values and
 // of keys is another (Q and P are laid out to it).
+//
+// What bounds it.  Long caches: memory.  TB/s of K and V (a kernel that only reads
+// reaches 6.2): head size 64 5.4, 128 5.6 (pages of 16 tokens 5.4), 256 5.4, 512
+// 5.5; with two row tiles 5.3, at 512 4.7 (its P takes as many instructions as its
+// loads); q8_0 5.0 to 5.2, at 512 4.9 (the conversions).  Short ones: the chain of
+// lengths, page table, K, scores, V, result, each a memory latency: 7.7 us for 700
+// keys, and 24.6 us for 11203 keys of head size 512, of which a workgroup's unit is
+// 256 KB.  What the choices were worth (us of the kernel):
+//   the line in half units, a half for each piece    48 ragged sequences   49 -> 45
+//   eight waves instead of four at head size 512     11203 keys            29 -> 25
+//   q8_0: two fp16 parts instead of three bf16       2 x 131072 keys     203 -> 172
+//   q8_0: 16-byte loads instead of 8                                     172 -> 118
+// As many runs as the card holds at once are enough: twice or three times as many
+// took 129 and 142 us instead of 124 for the 131072 keys, their units being shared
+// out evenly already.
 #pragma once
 
 #include <type_traits>

@@ -15,7 +15,11 @@ namespace dev {
 // workgroup takes 1024 / PG values of an item's tile, four a thread; its PG
 // groups of threads take every PG-th part, each under a running maximum of its
 // own, and are added in their order.  A part is read once, its maximum and sum
-// with its values, so that the loads of several parts are in flight.
+// with its values, so that the loads of several parts are in flight (a first pass
+// over the maxima, then the values: 4 tokens of 11203 keys with the attention
+// kernel 71 us, so 38).  A launch and a chain of four loads: 4.6 us for 700 keys,
+// 6.5 for the 177 parts of 11203, 8.5 for 48 sequences.  It is a kernel of its own
+// because no workgroup here waits for another one.
 template <int PG>
 __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, float p_shift) {
     constexpr int TPG = 256 / PG;
@@ -104,7 +108,10 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, f
 // written as they lie.  V: a thread converts a column's eight consecutive
 // positions, which are one 16-byte store in the transposed page; at the ends of a
 // run the positions that the call brings are stored one by one.  A thread asks for
-// all its values before it converts the first.
+// all its values before it converts the first.  Bound by memory: 2048 prompt tokens
+// of 8 heads of 256 from F32 into F16, 50 MB, 12.1 us (15 with K and V in one
+// workgroup; a large copy's rate would be 10); 4 tokens of 48 sequences 4.4 us, a
+// launch and three dependent loads.
 constexpr int APP_POS = 32;
 
 struct KvAppend {
@@ -278,8 +285,9 @@ void launch_append(const KvAppend & p, dim3 grid, hipStream_t s) {
 constexpr int KV_MAX_COUNT = 1 << 30;
 constexpr int PG_CHUNK = 16384;                                   // bytes a workgroup copies at a time
 
-// bytes [at, at + PG_CHUNK) of a page of `plane`, from one page to another:
-// four 128-bit loads in flight a lane
+// bytes [at, at + PG_CHUNK) of a page of `plane`, from one page to another: four
+// 128-bit loads in flight a lane.  Bound by memory: a compaction's moves of
+// 500 MB take 92 us, 5.5 TB/s of reads and writes; a large copy's rate is 5.0.
 __device__ __forceinline__ void copy_chunk(const llapis_kv_planes & p, int plane, int from, int to, uint64_t at) {
     const uint64_t n = p.bytes[plane];
     if (at >= n) return;
@@ -433,7 +441,9 @@ __global__ __launch_bounds__(SCAN_WG) void k_kv_plan(const int32_t * refs, int n
 }
 
 // All of the above for a pool and a table that one workgroup goes through in the
-// time of a few launches: the counts are in LDS.
+// time of a few launches: the counts are in LDS.  1024 pages and 64 sequences:
+// 11.8 us; four kernels' launches, 3.9 us each, are more than that.  (8192 counts are
+// 32 KB of LDS, 65536 entries 64 a thread.)
 constexpr int SMALL_PAGES = 8192, SMALL_ENTRIES = 65536;
 
 __global__ __launch_bounds__(SCAN_WG) void k_kv_plan_small(const int32_t * table, int64_t table_stride, int max_pages,

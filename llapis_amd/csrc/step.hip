@@ -57,6 +57,11 @@ __device__ __forceinline__ void put4(T * p, int i, int n, f4 x) {
 // weights, which it reads once for all its tokens.  The next token's values are
 // asked for before this one's sums.  The squares are summed per thread in order,
 // then over the wave, then over the waves in order.
+//
+// Bound by memory: 11200 tokens of 2816 bf16 values, a gate and two outputs, 69 us
+// (4.6 TB/s; a copy reaches 5.0), 88 with a workgroup a token, which reads the
+// weights each time.  4 tokens of F32: 4.7 us, a launch and the chain of one load,
+// two sums over the workgroup and a store.
 
 __device__ __forceinline__ float block_sum(float x, float * s_part) {
     for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, 64);
@@ -174,9 +179,16 @@ __global__ __launch_bounds__(THREADS) void k_block_norm(const llapis_block_norm_
 // k_verify_sum: every workgroup finds the number of taken drafts anew (a few
 // loads) and sums 4 segments of 1024 values of the row the next token comes from,
 // r, and p for the case that r is 0 everywhere.  (16 loads of 16 bytes a lane in two
-// batches, or in one at three waves a SIMD, took twice the time of one batch of 8.)  k_verify_pick: one workgroup a
-// sequence adds the segments in order, finds the one where the sum passes u_next
-// of the whole, and in it the token.
+// batches, or in one at three waves a SIMD, took twice the time of one batch of 8.)
+// k_verify_pick: one workgroup a sequence adds the segments in order, finds the one
+// where the sum passes u_next of the whole, and in it the token.
+//
+// Only the rows that the verdict names are read, about 50 MB for 32 sequences of
+// 262144 values: 11.5 and 4.5 us, 27 together with more batches of loads and with
+// LDS atomics for the pick's votes.  What bounds them is the chain: a sequence's
+// verdict (two dependent loads), its rows, its sums, the segment's values again.  One
+// sequence of 32003: 7.4 us together; one kernel of one workgroup, which saves a
+// launch, took 9.9, its rows coming through one CU.
 
 constexpr int VER_SEG = 1024;                   // values of a segment: 16 a lane, four a thread of the pick
 constexpr int VER_RUN = 4 * VER_SEG;            // values of a workgroup, a segment a wave
