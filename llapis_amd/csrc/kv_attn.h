@@ -42,8 +42,8 @@
 //
 // What bounds it.  Long caches: memory.  TB/s of K and V (a kernel that only reads
 // reaches 6.2): head size 64 5.4, 128 5.6 (pages of 16 tokens 5.4), 256 5.4, 512
-// 5.5; with two row tiles 5.3, at 512 4.7 (its P takes as many instructions as its
-// loads); q8_0 5.0 to 5.2, at 512 4.9 (the conversions).  Short ones: the chain of
+// 5.5; with two row tiles 5.3, at 512 4.7; q8_0 5.0 to 5.2, at 512 4.9 (its
+// conversions keep the VALU half busy).  Short ones: the chain of
 // lengths, page table, K, scores, V, result, each a memory latency: 7.7 us for 700
 // keys, and 24.6 us for 11203 keys of head size 512, of which a workgroup's unit is
 // 256 KB.  What the choices were worth (us of the kernel):
