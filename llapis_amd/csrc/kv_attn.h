@@ -241,6 +241,20 @@ __device__ __forceinline__ uint32_t pair_mask(uint32_t bits, int i) {
     return (a & 0xFFFFu) | (b & 0xFFFF0000u);
 }
 
+// A CU serves its oldest workgroup first: of three that share a CU for a whole long
+// call the first ended at 84 us, the last at 106, when it had the CU to itself.  With a
+// unit each at every priority in turn they go on together (TB/s of long caches: head
+// size 64 5.34 -> 5.46, 128 5.53 -> 5.61, 256 5.33 -> 5.44; q8_0 5.0 -> 5.2, 5.1 ->
+// 5.35; two or one to a CU: no difference).
+__device__ __forceinline__ void priority_in_turn(int turn) {
+    switch (turn & 3) {
+        case 0: __builtin_amdgcn_s_setprio(0); break;
+        case 1: __builtin_amdgcn_s_setprio(1); break;
+        case 2: __builtin_amdgcn_s_setprio(2); break;
+        default: __builtin_amdgcn_s_setprio(3);
+    }
+}
+
 constexpr float KV_LN2 = 0.69314718055994530942f, KV_LOG2E = 1.44269504088896340736f;
 
 // WIDE: fp32 results (q8_0: fp32 and fp16 ones)
@@ -512,6 +526,7 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
         int lv = lm;
         for (int key = cur.key_begin; key < key_end; key += UNIT) {
             asm volatile("" : "+v"(lv));              // V's offsets are formed anew, not held
+            if constexpr (kv_wgs(HD, NT) > 2) priority_in_turn(key / UNIT + (int)(blockIdx.x >> 8));
             bool full = key + UNIT <= min(all_to, key_end) && key >= all_from;
             uint32_t ok = 0;                          // bit i: the keys of the lane's load i have a page
             const uint8_t * va[NVL];
