@@ -41,8 +41,8 @@
 // of keys is another (Q and P are laid out to it).
 //
 // What bounds it.  Long caches: memory.  TB/s of K and V (a kernel that only reads
-// reaches 6.2): head size 64 5.4, 128 5.6 (pages of 16 tokens 5.4), 256 5.4, 512
-// 5.5; with two row tiles 5.3, at 512 4.7; q8_0 5.0 to 5.2, at 512 4.9 (its
+// reaches 6.2): head size 64 5.5, 128 5.6 (pages of 16 tokens 5.4), 256 5.4, 512
+// 5.3; with two row tiles 5.3, at 512 4.5; q8_0 5.2 to 5.35, at 512 4.9 (its
 // conversions keep the VALU half busy).  Short ones: the chain of
 // lengths, page table, K, scores, V, result, each a memory latency: 7.7 us for 700
 // keys, and 24.6 us for 11203 keys of head size 512, of which a workgroup's unit is
@@ -52,8 +52,10 @@
 //   q8_0: two fp16 parts instead of three bf16       2 x 131072 keys     203 -> 172
 //   q8_0: 16-byte loads instead of 8                                     172 -> 118
 // As many runs as the card holds at once are enough: twice or three times as many
-// took 129 and 142 us instead of 124 for the 131072 keys, their units being shared
-// out evenly already.
+// took 129 and 142 us instead of 124 for the 131072 keys.  Units are not parted
+// between runs: ends at a half of one (a quarter) took 55 to 59 (65) us instead of 53
+// for the 48 sequences with their join, since what a part of a unit costs is its chain
+// of latencies.
 #pragma once
 
 #include <type_traits>
