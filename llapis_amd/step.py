@@ -53,7 +53,8 @@ def _is(t, dtype, shape, dev, what):
 
 
 def _count(*values):
-    """Sizes as the library takes them: a larger one would wrap around in 32 bits."""
+    """Sizes as the library takes them: a larger one would wrap around in 32 bits.  (Calls
+    of a step ask with a shift first: the loop here costs them 0.3 us.)"""
     for x in values:
         if not 0 <= x < 1 << 31:
             raise ValueError(f"a size of {x} is negative or 2^31 and more")
@@ -201,7 +202,8 @@ class KvCache:
                   "lse must be a contiguous float32 [n_tokens, n_head]")
         if workspace is None:
             workspace = self.attention_workspace(batch, n_head)
-        _count(window)
+        if window >> 31:
+            _count(window)
         _need(workspace.device == self.device and workspace.is_contiguous(), "the workspace must be contiguous and on the cache's device")
         a = L.LlapisKvQuery(_tag(q.dtype), n_head, window, self.head_dim ** -0.5 if scale is None else scale,
                             q.data_ptr(), qs, out.data_ptr(), os_, _ptr(lse))
@@ -238,7 +240,8 @@ class KvPages:
                 or page_table.device != self.device):
             raise ValueError(f"page_table must be int32 [n_seq, max_pages] on {self.device}, rows of consecutive entries")
         _is(lens, torch.int32, (shape[0],), self.device, "lens")
-        _count(*shape)
+        if (shape[0] | shape[1]) >> 31:
+            _count(*shape)
         return page_table.data_ptr(), max(stride[0], shape[1]), shape[1]
 
     def copy(self, pairs):
@@ -316,7 +319,8 @@ def block_norm(h, y=None, post_weight=None, post_norm=True, gate=None, alpha=1.0
     shape, dtype, dev = h.shape, h.dtype, _on_gpu(h, "h")
     _need(len(shape) == 2 and h.stride(1) == 1, "h must be [T, d], rows of consecutive values")
     T, d = shape
-    _count(T, d)
+    if (T | d) >> 31:
+        _count(T, d)
 
     def row(t, what):
         stride = t.stride()
@@ -370,7 +374,8 @@ def verify_drafts(target, draft, drafts, u, u_next, n_draft=None, tokens=None, a
     shape, dtype, dev = target.shape, target.dtype, _on_gpu(target, "target")
     _need(len(shape) == 3 and shape[1] > 0, "target must be [n_seq, drafts + 1, vocab]")
     S, n, V = shape[0], shape[1] - 1, shape[2]
-    _count(S, n, V)
+    if (S | n | V) >> 31:
+        _count(S, n, V)
 
     def rows(t, k, what):
         stride = t.stride()
