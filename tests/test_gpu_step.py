@@ -877,3 +877,50 @@ def test_block_norm_most_tokens(gpu):
     for x in (h_out, out):
         for at in range(0, T, 1 << 29):
             assert bool((x[at:at + (1 << 29)] == 3.0).all())
+
+
+# ------------------------------------------------------------- two at once
+def test_two_threads_and_streams_at_once(gpu):
+    """Host threads with a stream and workspaces of their own run every operator at
+    once: as each does alone, bit for bit, and a refusal is its own thread's."""
+    import threading
+    f = Filled(gpu, 301, la.BF16, 128, 2, 16, [2500, 77, 0, 512], [4, 1, 0, 2], la.BF16)
+    g = torch.Generator().manual_seed(302)
+    q = [f.queries(303 + i, 8).to(gpu) for i in range(2)]
+    h, y = (torch.randn(2, 300, 777, generator=g).to(gpu) for _ in range(2))
+    target = torch.softmax(3 * torch.randn(2, 3, 4, 9001, generator=g), -1).to(gpu)
+    draft = torch.softmax(3 * torch.randn(2, 3, 3, 9001, generator=g), -1).to(gpu)
+    drafts = torch.randint(0, 9001, (3, 3), generator=g, dtype=torch.int32).to(gpu)
+    u, u_next = torch.rand(3, 3, generator=g).to(gpu), torch.rand(3, generator=g).to(gpu)
+
+    def work(i):
+        out = f.cache.attention(f.batch, q[i])
+        h2, (x,) = la.block_norm(h[i], y[i], weights=[None])
+        tokens, accepted = la.verify_drafts(target[i], draft[i], drafts, u, u_next)
+        return [out, h2, x, tokens, accepted]
+
+    alone = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = work(i)
+                    with pytest.raises(la.LlapisError, match="16384" if i else "16-byte aligned"):
+                        if i:
+                            la.block_norm(torch.zeros(1, 16385, device=gpu))
+                        else:
+                            f.cache.attention(f.batch, torch.zeros(8 * 8 * 128 + 1, device=gpu)[1:].view(8, 8, 128))
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, alone[i]))
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
