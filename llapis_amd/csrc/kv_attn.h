@@ -33,8 +33,9 @@
 // exponent range by powers of two: q's row is scaled to a maximum in [2^13,
 // 2^14), p by 2^15.  q8_0: an
 // int8 value times its scale is exact in two fp16 parts (18 bits; magnitudes
-// above 65504 become infinite, as an F16 cache's would), of which V's second is
-// left out for bf16 results (2^-12, an eighth of out's rounding).
+// above 65504 become infinite, as an F16 cache's would), K's and V's alike for
+// results of every type: fp16's 11 bits alone would be rounded a second time where
+// one key carries a row.
 //
 // q8_0's loads are 16 bytes a lane too: of a K row the lane's 16 values go to two
 // products, and of a V column 16 keys, so that the products' order of values and
@@ -259,7 +260,7 @@ __device__ __forceinline__ void priority_in_turn(int turn) {
 
 constexpr float KV_LN2 = 0.69314718055994530942f, KV_LOG2E = 1.44269504088896340736f;
 
-// WIDE: fp32 results (q8_0: fp32 and fp16 ones)
+// WIDE: fp32 queries and results
 template <int CT, bool WIDE, int HD, int NT>
 struct KvShape {
     static constexpr bool HALF = CT != KV_BF16;
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
     const int tid = threadIdx.x, lane = tid & 63, wave = same(tid >> 6);
     const int lm = lane & 15, lg = lane >> 4;
     const int page = 1 << p.page_shift, page_mask = page - 1;
-    const int type = WIDE && !Q8 ? (int)T_F32 : p.type;
+    const int type = WIDE ? (int)T_F32 : p.type;
     // run and tile: a run's tiles are eight workgroups apart, on one XCD
     const int octet = blockIdx.x >> 3, tile = octet % p.tiles, run = octet / p.tiles * 8 + (blockIdx.x & 7);
     auto units_at = [&](int s) { return seq_units(p.b, s, p.page_shift, p.window, UNIT); };
@@ -695,7 +696,7 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                         for (int q = 0; q < PP; ++q) acc[nt][t] = mfma16<HALF>(hi, bp[nt][q], acc[nt][t]);
-                        if (Q8 && WIDE) acc[nt][t] = mfma16<HALF>(lo, bp[nt][0], acc[nt][t]);
+                        if (Q8) acc[nt][t] = mfma16<HALF>(lo, bp[nt][0], acc[nt][t]);
                     }
                 }
             };
@@ -743,7 +744,7 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
                                 for (int q = 0; q < PP; ++q) {
                                     const u4 bp = *(const u4 *)(lds_p + ((b * NT + nt) * PP + q) * 1024 + lane * 16);
                                     d = mfma16<HALF>(hi, bp, d);
-                                    if (Q8 && WIDE && q == 0) d = mfma16<HALF>(lo, bp, d);
+                                    if (Q8 && q == 0) d = mfma16<HALF>(lo, bp, d);
                                 }
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) acc[nt][t][i] += tok_of[nt] == tok ? d[i] : 0.0f;
@@ -818,7 +819,7 @@ hipError_t launch_kv_attn_hd(const KvAttn & p, int head_dim, hipStream_t s) {
 
 template <int CT>
 hipError_t launch_kv_attn_type(const KvAttn & p, int head_dim, hipStream_t s) {
-    if (p.type == T_F32 || (CT == KV_Q8 && p.type == T_F16))
+    if (p.type == T_F32)
         return p.nt == 1 ? launch_kv_attn_hd<CT, true, 1>(p, head_dim, s) : launch_kv_attn_hd<CT, true, 2>(p, head_dim, s);
     return p.nt == 1 ? launch_kv_attn_hd<CT, false, 1>(p, head_dim, s) : launch_kv_attn_hd<CT, false, 2>(p, head_dim, s);
 }

@@ -207,6 +207,27 @@ def test_attention_window(gpu, tag, D, window):
     f.check(f.queries(6, 4), window=window)
 
 
+@pytest.mark.parametrize("n_head", [1, 20])
+@pytest.mark.parametrize("D,P", SHAPES)
+@pytest.mark.parametrize("io", [la.F32, la.F16, la.BF16])
+def test_attention_q8_values(gpu, io, D, P, n_head):
+    """8-bit values enter results with all their bits.  With queries of zeros every
+    weight is the same power of two, so that a row that sees one key is its value
+    rounded once, bit for bit; means of up to four keys are off by their rounding
+    and by what fp32 sums of four products, their number's reciprocal and the product
+    with it leave: six roundings, 6 * 4 * 2^-24 < 2^-19 of the largest value."""
+    f = Filled(gpu, D + n_head, la.Q8_0, D, 1, P, [1, 4], [1, 4], io)
+    q = torch.zeros(f.T, n_head, D, dtype=DT[io])
+    out = f.cache.attention(f.batch, q.to(gpu)).cpu()
+    for s, n in enumerate(f.lens):
+        _, v, _ = ref.sequence(f.cache, f.table[s], n)
+        assert torch.equal(out[f.start[s]], v[:, 0].to(DT[io]).expand(n_head, D))
+        for t in range(1, n):
+            want = v[:, :t + 1].mean(1)
+            off = (out[f.start[s] + t].double() - want).abs()
+            assert (off <= ref.EPS[io] * want.abs() + 2 ** -19 * v[:, :t + 1].abs().max()).all()
+
+
 def test_attention_empty_rows(gpu):
     """Sequences without tokens, without new ones, more new rows than tokens,
     and keys without a page: rows that see nothing get 0 and -inf."""
