@@ -76,6 +76,17 @@ def _call(name, dev, *args):
             check(fn(*args, stream), name)
 
 
+def _table_stride(table):
+    """Entries from a page table's row to the next.  A single row's stride says
+    nothing; the rows of several must not overlap (an expanded row has a stride of 0)."""
+    stride, (n, width) = table.stride(0), table.shape
+    if stride < width:
+        if n > 1:
+            raise ValueError("page_table's rows overlap: each sequence needs a row of its own")
+        return width
+    return stride
+
+
 def _on_gpu(t, what):
     _need(t.device.type == "cuda", f"{what} must be on the GPU")
     return t.device
@@ -105,7 +116,7 @@ class KvBatch:
         _count(n, n_tokens, max_new, page_table.shape[1])
         self.page_table, self.lens, self.new_start = page_table, lens, new_start
         self.n_seq, self.n_tokens, self.max_new, self.max_pages = n, n_tokens, max_new, page_table.shape[1]
-        self.struct = L.LlapisKvBatch(n, n_tokens, max_new, self.max_pages, max(page_table.stride(0), self.max_pages),
+        self.struct = L.LlapisKvBatch(n, n_tokens, max_new, self.max_pages, _table_stride(page_table),
                                       page_table.data_ptr(), lens.data_ptr(), _ptr(new_start))
         self._ref = C.byref(self.struct)
 
@@ -242,7 +253,7 @@ class KvPages:
         _is(lens, torch.int32, (shape[0],), self.device, "lens")
         if (shape[0] | shape[1]) >> 31:
             _count(*shape)
-        return page_table.data_ptr(), max(stride[0], shape[1]), shape[1]
+        return page_table.data_ptr(), _table_stride(page_table), shape[1]
 
     def copy(self, pairs):
         """Copy page pairs[i, 0] to page pairs[i, 1] (int32 [n, 2] on the GPU) in every layer."""
@@ -299,8 +310,8 @@ class KvPages:
         if len(self.structs) > 1 and table_out.data_ptr() == page_table.data_ptr():
             # every group of planes has to see the table as it was
             page_table = page_table.clone()
-            table, stride = page_table.data_ptr(), page_table.stride(0)
-            _need(stride == table_out.stride(0), "in place, more than 64 layers need a contiguous page_table")
+            table = page_table.data_ptr()
+            _need(_table_stride(page_table) == stride, "in place, more than 64 layers need a contiguous page_table")
         for s in self.structs:
             _call("llapis_kv_compact", self.device, C.byref(s), table, stride, width, lens.data_ptr(), table_out.shape[0],
                   table_out.data_ptr(), refs.data_ptr(), n_live.data_ptr(), workspace.data_ptr(),

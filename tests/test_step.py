@@ -216,6 +216,34 @@ def test_python_refuses_host_tensors():
         la.verify_drafts(torch.zeros(1, 2, 10), None, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 1), torch.zeros(1))
 
 
+def test_python_refuses_overlapping_table_rows(monkeypatch):
+    """Rows of a page table that share entries (one row for all sequences, expanded; rows
+    a few entries apart): the library would take them for rows of their whole width,
+    past the table's memory.  Host tensors stand in for the GPU's, and nothing is called."""
+    import torch
+    from llapis_amd import step
+    called = []
+    monkeypatch.setattr(step, "_on_gpu", lambda t, what: t.device)
+    monkeypatch.setattr(step, "_call", lambda *a: called.append(a))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    caches = [step.KvCache.empty(8, 16, 1, 64, la.F16, "cpu") for _ in range(2)]
+    pages, lens = step.KvPages(caches), i32(5, 5, 5)
+    one = i32([0, 1, 2, 3])
+    for table in (one.expand(3, 4), torch.arange(10, dtype=torch.int32).as_strided((3, 4), (3, 1))):
+        for call in (lambda: step.KvBatch(table, lens), lambda: step.KvBatch(table, lens, i32(0, 1, 2, 3), 3),
+                     lambda: pages.fork(table, lens, i32([0, 1, 6])), lambda: pages.refs(table, lens),
+                     lambda: pages.compact(table, lens), lambda: pages.compact(table, lens, table_out=table)):
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+    assert not called
+    # one row's stride says nothing, and rows may lie apart
+    assert step.KvBatch(one, lens[:1]).struct.table_stride == 4 == step.KvBatch(one.expand(1, 4), lens[:1]).struct.table_stride
+    assert step.KvBatch(one.as_strided((1, 4), (0, 1)), lens[:1]).struct.table_stride == 4
+    assert step.KvBatch(torch.zeros(3, 9, dtype=torch.int32)[:, 1:5], lens).struct.table_stride == 9
+    pages.refs(one.as_strided((1, 4), (0, 1)), lens[:1])
+    assert [a[5] for a in called] == [4]
+
+
 def test_largest_counts():
     """Counts that loops would run past 32 bits with are refused, and have no workspace."""
     lib, big = la.lib(), (1 << 30) + 1
