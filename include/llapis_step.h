@@ -61,7 +61,7 @@ uint64_t llapis_kv_page_bytes(int32_t type, int32_t n_kv, int32_t head_dim, int3
  * row.  What lies beyond them is not touched: rows past n_tokens, new tokens
  * past max_new of a sequence, keys past max_pages * page_size.  A table entry
  * outside 0 .. n_pages - 1 has no page: its keys are masked and what would be
- * appended there is dropped. */
+ * appended there is dropped.  An append takes fewer than 2^24 sequences. */
 typedef struct llapis_kv_batch {
     int32_t n_seq, n_tokens, max_new, max_pages;
     int64_t table_stride;          /* entries from a sequence's row to the next */
@@ -88,7 +88,8 @@ int32_t llapis_kv_append(const llapis_kv_cache * c, const llapis_kv_batch * b, i
  * out_stride values apart, 16-byte aligned, out apart from q; lse [n_tokens]
  * [n_head] or NULL.
  * Scores, sums and the running maximum are fp32; F32 queries are multiplied
- * as exact sums of 16-bit parts. */
+ * as exact sums of 16-bit parts.  Refused: 2^29 units of 64 keys a kv head in
+ * the whole batch, 2^24 blocks of up to 32 query rows of a sequence's kv heads. */
 typedef struct llapis_kv_query {
     int32_t type, n_head, window;
     float   scale;
@@ -109,7 +110,7 @@ int32_t  llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * 
  * Operations on whole pages, the same in every plane: a plane is one layer's
  * K or V pool, pages of `bytes` bytes (a multiple of 16) `stride` apart.  More
  * planes than LLAPIS_KV_MAX_PLANES take several calls.  n_pages and max_pages are
- * 2^30 at most. */
+ * 2^30 at most, n_seq below 2^24 in page_refs and compact, n_forks 65535 at most. */
 #define LLAPIS_KV_MAX_PLANES 128
 typedef struct llapis_kv_planes {
     int32_t n_planes, n_pages, page_size;

@@ -552,6 +552,12 @@ struct AttnPlan {
     uint64_t bytes() const { return base_bytes + ml_bytes + acc_bytes; }
 };
 
+// a launch has fewer than 2^32 threads in x: workgroups of 256
+constexpr int KV_MAX_GRID = 1 << 24;
+
+// an item may have several units, and parts to join
+bool needs_join(const llapis_kv_cache * c, const llapis_kv_batch * b) { return (int64_t)b->max_pages * c->page_size > kv_unit(c->head_dim); }
+
 const char * plan_attention(const llapis_kv_cache * c, const llapis_kv_batch * b, int n_head, AttnPlan & a) {
     const int max_new = b->new_start ? b->max_new : 1;
     if (n_head <= 0 || n_head > 1024 || n_head % c->n_kv) return "need n_head <= 1024, a multiple of n_kv";
@@ -561,8 +567,11 @@ const char * plan_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     a.tiles = (rows + 16 * a.nt - 1) / (16 * a.nt);
     const int unit = kv_unit(c->head_dim);
     const int64_t units = ((int64_t)b->max_pages * c->page_size + unit - 1) / unit + 1;
+    if (b->n_seq > 0 && units * c->n_kv > ((1 << 29) - 1) / b->n_seq) return "the batch has 2^29 units of work or more";
     const int64_t all = units * c->n_kv * b->n_seq;
-    if (all >= (int64_t)1 << 29) return "the batch has 2^29 units of work or more";
+    // the join has a workgroup for each (sequence, kv head, tile)
+    if (needs_join(c, b) && (int64_t)b->n_seq * c->n_kv * a.tiles >= KV_MAX_GRID)
+        return "2^24 or more (sequence, kv head, 32 query rows)";
     // as many workgroups as the card holds at once
     const int64_t most = std::max(256 * kv_wgs(c->head_dim, a.nt) / a.tiles, 8);
     a.runs = (int)((std::min(most, all) + 7) / 8 * 8);
@@ -595,6 +604,11 @@ const char * check_table(const void * table, int64_t stride, int max_pages, cons
     if (max_pages <= 0 || max_pages > KV_MAX_COUNT || stride < max_pages) return "need 0 < max_pages <= table_stride, max_pages <= 2^30";
     if (n_seq > 0 && (!table || !lens)) return "null page table or lengths";
     return nullptr;
+}
+
+// ... of calls with a workgroup for each row
+const char * check_rows(const void * table, int64_t stride, int max_pages, const void * lens, int n_seq) {
+    return n_seq >= KV_MAX_GRID ? "need n_seq < 2^24" : check_table(table, stride, max_pages, lens, n_seq);
 }
 
 dim3 table_grid(int n_seq, int max_pages) { return dim3(n_seq, std::min((max_pages + 255) / 256, 64)); }
@@ -642,6 +656,7 @@ int32_t llapis_kv_append(const llapis_kv_cache * c, const llapis_kv_batch * b, i
     const int64_t tiles = std::min<int64_t>(((int64_t)q.max_new + APP_POS - 2) / APP_POS + 1,
                                             ((int64_t)b->max_pages * c->page_size + APP_POS - 1) / APP_POS);
     if (tiles > 65535) return refuse_as(who, "more than 65535 * 32 new tokens of a sequence");
+    if (q.n_seq >= KV_MAX_GRID) return refuse_as(who, "need n_seq < 2^24");
     KvAppend p{q, (uint8_t *)c->k, (uint8_t *)c->v, c->k_stride, c->v_stride, c->n_pages, log2_of(c->page_size), c->n_kv,
                c->head_dim, x_type, k, v, k_stride, v_stride};
     const dim3 grid(q.n_seq, (unsigned)tiles, 2 * c->n_kv);
@@ -680,7 +695,6 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
         return refuse_as(who, "q and out must be 16-byte aligned, rows too");
     if (sq.n_tokens > 1 && (q->q_stride < width || q->out_stride < width)) return refuse_as(who, "rows shorter than n_head * head_dim");
     if (!workspace || !aligned16(workspace) || ws_bytes < a.bytes()) return refuse_as(who, "workspace too small or not 16-byte aligned");
-    if ((int64_t)sq.n_seq * c->n_kv * a.tiles >= (int64_t)1 << 31) return refuse_as(who, "2^31 items or more");
     KvAttn p{};
     p.b = sq;
     p.k = (const uint8_t *)c->k;
@@ -711,7 +725,7 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     if (c->type == T_F16) KV_TRY(launch_kv_attn_f16(p, c->head_dim, s));
     else if (c->type == T_BF16) KV_TRY(launch_kv_attn_bf16(p, c->head_dim, s));
     else KV_TRY(launch_kv_attn_q8(p, c->head_dim, s));
-    if ((int64_t)b->max_pages * c->page_size <= p.unit) return 0;      // every item is one unit
+    if (!needs_join(c, b)) return 0;                                   // every item is one unit
     // parts of an item, as many as the bounds suggest; workgroups by an item's rows
     const int64_t items = (int64_t)sq.n_seq * c->n_kv;
     const int parts = (int)(a.runs / items), pg = parts < 4 ? 1 : parts < 16 ? 4 : 16, per = 1024 / pg;
@@ -757,7 +771,7 @@ int32_t llapis_kv_fork(const llapis_kv_planes * p, int32_t * page_table, int64_t
 int32_t llapis_kv_page_refs(int32_t n_pages, int32_t page_size, const int32_t * page_table, int64_t table_stride,
                             int32_t max_pages, const int32_t * lens, int32_t n_seq, int32_t * refs, int32_t * free_pages,
                             int32_t * n_free, void * stream) {
-    const char * bad = check_table(page_table, table_stride, max_pages, lens, n_seq);
+    const char * bad = check_rows(page_table, table_stride, max_pages, lens, n_seq);
     if (!bad && (n_pages <= 0 || n_pages > KV_MAX_COUNT || page_size <= 0)) bad = "need 0 < n_pages <= 2^30 and page_size > 0";
     if (!bad && !refs) bad = "null refs";
     if (bad) return refuse_as("llapis_kv_page_refs", bad);
@@ -778,7 +792,7 @@ int32_t llapis_kv_compact(const llapis_kv_planes * p, const int32_t * page_table
     const char * who = "llapis_kv_compact";
     int chunks = 0;
     const char * bad = check_planes(p, chunks);
-    if (!bad) bad = check_table(page_table, table_stride, max_pages, lens, n_seq);
+    if (!bad) bad = check_rows(page_table, table_stride, max_pages, lens, n_seq);
     if (!bad && ((n_seq > 0 && !table_out) || !n_live)) bad = "null table_out or n_live";
     if (!bad && (!workspace || ((uintptr_t)workspace & 3) || ws_bytes < llapis_kv_compact_workspace_size(p->n_pages)))
         bad = "workspace too small";

@@ -216,6 +216,35 @@ def test_python_refuses_host_tensors():
         la.verify_drafts(torch.zeros(1, 2, 10), None, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 1), torch.zeros(1))
 
 
+def test_launch_limits():
+    """A launch has fewer than 2^32 threads in x.  Calls with a kernel past that, or whose
+    units of work pass 64 bits, are refused as calls, before a first kernel of theirs runs."""
+    lib, many = la.lib(), 1 << 24
+    b = batch(n_seq=many, n_tokens=many, max_new=1)
+    refused(lib.llapis_kv_append(C.byref(cache()), C.byref(b), la.F32, P, 128, P, 128, None), "llapis_kv_append", "2^24")
+    for n in (many, (1 << 31) - 1):
+        refused(lib.llapis_kv_page_refs(4, 16, P, 4, 4, P, n, P, P, P, None), "llapis_kv_page_refs", "2^24")
+        refused(lib.llapis_kv_compact(C.byref(planes()), P, 4, 4, P, n, P, None, P, P, 1 << 20, None), "llapis_kv_compact", "2^24")
+    # attention: (sequence, kv head, tile of query rows), which the second kernel has a workgroup for
+    many_heads = cache(n_kv=8, head_dim=64, page_size=256, k_stride=1 << 19, v_stride=1 << 19)
+    for c, b, n_head in ((many_heads, batch(n_seq=1 << 21, n_tokens=1 << 21), 8),
+                         (many_heads, batch(n_seq=1 << 17, n_tokens=1 << 21, max_new=16, new_start=P), 256)):
+        q = query(n_head=n_head, q_stride=64 * n_head, out_stride=64 * n_head)
+        assert lib.llapis_kv_attention_workspace_size(C.byref(c), C.byref(b), n_head) == 0
+        refused(lib.llapis_kv_attention(C.byref(c), C.byref(b), C.byref(q), P, 1 << 40, None), "llapis_kv_attention", "2^24")
+        b.n_seq -= 1
+        assert lib.llapis_kv_attention_workspace_size(C.byref(c), C.byref(b), n_head) > 0
+    # one kernel does where every item is a unit, whatever their number (a page of 16 keys)
+    c, b = cache(n_kv=8, k_stride=1 << 14, v_stride=1 << 14), batch(n_seq=1 << 21, n_tokens=1 << 21, max_pages=1, table_stride=1)
+    assert lib.llapis_kv_attention_workspace_size(C.byref(c), C.byref(b), 8) > 0
+    # 2^24 units of a sequence, 1024 heads and 2^30 sequences: 2^64
+    c = cache(n_kv=1024, head_dim=512, page_size=256, k_stride=1 << 28, v_stride=1 << 28)
+    b = batch(n_seq=1 << 30, n_tokens=1, max_pages=1 << 22, table_stride=1 << 22)
+    q = query(n_head=1024, q_stride=1 << 19, out_stride=1 << 19)
+    assert lib.llapis_kv_attention_workspace_size(C.byref(c), C.byref(b), 1024) == 0
+    refused(lib.llapis_kv_attention(C.byref(c), C.byref(b), C.byref(q), P, 1 << 62, None), "units")
+
+
 def test_python_refuses_overlapping_table_rows(monkeypatch):
     """Rows of a page table that share entries (one row for all sequences, expanded; rows
     a few entries apart): the library would take them for rows of their whole width,
