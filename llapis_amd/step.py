@@ -87,6 +87,13 @@ def _table_stride(table):
     return stride
 
 
+def _scratch(workspace, dev):
+    """(address, bytes) of a caller's workspace"""
+    if workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"the workspace must be contiguous and on {dev}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _on_gpu(t, what):
     _need(t.device.type == "cuda", f"{what} must be on the GPU")
     return t.device
@@ -215,11 +222,9 @@ class KvCache:
             workspace = self.attention_workspace(batch, n_head)
         if window >> 31:
             _count(window)
-        _need(workspace.device == self.device and workspace.is_contiguous(), "the workspace must be contiguous and on the cache's device")
         a = L.LlapisKvQuery(_tag(q.dtype), n_head, window, self.head_dim ** -0.5 if scale is None else scale,
                             q.data_ptr(), qs, out.data_ptr(), os_, _ptr(lse))
-        _call("llapis_kv_attention", self.device, self._ref, batch._ref, C.byref(a), workspace.data_ptr(),
-              workspace.numel() * workspace.element_size())
+        _call("llapis_kv_attention", self.device, self._ref, batch._ref, C.byref(a), *_scratch(workspace, self.device))
         return out
 
 
@@ -307,6 +312,7 @@ class KvPages:
         _is(n_live, torch.int32, (1,), self.device, "n_live")
         if workspace is None:
             workspace = self.workspace()
+        scratch = _scratch(workspace, self.device)
         if len(self.structs) > 1 and table_out.data_ptr() == page_table.data_ptr():
             # every group of planes has to see the table as it was
             page_table = page_table.clone()
@@ -314,8 +320,7 @@ class KvPages:
             _need(_table_stride(page_table) == stride, "in place, more than 64 layers need a contiguous page_table")
         for s in self.structs:
             _call("llapis_kv_compact", self.device, C.byref(s), table, stride, width, lens.data_ptr(), table_out.shape[0],
-                  table_out.data_ptr(), refs.data_ptr(), n_live.data_ptr(), workspace.data_ptr(),
-                  workspace.numel() * workspace.element_size())
+                  table_out.data_ptr(), refs.data_ptr(), n_live.data_ptr(), *scratch)
         return table_out, refs, n_live
 
 
@@ -413,5 +418,5 @@ def verify_drafts(target, draft, drafts, u, u_next, n_draft=None, tokens=None, a
         workspace = verify_workspace(S, V, dev)
     a = L.LlapisVerifyArgs(_tag(dtype), S, n, V, *target_rows, *draft_rows, drafts.data_ptr(), _ptr(n_draft), u.data_ptr(),
                            u_next.data_ptr(), tokens.data_ptr(), accepted.data_ptr())
-    _call("llapis_verify_drafts", dev, C.byref(a), workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _call("llapis_verify_drafts", dev, C.byref(a), *_scratch(workspace, dev))
     return tokens, accepted

@@ -273,6 +273,31 @@ def test_python_refuses_overlapping_table_rows(monkeypatch):
     assert [a[5] for a in called] == [4]
 
 
+@pytest.mark.parametrize("bad", ["expanded", "elsewhere"])
+def test_python_checks_workspaces(monkeypatch, bad):
+    """A workspace has to be memory of the call's device, all of it: one value expanded to the
+    size, or memory of another device, is no workspace.  Host tensors stand in for the GPU's."""
+    import torch
+    from llapis_amd import step
+    called = []
+    monkeypatch.setattr(step, "_on_gpu", lambda t, what: t.device)
+    monkeypatch.setattr(step, "_call", lambda *a: called.append(a))
+    ws = torch.zeros(1, dtype=torch.uint8).expand(1 << 24) if bad == "expanded" else torch.empty(1 << 24, dtype=torch.uint8, device="meta")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    cache = step.KvCache.empty(8, 16, 1, 64, la.F16, "cpu")
+    table, lens = i32([0, 1], [2, 3]), i32(5, 7)
+    calls = (lambda w: cache.attention(step.KvBatch(table, lens), torch.zeros(2, 4, 64), workspace=w),
+             lambda w: step.KvPages([cache]).compact(table, lens, workspace=w),
+             lambda w: step.verify_drafts(torch.rand(2, 2, 9), None, torch.zeros(2, 1, dtype=torch.int32), torch.rand(2, 1), torch.rand(2), workspace=w))
+    for call in calls:
+        with pytest.raises(ValueError, match="workspace"):
+            call(ws)
+    assert not called
+    for call in calls:
+        call(torch.empty(1 << 24, dtype=torch.uint8))
+    assert [a[0] for a in called] == ["llapis_kv_attention", "llapis_kv_compact", "llapis_verify_drafts"]
+
+
 def test_largest_counts():
     """Counts that loops would run past 32 bits with are refused, and have no workspace."""
     lib, big = la.lib(), (1 << 30) + 1
