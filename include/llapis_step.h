@@ -37,8 +37,9 @@ enum { LLAPIS_T_F16 = 1, LLAPIS_T_BF16 = 30 };
  * (K's and V's alike), one for 32 consecutive values of a token's vector:
  * ggml's q8_0 blocks with the planes apart (d = amax / 127 rounded to fp16,
  * q = x times the fp32 reciprocal of the unrounded d, rounded to nearest even; a
- * block with a NaN has a NaN scale).  Attention reads magnitudes above 65504 as
- * infinite, as an F16 cache holds them.
+ * block with a NaN has a NaN scale, one with an infinity an infinite one: either is
+ * NaN throughout).  Attention takes a value q d from fp16 parts: one that rounds
+ * past fp16's largest, 65504, which takes a scale of 515 and more, is read as NaN.
  * Page p is at base + p * stride bytes; strides are multiples of 16 and at
  * least llapis_kv_page_bytes (pages of several layers may interleave). */
 typedef struct llapis_kv_cache {

@@ -32,10 +32,12 @@
 // two bf16 parts (2^-17) is far below out's rounding.  fp16 parts keep their
 // exponent range by powers of two: q's row is scaled to a maximum in [2^13,
 // 2^14), p by 2^15.  q8_0: an
-// int8 value times its scale is exact in two fp16 parts (18 bits; magnitudes
-// above 65504 become infinite, as an F16 cache's would), K's and V's alike for
-// results of every type: fp16's 11 bits alone would be rounded a second time where
-// one key carries a row.
+// int8 value times its scale is exact in two fp16 parts (18 bits), K's and V's alike
+// for results of every type: fp16's 11 bits alone would be rounded a second time
+// where one key carries a row.  Past 65504 the first part is infinite and the second
+// of the other sign, so that such a value is NaN (a remainder kept finite takes two
+// more instructions for two values, 7 % of a long cache's time, and sums of its own
+// for the remainders 2.5 % and spilled registers at three head sizes).
 //
 // q8_0's loads are 16 bytes a lane too: of a K row the lane's 16 values go to two
 // products, and of a V column 16 keys, so that the products' order of values and

@@ -207,6 +207,44 @@ def test_attention_window(gpu, tag, D, window):
     f.check(f.queries(6, 4), window=window)
 
 
+@pytest.mark.parametrize("io", [la.F32, la.F16, la.BF16])
+@pytest.mark.parametrize("D", [64, 256])
+def test_attention_q8_range(gpu, io, D):
+    """Values up to 65504 are read as they are, larger ones as NaN: a key of them in the
+    rows that see it, a value in its column of them.
+
+    Filled.check's bound on lse is for scores near 1.  Here they reach 6e4, with sums of
+    products several times as large: as a function of the scores lse moves by no more
+    than the score that moves most, and a score by (D + 8) 2^-24 + 2^-22 of its sum of
+    |q k| (ref.attention)."""
+    P, n, at = 16, 40, 38
+    f = Filled(gpu, 25, la.Q8_0, D, 1, P, [n], [3], io)
+    q = f.queries(26, 4)
+    clean = f.check(q)
+    pg, slot = f.table[0][at // P], at % P
+    half = lambda t: t[pg].view(torch.float16)[P * D // 2:].view(D // 32, P)
+    k_was = half(f.cache.k)[0, slot].clone()
+    for t in (f.cache.k, f.cache.v):
+        half(t)[0, slot] = 515.0                              # 127 * 515 = 65405
+        lse = torch.empty(q.shape[:2], device=gpu)
+        out = f.cache.attention(f.batch, q.to(gpu), lse=lse).cpu()
+        want, want_lse, tol = ref.attention(f.cache, f.table, f.lens, f.start, q, D ** -0.5)
+        assert ((out.double() - want).abs() <= tol).all()
+        keys = ref.sequence(f.cache, f.table[0], n)[0][0].abs()
+        ds = ((D + 8) * 2 ** -24 + 2 ** -22) * D ** -0.5 * (q.double().abs() @ keys.T).amax(-1)
+        assert ((lse.cpu().double() - want_lse).abs() <= 2e-5 + 2 ** -22 * want_lse.abs() + ds).all()
+    half(f.cache.k)[0, slot] = 600.0
+    got = f.cache.attention(f.batch, q.to(gpu)).cpu()
+    assert torch.equal(got[0], clean[0]) and torch.isnan(got[1:]).all()
+    half(f.cache.k)[0, slot] = k_was
+    half(f.cache.v)[0, slot] = 600.0
+    got = f.cache.attention(f.batch, q.to(gpu)).cpu()
+    past = ref.unpack(f.cache, pg, True)[0, slot].abs() >= 65520      # halfway to fp16's next
+    assert past.any() and not past.all()
+    assert torch.equal(got[0], clean[0])
+    assert torch.equal(torch.isnan(got[1:]), past.expand(2, 4, D))
+
+
 @pytest.mark.parametrize("n_head", [1, 20])
 @pytest.mark.parametrize("D,P", SHAPES)
 @pytest.mark.parametrize("io", [la.F32, la.F16, la.BF16])
