@@ -88,9 +88,13 @@ int32_t llapis_kv_append(const llapis_kv_cache * c, const llapis_kv_batch * b, i
  * places hold.  q, out: [n_tokens][n_head][head_dim] of `type`, rows q_stride /
  * out_stride values apart, 16-byte aligned, out apart from q; lse [n_tokens]
  * [n_head] or NULL.
- * Scores, sums and the running maximum are fp32; F32 queries are multiplied
- * as exact sums of 16-bit parts.  Refused: 2^29 units of 64 keys a kv head in
- * the whole batch, 2^24 blocks of up to 32 query rows of a sequence's kv heads. */
+ * Scores, sums and the running maximum are fp32, and cached values enter with all
+ * their bits.  Queries and probabilities are multiplied as sums of 16-bit parts, equal
+ * to them to 2^-22 and better (a part in 2^37 of the row's largest is the least); 16-bit
+ * queries exactly; the probabilities of 16-bit results over BF16 pages to 2^-17, a
+ * 64th of an F16 result's own rounding, a 512th of a BF16 one's.
+ * Refused: batches of 2^29 and more (kv head, 64 keys), of 2^24 and more (sequence,
+ * kv head, 32 query rows). */
 typedef struct llapis_kv_query {
     int32_t type, n_head, window;
     float   scale;
