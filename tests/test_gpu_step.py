@@ -207,6 +207,46 @@ def test_attention_window(gpu, tag, D, window):
     f.check(f.queries(6, 4), window=window)
 
 
+@pytest.mark.parametrize("group,new", [(8, [4, 3, 1, 2]), (3, [16, 1, 11, 2])])
+@pytest.mark.parametrize("D,P", SHAPES)
+@pytest.mark.parametrize("io", [la.F32, la.F16, la.BF16])
+@pytest.mark.parametrize("tag", [la.F16, la.BF16, la.Q8_0])
+def test_attention_types_two_tiles(gpu, tag, io, D, P, group, new):
+    """The same with 32 query rows a kv head, and with 48: two tiles of 16 rows in
+    a workgroup, a second workgroup that is half empty, items that several runs
+    share, and a window of fewer keys than new tokens."""
+    f = Filled(gpu, D + group, tag, D, 2, P, [4, 700, 45, 129], new, io)
+    q = f.queries(D + 1, 2 * group)
+    f.check(q)
+    f.check(q, window=3)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("tag,D", [(la.F16, 512), (la.BF16, 512), (la.Q8_0, 512), (la.F16, 96), (la.BF16, 192), (la.Q8_0, 192),
+                                   (la.Q8_0, 64)])
+def test_attention_hidden_non_finite_two_tiles(gpu, tag, D, bad):
+    """What the step's earlier tokens and the window's later ones do not see, with 40 query rows a kv head."""
+    P, N, n, window = 16, 4, 140, 20
+    f = Filled(gpu, 23, tag, D, 1, P, [n], [N], la.F32)
+    q = f.queries(24, 10)
+    clean = f.check(q, window=window)
+    for at, seen in ((n - 2, (2, 3)), (n - N + 1 - window + 1, (0, 1))):
+        pg, slot = f.table[0][at // P], at % P
+        pools = [(t[pg].view(torch.float16)[P * D // 2:].view(D // 32, P)[:, slot] if tag == la.Q8_0 else
+                  t[pg, 0, slot] if t is f.cache.k else t[pg, 0, :, slot]) for t in (f.cache.k, f.cache.v)]
+        held = [t.clone() for t in pools]
+        for t in pools:
+            t.fill_(bad)
+        got = f.cache.attention(f.batch, q.to(gpu), window=window).cpu()
+        for t, was in zip(pools, held):
+            t.copy_(was)
+        for j in range(N):
+            if j in seen:
+                assert not torch.isfinite(got[j]).any(-1).all()
+            else:
+                assert torch.equal(got[j], clean[j])
+
+
 @pytest.mark.parametrize("io", [la.F32, la.F16, la.BF16])
 @pytest.mark.parametrize("D", [64, 256])
 def test_attention_q8_range(gpu, io, D):
