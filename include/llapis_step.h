@@ -93,8 +93,8 @@ int32_t llapis_kv_append(const llapis_kv_cache * c, const llapis_kv_batch * b, i
  * to them to 2^-22 and better (a part in 2^37 of the row's largest is the least); 16-bit
  * queries exactly; the probabilities of 16-bit results over BF16 pages to 2^-17, a
  * 64th of an F16 result's own rounding, a 512th of a BF16 one's.
- * Refused: batches of 2^29 and more (kv head, 64 keys), of 2^24 and more (sequence,
- * kv head, 32 query rows). */
+ * Refused: batches of 2^29 and more units of work (64 or 128 keys of a kv head), and
+ * with several units a head of 2^24 and more (sequence, kv head, 32 query rows). */
 typedef struct llapis_kv_query {
     int32_t type, n_head, window;
     float   scale;
