@@ -598,6 +598,41 @@ def test_compact(gpu, n_seq, width, n_pages, layers):
     check_moved(before, planes_of(p), [])
 
 
+@pytest.mark.parametrize("n_seq,width,n_pages,layers", [(30, 40, 8193, 1), (300, 230, 1000, 2), (220, 300, 20000, 1), (5, 13200, 8500, 66)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_compact_large(gpu, n_seq, width, n_pages, layers, in_place):
+    """Pools of more than 8192 pages and tables of more than 65536 entries, moved
+    in place too, and by two calls a compaction in the last case."""
+    P = 16
+    table, lens = random_tables(n_pages + 1, n_seq, width, n_pages, P)
+    p = pools(gpu, 6, n_pages, layers, H=1)
+    tb, ln = i32(table, gpu), i32(lens, gpu)
+    before = [c.k.clone() for c in p.caches] + [c.v.clone() for c in p.caches]
+    out, refs, n_live = p.compact(tb, ln, table_out=tb if in_place else None)
+    want, after, n, moves = ref.compact(table, lens, P, n_pages)
+    assert out.tolist() == want and refs.tolist() == after and int(n_live) == n
+    assert in_place or tb.tolist() == table
+    assert len(moves) > 0
+    frm, to = torch.tensor(moves).to(gpu).T
+    for was, now in zip(before, [c.k for c in p.caches] + [c.v for c in p.caches]):
+        was.view(torch.int16)[to] = was.view(torch.int16)[frm]
+        assert torch.equal(was.view(torch.int16), now.view(torch.int16))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_compact_many_planes(gpu, in_place):
+    """More planes than a call takes, pages that do move: every plane's move and the table's are the same."""
+    P, n_pages = 16, 40
+    table, lens = [[39, 3, 38, 20], [20, 1, 37, -1], [30, 31, 32, 33]], [64, 40, 17]
+    p = pools(gpu, 7, n_pages, 67, H=1)
+    tb, ln, before = i32(table, gpu), i32(lens, gpu), planes_of(p)
+    out, refs, n_live = p.compact(tb, ln, table_out=tb if in_place else None)
+    want, after, n, moves = ref.compact(table, lens, P, n_pages)
+    assert len(moves) == 6 and n == 8
+    assert out.tolist() == want and refs.tolist() == after and int(n_live) == n
+    check_moved(before, planes_of(p), moves)
+
+
 def test_compact_full_and_empty(gpu):
     p = pools(gpu, 5, 8, 1)
     full = [[7, 6, 5, 4], [3, 2, 1, 0]]
