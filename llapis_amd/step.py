@@ -18,9 +18,6 @@ import ctypes as C
 from . import _lib as L
 from ._lib import BF16, F16, F32, Q8_0, check, lib
 
-KV_MAX_NEW = 16
-
-
 _module = None
 _tags = {}
 
