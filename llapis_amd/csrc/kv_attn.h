@@ -45,15 +45,16 @@
 //
 // What bounds it.  Long caches: memory.  TB/s of K and V (a kernel that only reads
 // reaches 6.2): head size 64 5.5, 128 5.6 (pages of 16 tokens 5.4), 256 5.4, 512
-// 5.3; with two row tiles 5.3, at 512 4.5; q8_0 5.2 to 5.35, at 512 4.9 (its
-// conversions keep the VALU half busy).  Short ones: the chain of
-// lengths, page table, K, scores, V, result, each a memory latency: 7.7 us for 700
+// 5.3; with two row tiles 5.3, at 512 4.5; q8_0 4.8 to 5.2, at 512 4.65 (its
+// conversions keep the VALU busy for 60 % of the time).  Short ones: the chain of
+// lengths, page table, K, scores, V, result, each a memory latency: 7.6 us for 700
 // keys, and 24.6 us for 11203 keys of head size 512, of which a workgroup's unit is
-// 256 KB.  What the choices were worth (us of the kernel):
+// 256 KB.  What the choices were worth, and cost (us of the kernel):
 //   the line in half units, a half for each piece    48 ragged sequences   49 -> 45
 //   eight waves instead of four at head size 512     11203 keys            29 -> 25
 //   q8_0: two fp16 parts instead of three bf16       2 x 131072 keys     203 -> 172
 //   q8_0: 16-byte loads instead of 8                                     172 -> 118
+//   q8_0: V's second part for 16-bit results too, all else as it is      107 -> 116
 // As many runs as the card holds at once are enough: twice or three times as many
 // took 129 and 142 us instead of 124 for the 131072 keys.  Units are not parted
 // between runs: ends at a half of one (a quarter) took 55 to 59 (65) us instead of 53
@@ -249,8 +250,8 @@ __device__ __forceinline__ uint32_t pair_mask(uint32_t bits, int i) {
 // A CU serves its oldest workgroup first: of three that share a CU for a whole long
 // call the first ended at 84 us, the last at 106, when it had the CU to itself.  With a
 // unit each at every priority in turn they go on together (TB/s of long caches: head
-// size 64 5.34 -> 5.46, 128 5.53 -> 5.61, 256 5.33 -> 5.44; q8_0 5.0 -> 5.2, 5.1 ->
-// 5.35; two or one to a CU: no difference).
+// size 64 5.34 -> 5.46, 128 5.53 -> 5.61, 256 5.33 -> 5.44; q8_0, still without
+// V's second part, 5.0 -> 5.2, 5.1 -> 5.35; two or one to a CU: no difference).
 __device__ __forceinline__ void priority_in_turn(int turn) {
     switch (turn & 3) {
         case 0: __builtin_amdgcn_s_setprio(0); break;

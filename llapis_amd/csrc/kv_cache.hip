@@ -17,9 +17,10 @@ namespace dev {
 // own, and are added in their order.  A part is read once, its maximum and sum
 // with its values, so that the loads of several parts are in flight (a first pass
 // over the maxima, then the values: 4 tokens of 11203 keys with the attention
-// kernel 71 us, so 38).  A launch and a chain of four loads: 4.6 us for 700 keys,
-// 6.5 for the 177 parts of 11203, 8.5 for 48 sequences.  It is a kernel of its own
-// because no workgroup here waits for another one.
+// kernel 71 us, so 38).  A launch and a chain of four loads: 4.7 us for 700 keys,
+// 6.8 for the 88 parts a head of 11203, 8.5 for 48 sequences.  It is a kernel of its
+// own: added by the workgroup that ends last, the parts would need counters that are 0
+// before the call, and the workspace, which calls share, carries nothing over.
 template <int PG>
 __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, float p_shift) {
     constexpr int TPG = 256 / PG;
@@ -286,8 +287,8 @@ constexpr int KV_MAX_COUNT = 1 << 30;
 constexpr int PG_CHUNK = 16384;                                   // bytes a workgroup copies at a time
 
 // bytes [at, at + PG_CHUNK) of a page of `plane`, from one page to another: four
-// 128-bit loads in flight a lane.  Bound by memory: a compaction's moves of
-// 500 MB take 92 us, 5.5 TB/s of reads and writes; a large copy's rate is 5.0.
+// 128-bit loads in flight a lane.  Bound by memory: a compaction's moves of 500 MB of
+// reads and writes take 97 to 100 us, 5.0 to 5.2 TB/s; a large copy's rate is 5.0.
 __device__ __forceinline__ void copy_chunk(const llapis_kv_planes & p, int plane, int from, int to, uint64_t at) {
     const uint64_t n = p.bytes[plane];
     if (at >= n) return;
