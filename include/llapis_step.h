@@ -104,7 +104,8 @@ typedef struct llapis_kv_query {
     int64_t out_stride;
     float * lse;
 } llapis_kv_query;
-/* Device scratch (bytes) of an attention call; 0 if it would be refused.
+/* Device scratch (bytes) of an attention call; 0 if it would be refused.  It serves
+ * every call of fewer sequences, new tokens and pages too.
  * Reads c's geometry, b's n_seq, max_new and max_pages, and n_head. */
 uint64_t llapis_kv_attention_workspace_size(const llapis_kv_cache * c, const llapis_kv_batch * b, int32_t n_head);
 int32_t  llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * a,

@@ -674,7 +674,13 @@ uint64_t llapis_kv_attention_workspace_size(const llapis_kv_cache * c, const lla
     if (!c || !b || !llapis_kv_page_bytes(c->type, c->n_kv, c->head_dim, c->page_size) || b->n_seq < 0 || b->max_pages <= 0 ||
         (int64_t)b->max_pages * c->page_size > (1 << 30) || plan_attention(c, b, n_head, a))
         return 0;
-    return a.bytes();
+    // three tiles a run have more workgroups in their multiple of eight runs than four:
+    // the most of what fewer new tokens take
+    uint64_t most = a.bytes();
+    llapis_kv_batch less = *b;
+    for (less.max_new = 1; b->new_start && less.max_new < b->max_new; ++less.max_new)
+        if (!plan_attention(c, &less, n_head, a)) most = std::max(most, a.bytes());
+    return most;
 }
 
 int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * q, void * workspace,

@@ -188,8 +188,8 @@ class KvCache:
         _call("llapis_kv_append", self.device, self._ref, batch._ref, _tag(k.dtype), k.data_ptr(), ks, v.data_ptr(), vs)
 
     def attention_workspace(self, batch, n_head):
-        """Scratch for attention calls of this geometry, for a caller that keeps
-        it: calls that share it must not overlap."""
+        """Scratch for attention calls of this geometry and of batches within this one's
+        bounds, for a caller that keeps it: calls that share it must not overlap."""
         n = int(lib().llapis_kv_attention_workspace_size(self._ref, batch._ref, n_head))
         if n == 0:
             raise ValueError("attention: unsupported geometry (n_head, max_new or lengths)")

@@ -110,6 +110,23 @@ def test_attention_limits():
         assert la.lib().llapis_kv_append(C.byref(c), C.byref(b), la.F32, P, 128, P, 128, None) == 0
 
 
+@pytest.mark.parametrize("head_dim", [64, 96, 128, 256, 512])
+@pytest.mark.parametrize("n_kv,group", [(8, 1), (8, 8), (2, 9), (1, 64), (1, 1024)])
+def test_attention_workspace_serves_less(head_dim, n_kv, group):
+    """A workspace for the most sequences, new tokens and pages of a program serves each of its smaller steps."""
+    lib, n_head = la.lib(), n_kv * group
+    c = cache(n_kv=n_kv, head_dim=head_dim, page_size=64, k_stride=1 << 20, v_stride=1 << 20)
+
+    def size(n_seq, new, pages):
+        b = batch(n_seq=n_seq, n_tokens=n_seq * new, max_new=new, max_pages=pages, table_stride=pages, new_start=P)
+        return lib.llapis_kv_attention_workspace_size(C.byref(c), C.byref(b), n_head)
+
+    for n_seq, new, pages in ((1, 16, 3), (7, 16, 40), (64, 16, 512), (300, 9, 100)):
+        most = size(n_seq, new, pages)
+        for less in [(n_seq, i, pages) for i in range(1, new)] + [(max(n_seq - 1, 1), new, pages), (n_seq, new, pages - 1), (1, 1, 1)]:
+            assert 0 < size(*less) <= most, less
+
+
 def test_append_refusals():
     c, b = cache(), batch(n_seq=2, n_tokens=2)
     call = lambda t=la.F32, k=P, ks=128, v=P, vs=128: la.lib().llapis_kv_append(C.byref(c), C.byref(b), t, k, ks, v, vs, None)
