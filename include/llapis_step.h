@@ -1,8 +1,9 @@
 /*
  * llapis_step.h -- the operators of a decode step around the MoE layer
  * (llapis_moe.h): a paged key-value cache with its append, attention and page
- * operations, the norms before and after a block, and the verification of
- * drafted tokens.
+ * operations, pages and slots for a step's new tokens, the norms and rotary
+ * positions of queries and keys, the norms before and after a block, sampling
+ * and the verification of drafted tokens.
  *
  * The conventions are llapis_moe.h's: device pointers and a hipStream_t of the
  * current device passed as void*, nothing allocated, launches on that stream
@@ -167,6 +168,93 @@ int32_t  llapis_kv_compact(const llapis_kv_planes * p, const int32_t * page_tabl
                            int32_t max_pages, const int32_t * lens, int32_t n_seq, int32_t * table_out, int32_t * refs,
                            int32_t * n_live, void * workspace, uint64_t ws_bytes, void * stream);
 
+/* ------------------------------------------- pages and slots of a step
+ *
+ * Make room for the new tokens of a step: sequence s of lens[s] tokens asks for
+ * n_new[s] more (negative numbers count as 0).  A sequence gets all that it asks
+ * for or nothing.  It gets nothing where
+ *   - lens[s] + n_new[s] tokens are more than its row's max_pages hold, else where
+ *   - the asked of sequences 0 .. s that passed are more than n_tokens, else where
+ *   - it needs a page, and the pages that sequences 0 .. s need that passed are
+ *     more than n_free.
+ * Pages come from the end of free_pages (an array of n_pages entries, of which the
+ * first n_free[0] are free), sequence by sequence: entry ceil(lens / page_size) of
+ * a row and those behind it.  Then, each array as long as the new state needs:
+ *   lens_out [n_seq]       lengths with the new tokens (may be lens)
+ *   n_free_out [1]         the free pages left, the first of free_pages (may be n_free)
+ *   new_start [n_seq + 1]  first row of each sequence's new tokens: llapis_kv_batch's
+ *   pos, seq [n_tokens]    a row's position in its sequence, and which that is
+ *   slots [n_tokens]       page * page_size + place in the page; -1 without a page
+ * with -1 in rows past the last token; pos, seq and slots may be NULL.  n_seq is
+ * below 2^24, n_tokens, n_pages and max_pages * page_size 2^30 at most. */
+typedef struct llapis_kv_extend_args {
+    int32_t page_size, n_pages, n_seq, n_tokens, max_pages;
+    int32_t reserved;
+    int64_t table_stride;
+    int32_t * page_table;
+    const int32_t * lens;
+    const int32_t * n_new;
+    const int32_t * free_pages;
+    const int32_t * n_free;
+    int32_t * lens_out;
+    int32_t * n_free_out;
+    int32_t * new_start;
+    int32_t * pos;
+    int32_t * seq;
+    int64_t * slots;
+} llapis_kv_extend_args;
+uint64_t llapis_kv_extend_workspace_size(int32_t n_seq);
+int32_t  llapis_kv_extend(const llapis_kv_extend_args * a, void * workspace, uint64_t ws_bytes, void * stream);
+
+/* ------------------------------------- norms and positions of q and k
+ *
+ * Frequencies of a rotation, computed on the host: freq[i], i < rot_dim / 2, is
+ * base^(-2 i / rot_dim), divided by divisors[i] (NULL: none), and with `kind`
+ *   LINEAR  divided by factor;
+ *   NTK     from the base  base * factor^(rot_dim / (rot_dim - 2));
+ *   YARN    f (1 - r) + f / factor r, r = (i - lo) / (hi - lo) within 0 .. 1,
+ *           lo = floor(d(high)) >= 0, hi = ceil(d(low)) <= rot_dim - 1 (0.001 apart at
+ *           least), d(t) = rot_dim ln(trained / (2 pi t)) / (2 ln base);
+ *   BANDS   f s + f / factor (1 - s), s = (trained f / (2 pi) - low) / (high - low)
+ *           within 0 .. 1.
+ * low and high are turns over the trained length (YARN: 1 and 32, BANDS: 1 and 4
+ * are usual).  *magnitude, what cosine and sine are multiplied by: 0.1 ln factor + 1
+ * for YARN with a factor above 1, else 1. */
+enum { LLAPIS_ROPE_PLAIN = 0, LLAPIS_ROPE_LINEAR = 1, LLAPIS_ROPE_NTK = 2, LLAPIS_ROPE_YARN = 3, LLAPIS_ROPE_BANDS = 4 };
+typedef struct llapis_rope_rule {
+    int32_t kind, rot_dim;
+    double  base, factor, trained, low, high;
+    const double * divisors;
+} llapis_rope_rule;
+int32_t llapis_rope_frequencies(const llapis_rope_rule * rule, double * freq, float * magnitude);
+
+/* The norms of queries and keys for each head, and their rotary positions, in
+ * one pass: for every head x of head_dim values (up to 512) of a token at pos[t]
+ *   y = norm ? x / sqrt(mean x^2 + eps) * weight : x
+ *   (y_a, y_b) -> magnitude (y_a cos z - y_b sin z, y_b cos z + y_a sin z),  z = pos[t] freq[i]
+ * for i < rot_dim / 2 with, by `layout`, (a, b) = (i, i + rot_dim / 2) or (2 i, 2 i + 1);
+ * values from rot_dim on are not rotated (rot_dim 0: none are).  Angles are formed in
+ * 64 bits, the rest in fp32, and rounded once.  q [n_tokens][n_head][head_dim] and k
+ * [n_tokens][n_kv][head_dim] (n_kv 0: no k) are of `type`, rows q_stride values apart
+ * and so on, in any alignment to a value; outputs may lie on inputs row for row, and
+ * overlap them in no other way.  Weights fp32 [head_dim] or NULL (ones).  A row with
+ * pos[t] < 0 is neither read nor written. */
+enum { LLAPIS_ROPE_HALF = 0, LLAPIS_ROPE_PAIRS = 1 };
+typedef struct llapis_qk_rope_args {
+    int32_t type;                  /* LLAPIS_T_F32, LLAPIS_T_F16 or LLAPIS_T_BF16 */
+    int32_t n_tokens, n_head, n_kv, head_dim, rot_dim, layout, norm;
+    float   eps, magnitude;
+    const int32_t * pos;           /* [n_tokens]; NULL with rot_dim 0: every row */
+    const double *  freq;          /* [rot_dim / 2] */
+    const void *  q;      int64_t q_stride;
+    void *        q_out;  int64_t q_out_stride;
+    const float * q_weight;
+    const void *  k;      int64_t k_stride;
+    void *        k_out;  int64_t k_out_stride;
+    const float * k_weight;
+} llapis_qk_rope_args;
+int32_t llapis_qk_rope(const llapis_qk_rope_args * a, void * stream);
+
 /* -------------------------------------------------------- block norms
  *
  * What lies between one block and the next of a residual stream, in one
@@ -198,6 +286,40 @@ typedef struct llapis_block_norm_args {
     int64_t x_stride[LLAPIS_NORM_MAX_OUT];
 } llapis_block_norm_args;
 int32_t llapis_block_norm(const llapis_block_norm_args * a, void * stream);
+
+/* ----------------------------------------------------------- sampling
+ *
+ * The next token of each sequence from its logits [n_seq][vocab] of `type`, rows
+ * logits_stride values apart, with numbers u [n_seq] in [0, 1) that the caller
+ * draws.  With M a row's largest logit, values in the order (value descending,
+ * index ascending) and w_i = e^((x_i - M) / temperature):
+ *   top_k   keeps the first top_k values (0 and less: all);
+ *   top_p   keeps of those the fewest first ones whose weights' sum is at least
+ *           top_p of theirs (1 and more: all), the first always;
+ *   min_p   keeps of those the ones with w_i >= min_p (M's weight is 1);
+ *   the token is the smallest v for which the kept w_0 + .. + w_v > u sum w.
+ * A temperature that is not positive, and a min_p above 1, take the first value.
+ * The settings are read on the device, one for each sequence; NULL: temperature 1,
+ * the others off.  Weights and sums are fp64.  NaN and -infinity are no values (the
+ * token of a row without any is -1); where +infinity is the largest, the others have no
+ * weight.  With top_k or top_p a value whose weight is below 2^-63 may not be kept.
+ * probs [n_seq][vocab] of `type`, rows probs_stride apart, or NULL: the probabilities
+ * that the token was drawn with, rounded once (what llapis_verify_drafts takes as a
+ * draft's); not on logits.  n_seq is 65535 at most, vocab 2^30 (else the workspace size is 0). */
+typedef struct llapis_sample_args {
+    int32_t type;                  /* LLAPIS_T_F32, LLAPIS_T_F16 or LLAPIS_T_BF16 */
+    int32_t n_seq, vocab;
+    const void *    logits;  int64_t logits_stride;
+    const float *   u;
+    const float *   temperature;
+    const int32_t * top_k;
+    const float *   top_p;
+    const float *   min_p;
+    int32_t *       tokens;
+    void *          probs;   int64_t probs_stride;
+} llapis_sample_args;
+uint64_t llapis_sample_workspace_size(int32_t n_seq, int32_t vocab);
+int32_t  llapis_sample(const llapis_sample_args * a, void * workspace, uint64_t ws_bytes, void * stream);
 
 /* ------------------------------------------------ draft verification
  *

@@ -156,6 +156,34 @@ class LlapisVerifyArgs(C.Structure):
                 ("tokens", vp), ("accepted", vp)]
 
 
+class LlapisKvExtendArgs(C.Structure):
+    _fields_ = [("page_size", i32), ("n_pages", i32), ("n_seq", i32), ("n_tokens", i32), ("max_pages", i32), ("reserved", i32),
+                ("table_stride", i64), ("page_table", vp), ("lens", vp), ("n_new", vp), ("free_pages", vp), ("n_free", vp),
+                ("lens_out", vp), ("n_free_out", vp), ("new_start", vp), ("pos", vp), ("seq", vp), ("slots", vp)]
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = 0, 1, 2, 3, 4
+ROPE_HALF, ROPE_PAIRS = 0, 1
+
+
+class LlapisRopeRule(C.Structure):
+    _fields_ = [("kind", i32), ("rot_dim", i32), ("base", C.c_double), ("factor", C.c_double), ("trained", C.c_double),
+                ("low", C.c_double), ("high", C.c_double), ("divisors", vp)]
+
+
+class LlapisQkRopeArgs(C.Structure):
+    _fields_ = [("type", i32), ("n_tokens", i32), ("n_head", i32), ("n_kv", i32), ("head_dim", i32), ("rot_dim", i32),
+                ("layout", i32), ("norm", i32), ("eps", f32), ("magnitude", f32), ("pos", vp), ("freq", vp), ("q", vp),
+                ("q_stride", i64), ("q_out", vp), ("q_out_stride", i64), ("q_weight", vp), ("k", vp), ("k_stride", i64),
+                ("k_out", vp), ("k_out_stride", i64), ("k_weight", vp)]
+
+
+class LlapisSampleArgs(C.Structure):
+    _fields_ = [("type", i32), ("n_seq", i32), ("vocab", i32), ("logits", vp), ("logits_stride", i64), ("u", vp),
+                ("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp), ("tokens", vp), ("probs", vp),
+                ("probs_stride", i64)]
+
+
 STEP_SIGNATURES = {
     "llapis_kv_page_bytes": (u64, [i32, i32, i32, i32]),
     "llapis_kv_append": (i32, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), i32, vp, i64, vp, i64, vp]),
@@ -166,7 +194,13 @@ STEP_SIGNATURES = {
     "llapis_kv_page_refs": (i32, [i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp]),
     "llapis_kv_compact_workspace_size": (u64, [i32]),
     "llapis_kv_compact": (i32, [C.POINTER(LlapisKvPlanes), vp, i64, i32, vp, i32, vp, vp, vp, vp, u64, vp]),
+    "llapis_kv_extend_workspace_size": (u64, [i32]),
+    "llapis_kv_extend": (i32, [C.POINTER(LlapisKvExtendArgs), vp, u64, vp]),
+    "llapis_rope_frequencies": (i32, [C.POINTER(LlapisRopeRule), vp, C.POINTER(f32)]),
+    "llapis_qk_rope": (i32, [C.POINTER(LlapisQkRopeArgs), vp]),
     "llapis_block_norm": (i32, [C.POINTER(LlapisBlockNormArgs), vp]),
+    "llapis_sample_workspace_size": (u64, [i32, i32]),
+    "llapis_sample": (i32, [C.POINTER(LlapisSampleArgs), vp, u64, vp]),
     "llapis_verify_drafts_workspace_size": (u64, [i32, i32]),
     "llapis_verify_drafts": (i32, [C.POINTER(LlapisVerifyArgs), vp, u64, vp]),
 }

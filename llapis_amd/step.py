@@ -4,8 +4,11 @@
   new keys and values, ``attention`` attends the new tokens over it.
 * ``KvBatch`` -- a step's sequences: page table, lengths, new tokens.
 * ``KvPages`` -- page operations over every layer's pools at once: copy, fork,
-  references and free pages, compaction.
+  references and free pages, compaction, room for a step's new tokens.
+* ``qk_rope`` -- the norms of queries and keys and their rotary positions, whose
+  frequencies ``rope_frequencies`` computes.
 * ``block_norm`` -- post-norm, gate, residual and the next block's norms.
+* ``sample`` -- the next tokens from logits, with the probabilities they were drawn with.
 * ``verify_drafts`` -- accept or refuse drafted tokens, draw the next one.
 
 torch is used for device memory and the current stream alone.  A call runs on
@@ -82,6 +85,11 @@ def _table_stride(table):
             raise ValueError("page_table's rows overlap: each sequence needs a row of its own")
         return width
     return stride
+
+
+def _bytes(sizer, dev, *args):
+    """A workspace of the size that the library names"""
+    return _torch().empty(int(getattr(lib(), sizer)(*args)), dtype=_torch().uint8, device=dev)
 
 
 def _scratch(workspace, dev):
@@ -321,6 +329,120 @@ class KvPages:
         return table_out, refs, n_live
 
 
+    def extend_workspace(self, n_seq):
+        """Scratch for extend with up to n_seq sequences, for a caller that keeps it: calls that share it must not overlap."""
+        return _bytes("llapis_kv_extend_workspace_size", self.device, n_seq)
+
+    def extend(self, page_table, lens, n_new, free, n_free, n_tokens, lens_out=None, n_free_out=None, new_start=None, pos=None,
+               seq=None, slots=None, workspace=None):
+        """Make room for n_new [n_seq] more tokens of each sequence -> (new_start
+        [n_seq + 1], pos, seq [n_tokens] int32, slots [n_tokens] int64).  free
+        [n_pages], of which the first n_free [1] are free pages (as refs returns
+        them): the last of them are taken first, entered into page_table and off
+        n_free.  A sequence gets room for all of its new tokens or, where its row,
+        the n_tokens rows or the free pages do not suffice for it and those before it,
+        for none.  lens and n_free are updated in place unless lens_out and n_free_out
+        are given.  pos, seq, slots: each row's position, sequence and page * page_size
+        + place, -1 past the last row (or without a page)."""
+        torch = _torch()
+        table, stride, width = self._table(page_table, lens)
+        n, dev, int32 = page_table.shape[0], self.device, torch.int32
+        _is(n_new, int32, (n,), dev, "n_new")
+        _is(free, int32, (self.n_pages,), dev, "free")
+        _is(n_free, int32, (1,), dev, "n_free")
+        _count(n_tokens)
+        if lens_out is None:
+            lens_out = lens
+        if n_free_out is None:
+            n_free_out = n_free
+
+        def made(t, shape, dtype, what):
+            if t is None:
+                return torch.empty(shape, dtype=dtype, device=dev)
+            _is(t, dtype, shape, dev, what)
+            return t
+
+        _is(lens_out, int32, (n,), dev, "lens_out")
+        _is(n_free_out, int32, (1,), dev, "n_free_out")
+        new_start = made(new_start, (n + 1,), int32, "new_start")
+        pos, seq = made(pos, (n_tokens,), int32, "pos"), made(seq, (n_tokens,), int32, "seq")
+        slots = made(slots, (n_tokens,), torch.int64, "slots")
+        if workspace is None:
+            workspace = self.extend_workspace(n)
+        a = L.LlapisKvExtendArgs(self.page_size, self.n_pages, n, n_tokens, width, 0, stride, table, lens.data_ptr(),
+                                 n_new.data_ptr(), free.data_ptr(), n_free.data_ptr(), lens_out.data_ptr(),
+                                 n_free_out.data_ptr(), new_start.data_ptr(), pos.data_ptr(), seq.data_ptr(), slots.data_ptr())
+        _call("llapis_kv_extend", dev, C.byref(a), *_scratch(workspace, dev))
+        return new_start, pos, seq, slots
+
+
+def rope_frequencies(rot_dim, base=10000.0, kind=L.ROPE_PLAIN, factor=1.0, trained=0.0, low=1.0, high=None, divisors=None,
+                     device="cuda"):
+    """(freq float64 [rot_dim / 2] on `device`, magnitude): the frequencies of a
+    rotation of rot_dim values, computed on the host.  kind: ROPE_PLAIN,
+    ROPE_LINEAR, ROPE_NTK, ROPE_YARN or ROPE_BANDS, stretched by `factor` over the
+    `trained` length; low and high (32, for ROPE_BANDS 4): the turns over that length
+    from which a frequency starts to be kept and is kept whole; divisors [rot_dim /
+    2]: numbers that the frequencies are divided by."""
+    torch = _torch()
+    n = max(rot_dim // 2, 0)
+    if divisors is not None:
+        divisors = torch.as_tensor(divisors, dtype=torch.float64, device="cpu").contiguous()
+        _need(divisors.shape == (n,), f"divisors must be {n} numbers")
+    freq, magnitude = torch.empty(n, dtype=torch.float64), C.c_float()
+    rule = L.LlapisRopeRule(kind, rot_dim, base, factor, trained, low, (4.0 if kind == L.ROPE_BANDS else 32.0) if high is None else high,
+                            _ptr(divisors))
+    check(lib().llapis_rope_frequencies(C.byref(rule), freq.data_ptr(), C.byref(magnitude)), "llapis_rope_frequencies")
+    return freq.to(device), magnitude.value
+
+
+def qk_rope(q, k=None, pos=None, freq=None, q_weight=None, k_weight=None, norm=True, eps=1e-6, magnitude=1.0, layout=L.ROPE_HALF,
+            q_out=None, k_out=None):
+    """Norm each head of q [T, n_head, head_dim] and k [T, n_kv, head_dim] (None:
+    no k; float32, float16 or bfloat16) and turn its first 2 len(freq) values by
+    pos [T] (int32) times freq (float64; None: not turned) -> (q_out, k_out), which may be q and k.
+    norm: x / rms(x) * weight, weights float32 [head_dim] or None; layout:
+    ROPE_HALF pairs value i with i + len(freq), ROPE_PAIRS 2 i with 2 i + 1;
+    magnitude: factor on cosine and sine.  Rows with a negative position are
+    left as they are (in outputs made here: as the allocation holds them)."""
+    torch = _torch()
+    shape, dtype, dev = q.shape, q.dtype, _on_gpu(q, "q")
+    _need(len(shape) == 3, "q must be [T, n_head, head_dim]")
+    T, n_head, D = shape
+    if (T | n_head | D) >> 31:
+        _count(T, n_head, D)
+
+    def heads(t, n, what):
+        s, stride = t.shape, t.stride()
+        if len(s) != 3 or s[0] != T or s[1] != n or s[2] != D or t.dtype != dtype or t.device != dev or (D > 1 and stride[2] != 1) or (n > 1 and stride[1] != D):
+            raise ValueError(f"{what} must be [{T}, {n}, {D}] of q's type and device, rows of consecutive values")
+        return t.data_ptr(), stride[0]
+
+    rot = 0
+    if freq is not None:
+        rot = 2 * freq.shape[0]
+        _is(freq, torch.float64, (rot // 2,), dev, "freq")
+        _need(pos is not None, "freq needs pos")
+    if pos is not None:
+        _is(pos, torch.int32, (T,), dev, "pos")
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=dtype, device=dev)
+    n_kv, k_in, k_to = 0, (None, 0), (None, 0)
+    if k is not None:
+        _need(len(k.shape) == 3, "k must be [T, n_kv, head_dim]")
+        n_kv = k.shape[1]
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+        k_in, k_to = heads(k, n_kv, "k"), heads(k_out, n_kv, "k_out")
+    for w in (q_weight, k_weight):
+        if w is not None:
+            _is(w, torch.float32, (D,), dev, "weights")
+    a = L.LlapisQkRopeArgs(_tag(dtype), T, n_head, n_kv, D, rot, layout, int(norm), eps, magnitude, _ptr(pos), _ptr(freq),
+                           *heads(q, n_head, "q"), *heads(q_out, n_head, "q_out"), _ptr(q_weight), *k_in, *k_to, _ptr(k_weight))
+    _call("llapis_qk_rope", dev, C.byref(a))
+    return q_out, k_out
+
+
 def block_norm(h, y=None, post_weight=None, post_norm=True, gate=None, alpha=1.0, beta=1.0, weights=(), eps=1e-6,
                h_out=None, out=None):
     """h' = alpha h + beta gate u, u = rms_norm(y) * post_weight (post_norm) or
@@ -368,6 +490,50 @@ def block_norm(h, y=None, post_weight=None, post_norm=True, gate=None, alpha=1.0
         x_at[i], x_stride[i] = row(x, "out")
     _call("llapis_block_norm", dev, C.byref(a))
     return h_out, out
+
+
+def sample_workspace(n_seq, vocab, device="cuda"):
+    """Scratch for sample, for a caller that keeps it: calls that share it must not overlap."""
+    return _bytes("llapis_sample_workspace_size", device, n_seq, vocab)
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None, workspace=None):
+    """The next token of each sequence -> tokens [n_seq] int32, from logits [n_seq,
+    vocab] (float32, float16 or bfloat16) and u [n_seq] float32 in [0, 1): softmax at
+    the temperature, the top_k most probable (0: all), of those the fewest whose
+    probability is top_p of theirs (1: all), of those the ones of at least min_p
+    times the largest probability; the first token in the vocabulary's order at which the sum of what is left
+    passes u of the whole.  Settings are tensors [n_seq] (float32, top_k int32) or None:
+    temperature 1, the others off; a temperature of 0 takes the most probable.  Ties go
+    to the lowest index.  probs [n_seq, vocab] of the logits' type receives the
+    probabilities drawn with, as verify_drafts takes them."""
+    torch = _torch()
+    shape, dtype, dev = logits.shape, logits.dtype, _on_gpu(logits, "logits")
+    _need(len(shape) == 2, "logits must be [n_seq, vocab]")
+    S, V = shape
+    if (S | V) >> 31:
+        _count(S, V)
+    f32 = torch.float32
+
+    def rows(t, what):
+        stride = t.stride()
+        if t.shape != shape or t.dtype != dtype or t.device != dev or (V > 1 and stride[1] != 1):
+            raise ValueError(f"{what} must be [{S}, {V}] of the logits' type and device, rows of consecutive values")
+        return t.data_ptr(), stride[0] if S > 1 else V
+
+    _is(u, f32, (S,), dev, "u")
+    for t, dt, what in ((temperature, f32, "temperature"), (top_k, torch.int32, "top_k"), (top_p, f32, "top_p"), (min_p, f32, "min_p")):
+        if t is not None:
+            _is(t, dt, (S,), dev, what)
+    if tokens is None:
+        tokens = torch.empty(S, dtype=torch.int32, device=dev)
+    _is(tokens, torch.int32, (S,), dev, "tokens")
+    if workspace is None:
+        workspace = sample_workspace(S, V, dev)
+    a = L.LlapisSampleArgs(_tag(dtype), S, V, *rows(logits, "logits"), u.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                           _ptr(min_p), tokens.data_ptr(), *((None, 0) if probs is None else rows(probs, "probs")))
+    _call("llapis_sample", dev, C.byref(a), *_scratch(workspace, dev))
+    return tokens
 
 
 def verify_workspace(n_seq, vocab, device="cuda"):

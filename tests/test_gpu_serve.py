@@ -1,0 +1,367 @@
+"""Pages and slots, query and key norms with positions, and sampling (llapis_step.h) on
+the GPU against their plain 64-bit forms (serve_ref.py)."""
+import math
+
+import pytest
+import torch
+
+import llapis_amd as la
+import serve_ref as ref
+from step_ref import DT, EPS
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(v, dev):
+    return torch.tensor(v, dtype=torch.int32).to(dev)
+
+
+def f32(v, dev):
+    return torch.tensor(v, dtype=torch.float32).to(dev)
+
+
+# -------------------------------------------------------------- extend
+
+def pages(gpu, n_pages, P):
+    return la.KvPages([la.KvCache.empty(n_pages, P, 1, 64, la.F16, gpu)]) if P in (16, 32, 64, 128, 256) else None
+
+
+def run_extend(gpu, P, table, lens, n_new, free, n_free, n_tokens, in_place=False):
+    n_pages = len(free)
+    pg = pages(gpu, n_pages, P)
+    S, width = len(table), len(table[0])
+    tb = torch.full((S, width + 3), 12345, dtype=torch.int32, device=gpu)      # rows apart
+    tb[:, 1:1 + width] = i32(table, gpu).reshape(S, width)
+    view = tb[:, 1:1 + width]
+    ln, nf = i32(lens, gpu), i32([n_free], gpu)
+    out = (None, None) if in_place else (torch.full_like(ln, 777), torch.full_like(nf, 777))
+    got = pg.extend(view, ln, i32(n_new, gpu), i32(free, gpu), nf, n_tokens, lens_out=out[0], n_free_out=out[1])
+    want = ref.extend(table, lens, n_new, free, n_free, n_tokens, P, n_pages)
+    assert view.tolist() == want[0]
+    assert (tb[:, 0] == 12345).all() and (tb[:, 1 + width:] == 12345).all()
+    assert (ln if in_place else out[0]).tolist() == want[1]
+    assert int(nf if in_place else out[1]) == want[2]
+    if not in_place:
+        assert ln.tolist() == lens and int(nf) == n_free
+    for g, w in zip(got, want[3:]):
+        assert g.tolist() == w
+    return want
+
+
+def batch_of(seed, S, width, P, most_new, spare, holes=False):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda lo, hi: torch.randint(lo, hi + 1, (S,), generator=g).tolist()
+    lens = [min(n, width * P) for n in r(0, width * P)]
+    n_new = r(0, most_new)
+    held = [-(-n // P) for n in lens]
+    n_pages = sum(held) + spare
+    order = torch.randperm(n_pages, generator=g).tolist()
+    table = [[order.pop() if i < k else -1 for i in range(width)] for k in held]
+    if holes:
+        for s in range(0, S, 3):
+            if held[s]:
+                table[s][held[s] - 1] = (-1, n_pages, 2 ** 31 - 1)[s % 2 + s % 3 // 2]
+    free = order + [-1] * (n_pages - spare)
+    return table, lens, n_new, free, spare
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("S,width,P,new,spare", [(1, 1, 16, 1, 1), (1, 4, 16, 20, 5), (7, 6, 32, 40, 9), (48, 12, 16, 1, 60),
+                                                 (1023, 3, 16, 4, 900), (1025, 3, 16, 4, 700), (2047, 2, 16, 3, 2000),
+                                                 (2049, 2, 16, 1, 2500), (5000, 2, 16, 2, 3000)])
+def test_extend(gpu, S, width, P, new, spare, in_place):
+    """Every combination of sums cut short: rows, pages, the table's width."""
+    table, lens, n_new, free, n_free = batch_of(S + width, S, width, P, new, spare, holes=S > 5)
+    total = sum(n_new)
+    for n_tokens, n in ((total + 3, n_free), (total // 2, n_free), (total + 3, n_free // 2), (total, 0), (0, n_free)):
+        run_extend(gpu, P, table, lens, n_new, free, n, n_tokens, in_place)
+
+
+@pytest.mark.parametrize("n_tokens", [4095, 4096, 4097, 30000])
+def test_extend_prompts(gpu, n_tokens):
+    """Prompt chunks: many rows and pages a sequence, on either side of the rows that one workgroup fills."""
+    want = run_extend(gpu, 16, [[-1] * 700 for _ in range(9)], [0, 5, 16, 17, 0, 300, 0, 1, 33][:9],
+                      [5000, 1, 0, 4000, 300, 700, 11200, 11200, 9000], list(range(5000)), 3000, n_tokens, n_tokens % 2 == 0)
+    assert want[3][-1] <= n_tokens
+
+
+def test_extend_corners(gpu):
+    """Negative lengths and numbers, lengths past the table, a count of free pages outside the
+    list, free pages that are none, page sizes that are no power of two are the library's alone."""
+    run_extend(gpu, 16, [[3, -1], [4, 5], [-1, -1], [6, 7]], [-5, 40, 0, 32], [4, 1, -3, 1], [0, 1, 2, -1, 9, 99, -7, 8], 8, 10)
+    run_extend(gpu, 16, [[3, -1], [4, -1]], [16, 16], [1, 1], [0, 1, 2, 5, 6], 99, 4)
+    run_extend(gpu, 16, [[3, -1], [4, -1]], [16, 15], [1, 1], [0, 1, 2, 5, 6], -4, 4)
+    run_extend(gpu, 16, [[0, -1]], [2 ** 31 - 1], [2 ** 31 - 1], [1], 1, 4)
+    # no sequences
+    pg = pages(gpu, 4, 16)
+    nf = i32([3], gpu)
+    got = pg.extend(torch.zeros(0, 2, dtype=torch.int32, device=gpu), i32([], gpu), i32([], gpu), i32([0, 1, 2, -1], gpu), nf, 5)
+    assert got[0].tolist() == [0] and int(nf) == 3 and all(t.tolist() == [-1] * 5 for t in got[1:])
+
+
+def test_extend_graph(gpu):
+    """A captured step grows its sequences in place at every replay, as eager calls do."""
+    P, S = 16, 5
+    pg = pages(gpu, 64, P)
+    new, free = i32([1, 3, 0, 16, 1], gpu), i32(list(range(64)), gpu)
+
+    def state():
+        return torch.full((S, 12), -1, dtype=torch.int32, device=gpu), i32([0] * S, gpu), i32([64], gpu)
+
+    a, b = state(), state()
+    ws = pg.extend_workspace(S)
+    outs = pg.extend(*a[:2], new, free, a[2], 30, workspace=ws)
+    pg.extend(*b[:2], new, free, b[2], 30)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pg.extend(*a[:2], new, free, a[2], 30, new_start=outs[0], pos=outs[1], seq=outs[2], slots=outs[3], workspace=ws)
+    for _ in range(13):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = pg.extend(*b[:2], new, free, b[2], 30)
+        assert all(torch.equal(x, y) for x, y in zip((*a, *outs), (*b, *want)))
+    assert b[1].tolist()[3] == 192          # its row is full
+
+
+# ---------------------------------------------------------------- rope
+
+def run_rope(gpu, seed, T, n_head, n_kv, D, rot, half, tag, norm, weights=True, magnitude=1.0, pos=None, eps=1e-6, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    qkv = (scale * torch.randn(T, n_head + 2 * n_kv + 1, D, generator=g)).to(DT[tag])
+    q, k = qkv[:, :n_head], qkv[:, n_head:n_head + n_kv]
+    wq, wk = ((1 + 0.3 * torch.randn(D, generator=g)) if weights else None for _ in range(2))
+    pos = torch.randint(0, 40000, (T,), generator=g, dtype=torch.int32) if pos is None else pos
+    freq, _ = la.rope_frequencies(rot, device="cpu") if rot else (None, 1)
+    to = lambda t: None if t is None else t.to(gpu)
+    dq = qkv.to(gpu)
+    out_q = torch.full((T, n_head + 1, D), 5.0, dtype=DT[tag], device=gpu)[:, :n_head]
+    got = la.qk_rope(dq[:, :n_head], dq[:, n_head:n_head + n_kv] if n_kv else None, pos.to(gpu), to(freq), q_weight=to(wq),
+                     k_weight=to(wk), norm=norm, eps=eps, magnitude=magnitude, layout=la.ROPE_HALF if half else la.ROPE_PAIRS,
+                     q_out=out_q)
+    for x, w, y in ((q, wq, got[0]), (k, wk, got[1])):
+        if y is None:
+            continue
+        want, tol = ref.rope(x, pos, freq, w, norm, eps, magnitude, half, tag)
+        live = pos >= 0
+        off = (y.cpu().double() - want).abs()[live]
+        assert (off <= tol[live] + (2 ** -25 if tag == la.F16 else 0)).all(), f"off by {float((off / (tol[live] + 1e-30)).max()):.3g} of the bound"
+    assert torch.equal(dq.cpu(), qkv)
+    return got
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("D,rot", [(64, 64), (96, 96), (96, 24), (128, 32), (192, 192), (256, 64), (512, 512), (512, 0), (80, 20),
+                                   (10, 6), (7, 2), (1, 0), (333, 130)])
+@pytest.mark.parametrize("tag", [la.F32, la.F16, la.BF16])
+def test_rope(gpu, tag, D, rot, half, norm):
+    """Every type, both layouts, heads of vectors and odd ones, whole, part and none of a head turned."""
+    run_rope(gpu, D + rot, 5, 3, 2, D, rot, half, tag, norm, magnitude=1.25)
+
+
+@pytest.mark.parametrize("T,n_head,n_kv", [(1, 1, 0), (1, 16, 8), (2047, 3, 1), (2048, 3, 1), (2049, 5, 3), (3, 300, 7)])
+def test_rope_shapes(gpu, T, n_head, n_kv):
+    """One token and many, both sides of the change to several tokens a workgroup, many heads."""
+    run_rope(gpu, T, T, n_head, n_kv, 128, 128, True, la.BF16, True)
+    run_rope(gpu, T, T, n_head, n_kv, 64, 32, False, la.F32, True)
+
+
+def test_rope_far_positions(gpu):
+    """Positions up to 2^31 - 1, and the first."""
+    pos = torch.tensor([0, 1, 131071, 1000003, 16777217, 2 ** 31 - 1], dtype=torch.int32)
+    run_rope(gpu, 1, 6, 2, 1, 64, 64, True, la.F32, False, pos=pos)
+
+
+def test_rope_rows_left(gpu):
+    """Rows of a negative position are neither read nor written, in place or not; a turned pair of the others only."""
+    D, pos = 64, torch.tensor([3, -1, 7, -2 ** 31, 0], dtype=torch.int32)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(5, 2, D, generator=g)
+    x[1], x[3] = float("nan"), float("inf")
+    freq, _ = la.rope_frequencies(D, device=gpu)
+    dx, out = x.to(gpu), torch.full((5, 2, D), 9.0, device=gpu)
+    la.qk_rope(dx, None, pos.to(gpu), freq, q_out=out)
+    assert (out[[1, 3]] == 9).all() and torch.isfinite(out).all()
+    la.qk_rope(dx, None, pos.to(gpu), freq, q_out=dx)
+    assert torch.equal(dx[[0, 2, 4]], out[[0, 2, 4]]) and torch.isnan(dx[1]).all() and torch.isinf(dx[3]).all()
+
+
+def test_rope_norms(gpu):
+    """Without weights, rows of zeros, a large eps, values whose squares are small; norms alone without positions."""
+    run_rope(gpu, 4, 4, 2, 1, 128, 128, True, la.F32, True, weights=False)
+    run_rope(gpu, 5, 4, 2, 1, 128, 64, False, la.F32, True, eps=3.0)
+    run_rope(gpu, 6, 4, 2, 1, 128, 64, False, la.F32, True, scale=1e-6, eps=1e-12)
+    z = torch.zeros(3, 2, 64, device=gpu)
+    freq, _ = la.rope_frequencies(64, device=gpu)
+    assert (la.qk_rope(z, None, i32([1, 2, 3], gpu), freq)[0] == 0).all()
+    x = torch.randn(3, 2, 64, device=gpu)
+    want, tol = ref.rope(x.cpu(), None, None, None, True, 1e-6, 1.0, True, la.F32)
+    assert ((la.qk_rope(x)[0].cpu().double() - want).abs() <= tol).all()
+
+
+def test_rope_unaligned(gpu):
+    """Rows that start at any value."""
+    base = torch.randn(1 + 4 * 301, device=gpu).half()
+    x = base[1:].as_strided((4, 2, 128), (301, 128, 1), 1)
+    freq, _ = la.rope_frequencies(128, device=gpu)
+    pos = i32([5, 6, 7, 8], gpu)
+    got, _ = la.qk_rope(x, None, pos, freq)
+    assert torch.equal(got, la.qk_rope(x.contiguous(), None, pos, freq)[0])
+
+
+def test_rope_graph_and_stream(gpu):
+    freq, _ = la.rope_frequencies(64, device=gpu)
+    q, k, pos = torch.randn(4, 3, 64, device=gpu), torch.randn(4, 1, 64, device=gpu), i32([1, 2, 3, 4], gpu)
+    qo, ko = la.qk_rope(q, k, pos, freq)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        la.qk_rope(q, k, pos, freq, q_out=qo, k_out=ko)
+    for _ in range(3):
+        pos.add_(1000)
+        qo.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = la.qk_rope(q, k, pos, freq)
+        assert torch.equal(qo, want[0]) and torch.equal(ko, want[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = la.qk_rope(q, k, pos, freq)
+    side.synchronize()
+    assert torch.equal(got[0], want[0])
+
+
+# -------------------------------------------------------------- sample
+
+def run_sample(gpu, logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    dev = lambda v, t: None if v is None else torch.tensor(v, dtype=t).to(gpu)
+    S, V = logits.shape
+    wide = torch.full((S, V + 5), 50.0, dtype=logits.dtype)
+    wide[:, 2:2 + V] = logits
+    wide = wide.to(gpu)
+    probs = torch.full((S, V + 3), 7.0, dtype=logits.dtype, device=gpu)
+    args = (dev(temperature, torch.float32), dev(top_k, torch.int32), dev(top_p, torch.float32), dev(min_p, torch.float32))
+    got = la.sample(wide[:, 2:2 + V], f32(u, gpu), *args, probs=probs[:, 1:1 + V])
+    up = lambda v: None if v is None else torch.tensor(v, dtype=torch.float32).tolist()
+    tokens, want = ref.sample(logits, f32(u, "cpu"), up(temperature), top_k, up(top_p), up(min_p))
+    assert got.tolist() == tokens
+    # rounded once; fp16's least step
+    tag = {v: k for k, v in DT.items()}[logits.dtype]
+    p = probs[:, 1:1 + V].cpu().double()
+    off = (p - want).abs()
+    assert (off <= want * (EPS[tag] + 1e-12) + (2 ** -25 if tag == la.F16 else 2 ** -63)).all(), float(off.max())
+    assert (probs[:, 0] == 7).all() and (probs[:, 1 + V:] == 7).all()
+    # without probabilities, and again
+    for _ in range(2):
+        assert la.sample(wide[:, 2:2 + V], f32(u, gpu), *args).tolist() == tokens
+    return tokens, want
+
+
+def logits_of(seed, S, V, tag, width=2.5):
+    g = torch.Generator().manual_seed(seed)
+    x = width * torch.randn(S, V, generator=g)
+    x[:, ::max(V // 7, 1)] += 5
+    return x.to(DT[tag]), torch.rand(S, generator=g).tolist()
+
+
+@pytest.mark.parametrize("V", [1, 2, 37, 1000, 2048, 2049, 32003, 32768, 32769, 128001])
+@pytest.mark.parametrize("tag", [la.F32, la.F16, la.BF16])
+def test_sample(gpu, tag, V):
+    """Each filter alone, pairs, all and none, sizes around segments and chunks, types whose values tie."""
+    settings = [(1.0, 0, 1.0, 0.0), (0.7, 40, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.3, 0, 1.0, 0.05), (0.8, 40, 0.95, 0.05), (1.0, 1000, 0.999, 0.0),
+                (0.0, 5, 0.5, 0.5), (2.0, 1, 0.9, 0.0), (0.3, 3, 0.3, 0.0), (5.0, 500, 0.5, 0.001), (1.0, 10 ** 9, 0.01, 1.0), (0.1, 2000, 0.9999, 0.0)]
+    x, u = logits_of(V, len(settings), V, tag)
+    run_sample(gpu, x, u, *zip(*settings))
+
+
+@pytest.mark.parametrize("S", [1, 3, 64])
+def test_sample_large(gpu, S):
+    x, u = logits_of(S, S, 262144, la.F32, 2.2)
+    run_sample(gpu, x, u, [1.0] * S, [64 * (i % 3) for i in range(S)], [(0.9, 0.99, 1.0)[i % 3 - 1] for i in range(S)], None)
+
+
+@pytest.mark.parametrize("V,k,p", [(20000, 7000, 1.0), (20000, 0, 0.4), (20000, 9000, 0.5), (5000, 4999, 0.999), (70000, 69999, 0.7),
+                                   (4096, 100, 0.5), (4097, 4000, 0.9)])
+def test_sample_ties(gpu, V, k, p):
+    """Equal logits: the first indices are kept, by candidates that are sorted and by more than that."""
+    x = torch.full((3, V), 1.5)
+    x[1, V // 3::5] = 2.0
+    x[2] = torch.randint(0, 3, (V,), generator=torch.Generator().manual_seed(V)) / 64.0
+    _, want = run_sample(gpu, x, [0.1, 0.9, 0.5], None, [k] * 3, [p] * 3)
+    if p == 1.0:
+        assert (want[0, :k] > 0).all() and (want[0, k:] == 0).all()
+
+
+def test_sample_values(gpu):
+    """NaN and infinities, rows without a value, zeros of both signs, far temperatures and settings off the scale."""
+    inf, nan, V = math.inf, math.nan, 300
+    x = torch.randn(12, V, generator=torch.Generator().manual_seed(5))
+    x[0] = -inf
+    x[1] = nan
+    x[2, ::2] = nan
+    x[3, 1::3] = -inf
+    x[4, [7, 90]] = inf
+    x[5, 10:] = -inf
+    x[6] = 0.0
+    x[6, ::2] = -0.0
+    x[7] *= 1e30
+    x[8] *= 1e-30
+    x[9, 5] = 3e38
+    x[10, 5] = -3e38
+    u = [0.5, 0.5, 0.7, 0.2, 0.6, 0.99, 0.4, 0.5, 0.3, 0.9, 0.1, 0.0]
+    for k, p, m in ((0, 1.0, 0.0), (5, 1.0, 0.0), (0, 0.8, 0.0), (20, 0.9, 0.1), (1, 1.0, 0.0), (-3, 1.5, -1.0), (10, 0.0, 0.0), (10, -1.0, 0.0), (0, 1.0, 1.0),
+                    (0, 1.0, 1.5), (2 ** 31 - 1, 0.5, 0.0)):
+        for t in (1.0, 0.0, -1.0, 1e-40, 1e30, inf, nan):
+            run_sample(gpu, x, u, [t] * 12, [k] * 12, [p] * 12, [m] * 12)
+    # settings that are no numbers are off
+    a = run_sample(gpu, x, u, None, [5] * 12, [nan] * 12, [nan] * 12)
+    assert a[0] == run_sample(gpu, x, u, None, [5] * 12)[0]
+
+
+def test_sample_draws(gpu):
+    """u of 0, next to 1, and outside [0, 1): the first and the last kept value."""
+    x, _ = logits_of(8, 6, 5000, la.F32)
+    run_sample(gpu, x, [0.0, 1 - 2 ** -24, 1.0, 7.0, -0.5, 0.5], None, [50] * 6)
+    run_sample(gpu, x, [0.0, 1 - 2 ** -24, 1.0, 7.0, -0.5, 0.5])
+    # every value is drawn where its share of u is
+    y = torch.tensor([[1.0, 2.0, 0.5, 3.0]]).log().expand(13, 4).contiguous()
+    got, _ = run_sample(gpu, y, [(i + 0.5) / 13 for i in range(13)])
+    assert got == [0] * 2 + [1] * 4 + [2] + [3] * 6
+
+
+def test_sample_feeds_verification(gpu):
+    """Drafts sampled with their probabilities, then verified against the same model's: all are taken."""
+    S, V = 4, 3001
+    x, u = logits_of(9, S, V, la.F32)
+    x = x.to(gpu)
+    probs = torch.empty(S, V, device=gpu)
+    k = i32([50] * S, gpu)
+    d = la.sample(x, f32(u, gpu), top_k=k, probs=probs)
+    target = torch.stack([probs, probs], 1)
+    tokens, accepted = la.verify_drafts(target, probs[:, None], d[:, None].contiguous(), f32([[0.99]] * S, gpu), f32(u, gpu))
+    assert accepted.tolist() == [1] * S and torch.equal(tokens[:, 0], d)
+    assert torch.equal(tokens[:, 1], d)                 # the same u, the same probabilities
+
+
+def test_sample_graphs_share_a_workspace(gpu):
+    x = [logits_of(i, 3, 40000 + i, la.BF16)[0].to(gpu) for i in range(2)]
+    u, p = f32([0.2, 0.6, 0.9], gpu), f32([0.9, 0.95, 1.0], gpu)
+    ws = la.sample_workspace(3, 40001, gpu)
+    toks, graphs = [], []
+    for y in x:
+        tok = la.sample(y, u, top_p=p, workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            la.sample(y, u, top_p=p, tokens=tok, workspace=ws)
+        toks.append(tok)
+        graphs.append(g)
+    for step in range(4):
+        for y, tok, g in zip(x, toks, graphs):
+            tok.fill_(-5)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(tok, la.sample(y, u, top_p=p))
+        u.mul_(0.7)

@@ -1,0 +1,214 @@
+"""The operators before and after a step's attention (llapis_step.h) without a GPU: struct
+layouts, sizes, rotary frequencies, and the calls that are refused before anything is launched."""
+import ctypes as C
+import math
+
+import pytest
+
+import llapis_amd as la
+from llapis_amd import _lib
+from test_abi import INCLUDE, compile_layouts
+from test_step import P, refused
+
+STRUCTS = {
+    "llapis_kv_extend_args": _lib.LlapisKvExtendArgs, "llapis_rope_rule": _lib.LlapisRopeRule,
+    "llapis_qk_rope_args": _lib.LlapisQkRopeArgs, "llapis_sample_args": _lib.LlapisSampleArgs,
+}
+
+
+def test_ctypes_mirror_matches_header(tmp_path):
+    structs = {k: [f[0] for f in v._fields_] for k, v in STRUCTS.items()}
+    got = compile_layouts(tmp_path, str(INCLUDE / "llapis_step.h"), structs)
+    for s, cls in STRUCTS.items():
+        assert got[(s, "sizeof")] == C.sizeof(cls), s
+        for f in structs[s]:
+            assert got[(s, f)] == getattr(cls, f).offset, (s, f)
+
+
+# -------------------------------------------------------------- extend
+
+def extend_args(**kw):
+    a = dict(page_size=16, n_pages=8, n_seq=2, n_tokens=4, max_pages=4, table_stride=4, page_table=P, lens=P, n_new=P, free_pages=P,
+             n_free=P, lens_out=P, n_free_out=P, new_start=P, pos=P, seq=P, slots=P)
+    a.update(kw)
+    return _lib.LlapisKvExtendArgs(**a)
+
+
+@pytest.mark.parametrize("bad", [dict(page_size=0), dict(n_pages=0), dict(n_pages=(1 << 30) + 1), dict(n_seq=-1), dict(n_seq=1 << 24),
+                                 dict(n_tokens=-1), dict(n_tokens=(1 << 30) + 1), dict(max_pages=0), dict(table_stride=3),
+                                 dict(max_pages=1 << 27, table_stride=1 << 27), dict(page_table=None), dict(lens=None), dict(n_new=None),
+                                 dict(free_pages=None), dict(n_free=None), dict(lens_out=None), dict(n_free_out=None),
+                                 dict(new_start=None)], ids=str)
+def test_extend_refusals(bad):
+    a = extend_args(**bad)
+    refused(la.lib().llapis_kv_extend(C.byref(a), P, 1 << 40, None), "llapis_kv_extend")
+
+
+def test_extend_workspace():
+    a, lib = extend_args(), la.lib()
+    need = lib.llapis_kv_extend_workspace_size(2)
+    assert need > 0 and lib.llapis_kv_extend_workspace_size(1 << 24) == 0 == lib.llapis_kv_extend_workspace_size(-1)
+    for n in (0, 1, 1000):
+        assert 0 < lib.llapis_kv_extend_workspace_size(n) < lib.llapis_kv_extend_workspace_size(n + 1)
+    refused(lib.llapis_kv_extend(C.byref(a), P, need - 1, None), "workspace")
+    refused(lib.llapis_kv_extend(C.byref(a), P + 2, need, None), "workspace")
+    refused(lib.llapis_kv_extend(C.byref(a), None, need, None), "workspace")
+    refused(lib.llapis_kv_extend(None, P, need, None), "null")
+
+
+# ---------------------------------------------------------------- rope
+
+def test_frequencies():
+    freq = lambda *a, **kw: (lambda f, m: (f.tolist(), m))(*la.rope_frequencies(*a, device="cpu", **kw))
+    f, m = freq(64, 10000.0)
+    assert m == 1.0 and f == pytest.approx([10000.0 ** (-i / 32) for i in range(32)], rel=1e-14)
+    f2, _ = freq(64, 10000.0, divisors=[1.0 + i for i in range(32)])
+    assert f2 == pytest.approx([x / (1 + i) for i, x in enumerate(f)], rel=1e-14)
+    assert freq(64, 10000.0, la.ROPE_LINEAR, 4.0)[0] == pytest.approx([x / 4 for x in f], rel=1e-14)
+    # the base grows such that the slowest frequency is divided by the factor, the fastest kept
+    f3, _ = freq(64, 10000.0, la.ROPE_NTK, 4.0)
+    assert f3[0] == 1.0 and f3[-1] == pytest.approx(f[-1] / 4, rel=1e-13)
+    # by turns over the trained length: above `high` kept, below `low` divided
+    for kind, low, high in ((la.ROPE_YARN, 1.0, 32.0), (la.ROPE_BANDS, 1.0, 4.0)):
+        g, m = freq(128, 500000.0, kind, 8.0, 8192.0)
+        h, _ = freq(128, 500000.0)
+        assert m == pytest.approx(0.1 * math.log(8) + 1 if kind == la.ROPE_YARN else 1.0, rel=1e-7)
+        between = 0
+        for i, (x, y) in enumerate(zip(g, h)):
+            turns = 8192 * y / (2 * math.pi)
+            if kind == la.ROPE_BANDS:
+                s = min(max((turns - low) / (high - low), 0), 1)
+            else:
+                at = lambda t: 128 * math.log(8192 / (t * 2 * math.pi)) / (2 * math.log(500000.0))
+                lo, hi = math.floor(at(high)), math.ceil(at(low))
+                s = 1 - min(max((i - lo) / (hi - lo), 0), 1)
+            between += 0 < s < 1
+            assert x == pytest.approx(y * s + y / 8 * (1 - s), rel=1e-12), i
+        assert between > 2 and g[0] == h[0] and g[-1] == pytest.approx(h[-1] / 8, rel=1e-13)
+    # ramps of no width, one pair, no stretching
+    assert freq(2, 10000.0, la.ROPE_NTK, 4.0)[0] == [1.0]
+    assert freq(2, 10000.0, la.ROPE_YARN, 1.0, 10.0)[1] == 1.0
+    assert all(math.isfinite(x) for x in freq(4, 1e6, la.ROPE_YARN, 16.0, 5.0, low=1.0, high=1.5)[0])
+
+
+@pytest.mark.parametrize("bad", [dict(rot_dim=0), dict(rot_dim=7), dict(rot_dim=514), dict(kind=5), dict(kind=-1), dict(base=1.0),
+                                 dict(base=math.nan), dict(base=math.inf), dict(kind=1, factor=0.0), dict(kind=2, factor=math.inf),
+                                 dict(kind=3, factor=math.nan), dict(kind=3, factor=2.0), dict(kind=4, factor=2.0, trained=100.0, low=4.0, high=4.0),
+                                 dict(kind=4, factor=2.0, trained=100.0, low=0.0, high=4.0)], ids=str)
+def test_frequency_refusals(bad):
+    a = dict(kind=0, rot_dim=64, base=10000.0, factor=1.0, trained=0.0, low=1.0, high=32.0)
+    a.update(bad)
+    rule, out, m = _lib.LlapisRopeRule(**a), (C.c_double * 256)(), C.c_float()
+    refused(la.lib().llapis_rope_frequencies(C.byref(rule), out, C.byref(m)), "llapis_rope_frequencies")
+    assert not any(out) and m.value == 0
+    refused(la.lib().llapis_rope_frequencies(None, out, C.byref(m)), "null")
+    zero = (C.c_double * 32)()
+    rule = _lib.LlapisRopeRule(kind=0, rot_dim=64, base=10000.0, divisors=C.addressof(zero))
+    refused(la.lib().llapis_rope_frequencies(C.byref(rule), out, C.byref(m)), "divisors")
+
+
+def rope_args(**kw):
+    a = dict(type=la.F32, n_tokens=2, n_head=4, n_kv=2, head_dim=64, rot_dim=64, layout=0, norm=1, eps=1e-6, magnitude=1.0, pos=P, freq=P,
+             q=P, q_stride=256, q_out=P, q_out_stride=256, k=P, k_stride=128, k_out=P, k_out_stride=128)
+    a.update(kw)
+    return _lib.LlapisQkRopeArgs(**a)
+
+
+@pytest.mark.parametrize("bad", [dict(type=la.Q8_0), dict(n_tokens=-1), dict(n_tokens=1 << 24), dict(n_head=-1), dict(n_kv=-1), dict(n_head=65537),
+                                 dict(n_kv=65537), dict(head_dim=0), dict(head_dim=513), dict(rot_dim=65), dict(rot_dim=66), dict(rot_dim=-2),
+                                 dict(layout=2), dict(layout=-1), dict(pos=None), dict(freq=None), dict(q=None), dict(q_out=None), dict(k=None),
+                                 dict(k_out=None), dict(q_out_stride=255), dict(k_out_stride=127)], ids=str)
+def test_rope_refusals(bad):
+    a = rope_args(**bad)
+    refused(la.lib().llapis_qk_rope(C.byref(a), None), "llapis_qk_rope")
+
+
+def test_rope_of_nothing():
+    for nothing in (dict(n_tokens=0), dict(n_head=0, n_kv=0)):
+        a = rope_args(**nothing)
+        assert la.lib().llapis_qk_rope(C.byref(a), None) == 0
+    refused(la.lib().llapis_qk_rope(None, None), "null")
+
+
+# -------------------------------------------------------------- sample
+
+def sample_args(**kw):
+    a = dict(type=la.F32, n_seq=2, vocab=100, logits=P, logits_stride=100, u=P, tokens=P, probs=P, probs_stride=100)
+    a.update(kw)
+    return _lib.LlapisSampleArgs(**a)
+
+
+@pytest.mark.parametrize("bad", [dict(type=la.Q8_0), dict(n_seq=-1), dict(n_seq=65536), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(logits=None),
+                                 dict(u=None), dict(tokens=None), dict(logits_stride=99), dict(probs_stride=99)], ids=str)
+def test_sample_refusals(bad):
+    a = sample_args(**bad)
+    refused(la.lib().llapis_sample(C.byref(a), P, 1 << 50, None), "llapis_sample")
+
+
+def test_sample_workspace():
+    a, lib = sample_args(), la.lib()
+    need = lib.llapis_sample_workspace_size(2, 100)
+    assert need > 0
+    refused(lib.llapis_sample(C.byref(a), P, need - 1, None), "workspace")
+    refused(lib.llapis_sample(C.byref(a), P + 8, need, None), "workspace")
+    refused(lib.llapis_sample(C.byref(a), None, need, None), "workspace")
+    refused(lib.llapis_sample(None, P, need, None), "null")
+    a = sample_args(n_seq=0)
+    assert lib.llapis_sample(C.byref(a), None, 0, None) == 0
+    for s, v in ((0, 10), (65536, 10), (1, 0), (1, (1 << 30) + 1), (-1, 5)):
+        assert lib.llapis_sample_workspace_size(s, v) == 0
+    # a workspace for more serves less
+    for s, v in ((1, 1), (3, 32768), (64, 128001)):
+        n = lib.llapis_sample_workspace_size(s, v)
+        assert 0 < n <= lib.llapis_sample_workspace_size(s + 1, v) and n <= lib.llapis_sample_workspace_size(s, v + 1)
+    assert lib.llapis_sample_workspace_size(65535, 1 << 30) > 1 << 48
+
+
+# -------------------------------------------------------------- python
+
+def test_python_refuses_host_tensors():
+    import torch
+    with pytest.raises(ValueError, match="GPU"):
+        la.qk_rope(torch.zeros(2, 2, 64))
+    with pytest.raises(ValueError, match="GPU"):
+        la.sample(torch.zeros(2, 10), torch.zeros(2))
+
+
+def test_python_checks(monkeypatch):
+    """Host tensors stand in for the GPU's, and nothing is called."""
+    import torch
+    from llapis_amd import step
+    called = []
+    monkeypatch.setattr(step, "_on_gpu", lambda t, what: t.device)
+    monkeypatch.setattr(step, "_call", lambda *a: called.append(a[0]))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    pages = step.KvPages([step.KvCache.empty(4, 16, 1, 64, la.F16, "cpu")])
+    table, lens, new, free, one = i32([0, -1], [1, -1]), i32(3, 4), i32(1, 1), i32(2, 3, -1, -1), i32(2)
+    extend = lambda **kw: pages.extend(*(kw.get(k, v) for k, v in (("table", table), ("lens", lens), ("new", new), ("free", free), ("one", one), ("n", 4))),
+                                       **{k: v for k, v in kw.items() if k not in ("table", "lens", "new", "free", "one", "n")})
+    extend()
+    for bad, what in ((dict(table=table.long()), "page_table"), (dict(table=table[:1].expand(2, 2)), "overlap"), (dict(lens=i32(3)), "lens"),
+                      (dict(new=i32(1)), "n_new"), (dict(free=i32(2, 3)), "free"), (dict(one=i32(2, 2)), "n_free"), (dict(n=1 << 32), "2\\^31"),
+                      (dict(lens_out=i32(3)), "lens_out"), (dict(n_free_out=lens), "n_free_out"), (dict(new_start=lens), "new_start"),
+                      (dict(pos=lens), "pos"), (dict(seq=lens), "seq"), (dict(slots=torch.zeros(4, dtype=torch.int32)), "slots"),
+                      (dict(workspace=torch.zeros(1, dtype=torch.uint8).expand(1 << 20)), "workspace")):
+        with pytest.raises(ValueError, match=what):
+            extend(**bad)
+    q, k, pos, freq = torch.zeros(3, 4, 64), torch.zeros(3, 2, 64), i32(1, 2, 3), torch.ones(32, dtype=torch.float64)
+    step.qk_rope(q, k, pos, freq)
+    for bad, what in ((dict(q=q[0]), "q must"), (dict(k=k[:2]), "k must"), (dict(k=k.half()), "k must"), (dict(k=k[0]), "k must"), (dict(pos=None), "pos"),
+                      (dict(pos=pos.long()), "pos"), (dict(freq=freq.float()), "freq"), (dict(q=q.transpose(0, 1), k=None, pos=None, freq=None), "q must"),
+                      (dict(q=q.to(torch.int32), k=None, pos=None, freq=None), "float32"), (dict(q_weight=freq), "weights"), (dict(k_weight=torch.ones(63)), "weights"),
+                      (dict(q_out=k), "q_out"), (dict(k_out=q), "k_out"), (dict(q=torch.zeros(3, 4, 128)[..., ::2], k=None, pos=None, freq=None), "q must"),
+                      (dict(q=torch.zeros(1, 1, 1).expand((1 << 32) + 1, 1, 1)), "2\\^31")):
+        with pytest.raises(ValueError, match=what):
+            step.qk_rope(**{**dict(q=q, k=k, pos=pos, freq=freq), **bad})
+    x, u = torch.zeros(2, 10), torch.zeros(2)
+    step.sample(x, u, workspace=torch.empty(1 << 20, dtype=torch.uint8))
+    for bad, what in ((dict(logits=x[0]), "logits"), (dict(logits=torch.zeros(10, 2).t()), "logits"), (dict(logits=x.to(torch.int32)), "float32"), (dict(u=u.double()), "u must"),
+                      (dict(temperature=u.half()), "temperature"), (dict(top_k=u), "top_k"), (dict(top_p=u[:1]), "top_p"), (dict(min_p=1.0 * pos), "min_p"),
+                      (dict(tokens=u), "tokens"), (dict(probs=x.half()), "probs"), (dict(probs=x[:, :5]), "probs"),
+                      (dict(workspace=torch.zeros(1, dtype=torch.uint8).expand(1 << 20)), "workspace")):
+        with pytest.raises(ValueError, match=what):
+            step.sample(**{**dict(logits=x, u=u), **bad})
+    assert called == ["llapis_kv_extend", "llapis_qk_rope", "llapis_sample"]
