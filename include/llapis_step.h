@@ -112,6 +112,29 @@ uint64_t llapis_kv_attention_workspace_size(const llapis_kv_cache * c, const lla
 int32_t  llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * a,
                              void * workspace, uint64_t ws_bytes, void * stream);
 
+/* The same attention (without a window) of a batch whose sequences begin with the
+ * same tokens on the same pages, as llapis_kv_fork leaves them: group g is the
+ * sequences groups[g] .. groups[g + 1] - 1, in whose rows of the page table the first
+ * prefix[g] tokens' entries are the same; they are read from the first of them with new
+ * tokens, once for the whole group (in tiles of 64 to 256 query rows of a kv head),
+ * and each sequence's other keys are attended as above.  Both arrays are read on the device; groups
+ * are in order (as the rows of new_start are), sequences before the first and behind the
+ * last share nothing.  A prefix is cut to what every sequence of its group with new tokens had before
+ * them, and to a multiple of 64 tokens and of a page; what is cut off counts as each one's own.  Results are
+ * llapis_kv_attention's but for the order of sums.  n_group is 256 at most.  Refused:
+ * what attention refuses, and prefixes of 2^30 and more units of work (32 or 64 keys of
+ * a kv head for a tile of rows).  The workspace serves every call of fewer sequences, rows, new
+ * tokens, pages and groups too; its size reads b's n_tokens beside what attention's does. */
+typedef struct llapis_kv_prefix {
+    int32_t n_group;
+    const int32_t * groups;        /* [n_group + 1] */
+    const int32_t * prefix;        /* [n_group] */
+} llapis_kv_prefix;
+uint64_t llapis_kv_prefix_attention_workspace_size(const llapis_kv_cache * c, const llapis_kv_batch * b, int32_t n_head,
+                                                   int32_t n_group);
+int32_t  llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * a,
+                                    const llapis_kv_prefix * x, void * workspace, uint64_t ws_bytes, void * stream);
+
 /* ------------------------------------------------------------- pages
  *
  * Operations on whole pages, the same in every plane: a plane is one layer's

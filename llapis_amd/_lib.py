@@ -156,6 +156,10 @@ class LlapisVerifyArgs(C.Structure):
                 ("tokens", vp), ("accepted", vp)]
 
 
+class LlapisKvPrefix(C.Structure):
+    _fields_ = [("n_group", i32), ("groups", vp), ("prefix", vp)]
+
+
 class LlapisKvExtendArgs(C.Structure):
     _fields_ = [("page_size", i32), ("n_pages", i32), ("n_seq", i32), ("n_tokens", i32), ("max_pages", i32), ("reserved", i32),
                 ("table_stride", i64), ("page_table", vp), ("lens", vp), ("n_new", vp), ("free_pages", vp), ("n_free", vp),
@@ -189,6 +193,9 @@ STEP_SIGNATURES = {
     "llapis_kv_append": (i32, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), i32, vp, i64, vp, i64, vp]),
     "llapis_kv_attention_workspace_size": (u64, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), i32]),
     "llapis_kv_attention": (i32, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), C.POINTER(LlapisKvQuery), vp, u64, vp]),
+    "llapis_kv_prefix_attention_workspace_size": (u64, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), i32, i32]),
+    "llapis_kv_prefix_attention": (i32, [C.POINTER(LlapisKvCache), C.POINTER(LlapisKvBatch), C.POINTER(LlapisKvQuery),
+                                         C.POINTER(LlapisKvPrefix), vp, u64, vp]),
     "llapis_kv_copy_pages": (i32, [C.POINTER(LlapisKvPlanes), vp, i32, vp]),
     "llapis_kv_fork": (i32, [C.POINTER(LlapisKvPlanes), vp, i64, i32, vp, i32, vp, i32, vp]),
     "llapis_kv_page_refs": (i32, [i32, i32, vp, i64, i32, vp, i32, vp, vp, vp, vp]),

@@ -20,7 +20,8 @@ LIB = PKG / "libllapis_moe.so"
 ARCH = "gfx950"
 
 HIP_SOURCES = ["mmv.hip", "decode.hip", "prefill.hip", "small_kernels.hip", "transfer.hip", "model_files.hip",
-               "residency.hip", "kv_attn_f16.hip", "kv_attn_bf16.hip", "kv_attn_q8.hip", "kv_cache.hip", "kv_extend.hip",
+               "residency.hip", "kv_attn_f16.hip", "kv_attn_bf16.hip", "kv_attn_q8.hip", "kv_prefix_f16.hip",
+               "kv_prefix_bf16.hip", "kv_prefix_q8.hip", "kv_cache.hip", "kv_extend.hip",
                "rope.hip", "step.hip", "sample.hip", "api.hip"]
 HOST_SOURCES = ["quantize.cpp", "policy.cpp", "kfit.cpp"]
 

@@ -37,7 +37,7 @@ struct KvAttn {
     int n_kv, group;                 // query heads of a kv head
     int window, unit;
     float scale;
-    int type;                        // of q and out
+    int type, out_type;              // of q, of out
     const void * q;
     int64_t q_stride;
     void * out;

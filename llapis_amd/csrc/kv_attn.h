@@ -780,7 +780,7 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
 #pragma unroll
                 for (int t = 0; t < NVW; ++t)
                     if (v_tile + t < NV)
-                        store4(p.out, type, out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
+                        store4(p.out, WIDE ? (int)T_F32 : p.out_type, out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
                 if (p.lse && wave == 0 && lg == 0)
                     p.lse[out_row * (p.group * p.n_kv) + hq] =
                         sum == 0.0f ? -__builtin_inff() : (m[nt] + (__builtin_amdgcn_logf(sum) - P_SHIFT)) * KV_LN2;

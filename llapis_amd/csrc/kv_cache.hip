@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <cstdio>
 
-#include "kv_attn.h"
+#include "kv_prefix.h"
 
 namespace llapis {
 namespace dev {
@@ -97,9 +97,127 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, f
     const int rr = tile * tile_rows + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
     const int64_t row = su.r.row0 + tok;
     const float inv = 1.0f / l;
-    store4(p.out, p.type, row * p.out_stride + (int64_t)hq * head_dim + d, l == 0.0f ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : a * inv);
+    store4(p.out, p.out_type, row * p.out_stride + (int64_t)hq * head_dim + d, l == 0.0f ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : a * inv);
     if (p.lse && d == 0)
         p.lse[row * (p.n_kv * p.group) + hq] = l == 0.0f ? -__builtin_inff() : (m + (__builtin_amdgcn_logf(l) - p_shift)) * KV_LN2;
+}
+
+// --------------------------------------------------- join with a prefix
+//
+// As k_kv_join, of the parts of a row's prefix (k_kv_prefix) and those of its own keys,
+// which are parts of k_kv_attn or, where one run had them all, its result with the
+// logarithm of its sum.
+struct KvResult {
+    void * out;
+    int64_t out_stride;
+    float * lse;
+    int type;
+};
+
+template <int PG>
+__global__ __launch_bounds__(256) void k_kv_prefix_join(const KvAttn p, const KvPrefix x, const KvResult o, int head_dim,
+                                                        int prefix_rows, float p_shift) {
+    constexpr int TPG = 256 / PG;
+    __shared__ f4v s_acc[PG][TPG];
+    __shared__ float s_m[PG][TPG], s_l[PG][TPG];
+    const int tid = threadIdx.x, g = tid / TPG, e = tid - g * TPG, tile_rows = 16 * p.nt;
+    const int seq = blockIdx.x / (p.n_kv * p.tiles), rest = blockIdx.x - seq * p.n_kv * p.tiles;
+    const int total = p.base[p.b.n_seq], base = p.base[seq], grp = x.seq_group[seq], p_total = x.total[0];
+    const SeqUnits su = seq_units(p.b, seq, p.page_shift, 0, p.unit);
+    const int head = rest / p.tiles, tile = rest - head * p.tiles;
+    const int n_rows = min(su.r.n * p.group - tile * tile_rows, tile_rows);
+    const int at = (blockIdx.y * TPG + e) * 4, r = at / head_dim, d = at - r * head_dim;
+    if ((int)(blockIdx.y * TPG * 4) >= n_rows * head_dim) return;      // also: no such item
+    const bool live = r < n_rows;
+    const int rr = tile * tile_rows + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
+    const int64_t row = su.r.row0 + tok;
+    // the runs of the item's first and last unit, here and in the prefix
+    const Runs runs(total, runs_of(p.runs, total));
+    const int first = base + head * item_steps(su.units);
+    const int w0 = runs.owner(first + 1), n_own = runs.owner(first + 2 * su.units - 1) - w0 + 1;
+    int n_pre = 0;
+    int64_t pre_row = 0;                                               // the first part's
+    if (grp >= 0 && p_total > 0) {
+        const KvGroup gr = x.plan[grp];
+        const int pr = (int)(row - gr.row0) * p.group + rr - tok * p.group;
+        if (row >= gr.row0 && pr < gr.rows) {
+            const Runs pre(p_total, runs_of(x.runs, p_total));
+            const int tiles = (gr.rows + prefix_rows - 1) / prefix_rows, item = head * tiles + pr / prefix_rows;
+            const int begin = gr.base + item * item_steps(gr.units), v0 = pre.owner(begin + 1);
+            n_pre = pre.owner(begin + 2 * gr.units - 1) - v0 + 1;
+            const int64_t slot = (int64_t)gr.item + item + v0;
+            n_pre = (int)min((int64_t)n_pre, x.slots - slot);
+            pre_row = slot * prefix_rows + pr % prefix_rows;
+        }
+    }
+    f4v a = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -__builtin_inff(), l = 0.0f;
+    constexpr int UN = 8;
+    for (int i0 = g; i0 < n_pre + n_own; i0 += PG * UN) {
+        f4v v[UN];
+        float vm[UN], vl[UN];
+#pragma unroll
+        for (int j = 0; j < UN; ++j) {
+            const int i = i0 + PG * j;
+            v[j] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            vm[j] = -__builtin_inff();
+            vl[j] = 0.0f;
+            if (!live || i >= n_pre + n_own) continue;
+            if (i < n_pre) {
+                const int64_t at_row = pre_row + (int64_t)i * prefix_rows;
+                v[j] = *(const f4v *)(x.acc + at_row * head_dim + d);
+                vm[j] = x.ml[2 * at_row];
+                vl[j] = x.ml[2 * at_row + 1];
+            } else if (n_own == 1) {
+                v[j] = *(const f4v *)((const float *)p.out + row * p.out_stride + (int64_t)hq * head_dim + d) * __builtin_ldexpf(1.0f, (int)p_shift);
+                vm[j] = p.lse[row * (p.n_kv * p.group) + hq] * KV_LOG2E;
+                vl[j] = vm[j] == -__builtin_inff() ? 0.0f : __builtin_ldexpf(1.0f, (int)p_shift);
+            } else {
+                const int64_t at_row = (((int64_t)(w0 + i - n_pre) * p.tiles + tile) * 2 + (i == n_pre)) * tile_rows + r;
+                v[j] = *(const f4v *)(p.acc + at_row * head_dim + d);
+                vm[j] = p.ml[2 * at_row];
+                vl[j] = p.ml[2 * at_row + 1];
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < UN; ++j) top = fmaxf(top, vm[j]);
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        a *= f;
+        l *= f;
+        m = top;
+#pragma unroll
+        for (int j = 0; j < UN; ++j) {
+            const float w = __builtin_amdgcn_exp2f(vm[j] - ref);
+            a += w * v[j];
+            l += w * vl[j];
+        }
+    }
+    if (PG > 1) {
+        s_acc[g][e] = a;
+        s_m[g][e] = m;
+        s_l[g][e] = l;
+        __syncthreads();
+        if (g > 0) return;
+        float top = m;
+        for (int i = 1; i < PG; ++i) top = fmaxf(top, s_m[i][e]);
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        a *= f;
+        l *= f;
+        m = top;
+        for (int i = 1; i < PG; ++i) {
+            const float w = __builtin_amdgcn_exp2f(s_m[i][e] - ref);
+            a += w * s_acc[i][e];
+            l += w * s_l[i][e];
+        }
+    }
+    if (!live) return;
+    const float inv = 1.0f / l;
+    store4(o.out, o.type, row * o.out_stride + (int64_t)hq * head_dim + d, l == 0.0f ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : a * inv);
+    if (o.lse && d == 0)
+        o.lse[row * (p.n_kv * p.group) + hq] = l == 0.0f ? -__builtin_inff() : (m + (__builtin_amdgcn_logf(l) - p_shift)) * KV_LN2;
 }
 
 // -------------------------------------------------------------- append
@@ -583,6 +701,97 @@ const char * plan_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     return nullptr;
 }
 
+// a query's own terms; nothing is asked of one without rows
+const char * check_query(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * q) {
+    if (!act_type(q->type)) return "need F32, F16 or BF16 queries";
+    if (q->window < 0 || !(q->scale == q->scale)) return "negative window or no scale";
+    const KvSeqs sq = seqs_of(b);
+    if (sq.n_seq == 0 || sq.n_tokens == 0 || sq.max_new == 0) return nullptr;
+    const int es = el_bytes(q->type), width = q->n_head * c->head_dim;
+    if (!q->q || !q->out) return "null q or out";
+    if (q->q == q->out) return "out may not be q: its rows are read by several workgroups";
+    if (!aligned16(q->q) || !aligned16(q->out) || (q->q_stride * es) % 16 || (q->out_stride * es) % 16)
+        return "q and out must be 16-byte aligned, rows too";
+    if (sq.n_tokens > 1 && (q->q_stride < width || q->out_stride < width)) return "rows shorter than n_head * head_dim";
+    return nullptr;
+}
+
+KvAttn attn_of(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * q, const AttnPlan & a, void * workspace) {
+    KvAttn p{};
+    p.b = seqs_of(b);
+    p.k = (const uint8_t *)c->k;
+    p.v = (const uint8_t *)c->v;
+    p.k_stride = c->k_stride;
+    p.v_stride = c->v_stride;
+    p.n_pages = c->n_pages;
+    p.page_shift = log2_of(c->page_size);
+    p.n_kv = c->n_kv;
+    p.group = q->n_head / c->n_kv;
+    p.window = std::min(q->window, 0x7FFFFF00);            // leaves room for sums with it
+    p.unit = kv_unit(c->head_dim);
+    p.scale = q->scale;
+    p.type = p.out_type = q->type;
+    p.q = q->q;
+    p.q_stride = q->q_stride;
+    p.out = q->out;
+    p.out_stride = q->out_stride;
+    p.lse = q->lse;
+    uint8_t * ws = (uint8_t *)workspace;
+    p.base = (int32_t *)ws;
+    p.ml = (float *)(ws + a.base_bytes);
+    p.acc = (float *)(ws + a.base_bytes + a.ml_bytes);
+    p.nt = a.nt;
+    p.runs = a.runs;
+    p.tiles = a.tiles;
+    return p;
+}
+
+hipError_t launch_attn(const llapis_kv_cache * c, const KvAttn & p, hipStream_t s) {
+    if (c->type == T_F16) return launch_kv_attn_f16(p, c->head_dim, s);
+    if (c->type == T_BF16) return launch_kv_attn_bf16(p, c->head_dim, s);
+    return launch_kv_attn_q8(p, c->head_dim, s);
+}
+
+constexpr int KVP_RUNS = 256;                            // a workgroup a CU
+
+// a prefix call's workspace: places of its parts, behind attention's own
+struct PrefixPlan {
+    int rows, slots;
+    int64_t max_steps;
+    uint64_t lens, table, seq_group, plan, total, out, lse, ml, acc, bytes;
+};
+
+const char * plan_prefix(const llapis_kv_cache * c, const llapis_kv_batch * b, int n_head, int n_group, bool wide, int attn_tiles,
+                         uint64_t own, PrefixPlan & f) {
+    const int hd = c->head_dim, half = c->type != T_BF16, group = n_head / c->n_kv;
+    f.rows = kvp_rows(half, wide, hd);
+    const int64_t tokens = b->n_tokens, tiles = (tokens * group + f.rows - 1) / f.rows + n_group;
+    const int64_t units = (int64_t)b->max_pages * c->page_size / kvp_unit(hd);
+    f.max_steps = tiles * c->n_kv * (2 * units + 1);
+    if (tokens > 1 << 24 || f.max_steps >= (int64_t)1 << 31) return "the groups' prefixes have 2^30 units of work or more";
+    // the join has a workgroup for each (sequence, kv head, tile)
+    if ((int64_t)b->n_seq * c->n_kv * attn_tiles >= KV_MAX_GRID) return "2^24 or more (sequence, kv head, 32 query rows)";
+    f.slots = (int)(tiles * c->n_kv + KVP_RUNS);
+    uint64_t at = own;
+    auto part = [&](uint64_t & place, uint64_t bytes) {
+        at = (at + 255) / 256 * 256;
+        place = at;
+        at += bytes;
+    };
+    const uint64_t n_seq = b->n_seq, width = (uint64_t)n_head * hd;
+    part(f.lens, n_seq * 4);
+    part(f.table, n_seq * b->max_pages * 4);
+    part(f.seq_group, n_seq * 4);
+    part(f.plan, KVP_GROUPS * sizeof(KvGroup));
+    part(f.total, 4);
+    part(f.out, (uint64_t)b->n_tokens * width * 4);
+    part(f.lse, (uint64_t)b->n_tokens * n_head * 4);
+    part(f.ml, (uint64_t)f.slots * f.rows * 8);
+    part(f.acc, (uint64_t)f.slots * f.rows * hd * 4);
+    f.bytes = at;
+    return nullptr;
+}
+
 // chunks of the longest plane's page; 0 where a plane is refused
 const char * check_planes(const llapis_kv_planes * p, int & chunks) {
     if (!p) return "null planes";
@@ -691,47 +900,13 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     AttnPlan a{};
     if (!bad) bad = q ? plan_attention(c, b, q->n_head, a) : "null query";
     if (bad) return refuse_as(who, bad);
-    if (!act_type(q->type)) return refuse_as(who, "need F32, F16 or BF16 queries");
-    if (q->window < 0 || !(q->scale == q->scale)) return refuse_as(who, "negative window or no scale");
+    if ((bad = check_query(c, b, q))) return refuse_as(who, bad);
     const KvSeqs sq = seqs_of(b);
     if (sq.n_seq == 0 || sq.n_tokens == 0 || sq.max_new == 0) return 0;
-    const int es = el_bytes(q->type), width = q->n_head * c->head_dim;
-    if (!q->q || !q->out) return refuse_as(who, "null q or out");
-    if (q->q == q->out) return refuse_as(who, "out may not be q: its rows are read by several workgroups");
-    if (!aligned16(q->q) || !aligned16(q->out) || (q->q_stride * es) % 16 || (q->out_stride * es) % 16)
-        return refuse_as(who, "q and out must be 16-byte aligned, rows too");
-    if (sq.n_tokens > 1 && (q->q_stride < width || q->out_stride < width)) return refuse_as(who, "rows shorter than n_head * head_dim");
     if (!workspace || !aligned16(workspace) || ws_bytes < a.bytes()) return refuse_as(who, "workspace too small or not 16-byte aligned");
-    KvAttn p{};
-    p.b = sq;
-    p.k = (const uint8_t *)c->k;
-    p.v = (const uint8_t *)c->v;
-    p.k_stride = c->k_stride;
-    p.v_stride = c->v_stride;
-    p.n_pages = c->n_pages;
-    p.page_shift = log2_of(c->page_size);
-    p.n_kv = c->n_kv;
-    p.group = q->n_head / c->n_kv;
-    p.window = std::min(q->window, 0x7FFFFF00);            // leaves room for sums with it
-    p.unit = kv_unit(c->head_dim);
-    p.scale = q->scale;
-    p.type = q->type;
-    p.q = q->q;
-    p.q_stride = q->q_stride;
-    p.out = q->out;
-    p.out_stride = q->out_stride;
-    p.lse = q->lse;
-    uint8_t * ws = (uint8_t *)workspace;
-    p.base = (int32_t *)ws;
-    p.ml = (float *)(ws + a.base_bytes);
-    p.acc = (float *)(ws + a.base_bytes + a.ml_bytes);
-    p.nt = a.nt;
-    p.runs = a.runs;
-    p.tiles = a.tiles;
+    const KvAttn p = attn_of(c, b, q, a, workspace);
     hipStream_t s = (hipStream_t)stream;
-    if (c->type == T_F16) KV_TRY(launch_kv_attn_f16(p, c->head_dim, s));
-    else if (c->type == T_BF16) KV_TRY(launch_kv_attn_bf16(p, c->head_dim, s));
-    else KV_TRY(launch_kv_attn_q8(p, c->head_dim, s));
+    KV_TRY(launch_attn(c, p, s));
     if (!needs_join(c, b)) return 0;                                   // every item is one unit
     // parts of an item, as many as the bounds suggest; workgroups by an item's rows
     const int64_t items = (int64_t)sq.n_seq * c->n_kv;
@@ -742,6 +917,94 @@ int32_t llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * b
     if (pg == 1) hipLaunchKernelGGL(k_kv_join<1>, grid, wg, 0, s, p, c->head_dim, shift);
     else if (pg == 4) hipLaunchKernelGGL(k_kv_join<4>, grid, wg, 0, s, p, c->head_dim, shift);
     else hipLaunchKernelGGL(k_kv_join<16>, grid, wg, 0, s, p, c->head_dim, shift);
+    KV_TRY(hipGetLastError());
+    return 0;
+}
+
+uint64_t llapis_kv_prefix_attention_workspace_size(const llapis_kv_cache * c, const llapis_kv_batch * b, int32_t n_head,
+                                                   int32_t n_group) {
+    const uint64_t own = llapis_kv_attention_workspace_size(c, b, n_head);
+    if (!own || n_group < 0 || n_group > KVP_GROUPS || b->n_tokens < 0) return 0;
+    AttnPlan a;
+    PrefixPlan wide, narrow;
+    plan_attention(c, b, n_head, a);
+    if (plan_prefix(c, b, n_head, n_group, true, a.tiles, own, wide) || plan_prefix(c, b, n_head, n_group, false, a.tiles, own, narrow)) return 0;
+    return std::max(wide.bytes, narrow.bytes);
+}
+
+int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * q,
+                                   const llapis_kv_prefix * x, void * workspace, uint64_t ws_bytes, void * stream) {
+    const char * who = "llapis_kv_prefix_attention";
+    const char * bad = check_cache(c);
+    if (!bad) bad = check_batch(b, c->page_size);
+    AttnPlan a{};
+    if (!bad) bad = q ? plan_attention(c, b, q->n_head, a) : "null query";
+    if (!bad && !x) bad = "null prefix";
+    if (!bad && (x->n_group < 0 || x->n_group > KVP_GROUPS)) bad = "need 0 <= n_group <= 256";
+    if (!bad && q->window != 0) bad = "a window is llapis_kv_attention's";
+    if (!bad) bad = check_query(c, b, q);
+    PrefixPlan f{};
+    if (!bad) bad = plan_prefix(c, b, q->n_head, x->n_group, q->type == T_F32, a.tiles, a.bytes(), f);
+    if (bad) return refuse_as(who, bad);
+    const KvSeqs sq = seqs_of(b);
+    if (sq.n_seq == 0 || sq.n_tokens == 0 || sq.max_new == 0) return 0;
+    if (x->n_group > 0 && (!x->groups || !x->prefix)) return refuse_as(who, "null groups or prefix");
+    if (!workspace || !aligned16(workspace) || ws_bytes < f.bytes) return refuse_as(who, "workspace too small or not 16-byte aligned");
+    if (x->n_group == 0) return llapis_kv_attention(c, b, q, workspace, ws_bytes, stream);
+    uint8_t * ws = (uint8_t *)workspace;
+    KvPrefix p{};
+    p.b = sq;
+    p.k = (const uint8_t *)c->k;
+    p.v = (const uint8_t *)c->v;
+    p.k_stride = c->k_stride;
+    p.v_stride = c->v_stride;
+    p.n_pages = c->n_pages;
+    p.page_shift = log2_of(c->page_size);
+    p.n_kv = c->n_kv;
+    p.group = q->n_head / c->n_kv;
+    p.scale = q->scale;
+    p.type = q->type;
+    p.q = q->q;
+    p.q_stride = q->q_stride;
+    p.groups = x->groups;
+    p.prefix = x->prefix;
+    p.n_group = x->n_group;
+    p.runs = KVP_RUNS;
+    p.slots = f.slots;
+    p.max_steps = f.max_steps;
+    p.lens = (int32_t *)(ws + f.lens);
+    p.table = (int32_t *)(ws + f.table);
+    p.seq_group = (int32_t *)(ws + f.seq_group);
+    p.plan = (KvGroup *)(ws + f.plan);
+    p.total = (int32_t *)(ws + f.total);
+    p.ml = (float *)(ws + f.ml);
+    p.acc = (float *)(ws + f.acc);
+    hipStream_t s = (hipStream_t)stream;
+    KV_TRY(c->type == T_F16 ? launch_kv_prefix_f16(p, c->head_dim, s)
+                            : c->type == T_BF16 ? launch_kv_prefix_bf16(p, c->head_dim, s) : launch_kv_prefix_q8(p, c->head_dim, s));
+    // the sequences' own keys, with results in fp32
+    llapis_kv_batch rest = *b;
+    rest.page_table = p.table;
+    rest.table_stride = b->max_pages;
+    rest.lens = p.lens;
+    llapis_kv_query to = *q;
+    to.out = ws + f.out;
+    to.out_stride = (int64_t)q->n_head * c->head_dim;
+    to.lse = (float *)(ws + f.lse);
+    KvAttn k = attn_of(c, &rest, &to, a, ws);
+    k.out_type = T_F32;
+    KV_TRY(launch_attn(c, k, s));
+    const KvResult o{q->out, q->out_stride, q->lse, q->type};
+    const int64_t items = (int64_t)sq.n_seq * c->n_kv;
+    const int tiles = (sq.n_tokens * p.group + f.rows - 1) / f.rows;
+    const int parts = KVP_RUNS / std::max((int)std::min<int64_t>((int64_t)c->n_kv * std::max(tiles, x->n_group), KVP_RUNS), 1) + 1;
+    const int pg = parts < 4 ? 1 : parts < 16 ? 4 : 16, per = 1024 / pg;
+    const int rows = std::min(p.group * sq.max_new, 16 * a.nt);
+    const dim3 grid((unsigned)(items * a.tiles), (rows * c->head_dim + per - 1) / per), wg(256);
+    const float shift = c->type == T_BF16 ? 0.0f : 15.0f;
+    if (pg == 1) hipLaunchKernelGGL(k_kv_prefix_join<1>, grid, wg, 0, s, k, p, o, c->head_dim, f.rows, shift);
+    else if (pg == 4) hipLaunchKernelGGL(k_kv_prefix_join<4>, grid, wg, 0, s, k, p, o, c->head_dim, f.rows, shift);
+    else hipLaunchKernelGGL(k_kv_prefix_join<16>, grid, wg, 0, s, k, p, o, c->head_dim, f.rows, shift);
     KV_TRY(hipGetLastError());
     return 0;
 }

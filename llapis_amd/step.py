@@ -210,6 +210,14 @@ class KvCache:
         most, itself the last; lse [rows, n_head] float32 receives the logarithm
         of the softmax sums.  Rows of no sequence are left as they are (in an
         out made here: as the allocation holds them)."""
+        a = self._query(batch, q, scale, window, out, lse)
+        if workspace is None:
+            workspace = self.attention_workspace(batch, a.n_head)
+        _call("llapis_kv_attention", self.device, self._ref, batch._ref, C.byref(a), *_scratch(workspace, self.device))
+        return a.result
+
+    def _query(self, batch, q, scale, window, out, lse):
+        """Attention's arguments, the output among them as `result`"""
         torch = _torch()
         _need(q.dim() == 3 and batch.device == self.device, "q must be [n_tokens, n_head, head_dim], the batch on its device")
         n_head = q.shape[1]
@@ -223,14 +231,36 @@ class KvCache:
             _need(lse.dtype == torch.float32 and lse.device == self.device and lse.is_contiguous() and len(shape) == 2
                   and shape[0] >= batch.n_tokens and shape[1] == n_head,
                   "lse must be a contiguous float32 [n_tokens, n_head]")
-        if workspace is None:
-            workspace = self.attention_workspace(batch, n_head)
         if window >> 31:
             _count(window)
         a = L.LlapisKvQuery(_tag(q.dtype), n_head, window, self.head_dim ** -0.5 if scale is None else scale,
                             q.data_ptr(), qs, out.data_ptr(), os_, _ptr(lse))
-        _call("llapis_kv_attention", self.device, self._ref, batch._ref, C.byref(a), *_scratch(workspace, self.device))
-        return out
+        a.result = out
+        return a
+
+    def prefix_workspace(self, batch, n_head, n_group):
+        """Scratch for prefix_attention calls of this geometry and of batches and groups within these bounds."""
+        n = int(lib().llapis_kv_prefix_attention_workspace_size(self._ref, batch._ref, n_head, n_group))
+        if n == 0:
+            raise ValueError("prefix_attention: unsupported geometry (n_head, max_new, groups or lengths)")
+        return _torch().empty(n, dtype=_torch().uint8, device=self.device)
+
+    def prefix_attention(self, batch, q, groups, prefix, scale=None, out=None, lse=None, workspace=None):
+        """attention without a window where sequences begin on the same pages (as
+        fork leaves them): sequences groups[g] .. groups[g + 1] - 1 share their first
+        prefix[g] tokens, which are read once for all of them.  groups int32
+        [n_group + 1] in order, prefix int32 [n_group], on the GPU; sequences in no group share nothing."""
+        torch = _torch()
+        n = prefix.shape[0] if prefix.dim() == 1 else -1
+        _is(prefix, torch.int32, (n,), self.device, "prefix")
+        _is(groups, torch.int32, (n + 1,), self.device, "groups")
+        a = self._query(batch, q, scale, 0, out, lse)
+        if workspace is None:
+            workspace = self.prefix_workspace(batch, a.n_head, n)
+        x = L.LlapisKvPrefix(n, groups.data_ptr(), prefix.data_ptr())
+        _call("llapis_kv_prefix_attention", self.device, self._ref, batch._ref, C.byref(a), C.byref(x),
+              *_scratch(workspace, self.device))
+        return a.result
 
 
 class KvPages:

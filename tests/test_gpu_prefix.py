@@ -1,0 +1,304 @@
+"""Attention of sequences that share a prefix (llapis_kv_prefix_attention) on the GPU against
+the plain 64-bit form of attention (step_ref.py), which reads every sequence's own row of the page table.
+
+The bound is step_ref.attention's.  What the prefix adds to its error: the weight of a
+sequence's own keys comes from the logarithm of their sum, rounded twice, 2^-23 |lse| of it, and |lse| is
+at most the largest score and the logarithm of their number: within the bound's 2^-22
+(|s| + |m|) and its 2^-21."""
+import math
+
+import pytest
+import torch
+
+import llapis_amd as la
+import step_ref as ref
+from test_gpu_step import i32, poisoned
+
+pytestmark = pytest.mark.gpu
+
+DT = ref.DT
+
+
+class Shared:
+    """Groups of sequences on the same first pages, every other place NaN.  groups: (shared
+    tokens, [(own tokens, new ones among them)]) each; a lone sequence is a group of nothing shared."""
+
+    def __init__(self, gpu, seed, tag, D, H, P, groups, io, before=0, spare=3):
+        g = torch.Generator().manual_seed(seed)
+        self.P, self.io = P, io
+        self.lens, self.new, first, rows = [], [], [before], []
+        need = sum(-(-n // P) + sum(-(-t // P) for t, _ in m) for n, m in groups) + before
+        n_pages = need + spare
+        order = torch.randperm(n_pages, generator=g).tolist()
+        for _ in range(before):
+            self.lens.append(P // 2)
+            self.new.append(1)
+            rows.append([order.pop()])
+        for n, members in groups:
+            assert n % P == 0
+            head = [order.pop() for _ in range(n // P)]
+            for t, k in members:
+                rows.append(head + [order.pop() for _ in range(-(-t // P))])
+                self.lens.append(n + t)
+                self.new.append(k)
+            first.append(first[-1] + len(members))
+        width = max(len(r) for r in rows) + 1
+        self.table = [r + [-1] * (width - len(r)) for r in rows]
+        self.cache = poisoned(la.KvCache.empty(n_pages, P, H, D, tag, gpu))
+        self.tb = i32(self.table, gpu)
+        kv = lambda n: [torch.randn(max(n, 1), H, D, generator=g).to(gpu) for _ in range(2)]
+        # whole sequences as prompts, one of each group first: the others' prefix is the same
+        lead = {}
+        for s, (n, i) in enumerate(zip(self.lens, range(len(self.lens)))):
+            g_i = next((j for j in range(len(groups)) if first[j] <= s < first[j + 1]), None)
+            skip = 0
+            if g_i is not None:
+                skip = groups[g_i][0] if g_i in lead else 0
+                if n >= groups[g_i][0]:
+                    lead.setdefault(g_i, s)
+            new = n - skip
+            if new > 0:
+                b = la.KvBatch(self.tb[s:s + 1], i32([n], gpu), i32([0, new], gpu), n_tokens=new, max_new=new)
+                self.cache.append(b, *kv(new))
+        self.start = [0]
+        for k in self.new:
+            self.start.append(self.start[-1] + k)
+        self.T = self.start[-1]
+        self.groups, self.prefix = i32(first, gpu), i32([n for n, _ in groups], gpu)
+        self.first, self.shared = first, [n for n, _ in groups]
+        self.batch = la.KvBatch(self.tb, i32(self.lens, gpu), i32(self.start, gpu), n_tokens=self.T, max_new=max(max(self.new), 1))
+
+    def queries(self, seed, n_head, factor=1.5):
+        g = torch.Generator().manual_seed(seed)
+        return (factor * torch.randn(max(self.T, 1), n_head, self.cache.head_dim, generator=g)).to(DT[self.io])
+
+    def check(self, q, scale=None, groups=None, prefix=None, table=None):
+        dev = self.cache.device
+        scale = self.cache.head_dim ** -0.5 if scale is None else scale
+        lse = torch.full(q.shape[:2], 7.0, device=dev)
+        out = torch.full((q.shape[0], q.shape[1] + 1, q.shape[2]), 5.0, dtype=q.dtype, device=dev)[:, :q.shape[1]]
+        self.cache.prefix_attention(self.batch, q.to(dev), self.groups if groups is None else groups,
+                                    self.prefix if prefix is None else prefix, scale=scale, out=out, lse=lse)
+        want, want_lse, tol = ref.attention(self.cache, self.table if table is None else table, self.lens, self.start, q, scale)
+        out, lse = out.cpu(), lse.cpu()
+        off = (out.double() - want).abs()
+        assert not torch.isnan(out[:self.T]).any()
+        assert (off <= tol)[:self.T].all(), f"off by {float((off / (tol + 1e-30))[:self.T].max()):.3g} of the bound"
+        empty = want_lse == -math.inf
+        assert (lse[empty] == -math.inf).all() and (out[empty] == 0).all()
+        near = (lse.double() - want_lse).abs()[~empty]
+        assert (near <= 2e-5 + 2 ** -22 * want_lse[~empty].abs()).all(), float(near.max())
+        return out
+
+
+SHAPES = [(64, 16), (96, 32), (128, 64), (192, 128), (256, 256), (512, 64)]
+
+
+@pytest.mark.parametrize("D,P", SHAPES)
+@pytest.mark.parametrize("io", [la.F32, la.F16, la.BF16])
+@pytest.mark.parametrize("tag", [la.F16, la.BF16, la.Q8_0])
+def test_types(gpu, tag, io, D, P):
+    """Every cache type, query type and head size: two groups, a sequence before them, several tokens."""
+    n = max(P, 64)
+    s = Shared(gpu, D, tag, D, 2, P, [(5 * n, [(3, 1), (70, 3), (1, 1), (P, 2)]), (2 * n, [(40, 1), (9, 4)])], io, before=1)
+    s.check(s.queries(D + 1, 6))
+
+
+@pytest.mark.parametrize("n_seq,group,H", [(1, 1, 1), (2, 1, 3), (5, 3, 2), (17, 4, 1), (40, 8, 2), (70, 5, 1)])
+@pytest.mark.parametrize("io,tag,D", [(la.F32, la.F16, 64), (la.BF16, la.BF16, 128), (la.F32, la.BF16, 128), (la.F16, la.Q8_0, 256)])
+def test_rows(gpu, n_seq, group, H, io, tag, D):
+    """Query rows from one to several tiles of a group, tiles of all, some and one of a workgroup's waves."""
+    s = Shared(gpu, n_seq, tag, D, H, 16, [(320, [(1 + (7 * i) % 50, 1 + (i % 2 if (7 * i) % 50 else 0)) for i in range(n_seq)])], io)
+    s.check(s.queries(4, group * H))
+
+
+@pytest.mark.parametrize("n", [64, 128, 192, 1024, 2048, 6400])
+def test_lengths(gpu, n):
+    """Prefixes of one unit and of many, in runs that end inside them."""
+    s = Shared(gpu, n, la.F16, 64, 1, 64, [(n, [(5, 1), (300, 2)]), (64, [(1, 1)])], la.F32)
+    s.check(s.queries(n, 3))
+
+
+@pytest.mark.parametrize("given", [-5, 0, 1, 63, 64, 100, 319, 320, 330, 10 ** 9])
+def test_cut(gpu, given):
+    """A prefix that is no multiple of a unit, none, or longer than what the sequences share or hold: it
+    is cut to what each had before its new tokens."""
+    s = Shared(gpu, 3, la.F16, 64, 2, 16, [(320, [(1, 1), (4, 4), (90, 1)])], la.F32)
+    q = s.queries(5, 4)
+    if given > 320:
+        # longer than the shared pages' tokens, but not than the shortest sequence's own before its new ones
+        assert min(n - k for n, k in zip(s.lens, s.new)) == 320
+    s.check(q, prefix=i32([given], gpu))
+
+
+def test_members(gpu):
+    """A group's first sequence ended, members without new tokens, a member shorter than the
+    prefix, groups of one and of none, sequences in no group."""
+    s = Shared(gpu, 6, la.BF16, 128, 2, 32, [(256, [(0, 0), (40, 0), (3, 1), (65, 2)]), (128, [(20, 1)]), (64, [])], la.BF16, before=2)
+    s.lens[2] = 0
+    s.batch.lens[2] = 0
+    s.tb[2] = 12345
+    s.table[2] = [12345] * len(s.table[2])
+    q = s.queries(7, 8)
+    s.check(q)
+    # a member with new tokens that has less than the others share: the prefix is cut for all
+    s.lens[4] = s.lens[4] - 200
+    s.batch.lens[4] = s.lens[4]
+    s.check(q)
+    s.lens[4] = 1
+    s.batch.lens[4] = 1
+    s.check(q)
+    s.lens[4] = 0                      # more new tokens than tokens
+    s.batch.lens[4] = 0
+    s.check(q)
+    # groups that leave all sequences out, and no groups at all
+    for groups, prefix in (([6, 6], [128]), ([0, 0], [128]), ([2], [])):
+        s.check(q, groups=i32(groups, gpu), prefix=i32(prefix, gpu))
+
+
+def test_holes(gpu):
+    """Entries without a page, in the prefix and behind it: their keys are masked."""
+    s = Shared(gpu, 8, la.F16, 64, 1, 16, [(256, [(30, 1), (50, 2)])], la.F32)
+    for i, pg in ((3, -1), (7, 10 ** 6), (8, -7)):
+        for r in range(2):
+            s.tb[r, i] = pg
+            s.table[r][i] = pg
+    s.tb[1, 17] = -1
+    s.table[1][17] = -1
+    q = s.queries(9, 2)
+    s.check(q)
+    for r in range(2):
+        s.tb[r, :16] = -1
+        s.table[r][:16] = [-1] * 16
+    s.check(q)
+    # nothing left to see
+    s.tb[:] = -1
+    s.table = [[-1] * len(r) for r in s.table]
+    assert (s.check(q) == 0).all()
+
+
+@pytest.mark.parametrize("tag,D", [(la.F16, 128), (la.BF16, 128), (la.Q8_0, 64), (la.F16, 512), (la.Q8_0, 512)])
+def test_hidden_non_finite(gpu, tag, D):
+    """A later draft's NaN key and value stay out of the rows that do not see it; one in the prefix is in every row."""
+    P, N = 16, 4
+    s = Shared(gpu, 10, tag, D, 1, P, [(128, [(20, N), (7, 1)])], la.F32)
+    q = s.queries(11, 2)
+    clean = s.check(q)
+
+    def poison(row, at):
+        pg, slot = s.table[row][at // P], at % P
+        for t in (s.cache.k, s.cache.v):
+            if tag == la.Q8_0:
+                t[pg].view(torch.float16)[P * D // 2:].view(D // 32, P)[:, slot] = float("nan")
+            elif t is s.cache.k:
+                t[pg, 0, slot] = float("nan")
+            else:
+                t[pg, 0, :, slot] = float("nan")
+
+    run = lambda: s.cache.prefix_attention(s.batch, q.to(gpu), s.groups, s.prefix).cpu()
+    poison(0, s.lens[0] - 2)
+    got = run()
+    assert torch.equal(got[[0, 1, 4]], clean[[0, 1, 4]]) and torch.isnan(got[2:4]).all()
+    poison(0, 70)
+    assert torch.isnan(run()).all()
+
+
+def test_scores(gpu):
+    """Scores all equal, far apart, of either sign of scale; the prefix far above the rest and far below it."""
+    s = Shared(gpu, 12, la.F16, 128, 1, 64, [(640, [(30, 1), (200, 2)])], la.F32)
+    q = s.queries(13, 4)
+    s.check(torch.zeros_like(q))
+    s.check(q * 300)
+    s.check(q, scale=-0.3)
+    s.check(q * 1e-6)
+    for size, where in ((40.0, slice(0, 10)), (0.0, slice(0, 10))):
+        held = s.cache.k.clone()
+        s.cache.k[torch.tensor(s.table[0][where])] *= size
+        s.check(q)
+        s.cache.k.copy_(held)
+
+
+@pytest.mark.parametrize("size", [1e-9, 3e4])
+def test_query_range(gpu, size):
+    s = Shared(gpu, 14, la.F16, 64, 1, 16, [(128, [(30, 1)])], la.F32)
+    s.check(s.queries(15, 2) * size, scale=0.125 / size)
+
+
+def test_many(gpu):
+    """As many groups as a call takes, and one more; hundreds of sequences of one group."""
+    s = Shared(gpu, 16, la.F16, 64, 1, 16, [(64, [(1 + i % 5, 1)]) for i in range(256)], la.F16)
+    s.check(s.queries(17, 1))
+    with pytest.raises(ValueError, match="prefix_attention"):
+        s.cache.prefix_attention(s.batch, s.queries(17, 1).to(gpu), torch.zeros(258, dtype=torch.int32, device=gpu),
+                                 torch.zeros(257, dtype=torch.int32, device=gpu))
+    s = Shared(gpu, 18, la.BF16, 64, 1, 16, [(192, [(1 + i % 7, 1) for i in range(600)])], la.BF16)
+    s.check(s.queries(19, 2))
+
+
+def test_one_row_each(gpu):
+    """A batch without row starts."""
+    s = Shared(gpu, 20, la.F16, 64, 2, 16, [(128, [(5, 1), (33, 1), (2, 1)])], la.F32)
+    q = s.queries(21, 4).to(gpu)
+    b = la.KvBatch(s.tb, s.batch.lens)
+    assert torch.equal(s.cache.prefix_attention(b, q, s.groups, s.prefix), s.cache.prefix_attention(s.batch, q, s.groups, s.prefix))
+
+
+def test_out_of_order(gpu):
+    """Groups and row starts that are in no order, or past the batch: results are not defined, memory is safe."""
+    s = Shared(gpu, 22, la.F16, 64, 1, 16, [(128, [(5, 1), (33, 2)]), (64, [(2, 1)])], la.F32)
+    q = s.queries(23, 4).to(gpu)
+    out = torch.full((s.T + 2, 4, 64), 5.0, device=gpu)
+    for groups in ([3, 0, 2], [0, 99, 3], [-7, 2, 1], [2 ** 31 - 1, -2 ** 31, 5]):
+        s.cache.prefix_attention(s.batch, q, i32(groups, gpu), s.prefix, out=out)
+    for start in ([4, 0, 2, 1], [0, 2 ** 31 - 1, -5, 3], [9, 9, 9, 9]):
+        b = la.KvBatch(s.tb, s.batch.lens, i32(start, gpu), n_tokens=s.T, max_new=2)
+        s.cache.prefix_attention(b, q, s.groups, s.prefix, out=out)
+    assert (out[s.T:] == 5).all()
+    s.check(q.cpu())
+
+
+def test_repeats_and_graphs(gpu):
+    """Two captured graphs with one workspace, replayed in turn as the lengths and the prefix
+    change, equal to eager calls bit for bit; a call on another stream."""
+    s = [Shared(gpu, 24 + i, la.BF16, 128, 2, 16, [(640 * (1 + i), [(90, 1), (200, 2), (5, 1)])], la.BF16) for i in range(2)]
+    qs = [x.queries(26, 8).to(gpu) for x in s]
+    ws = max((x.cache.prefix_workspace(x.batch, 8, 1) for x in s), key=lambda t: t.numel())
+    outs, graphs = [], []
+    for x, q in zip(s, qs):
+        out = x.cache.prefix_attention(x.batch, q, x.groups, x.prefix, workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            x.cache.prefix_attention(x.batch, q, x.groups, x.prefix, out=out, workspace=ws)
+        outs.append(out)
+        graphs.append(g)
+    for step in range(4):
+        for x, q, out, g in zip(s, qs, outs, graphs):
+            ws.random_(0, 255)
+            out.fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, x.cache.prefix_attention(x.batch, q, x.groups, x.prefix))
+            x.prefix.sub_(100)
+            x.batch.lens.sub_(torch.tensor([20, 3, 0], dtype=torch.int32, device=gpu))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = s[0].cache.prefix_attention(s[0].batch, qs[0], s[0].groups, s[0].prefix)
+    side.synchronize()
+    assert torch.equal(got, s[0].cache.prefix_attention(s[0].batch, qs[0], s[0].groups, s[0].prefix))
+
+
+def test_refusals(gpu):
+    s = Shared(gpu, 30, la.F16, 64, 2, 16, [(64, [(5, 1)])], la.F32)
+    q = s.queries(31, 4).to(gpu)
+    call = lambda **kw: s.cache.prefix_attention(**{**dict(batch=s.batch, q=q, groups=s.groups, prefix=s.prefix), **kw})
+    for bad, what in ((dict(groups=s.groups[:1]), "groups"), (dict(groups=s.groups.long()), "groups"), (dict(prefix=s.prefix.float()), "prefix"),
+                      (dict(prefix=s.prefix[0]), "prefix"), (dict(q=q[:, :3]), "unsupported"), (dict(q=q.double()), "float32"),
+                      (dict(lse=torch.zeros(1, 3, device=gpu)), "lse"), (dict(out=q.half()), "out"), (dict(groups=s.groups.cpu()), "groups")):
+        with pytest.raises(ValueError, match=what):
+            call(**bad)
+    with pytest.raises(la.LlapisError, match="workspace"):
+        call(workspace=torch.empty(64, dtype=torch.uint8, device=gpu))
+    with pytest.raises(la.LlapisError, match="out may not be q"):
+        call(out=q)

@@ -13,6 +13,7 @@ from test_step import P, refused
 STRUCTS = {
     "llapis_kv_extend_args": _lib.LlapisKvExtendArgs, "llapis_rope_rule": _lib.LlapisRopeRule,
     "llapis_qk_rope_args": _lib.LlapisQkRopeArgs, "llapis_sample_args": _lib.LlapisSampleArgs,
+    "llapis_kv_prefix": _lib.LlapisKvPrefix,
 }
 
 
@@ -212,3 +213,62 @@ def test_python_checks(monkeypatch):
         with pytest.raises(ValueError, match=what):
             step.sample(**{**dict(logits=x, u=u), **bad})
     assert called == ["llapis_kv_extend", "llapis_qk_rope", "llapis_sample"]
+
+
+# -------------------------------------------------- attention with a prefix
+
+def test_prefix_refusals():
+    from test_step import BAD_BATCH, BAD_CACHE, batch, cache, query
+    lib = la.lib()
+    prefix = lambda **kw: _lib.LlapisKvPrefix(**{**dict(n_group=1, groups=P, prefix=P), **kw})
+
+    def call(c=cache(), b=batch(), q=query(), x=prefix(), ws=P, n=1 << 40):
+        ref = lambda s: None if s is None else C.byref(s)
+        return lib.llapis_kv_prefix_attention(ref(c), ref(b), ref(q), ref(x), ws, n, None)
+
+    who = "llapis_kv_prefix_attention"
+    for bad in BAD_CACHE:
+        refused(call(c=cache(**bad)), who)
+    for bad in BAD_BATCH:
+        refused(call(b=batch(**bad)), who)
+    two = batch(n_seq=2, n_tokens=2)
+    for bad in (dict(type=la.Q8_0), dict(n_head=3), dict(n_head=0), dict(n_head=2048), dict(window=-1), dict(window=5), dict(scale=float("nan")),
+                dict(q=None), dict(out=None), dict(q=P + 4), dict(q_stride=258), dict(out_stride=250), dict(out=P)):
+        refused(call(b=two, q=query(**bad)), who)
+    for bad in (dict(n_group=-1), dict(n_group=257), dict(groups=None), dict(prefix=None)):
+        refused(call(x=prefix(**bad)), who)
+    for bad in (dict(c=None), dict(b=None), dict(q=None), dict(x=None)):
+        refused(call(**bad), "null")
+    refused(call(b=batch(new_start=P, max_new=17, n_tokens=17)), "16 new tokens")
+    need = lib.llapis_kv_prefix_attention_workspace_size(C.byref(cache()), C.byref(batch()), 4, 1)
+    assert need > lib.llapis_kv_attention_workspace_size(C.byref(cache()), C.byref(batch()), 4)
+    refused(call(n=64), "workspace")
+    refused(call(ws=P + 8), "workspace")
+    refused(call(ws=None), "workspace")
+    # nothing to do is no error
+    for nothing in (dict(n_seq=0, page_table=None, lens=None), dict(n_tokens=0)):
+        assert call(b=batch(**nothing), ws=None, n=0) == 0
+    size = lambda c=cache(), b=batch(), h=4, g=1: lib.llapis_kv_prefix_attention_workspace_size(C.byref(c), C.byref(b), h, g)
+    assert size(h=3) == size(g=257) == size(g=-1) == size(b=batch(new_start=P, max_new=17)) == 0
+    # more units than 32 bits count: 1024 heads, 2^22 pages of 256 keys
+    big = cache(n_kv=1024, head_dim=512, page_size=256, k_stride=1 << 28, v_stride=1 << 28)
+    b = batch(max_pages=1 << 22, table_stride=1 << 22)
+    assert size(big, b, 1024) == 0
+    refused(call(c=big, b=b, q=query(n_head=1024, q_stride=1 << 19, out_stride=1 << 19)), who)
+
+
+@pytest.mark.parametrize("kind", [la.F16, la.BF16])
+@pytest.mark.parametrize("head_dim", [64, 128, 512])
+def test_prefix_workspace_serves_less(head_dim, kind):
+    from test_step import batch, cache
+    lib, c = la.lib(), cache(type=kind, n_kv=2, head_dim=head_dim, page_size=64, k_stride=1 << 20, v_stride=1 << 20)
+
+    def size(n_seq, new, pages, groups, tokens=None):
+        b = batch(n_seq=n_seq, n_tokens=n_seq * new if tokens is None else tokens, max_new=new, max_pages=pages, table_stride=pages, new_start=P)
+        return lib.llapis_kv_prefix_attention_workspace_size(C.byref(c), C.byref(b), 16, groups)
+
+    for n_seq, new, pages, groups in ((1, 16, 3, 1), (64, 16, 512, 7), (300, 9, 100, 256)):
+        most = size(n_seq, new, pages, groups)
+        for less in ((n_seq, new - 1, pages, groups), (max(n_seq - 1, 1), new, pages, groups), (n_seq, new, pages - 1, groups), (n_seq, new, pages, groups - 1),
+                     (n_seq, new, pages, groups, 1), (1, 1, 1, 0)):
+            assert 0 < size(*less) <= most, less
