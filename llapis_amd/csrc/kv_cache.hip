@@ -761,12 +761,12 @@ struct PrefixPlan {
     uint64_t lens, table, seq_group, plan, total, out, lse, ml, acc, bytes;
 };
 
-const char * plan_prefix(const llapis_kv_cache * c, const llapis_kv_batch * b, int n_head, int n_group, bool wide, int attn_tiles,
+const char * plan_prefix(const llapis_kv_cache * c, const llapis_kv_batch * b, int n_head, int n_group, int wave_tiles, int attn_tiles,
                          uint64_t own, PrefixPlan & f) {
-    const int hd = c->head_dim, half = c->type != T_BF16, group = n_head / c->n_kv;
-    f.rows = kvp_rows(half, wide, hd);
+    const int hd = c->head_dim, group = n_head / c->n_kv;
+    f.rows = 16 * wave_tiles * kvp_waves(hd);
     const int64_t tokens = b->n_tokens, tiles = (tokens * group + f.rows - 1) / f.rows + n_group;
-    const int64_t units = (int64_t)b->max_pages * c->page_size / kvp_unit(hd);
+    const int64_t units = (int64_t)b->max_pages * c->page_size / kvp_unit(c->type == LLAPIS_T_Q8_0, hd);
     f.max_steps = tiles * c->n_kv * (2 * units + 1);
     if (tokens > 1 << 24 || f.max_steps >= (int64_t)1 << 31) return "the groups' prefixes have 2^30 units of work or more";
     // the join has a workgroup for each (sequence, kv head, tile)
@@ -926,10 +926,10 @@ uint64_t llapis_kv_prefix_attention_workspace_size(const llapis_kv_cache * c, co
     const uint64_t own = llapis_kv_attention_workspace_size(c, b, n_head);
     if (!own || n_group < 0 || n_group > KVP_GROUPS || b->n_tokens < 0) return 0;
     AttnPlan a;
-    PrefixPlan wide, narrow;
+    PrefixPlan one, two;
     plan_attention(c, b, n_head, a);
-    if (plan_prefix(c, b, n_head, n_group, true, a.tiles, own, wide) || plan_prefix(c, b, n_head, n_group, false, a.tiles, own, narrow)) return 0;
-    return std::max(wide.bytes, narrow.bytes);
+    if (plan_prefix(c, b, n_head, n_group, 1, a.tiles, own, one) || plan_prefix(c, b, n_head, n_group, 2, a.tiles, own, two)) return 0;
+    return std::max(one.bytes, two.bytes);
 }
 
 int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapis_kv_query * q,
@@ -944,7 +944,9 @@ int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_ba
     if (!bad && q->window != 0) bad = "a window is llapis_kv_attention's";
     if (!bad) bad = check_query(c, b, q);
     PrefixPlan f{};
-    if (!bad) bad = plan_prefix(c, b, q->n_head, x->n_group, q->type == T_F32, a.tiles, a.bytes(), f);
+    // (how many rows a group has is the device's to know: the mean)
+    const int tiles = bad ? 1 : kvp_tiles(c->type != T_BF16, q->type, c->head_dim, (int64_t)b->n_tokens * (q->n_head / c->n_kv) / std::max(x->n_group, 1));
+    if (!bad) bad = plan_prefix(c, b, q->n_head, x->n_group, tiles, a.tiles, a.bytes(), f);
     if (bad) return refuse_as(who, bad);
     const KvSeqs sq = seqs_of(b);
     if (sq.n_seq == 0 || sq.n_tokens == 0 || sq.max_new == 0) return 0;
@@ -969,6 +971,7 @@ int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_ba
     p.groups = x->groups;
     p.prefix = x->prefix;
     p.n_group = x->n_group;
+    p.tiles = tiles;
     p.runs = KVP_RUNS;
     p.slots = f.slots;
     p.max_steps = f.max_steps;
@@ -996,10 +999,12 @@ int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_ba
     KV_TRY(launch_attn(c, k, s));
     const KvResult o{q->out, q->out_stride, q->lse, q->type};
     const int64_t items = (int64_t)sq.n_seq * c->n_kv;
-    const int tiles = (sq.n_tokens * p.group + f.rows - 1) / f.rows;
-    const int parts = KVP_RUNS / std::max((int)std::min<int64_t>((int64_t)c->n_kv * std::max(tiles, x->n_group), KVP_RUNS), 1) + 1;
-    const int pg = parts < 4 ? 1 : parts < 16 ? 4 : 16, per = 1024 / pg;
+    const int64_t tall = ((int64_t)sq.n_tokens * p.group + f.rows - 1) / f.rows;
+    const int parts = KVP_RUNS / (int)std::min<int64_t>(c->n_kv * std::max<int64_t>(tall, x->n_group), KVP_RUNS) + 1;
+    // parts that one thread adds, fewer where there are threads enough without
     const int rows = std::min(p.group * sq.max_new, 16 * a.nt);
+    const int64_t quads = items * a.tiles * rows * c->head_dim / 4;
+    const int pg = parts < 4 || quads >= 1 << 18 ? 1 : parts < 16 || quads >= 1 << 15 ? 4 : 16, per = 1024 / pg;
     const dim3 grid((unsigned)(items * a.tiles), (rows * c->head_dim + per - 1) / per), wg(256);
     const float shift = c->type == T_BF16 ? 0.0f : 15.0f;
     if (pg == 1) hipLaunchKernelGGL(k_kv_prefix_join<1>, grid, wg, 0, s, k, p, o, c->head_dim, f.rows, shift);

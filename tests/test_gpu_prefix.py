@@ -167,6 +167,8 @@ def test_holes(gpu):
     s.table[1][17] = -1
     q = s.queries(9, 2)
     s.check(q)
+    s.check(q, scale=0.0)
+    s.check(q, scale=-1e-38)
     for r in range(2):
         s.tb[r, :16] = -1
         s.table[r][:16] = [-1] * 16
