@@ -179,6 +179,9 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     const int page = 1 << p.page_shift, page_mask = page - 1, cap = p.b.max_pages << p.page_shift;
 
     // ---- the groups: their first sequence with new tokens, and what all of those have before them
+    // (a thread's first sequence is read beside the groups)
+    const SeqRows ahead_rows = tid < p.b.n_seq ? seq_rows(p.b, tid) : SeqRows{0, 0, 0};
+    const int wanted = tid < p.n_group ? p.prefix[tid] : 0;
     for (int g = tid; g <= p.n_group; g += WGT) {
         s_first[g] = min(max(p.groups[g], 0), p.b.n_seq);
         if (g < p.n_group) {
@@ -193,7 +196,7 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
         return s < s_first[g + 1] ? g : -1;
     };
     for (int s = tid; s < p.b.n_seq; s += WGT) {
-        const SeqRows r = seq_rows(p.b, s);
+        const SeqRows r = s == tid ? ahead_rows : seq_rows(p.b, s);
         const int g = r.n > 0 ? group_of(s) : -1;
         if (g >= 0) {
             atomicMin(&s_eff[g], max(r.len - r.n, 0));
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     if (tid < p.n_group && s_lead[tid] != 0x7FFFFFFF) {
         const int align = max(page, 64);
         mine.lead = s_lead[tid];
-        mine.eff = min(min(max(p.prefix[tid], 0), s_eff[tid]), cap) & ~(align - 1);
+        mine.eff = min(min(max(wanted, 0), s_eff[tid]), cap) & ~(align - 1);
         mine.units = mine.eff / UNIT;
         const int end = p.b.start ? p.b.start[s_first[tid + 1]] : s_first[tid + 1];
         mine.row0 = min(max(p.b.start ? p.b.start[s_first[tid]] : s_first[tid], 0), p.b.n_tokens);
@@ -226,23 +229,28 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     // (row starts that are not in order may give groups more rows than there are: no prefix then)
     const int n_steps = same(n_steps_all <= p.max_steps ? (int)n_steps_all : 0), n_runs = runs_of(p.runs, n_steps);
     if (blockIdx.x == 0 && tid == 0) p.total[0] = n_steps;
-    // ---- the sequences without their prefix, a wave each
-    for (int s = blockIdx.x * WAVES + wave; s < p.b.n_seq; s += gridDim.x * WAVES) {
-        const int g = same(group_of(s)), eff = g >= 0 ? same(s_plan[g].eff) : 0, len = min(max(p.b.lens[s], 0), 0x7FFFFFFF);
-        const int32_t * from = p.b.table + s * p.b.table_stride;
-        const int skip = eff >> p.page_shift;
-        if (lane == 0) {
-            p.lens[s] = len - min(eff, len);
-            p.seq_group[s] = eff > 0 ? g : -1;
+    // ---- the sequences without their prefix, a wave each; last, when their loads hold up nothing
+    auto write_rest = [&]() {
+        for (int s = blockIdx.x * WAVES + wave; s < p.b.n_seq; s += gridDim.x * WAVES) {
+            const int g = same(group_of(s)), eff = g >= 0 ? same(s_plan[g].eff) : 0, len = min(max(p.b.lens[s], 0), 0x7FFFFFFF);
+            const int32_t * from = p.b.table + s * p.b.table_stride;
+            const int skip = eff >> p.page_shift;
+            if (lane == 0) {
+                p.lens[s] = len - min(eff, len);
+                p.seq_group[s] = eff > 0 ? g : -1;
+            }
+            // entries to the end of the last unit, which its loads ask for
+            const int n = (min(len, cap) - min(eff, len) + kv_unit(HD)) / page + 1;
+            for (int i = lane; i < min(n, p.b.max_pages); i += 64)
+                p.table[(int64_t)s * p.b.max_pages + i] = i + skip < p.b.max_pages ? from[i + skip] : -1;
         }
-        // entries to the end of the last unit, which its loads ask for
-        const int n = (min(len, cap) - min(eff, len) + kv_unit(HD)) / page + 1;
-        for (int i = lane; i < min(n, p.b.max_pages); i += 64)
-            p.table[(int64_t)s * p.b.max_pages + i] = i + skip < p.b.max_pages ? from[i + skip] : -1;
-    }
+    };
     // consecutive runs on one XCD: they read the same head's keys, for the next rows or further on
     const int run = (blockIdx.x & 7) * (p.runs >> 3) + (blockIdx.x >> 3);
-    if (run >= n_runs) return;
+    if (run >= n_runs) {
+        write_rest();
+        return;
+    }
     const Runs runs(n_steps, n_runs);
     const int lo = same(runs.begin(run)), hi = same(runs.begin(run + 1));
 
@@ -600,8 +608,13 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     int step = lo, unit = 0, i = 0;
     bool busy = false;                                    // the wave has rows
     bool more = next_piece(step, cur);
-    if (!more) return;
+    if (!more) {
+        write_rest();
+        return;
+    }
     ask();
+    load_q(cur, rows_of(cur));                            // (its loads beside the pages')
+    busy = same(16 * wave < rows_of(cur));
     take_pages();
     load_next_k();
     ask();
@@ -614,8 +627,8 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     for (;; ++unit) {
         if (TWO) __builtin_amdgcn_s_setprio(1);
         if (unit > 0 && busy) products(lds_v + ((unit - 1) % BUFS) * PARTS * VB);
-        if (i == 0) {
-            if (unit > 0) write(past);
+        if (i == 0 && unit > 0) {
+            write(past);
             const int n_rows = rows_of(cur);
             load_q(cur, n_rows);
             busy = same(16 * wave < n_rows);
@@ -651,6 +664,7 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     }
     if (busy) products(lds_v + (unit % BUFS) * PARTS * VB);
     write(past);
+    write_rest();
     if (TWO && !second) barrier();                        // the other waves' last one
 }
 
