@@ -2,61 +2,63 @@
 //
 // With M the largest logit a value's weight is w = e^((x - M) / T), and every
 // filter keeps an upper part of the values in the order (value descending, index
-// ascending).  Three kernels find where that part ends and draw from it, without
+// ascending).  Four kernels find where that part ends and draw from it, without
 // sorting the row:
-//   k_sample_scan   a chunk's largest value, and where a top_k or top_p is to be found
-//                   a histogram of its values over SMP_BINS bins, 16 to a factor of 2
-//                   of the weight: their numbers and (roughly) their weights
-//   k_sample_cut    every workgroup adds the chunks' histograms, finds the few bins in
-//                   which top_k and top_p may end, and sorts its values into those
-//                   that are surely kept (summed), those that only count towards
-//                   top_k's weight (summed), and the candidates of those bins (listed)
-//   k_sample_pick   a workgroup a sequence orders the candidates, ends both filters
-//                   among them exactly, and finds the token: its segment of 2048
-//                   values by the segments' sums, then the value
-// and k_sample_probs writes probabilities if they are wanted.  The histogram's weights
-// are fp32 in fixed point: they only bound which bins are looked at, with a margin far
-// above their error.  What decides is fp64: weights, their sums and products, in a
-// fixed order, so that a draw next to a border falls as the definition says.
+//   k_sample_scan   a workgroup's values: the largest, and where a top_k or top_p is to be
+//                   found a histogram over SMP_BINS bins, 16 to a factor of 2 of the weight
+//   k_sample_find   a workgroup a sequence adds the histograms and finds the few bins in
+//                   which top_k and top_p may end, and the values that these begin with
+//   k_sample_split  a workgroup's values again: those above are surely kept (summed), those
+//                   between only count towards top_p's whole (summed), the candidates are listed
+//   k_sample_pick   a workgroup a sequence ends both filters among the candidates exactly
+//                   and finds the token: its segment by the segments' sums, then the value
+// and k_sample_probs writes probabilities if they are wanted.  A histogram's word holds a
+// bin's number of values and the sum of their places in it, in 32nds: a weight is 2^(place / 16)
+// times the bin's, so that both bound the bin's weight to 0.3 %.  They only say which
+// bins are looked at.  What decides is fp64 (and fixed point of 49 bits, where sums are
+// made by atomics): weights, their sums and products, in a fixed order, so that a draw next to a
+// border falls as the definition says.
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "kv.h"
 
 namespace llapis {
 namespace dev {
 
-constexpr int SMP_WG = 1024, SMP_WAVES = SMP_WG / 64;
-constexpr int SMP_LANE = 32;                              // values of a lane
-constexpr int SMP_SEG = 64 * SMP_LANE;                    // ... of a wave: a segment
-constexpr int SMP_CHUNK = SMP_WAVES * SMP_SEG;            // ... of a workgroup
-constexpr int SMP_BINS = 1024, SMP_OUT = SMP_BINS + 1;     // a value below all bins is in SMP_OUT
-constexpr double SMP_PER_OCTAVE = 16.0;
-constexpr int SMP_SORT = 4096;                            // candidates that are sorted in LDS
-// a histogram's word: the number of values (a chunk's at most) above 48 bits of their
-// weights' sum, 32 of them its fraction, each weight rounded down
-constexpr int SMP_COUNT_AT = 48;
-constexpr float SMP_ONE = 4294967296.0f;
-constexpr double SMP_LEAST = 1.0 / (1ull << 32);
-constexpr double SMP_MARGIN = 1.0 / 4096;                 // of a weight, whose error in fp32 is below 2^-16
+constexpr int SMP_WG = 256, SMP_WAVES = SMP_WG / 64;      // of the kernels that read rows
+constexpr int SMP_SEQ_WG = 1024, SMP_SEQ_WAVES = SMP_SEQ_WG / 64;     // of those with a workgroup a sequence
+// Values of a lane: 32, and 8 where rows are few and short, which then go to four times the
+// workgroups.  A wave's values are a segment, a workgroup's a chunk
+constexpr int smp_seg(int lane_values) { return 64 * lane_values; }
+constexpr int smp_chunk(int lane_values) { return SMP_WG * lane_values; }
+constexpr int SMP_BINS = 1024, SMP_OUT = SMP_BINS + 1;    // a value below all bins is in SMP_OUT
+constexpr float SMP_PER_OCTAVE = 16.0f;
+constexpr int SMP_FEW = 4096, SMP_HELD = 1024;            // candidates, and segments, that are held at once
+constexpr int SMP_LIST = 512;                             // candidates of a bucket that are ordered one by one
+// a histogram's word: the number of values above 18 bits of the sum of their places
+constexpr int SMP_COUNT_AT = 18;
+static_assert(smp_chunk(32) * 31 < 1 << SMP_COUNT_AT && smp_chunk(32) >> (32 - SMP_COUNT_AT) == 0, "a chunk's values fit in a word");
 
 struct SmpChunk { float top; int32_t at; };               // a chunk's largest value and its lowest index
 struct SmpSeg { double sure, draw, mid; int32_t n_sure, n_mid, n_cand, pad; };
-// a sequence's cut; bins are counted from the largest value's
+// A sequence's cut.  In the order of values: from x_sure on surely kept, from x_cand on
+// candidates, from x_mid on not kept by top_p, from x_end on candidates again (top_k's end); the rest is out
 struct SmpCut {
     float top;                     // M
-    int32_t lo, hi, last;          // candidates: bins lo .. hi and `last`, top_k's (SMP_BINS without one); those before lo are sure
+    float x_sure, x_cand, x_mid, x_end;
+    int32_t token;                 // the first value's index, -1 without one
     uint64_t key;                  // the last candidate that is kept, ~0 without one
-    double total;                  // the kept weights' sum; 0: nothing to draw from
-    int32_t token, pad;
+    double total;                  // the kept weights' sum
 };
 
 struct SmpWs {
+    SmpCut * cuts;                 // [n_seq]
     SmpChunk * chunks;             // [n_seq][n_chunks]
     SmpSeg * segs;                 // [n_seq][n_chunks * SMP_WAVES]
-    SmpCut * cuts;                 // [n_seq]
-    uint64_t * hist;               // [n_seq][n_chunks][SMP_BINS]
-    uint64_t * keys;               // [n_seq][n_chunks * SMP_CHUNK] candidates, by segment
+    uint32_t * hist;               // [n_seq][n_chunks][SMP_BINS]
+    uint64_t * keys;               // [n_seq][n_chunks * chunk] candidates, by segment
     int n_chunks;
 };
 
@@ -64,8 +66,9 @@ struct SmpWs {
 struct SmpSet {
     bool greedy, by_k, by_p;       // the largest value alone; a number of values; a part of their weight
     int k;
-    double inv_t, p, min_p;
-    double per_bin;                // bins a unit of x
+    double p, min_p;
+    double octaves;                // log2 of the weight a unit of x
+    float bins;                    // bins a unit of x; 0: one bin for all values
 };
 
 __device__ __forceinline__ SmpSet smp_settings(const llapis_sample_args & a, int seq) {
@@ -78,8 +81,9 @@ __device__ __forceinline__ SmpSet smp_settings(const llapis_sample_args & a, int
     s.greedy = !(t > 0.0f) || s.k == 1 || p <= 0.0f || m > 1.0f;
     s.p = (double)p;
     s.min_p = m > 0.0f ? (double)m : 0.0;
-    s.inv_t = 1.0 / (double)t;
-    s.per_bin = s.inv_t * (1.44269504088896340736 * SMP_PER_OCTAVE);
+    s.octaves = 1.44269504088896340736 / (double)t;
+    s.bins = (float)s.octaves * SMP_PER_OCTAVE;
+    if (!(s.bins < 0x1p60f)) s.bins = 0.0f;
     return s;
 }
 
@@ -96,13 +100,27 @@ __device__ __forceinline__ int smp_index(uint64_t key) { return (int)~(uint32_t)
 
 constexpr float SMP_NONE = -__builtin_inff();             // no value: it has no weight
 
-__device__ __forceinline__ double smp_weight(float x, float top, double inv_t) {
-    // (the difference with an infinite M, or times an infinite 1 / T, says nothing)
-    return x == top ? 1.0 : x == SMP_NONE || top == __builtin_inff() ? 0.0 : exp(((double)x - (double)top) * inv_t);
+// 2^t for t <= 0: the whole part in the exponent, the rest r by sum (r ln 2)^k / k! to k = 11, whose
+// remainder is 2^-47 of it at r = 1/2.  (The library's exp took half as long again.)
+__device__ __forceinline__ double smp_exp2(double t) {
+    constexpr double c[12] = {1.0, 0.69314718055994530942, 0.24022650695910071233, 0.055504108664821579953,
+                              0.0096181291076284771619, 0.0013333558146428443423, 1.5403530393381609954e-4,
+                              1.5252733804059840280e-5, 1.3215486790144309488e-6, 1.0178086009239699728e-7,
+                              7.0549116208011233299e-9, 4.4455382718708114976e-10};
+    const double n = rint(fmax(t, -2000.0)), r = t - n;
+    double y = c[11];
+#pragma unroll
+    for (int k = 10; k >= 0; --k) y = __builtin_fma(y, r, c[k]);
+    return t > -1100.0 ? __builtin_ldexp(y, (int)n) : 0.0;
 }
-// bins below the largest value's
-__device__ __forceinline__ int smp_bin(float x, float top, double per_bin) {
-    return x == top ? 0 : (int)fmin(floor((double)top * per_bin) - floor((double)x * per_bin), (double)SMP_OUT);
+__device__ __forceinline__ double smp_weight(float x, float top, double octaves) {
+    // (the difference with an infinite M, or times an infinite 1 / T, says nothing)
+    return x == top ? 1.0 : x == SMP_NONE || top == __builtin_inff() ? 0.0 : smp_exp2(((double)x - (double)top) * octaves);
+}
+// A value's bin below the largest's, the same wherever it is asked for, and never less for a
+// smaller value.  What lies below all bins, or too far for fp32, is in SMP_OUT
+__device__ __forceinline__ int smp_bin(float x, float top, float top_bin, float bins) {
+    return x == top ? 0 : (int)fminf(top_bin - floorf(x * bins), (float)SMP_OUT);
 }
 
 // a NaN counts as no value, -0 as 0
@@ -116,213 +134,295 @@ __device__ __forceinline__ int smp_at(int base, int j) {
     constexpr int W = 16 / sizeof(T);
     return base + (j / W * 64 + (threadIdx.x & 63)) * W + j % W;
 }
-template <class T>
-__device__ __forceinline__ void smp_read(const T * row, int base, int n, float (&x)[SMP_LANE]) {
+template <class T, int N>
+__device__ __forceinline__ void smp_read(const T * row, int base, int n, float (&x)[N]) {
     constexpr int W = 16 / sizeof(T);
-    if (base + SMP_SEG <= n) {
-        typename SmpVec<T>::v w[SMP_LANE / W];
+    if (base + smp_seg(N) <= n) {
+        typename SmpVec<T>::v w[N / W];
 #pragma unroll
-        for (int c = 0; c < SMP_LANE / W; ++c) w[c] = *(const typename SmpVec<T>::v *)(row + smp_at<T>(base, c * W));
+        for (int c = 0; c < N / W; ++c) w[c] = *(const typename SmpVec<T>::v *)(row + smp_at<T>(base, c * W));
 #pragma unroll
-        for (int j = 0; j < SMP_LANE; ++j) x[j] = smp_clean((float)w[j / W][j % W]);
+        for (int j = 0; j < N; ++j) x[j] = smp_clean((float)w[j / W][j % W]);
     } else {
 #pragma unroll
-        for (int j = 0; j < SMP_LANE; ++j) {
+        for (int j = 0; j < N; ++j) {
             const int i = smp_at<T>(base, j);
             x[j] = i < n ? smp_clean((float)row[i]) : SMP_NONE;
         }
     }
 }
 
-__device__ __forceinline__ uint64_t smp_max(uint64_t x) {
-    for (int o = 32; o; o >>= 1) {
-        const uint64_t y = __shfl_xor(x, o, 64);
-        x = y > x ? y : x;
+// ---- over a wave's lanes, by lane moves within rows of 16 and from row to row (a tenth of
+// the time of permutes through LDS).  What a lane has none of is 0
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t smp_move(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS, class V>
+__device__ __forceinline__ V smp_moved(V x) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, smp_move<CTRL, ROWS>(__builtin_bit_cast(uint32_t, x)));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        return __builtin_bit_cast(V, (uint64_t)smp_move<CTRL, ROWS>((uint32_t)(u >> 32)) << 32 | smp_move<CTRL, ROWS>((uint32_t)u));
     }
-    return x;
 }
-
-// the largest over a workgroup; s_part is read before the next barrier
-__device__ __forceinline__ uint64_t smp_max_wg(uint64_t x, uint64_t * s_part) {
-    x = smp_max(x);
-    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = 0;
-    for (int w = 0; w < SMP_WAVES; ++w) x = s_part[w] > x ? s_part[w] : x;
-    return x;
+// f over this lane and those before it in their row of 16
+template <class V, class F>
+__device__ __forceinline__ V smp_row(V x, F f) {
+    x = f(x, smp_moved<0x111, 0xF>(x));
+    x = f(x, smp_moved<0x112, 0xF>(x));
+    x = f(x, smp_moved<0x114, 0xF>(x));
+    return f(x, smp_moved<0x118, 0xF>(x));
 }
-
-// exclusive sums over the workgroup's threads in order, and the whole
+// ... and in the wave
+template <class V, class F>
+__device__ __forceinline__ V smp_wave(V x, F f) {
+    x = smp_row(x, f);
+    x = f(x, smp_moved<0x142, 0xA>(x));
+    return f(x, smp_moved<0x143, 0xC>(x));
+}
 template <class V>
-__device__ __forceinline__ V smp_scan(V x, V * s_part, V & total) {
+__device__ __forceinline__ V smp_lane(V x, int lane) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, x), lane));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        return __builtin_bit_cast(V, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), lane) << 32 |
+                                         (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, lane));
+    }
+}
+struct SmpAdd { template <class V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };
+struct SmpMax { template <class V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
+
+// ---- over a workgroup of WAVES <= 16 waves: a wave's last lane leaves its wave's, and
+// after a barrier every wave has those of all.  A `part` is used once between two barriers
+template <class V> __device__ __forceinline__ void smp_leave(V wave_value, V * part) {
+    if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = wave_value;
+}
+template <int WAVES, class V, class F>
+__device__ __forceinline__ V smp_all(const V * part, F f) {
+    const int lane = threadIdx.x & 63;
+    return smp_lane(smp_row(lane < WAVES ? part[lane] : V(0), f), WAVES - 1);
+}
+// what the waves before this one left, added
+template <int WAVES, class V>
+__device__ __forceinline__ V smp_before(const V * part, V & all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    V v = x;
-    for (int o = 1; o < 64; o <<= 1) {
-        const V y = __shfl_up(v, o, 64);
-        if (lane >= o) v += y;
-    }
-    __syncthreads();                                     // the last use of s_part is over
-    if (lane == 63) s_part[wave] = v;
+    const V x = smp_row(lane < WAVES ? part[lane] : V(0), SmpAdd());
+    all = smp_lane(x, WAVES - 1);
+    return wave ? smp_lane(x, __builtin_amdgcn_readfirstlane(wave - 1)) : V(0);
+}
+// exclusive sums over the threads in order, and the whole
+template <int WAVES, class V>
+__device__ __forceinline__ V smp_scan(V x, V * part, V & all) {
+    const V v = smp_wave(x, SmpAdd());
+    smp_leave(v, part);
     __syncthreads();
-    V before = 0;
-    total = 0;
-    for (int w = 0; w < SMP_WAVES; ++w) {
-        const V y = s_part[w];
-        if (w < wave) before += y;
-        total += y;
-    }
-    const V up = __shfl_up(v, 1, 64);
-    return before + (lane ? up : (V)0);
+    return smp_before<WAVES>(part, all) + smp_moved<0x138, 0xF>(v);
 }
 
-template <class T>
+// the first of the lowest wave's first lanes with `yes`, by a minimum in LDS that begins above
+__device__ __forceinline__ void smp_first(bool yes, int * at) {
+    const uint64_t votes = __ballot(yes);
+    if (votes && (threadIdx.x & 63) == 0) atomicMin(at, (int)threadIdx.x + (int)__builtin_ctzll(votes));
+}
+
+// ---------------------------------------------------------------- scan
+
+template <class T, int N>
 __global__ __launch_bounds__(SMP_WG) void k_sample_scan(const llapis_sample_args a, const SmpWs ws) {
-    __shared__ uint64_t s_hist[SMP_BINS];
+    __shared__ uint32_t s_hist[SMP_BINS];
     __shared__ uint64_t s_part[SMP_WAVES];
     const int seq = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
     const int64_t chunk = (int64_t)seq * ws.n_chunks + blockIdx.x;
-    const int base = blockIdx.x * SMP_CHUNK + wave * SMP_SEG;
-    float x[SMP_LANE];
+    const int base = blockIdx.x * smp_chunk(N) + wave * smp_seg(N);
+    float x[N];
     smp_read((const T *)a.logits + seq * a.logits_stride, base, a.vocab, x);
     const SmpSet s = smp_settings(a, seq);
-    s_hist[tid] = 0;
-    uint64_t best = 0;
 #pragma unroll
-    for (int j = 0; j < SMP_LANE; ++j) {
-        const uint64_t key = smp_key(x[j], smp_at<T>(base, j));
-        best = key > best ? key : best;
-    }
-    best = smp_max_wg(best, s_part);
+    for (int i = 0; i < SMP_BINS / SMP_WG; ++i) s_hist[i * SMP_WG + tid] = 0;
+    // the largest, then the lowest index that has it
+    float most = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) most = fmaxf(most, x[j]);
+    int where = 0;
+#pragma unroll
+    for (int j = N - 1; j >= 0; --j) where = x[j] == most ? j : where;
+    smp_leave(smp_wave(smp_key(most, smp_at<T>(base, where)), SmpMax()), s_part);
+    __syncthreads();
+    const uint64_t best = smp_all<SMP_WAVES>(s_part, SmpMax());
     const float top = smp_value(best);
     if (tid == 0) ws.chunks[chunk] = {top, smp_index(best)};
     if (s.greedy || !(s.by_k || s.by_p)) return;
-    const float per = (float)(s.inv_t * 1.44269504088896340736);
-    const double top_bin = floor((double)top * s.per_bin);
+    const float top_bin = floorf(top * s.bins);
 #pragma unroll
-    for (int j = 0; j < SMP_LANE; ++j) {
-        if (x[j] == SMP_NONE) continue;
-        const int b = x[j] == top ? 0 : (int)fmin(top_bin - floor((double)x[j] * s.per_bin), (double)SMP_OUT);
-        const float w = x[j] == top ? 1.0f : fmaxf(__builtin_amdgcn_exp2f((x[j] - top) * per), 0.0f);
-        if (b < SMP_BINS) atomicAdd((unsigned long long *)&s_hist[b], 1ull << SMP_COUNT_AT | (unsigned long long)(w * SMP_ONE));
+    for (int j = 0; j < N; ++j) {
+        const float at = x[j] * s.bins;
+        const int b = smp_bin(x[j], top, top_bin, s.bins);
+        // (the place says nothing for what is out of fp32's range, as its bin does)
+        const uint32_t place = min((uint32_t)((at - floorf(at)) * 32.0f), 31u);
+        if (x[j] != SMP_NONE && b < SMP_BINS) atomicAdd(&s_hist[b], 1u << SMP_COUNT_AT | place);
     }
     __syncthreads();
-    ws.hist[chunk * SMP_BINS + tid] = s_hist[tid];
+#pragma unroll
+    for (int i = 0; i < SMP_BINS / SMP_WG; ++i) ws.hist[chunk * SMP_BINS + i * SMP_WG + tid] = s_hist[i * SMP_WG + tid];
 }
 
-template <class T>
-__global__ __launch_bounds__(SMP_WG) void k_sample_cut(const llapis_sample_args a, const SmpWs ws) {
-    __shared__ uint64_t s_part[SMP_WAVES];
-    __shared__ double s_sum[SMP_WAVES];
-    __shared__ int s_count[SMP_WAVES], s_at[3];
-    __shared__ double s_mass[2];
-    const int seq = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+// ---------------------------------------------------------------- find
+
+__global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_args a, const SmpWs ws) {
+    __shared__ uint64_t s_best[SMP_SEQ_WAVES];
+    __shared__ int s_count[SMP_SEQ_WAVES], s_at[3];
+    __shared__ float s_low[SMP_SEQ_WAVES], s_high[SMP_SEQ_WAVES], s_mass[2];
+    const int seq = blockIdx.x, tid = threadIdx.x;
     const SmpSet s = smp_settings(a, seq);
     const SmpChunk * chunks = ws.chunks + (int64_t)seq * ws.n_chunks;
-    const int base = blockIdx.x * SMP_CHUNK + wave * SMP_SEG;
-    float x[SMP_LANE];
-    if (!s.greedy) smp_read((const T *)a.logits + seq * a.logits_stride, base, a.vocab, x);
     uint64_t best = 0;
-    for (int c = tid; c < ws.n_chunks; c += SMP_WG) {
+    for (int c = tid; c < ws.n_chunks; c += SMP_SEQ_WG) {
         const uint64_t key = smp_key(chunks[c].top, chunks[c].at);
         best = key > best ? key : best;
     }
-    best = smp_max_wg(best, s_part);
-    const float top = smp_value(best);
-    SmpCut cut = {top, SMP_OUT, SMP_OUT, SMP_OUT, ~0ull, 0.0, top == SMP_NONE ? -1 : smp_index(best), 0};
-    if (s.greedy || top == SMP_NONE) {
-        if (blockIdx.x == 0 && tid == 0) ws.cuts[seq] = cut;
+    smp_leave(smp_wave(best, SmpMax()), s_best);
+    if (tid == 0) s_at[0] = s_at[1] = s_at[2] = SMP_BINS - 1;
+    __syncthreads();
+    best = smp_all<SMP_SEQ_WAVES>(s_best, SmpMax());
+    const float top = smp_value(best), none = __builtin_nanf(""), least = -3.40282347e38f;
+    // without filters every value is surely kept
+    SmpCut cut = {top, least, none, none, none, top == SMP_NONE ? -1 : smp_index(best), ~0ull, 0.0};
+    if (s.greedy || top == SMP_NONE || !(s.by_k || s.by_p)) {
+        if (tid == 0) ws.cuts[seq] = cut;
         return;
     }
-    if (s.by_k || s.by_p) {
-        // ---- a thread's bin over all chunks
-        int count = 0;
-        double mass = 0.0;
-        const uint64_t * hist = ws.hist + (int64_t)seq * ws.n_chunks * SMP_BINS;
-        for (int c = 0; c < ws.n_chunks; ++c) {
-            const float its = chunks[c].top;
-            if (its == SMP_NONE) continue;
-            const int b = tid - smp_bin(its, top, s.per_bin);
-            if (b < 0) continue;
-            const uint64_t v = hist[(int64_t)c * SMP_BINS + b];
-            count += (int)(v >> SMP_COUNT_AT);
-            mass += (double)(v & ((1ull << SMP_COUNT_AT) - 1)) * SMP_LEAST * smp_weight(its, top, s.inv_t);
-        }
-        int n_all;
-        double all;
-        const int n_before = smp_scan(count, s_count, n_all);
-        const double before = smp_scan(mass, s_sum, all), upto = before + mass;
-        const int k = s.by_k ? min(s.k, n_all) : n_all;
-        if (tid == 0) s_at[0] = s_at[1] = s_at[2] = SMP_BINS - 1;
+    // ---- a thread's bin over all chunks
+    const float top_bin = floorf(top * s.bins);
+    int count = 0;
+    uint64_t places = 0;
+    const uint32_t * hist = ws.hist + (int64_t)seq * ws.n_chunks * SMP_BINS;
+#pragma unroll 8
+    for (int c = 0; c < ws.n_chunks; ++c) {
+        const float its = chunks[c].top;
+        const int b = tid - smp_bin(its, top, top_bin, s.bins);
+        const uint32_t v = its == SMP_NONE || b < 0 ? 0 : hist[(int64_t)c * SMP_BINS + b];
+        count += (int)(v >> SMP_COUNT_AT);
+        places += v & ((1u << SMP_COUNT_AT) - 1);
+    }
+    // the bin's weight: 2^((place - top's place) / 16) lies between 1 + 0.0433 place and 1 + 0.0443
+    // place times the bin's, a place between its 32nd and the next.  fp32 has each place to
+    // 2^-23 of its distance from 0
+    const float off = exp2f((fabsf(top * s.bins) + 2 * SMP_BINS) * 0x1p-22f / SMP_PER_OCTAVE) * (1.0f + 0x1p-14f);
+    const float unit = exp2f((top_bin - top * s.bins - (float)tid) / SMP_PER_OCTAVE);
+    const float low = unit * ((float)count + 0.0433f / 32 * (float)places);
+    const float high = unit * ((float)count + 0.0444f / 32 * ((float)places + (float)count));
+    const int count_w = smp_wave(count, SmpAdd());
+    const float low_w = smp_wave(low, SmpAdd()), high_w = smp_wave(high, SmpAdd());
+    smp_leave(count_w, s_count);
+    smp_leave(low_w, s_low);
+    smp_leave(high_w, s_high);
+    __syncthreads();
+    int n_all;
+    float all_low, all_high;
+    const int n_upto = smp_before<SMP_SEQ_WAVES>(s_count, n_all) + count_w, n_before = n_upto - count;
+    const float low_upto = smp_before<SMP_SEQ_WAVES>(s_low, all_low) + low_w;
+    const float high_upto = smp_before<SMP_SEQ_WAVES>(s_high, all_high) + high_w;
+    const int k = s.by_k ? min(s.k, n_all) : n_all;
+    if (n_before < k && k <= n_upto) {                     // one bin: top_k ends here
+        s_at[2] = tid;
+        s_mass[0] = s.by_k ? low_upto - low : all_low;
+        s_mass[1] = s.by_k ? high_upto : all_high;
+    }
+    __syncthreads();
+    const int last = s_at[2];
+    int lo = last, hi = last;
+    if (s.by_p) {
+        // the first bin in which the sum may, and in which it must have reached top_p's part
+        const float p = (float)s.p;
+        smp_first(high_upto * off * off >= p * s_mass[0] * (1.0f - 0x1p-14f), &s_at[0]);
+        smp_first(low_upto >= p * s_mass[1] * off * off, &s_at[1]);
         __syncthreads();
-        const int n_upto = n_before + count;
-        if (n_before < k && k <= n_upto) {                 // one bin: top_k ends here
-            s_at[2] = tid;
-            s_mass[0] = s.by_k ? before : all;
-            s_mass[1] = s.by_k ? upto + n_upto * SMP_LEAST : all + n_all * SMP_LEAST;
-        }
-        __syncthreads();
-        const int last = s_at[2];
-        if (s.by_p) {
-            // the first bin in which the sum may, and in which it must have reached top_p's part
-            const uint64_t may = __ballot((upto + n_upto * SMP_LEAST) * (1.0 + SMP_MARGIN) >= s.p * s_mass[0] * (1.0 - SMP_MARGIN));
-            const uint64_t must = __ballot(upto * (1.0 - SMP_MARGIN) >= s.p * s_mass[1] * (1.0 + SMP_MARGIN));
-            if (lane == 0) {
-                if (may) atomicMin(&s_at[0], tid + (int)__builtin_ctzll(may));
-                if (must) atomicMin(&s_at[1], tid + (int)__builtin_ctzll(must));
-            }
-            __syncthreads();
-            cut.lo = min(s_at[0], last);
-            cut.hi = min(s_at[1], last);
-        } else {
-            cut.lo = cut.hi = last;
-        }
-        cut.last = s.by_k ? last : SMP_BINS;
+        lo = s.bins > 0.0f ? min(s_at[0], last) : 0;
+        hi = s.bins > 0.0f ? min(s_at[1], last) : last;
     }
-    if (blockIdx.x == 0 && tid == 0) ws.cuts[seq] = cut;
-    // ---- the wave's segment
-    SmpSeg g = {0.0, 0.0, 0.0, 0, 0, 0, 0};
-    const int64_t seg = ((int64_t)seq * ws.n_chunks + blockIdx.x) * SMP_WAVES + wave;
-    uint64_t * list = ws.keys + seg * SMP_SEG;
-    const double top_bin = floor((double)top * s.per_bin);
-    const bool bins = s.by_k || s.by_p;
-#pragma unroll
-    for (int j = 0; j < SMP_LANE; ++j) {
-        const int b = !bins || x[j] == top ? 0 : (int)fmin(top_bin - floor((double)x[j] * s.per_bin), (double)SMP_OUT);
-        const bool there = x[j] != SMP_NONE, cand = there && ((b >= cut.lo && b <= cut.hi) || b == cut.last);
-        const bool sure = there && b < cut.lo, mid = there && b > cut.hi && b < cut.last;
-        if (sure || mid) {
-            const double w = smp_weight(x[j], top, s.inv_t);
-            if (sure) {
-                g.sure += w;
-                g.draw += w >= s.min_p ? w : 0.0;
-                ++g.n_sure;
-            } else {
-                g.mid += w;
-                ++g.n_mid;
-            }
+    // ---- the least value of bins lo - 1, hi and of those that top_k's end lies in, by bisection of the
+    // values' order; a lane each
+    const int of = tid == 0 ? lo - 1 : tid == 1 ? hi : tid == 2 ? (s.by_k ? last - 1 : SMP_BINS - 1) : last;
+    uint32_t below = (uint32_t)(smp_key(least, 0) >> 32) - 1, from = (uint32_t)(smp_key(top, 0) >> 32);
+    if (tid < 4) {
+        while (from - below > 1) {
+            const uint32_t mid = below + (from - below) / 2;
+            if (smp_bin(smp_value((uint64_t)mid << 32), top, top_bin, s.bins) <= of) from = mid;
+            else below = mid;
         }
-        const uint64_t votes = __ballot(cand);
-        if (cand) list[g.n_cand + __popcll(votes & ((1ull << lane) - 1))] = smp_key(x[j], smp_at<T>(base, j));
-        g.n_cand += __popcll(votes);
     }
-    for (int o = 32; o; o >>= 1) {
-        g.sure += __shfl_xor(g.sure, o, 64);
-        g.draw += __shfl_xor(g.draw, o, 64);
-        g.mid += __shfl_xor(g.mid, o, 64);
-        g.n_sure += __shfl_xor(g.n_sure, o, 64);
-        g.n_mid += __shfl_xor(g.n_mid, o, 64);
+    if (tid < 64) {
+        const float x = of < 0 ? none : smp_value((uint64_t)from << 32);
+        cut.x_sure = smp_lane(x, 0);
+        cut.x_cand = smp_lane(x, 1);
+        // (bins hi and last are one: no values between them)
+        cut.x_mid = s.by_k && last == hi ? cut.x_cand : smp_lane(x, 2);
+        cut.x_end = s.by_k && last > hi ? smp_lane(x, 3) : cut.x_mid;
+        if (tid == 0) ws.cuts[seq] = cut;
     }
-    if (lane == 0) ws.segs[seg] = g;
 }
 
-template <class T>
-__global__ __launch_bounds__(SMP_WG) void k_sample_pick(const llapis_sample_args a, const SmpWs ws) {
-    __shared__ uint64_t s_key[SMP_SORT];
-    __shared__ double s_sum[SMP_WAVES];
-    __shared__ int s_count[SMP_WAVES];
-    __shared__ unsigned long long s_mass[256];
-    __shared__ int s_n[256];
-    __shared__ int s_seg, s_last;
+// --------------------------------------------------------------- split
+
+template <class T, int N>
+__global__ __launch_bounds__(SMP_WG) void k_sample_split(const llapis_sample_args a, const SmpWs ws) {
+    // the values, which a loop goes through: unrolled, its code takes longer to fetch than to run
+    __shared__ float s_x[N][SMP_WG];
+    const int seq = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const SmpSet s = smp_settings(a, seq);
+    if (s.greedy) return;
+    const int base = blockIdx.x * smp_chunk(N) + wave * smp_seg(N);
+    {
+        float x[N];
+        smp_read((const T *)a.logits + seq * a.logits_stride, base, a.vocab, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) s_x[j][tid] = x[j];
+    }
+    const SmpCut cut = ws.cuts[seq];
+    if (cut.token < 0) return;
+    SmpSeg g = {0.0, 0.0, 0.0, 0, 0, 0, 0};
+    const int64_t seg = ((int64_t)seq * ws.n_chunks + blockIdx.x) * SMP_WAVES + wave;
+    uint64_t * list = ws.keys + seg * smp_seg(N);
+#pragma unroll 2
+    for (int j = 0; j < N; ++j) {
+        const float x = s_x[j][tid];
+        const bool sure = x >= cut.x_sure, mid = x >= cut.x_mid && x < cut.x_cand;
+        const bool cand = !sure && x >= cut.x_end && !mid;
+        if (sure || mid) {
+            const double w = smp_weight(x, cut.top, s.octaves);
+            g.sure += sure ? w : 0.0;
+            g.draw += sure && w >= s.min_p ? w : 0.0;
+            g.mid += sure ? 0.0 : w;
+            g.n_sure += sure;
+            g.n_mid += !sure;
+        }
+        const uint64_t votes = __ballot(cand);
+        if (votes) {
+            if (cand) list[g.n_cand + __popcll(votes & ((1ull << lane) - 1))] = smp_key(x, smp_at<T>(base, j));
+            g.n_cand += __popcll(votes);
+        }
+    }
+    g.sure = smp_wave(g.sure, SmpAdd());
+    g.draw = smp_wave(g.draw, SmpAdd());
+    g.mid = smp_wave(g.mid, SmpAdd());
+    g.n_sure = smp_wave(g.n_sure, SmpAdd());
+    g.n_mid = smp_wave(g.n_mid, SmpAdd());
+    if (lane == 63) ws.segs[seg] = g;
+}
+
+// ---------------------------------------------------------------- pick
+
+template <class T, int N>
+__global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_pick(const llapis_sample_args a, const SmpWs ws) {
+    constexpr int WG = SMP_SEQ_WG, WAVES = SMP_SEQ_WAVES, SEG = smp_seg(N), HOLD = SMP_FEW / WG;
+    __shared__ double s_sure[WAVES], s_mid[WAVES], s_sum[2][WAVES];
+    __shared__ int s_n[3][WAVES], s_count[WAVES], s_digit[256];
+    __shared__ uint64_t s_mass[WAVES];
+    __shared__ int s_first[SMP_HELD + 1], s_bucket_n[WG], s_list_n, s_found, s_last;
+    __shared__ unsigned long long s_bucket[WG], s_kept[SMP_HELD], s_weigh[256], s_all_k;
+    __shared__ uint64_t s_list[SMP_LIST], s_key;
+    __shared__ struct { int bucket, before, n; uint64_t mass; } s_sel;
     __shared__ double s_before;
     const int seq = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const SmpSet s = smp_settings(a, seq);
@@ -331,252 +431,380 @@ __global__ __launch_bounds__(SMP_WG) void k_sample_pick(const llapis_sample_args
         if (tid == 0) a.tokens[seq] = cut.token;
         return;
     }
-    const int n_segs = (a.vocab + SMP_SEG - 1) / SMP_SEG, per = (n_segs + SMP_WG - 1) / SMP_WG;
+    const int n_segs = (a.vocab + SEG - 1) / SEG, per = (n_segs + WG - 1) / WG;
     const int64_t seg0 = (int64_t)seq * ws.n_chunks * SMP_WAVES;
-    const SmpSeg * segs = ws.segs + seg0;
-    const uint64_t * keys = ws.keys + seg0 * SMP_SEG;
-    auto weight = [&](uint64_t key) { return smp_weight(smp_value(key), cut.top, s.inv_t); };
+    SmpSeg * segs = ws.segs + seg0;
+    const uint64_t * keys = ws.keys + seg0 * SEG;
+    auto weight = [&](uint64_t key) { return smp_weight(smp_value(key), cut.top, s.octaves); };
     // ---- a thread's segments are consecutive
-    SmpSeg mine = {0.0, 0.0, 0.0, 0, 0, 0, 0};
+    double sure = 0.0, mid = 0.0, draw = 0.0;
+    int n_sure = 0, n_mid = 0, n_mine = 0;
     for (int i = tid * per; i < min((tid + 1) * per, n_segs); ++i) {
         const SmpSeg g = segs[i];
-        mine.sure += g.sure;
-        mine.mid += g.mid;
-        mine.n_sure += g.n_sure;
-        mine.n_mid += g.n_mid;
-        mine.n_cand += g.n_cand;
+        sure += g.sure;
+        mid += g.mid;
+        draw += g.draw;
+        n_sure += g.n_sure;
+        n_mid += g.n_mid;
+        n_mine += g.n_cand;
     }
-    double sure, mid;
-    int n_sure, n_mid, n_cand;
-    smp_scan(mine.sure, s_sum, sure);
-    smp_scan(mine.mid, s_sum, mid);
-    smp_scan(mine.n_sure, s_count, n_sure);
-    smp_scan(mine.n_mid, s_count, n_mid);
-    const int at = smp_scan(mine.n_cand, s_count, n_cand);
-    // f(key) of each candidate, a wave a segment
-    auto each = [&](auto f) {
-        for (int i = wave; i < n_segs; i += SMP_WAVES) {
-            const int n = segs[i].n_cand;
-            for (int c = lane; c < n; c += 64) f(keys[(int64_t)i * SMP_SEG + c]);
-        }
-    };
+    const int cand_w = smp_wave(n_mine, SmpAdd());
+    smp_leave(cand_w, s_n[0]);
+    smp_leave(smp_wave(n_sure, SmpAdd()), s_n[1]);
+    smp_leave(smp_wave(n_mid, SmpAdd()), s_n[2]);
+    smp_leave(smp_wave(sure, SmpAdd()), s_sure);
+    smp_leave(smp_wave(mid, SmpAdd()), s_mid);
+    s_bucket_n[tid] = 0;
+    s_bucket[tid] = 0;
+    s_kept[tid] = 0;
+    if (tid == 0) {
+        s_list_n = 0;
+        s_all_k = 0;
+        s_found = 0x7FFFFFFF;
+        s_last = -1;
+    }
+    __syncthreads();
+    int n_cand;
+    const int first = smp_before<WAVES>(s_n[0], n_cand) + cand_w - n_mine;
     uint64_t key = ~0ull;                                  // the last that is kept
     if (n_cand > 0) {
+        n_sure = smp_all<WAVES>(s_n[1], SmpAdd());
+        n_mid = smp_all<WAVES>(s_n[2], SmpAdd());
+        sure = smp_all<WAVES>(s_sure, SmpAdd());
+        mid = smp_all<WAVES>(s_mid, SmpAdd());
         // candidates within top_k, the first of them in order
         const int n_k = s.by_k ? max(min(s.k - n_sure - n_mid, n_cand), 0) : n_cand;
-        if (n_cand <= SMP_SORT) {
-            int n2 = 64;
-            while (n2 < n_cand) n2 *= 2;
-            // each segment's list to its place
-            int to = at;
-            for (int i = tid * per; i < min((tid + 1) * per, n_segs); ++i) {
-                const int n = segs[i].n_cand;
-                for (int c = 0; c < n; ++c) s_key[to++] = keys[(int64_t)i * SMP_SEG + c];
-            }
-            for (int i = n_cand + tid; i < n2; i += SMP_WG) s_key[i] = 0;
+        bool few = n_cand <= SMP_FEW && per == 1;
+        if (few) {
+            // ---- the candidates in registers, and in buckets by value, thread b's the b-th from above.
+            // Weights are whole numbers of 2^-49 of the largest that a candidate may have
+            if (tid < n_segs) s_first[tid] = first;
+            if (tid == 0) s_first[n_segs] = n_cand;
             __syncthreads();
-            for (int size = 2; size <= n2; size *= 2)
-                for (int step = size / 2; step; step /= 2) {
-                    for (int i = tid; i < n2 / 2; i += SMP_WG) {
-                        const int l = (i / step) * 2 * step + i % step, r = l + step;
-                        const uint64_t u = s_key[l], v = s_key[r];
-                        if ((u < v) == ((l & size) == 0)) {
-                            s_key[l] = v;
-                            s_key[r] = u;
-                        }
+            const float upper = cut.x_sure == cut.x_sure ? cut.x_sure : cut.top;
+            const double scale = 0x1p49 / smp_weight(upper, cut.top, s.octaves);
+            const bool two = cut.x_end < cut.x_mid;         // candidates of top_k's end apart
+            const int n_upper = two ? WG / 2 : WG;
+            const double per_upper = n_upper / fmax((double)upper - (double)cut.x_cand, 1e-300);
+            const double per_lower = (WG / 2) / fmax((double)cut.x_mid - (double)cut.x_end, 1e-300);
+            uint64_t k[HOLD];
+            unsigned long long w[HOLD];
+            int bucket[HOLD], seg_of[HOLD];
+#pragma unroll
+            for (int e = 0; e < HOLD; ++e) {
+                const int r = tid + e * WG;
+                k[e] = 0;
+                w[e] = 0;
+                bucket[e] = -1;
+                seg_of[e] = 0;
+                if (r < n_cand) {
+                    int l = 0;
+                    for (int h = n_segs; h - l > 1;) {
+                        const int mid_seg = (l + h) >> 1;
+                        if (s_first[mid_seg] <= r) l = mid_seg;
+                        else h = mid_seg;
                     }
-                    __syncthreads();
+                    seg_of[e] = l;
+                    k[e] = keys[(int64_t)l * SEG + r - s_first[l]];
                 }
-            // a thread's keys are consecutive
-            const int each_n = (n2 + SMP_WG - 1) / SMP_WG;
-            double w[SMP_SORT / SMP_WG], sum = 0.0, within = 0.0;
-#pragma unroll
-            for (int i = 0; i < SMP_SORT / SMP_WG; ++i) {
-                const int r = tid * each_n + i;
-                w[i] = i < each_n && r < n_cand ? weight(s_key[r]) : 0.0;
-                sum += w[i];
-                within += r < n_k ? w[i] : 0.0;
             }
-            double all_k, all;
-            smp_scan(within, s_sum, all_k);
-            double before = sure + smp_scan(sum, s_sum, all);
-            const double goal = s.p * (sure + mid + all_k);
-            int kept = 0;
+#pragma unroll 1
+            for (int e = 0; e < HOLD && e * WG < n_cand; ++e) {
+                uint64_t u = 0;
 #pragma unroll
-            for (int i = 0; i < SMP_SORT / SMP_WG; ++i) {
-                const int r = tid * each_n + i;
-                if (i < each_n && r < n_k && (!s.by_p || before < goal)) ++kept;
-                before += w[i];
+                for (int i = 0; i < HOLD; ++i) u = i == e ? k[i] : u;
+                if (u) {
+                    const float x = smp_value(u);
+                    const unsigned long long y = (unsigned long long)(weight(u) * scale);
+                    const bool above = !two || x >= cut.x_cand;
+                    const double at = ((double)(above ? upper : cut.x_mid) - (double)x) * (above ? per_upper : per_lower);
+                    const int most = above ? n_upper - 1 : WG / 2 - 1;
+                    // (the largest of all may be infinite: it is first)
+                    const int b = x == upper ? 0 : (above ? 0 : n_upper) + (int)fmin(fmax(at, 0.0), (double)most);
+#pragma unroll
+                    for (int i = 0; i < HOLD; ++i)
+                        if (i == e) {
+                            bucket[i] = b;
+                            w[i] = y;
+                        }
+                    atomicAdd(&s_bucket_n[b], 1);
+                    atomicAdd(&s_bucket[b], y);
+                }
             }
-            int n_kept;
-            smp_scan(kept, s_count, n_kept);
-            if (n_kept > 0) key = s_key[n_kept - 1];
-        } else {
-            // too many: eight bits of the key at a time, the candidates counted (and
+            __syncthreads();
+            const int b_n = s_bucket_n[tid];
+            const uint64_t b_mass = s_bucket[tid];
+            const int b_n_w = smp_wave(b_n, SmpAdd());
+            const uint64_t b_mass_w = smp_wave(b_mass, SmpAdd());
+            smp_leave(b_n_w, s_count);
+            smp_leave(b_mass_w, s_mass);
+            __syncthreads();
+            int all_n;
+            uint64_t all_mass;
+            const int n_upto = smp_before<WAVES>(s_count, all_n) + b_n_w;
+            const uint64_t mass_upto = smp_before<WAVES>(s_mass, all_mass) + b_mass_w;
+            // ---- the bucket that a filter ends in, then the key: top_k's by number, top_p's by weight
+            uint64_t all_k = all_mass;
+            key = n_k > 0 ? 0 : ~0ull;
+            for (int pass = n_k < n_cand ? 0 : 1; pass < (s.by_p ? 2 : 1) && n_k > 0 && few; ++pass) {
+                const double whole = sure + mid + (double)all_k / scale;
+                const uint64_t goal = (uint64_t)ceil(fmax(s.p * whole - sure, 0.0) * scale);
+                const bool mine = b_n > 0 && (pass == 0 ? n_upto >= n_k && n_upto - b_n < n_k : mass_upto >= goal && (mass_upto - b_mass < goal || n_upto == b_n));
+                if (tid == 0) s_sel.bucket = -1;
+                __syncthreads();
+                if (mine) s_sel = {tid, n_upto - b_n, b_n, mass_upto - b_mass};
+                __syncthreads();
+                if (s_sel.bucket < 0) break;               // the weight of all is not top_p's part by a rounding: all are kept
+                const int n = s_sel.n;
+                if (n > SMP_LIST) {
+                    few = false;
+                    break;
+                }
+#pragma unroll
+                for (int e = 0; e < HOLD; ++e)
+                    if (bucket[e] == s_sel.bucket) s_list[atomicAdd(&s_list_n, 1)] = k[e];
+                __syncthreads();
+                if (tid < n) {
+                    // the list's keys that are not below this thread's
+                    const uint64_t u = s_list[tid];
+                    int rank = 0;
+                    uint64_t upto = 0;
+                    const uint64_t own_mass = (uint64_t)(weight(u) * scale);
+                    if (pass == 0) {
+                        for (int i = 0; i < n; ++i) rank += s_list[i] >= u;
+                        if (s_sel.before + rank <= n_k) atomicAdd(&s_all_k, own_mass);
+                        if (s_sel.before + rank == n_k) s_key = u;
+                    } else {
+                        for (int i = 0; i < n; ++i) {
+                            const uint64_t v = s_list[i];
+                            // (equal values have equal weights: most buckets hold one)
+                            upto += v >= u ? (v >> 32 == u >> 32 ? own_mass : (uint64_t)(weight(v) * scale)) : 0;
+                        }
+                        const uint64_t g = goal > s_sel.mass ? goal - s_sel.mass : 0;
+                        if (upto >= g && (upto - own_mass < g || upto == own_mass)) s_key = u;
+                    }
+                }
+                __syncthreads();
+                if (pass == 0) all_k = s_sel.mass + s_all_k;
+                key = s_key > key ? s_key : key;
+                if (tid == 0) s_list_n = 0;
+                __syncthreads();
+            }
+            // ---- the segments' kept weights
+            if (few) {
+#pragma unroll 1
+                for (int e = 0; e < HOLD && e * WG < n_cand; ++e) {
+                    uint64_t u = 0;
+                    unsigned long long y = 0;
+                    int at = 0;
+#pragma unroll
+                    for (int i = 0; i < HOLD; ++i)
+                        if (i == e) {
+                            u = k[i];
+                            y = w[i];
+                            at = seg_of[i];
+                        }
+                    if (u && u >= key && (s.min_p == 0.0 || weight(u) >= s.min_p)) atomicAdd(&s_kept[at], y);
+                }
+                __syncthreads();
+                draw += (double)s_kept[tid] / scale;
+            }
+        }
+        if (!few) {
+            // ---- too many at once: eight bits of the key at a time, the candidates counted (and
             // weighed in fixed point) by them: the first key at which the number or the
             // weight of what is not below it reaches the goal
+            auto each = [&](auto f) {                      // f(key) of each candidate, a wave a segment
+                for (int i = wave; i < n_segs; i += WAVES) {
+                    const int n = segs[i].n_cand;
+                    for (int c = lane; c < n; c += 64) f(keys[(int64_t)i * SEG + c]);
+                }
+            };
             int bits = 1;
             while (bits < 31 && (1 << bits) < n_cand) ++bits;
             const double scale = __builtin_ldexp(1.0, 61 - bits);
-            auto descend = [&](bool by_mass, int n_goal, double goal) {
+            double goal = 0.0;
+            key = n_k > 0 ? 0 : ~0ull;
+            for (int pass = n_k < n_cand ? 0 : 1; pass < (s.by_p ? 2 : 1) && n_k > 0; ++pass) {
+                const bool by_mass = pass == 1;
+                if (by_mass) {
+                    double within = 0.0, all_k;
+                    each([&](uint64_t u) { within += u >= key ? weight(u) : 0.0; });
+                    __syncthreads();
+                    smp_scan<WAVES>(within, s_sum[0], all_k);
+                    goal = s.p * (sure + mid + all_k) - sure;
+                }
                 uint64_t prefix = 0;
                 int n_above = 0;
                 unsigned long long above = 0;
                 const unsigned long long want = by_mass ? (unsigned long long)ceil(fmax(goal, 0.0) * scale) : 0;
                 for (int shift = 56; shift >= 0; shift -= 8) {
+                    __syncthreads();
                     if (tid < 256) {
-                        s_n[tid] = 0;
-                        s_mass[tid] = 0;
+                        s_digit[tid] = 0;
+                        s_weigh[tid] = 0;
                     }
                     __syncthreads();
                     each([&](uint64_t u) {
                         if (shift < 56 && (u >> (shift + 8)) != (prefix >> (shift + 8))) return;
                         const int d = (int)(u >> shift) & 255;
-                        atomicAdd(&s_n[d], 1);
-                        if (by_mass) atomicAdd(&s_mass[d], (unsigned long long)(weight(u) * scale));
+                        atomicAdd(&s_digit[d], 1);
+                        if (by_mass) atomicAdd(&s_weigh[d], (unsigned long long)(weight(u) * scale));
                     });
                     __syncthreads();
                     int d = 255, found = -1;
                     for (; d >= 0; --d) {
-                        if (s_n[d] == 0) continue;
+                        if (s_digit[d] == 0) continue;
                         found = d;
-                        if (by_mass ? above + s_mass[d] >= want : n_above + s_n[d] >= n_goal) break;
-                        n_above += s_n[d];
-                        above += s_mass[d];
+                        if (by_mass ? above + s_weigh[d] >= want : n_above + s_digit[d] >= n_k) break;
+                        n_above += s_digit[d];
+                        above += s_weigh[d];
                     }
                     if (d < 0) {                          // all of them: the last
-                        n_above -= s_n[found];
-                        above -= s_mass[found];
+                        n_above -= s_digit[found];
+                        above -= s_weigh[found];
                     }
                     prefix |= (uint64_t)found << shift;
-                    __syncthreads();
                 }
-                return prefix;
-            };
-            if (n_k > 0) {
-                key = n_k < n_cand ? descend(false, n_k, 0.0) : 0;
-                if (s.by_p) {
-                    double within = 0.0, all_k;
-                    each([&](uint64_t u) { within += u >= key ? weight(u) : 0.0; });
-                    smp_scan(within, s_sum, all_k);
-                    const uint64_t by_p = descend(true, 0, s.p * (sure + mid + all_k) - sure);
-                    key = by_p > key ? by_p : key;
-                }
+                key = prefix > key ? prefix : key;
             }
+            for (int i = wave; i < n_segs; i += WAVES) {
+                const int n = segs[i].n_cand;
+                double sum = 0.0;
+                for (int c = lane; c < n; c += 64) {
+                    const uint64_t u = keys[(int64_t)i * SEG + c];
+                    const double y = u >= key ? weight(u) : 0.0;
+                    sum += y >= s.min_p ? y : 0.0;
+                }
+                sum = smp_lane(smp_wave(sum, SmpAdd()), 63);
+                if (lane == 0) segs[i].draw += sum;
+            }
+            __syncthreads();
+            draw = 0.0;
+            for (int i = tid * per; i < min((tid + 1) * per, n_segs); ++i) draw += segs[i].draw;
         }
     }
-    // ---- the segments' kept weights, in their order
-    auto kept = [&](uint64_t u) {
-        const double w = u >= key ? weight(u) : 0.0;
-        return w >= s.min_p ? w : 0.0;
-    };
-    for (int i = wave; i < n_segs; i += SMP_WAVES) {
-        const int n = segs[i].n_cand;
-        double w = 0.0;
-        for (int c = lane; c < n; c += 64) w += kept(keys[(int64_t)i * SMP_SEG + c]);
-        if (n > 0) {
-            for (int o = 32; o; o >>= 1) w += __shfl_xor(w, o, 64);
-            if (lane == 0) ws.segs[seg0 + i].draw = segs[i].draw + w;
-        }
-    }
-    if (tid == 0) {
-        s_seg = 0x7FFFFFFF;
-        s_last = -1;
-    }
-    __syncthreads();
-    double sum = 0.0, total;
-    for (int i = tid * per; i < min((tid + 1) * per, n_segs); ++i) sum += ws.segs[seg0 + i].draw;
-    double cum = smp_scan(sum, s_sum, total);
-    const double goal = (double)a.u[seq] * total;
-    // the first thread in whose segments the sum passes the goal; without one
+    // ---- the first thread in whose segments the sum passes the goal; without one
     // (rounding, u of 1 and more) the last that has anything
-    const uint64_t any = __ballot(sum > 0.0), over = __ballot(sum > 0.0 && cum + sum > goal);
-    if (lane == 0) {
-        if (any) atomicMax(&s_last, tid + 63 - (int)__builtin_clzll(any));
-        if (over) atomicMin(&s_seg, tid + (int)__builtin_ctzll(over));
-    }
+    double total;
+    double cum = smp_scan<WAVES>(draw, s_sum[1], total);
+    const double goal = (double)a.u[seq] * total;
+    const uint64_t any = __ballot(draw > 0.0);
+    if (any && lane == 0) atomicMax(&s_last, tid + 63 - (int)__builtin_clzll(any));
+    smp_first(draw > 0.0 && cum + draw > goal, &s_found);
     __syncthreads();
-    const bool found = s_seg != 0x7FFFFFFF;
-    const int who = found ? s_seg : s_last;
+    const bool found = s_found != 0x7FFFFFFF;
+    const int who = found ? s_found : s_last;
     __syncthreads();
     if (tid == who) {
-        int seg = -1;
-        for (int i = tid * per; i < min((tid + 1) * per, n_segs); ++i) {
-            const double y = ws.segs[seg0 + i].draw;
-            if (!(y > 0.0)) continue;
+        int seg = tid;
+        if (per > 1) {
+            seg = -1;
+            for (int i = tid * per; i < min((tid + 1) * per, n_segs); ++i) {
+                const double y = segs[i].draw;
+                if (!(y > 0.0)) continue;
+                seg = i;
+                s_before = cum;
+                cum += y;
+                if (found && cum > goal) break;
+            }
+        } else {
             s_before = cum;
-            seg = i;
-            cum += y;
-            if (found && cum > goal) break;
         }
-        s_seg = seg;
+        s_found = seg;
+    }
+    if (tid == 0) {
         s_last = -1;
+        s_list_n = 0x7FFFFFFF;
     }
     __syncthreads();
-    // ---- the token: two consecutive values a thread
-    const int first = s_seg * SMP_SEG + tid * (SMP_SEG / SMP_WG);
+    // ---- the token: consecutive values a thread
+    constexpr int E = (SEG + WG - 1) / WG;
+    const int at = s_found * SEG + tid * E, end = min(s_found * SEG + SEG, a.vocab);
     const T * row = (const T *)a.logits + seq * a.logits_stride;
-    double w[SMP_SEG / SMP_WG];
-    sum = 0.0;
+    double w[E], sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < SMP_SEG / SMP_WG; ++i) {
-        const float x = first + i < a.vocab ? smp_clean((float)row[first + i]) : SMP_NONE;
-        const int b = !(s.by_k || s.by_p) ? 0 : smp_bin(x, cut.top, s.per_bin);
-        const bool keep = x != SMP_NONE && (b < cut.lo || ((b <= cut.hi || b == cut.last) && smp_key(x, first + i) >= key));
-        w[i] = keep ? smp_weight(x, cut.top, s.inv_t) : 0.0;
+    for (int i = 0; i < E; ++i) {
+        const float x = at + i < end ? smp_clean((float)row[at + i]) : SMP_NONE;
+        const bool keep = x >= cut.x_sure || (x >= cut.x_end && !(x >= cut.x_mid && x < cut.x_cand) && smp_key(x, at + i) >= key);
+        w[i] = keep ? smp_weight(x, cut.top, s.octaves) : 0.0;
         if (w[i] < s.min_p) w[i] = 0.0;
         sum += w[i];
     }
     double part;
-    cum = s_before + smp_scan(sum, s_sum, part);
+    cum = s_before + smp_scan<WAVES>(sum, s_sum[0], part);
     int token = -1, last = -1;
 #pragma unroll
-    for (int i = 0; i < SMP_SEG / SMP_WG; ++i) {
+    for (int i = 0; i < E; ++i) {
         cum += w[i];
         if (w[i] > 0.0) {
-            last = first + i;
-            if (token < 0 && found && cum > goal) token = first + i;
+            last = at + i;
+            if (token < 0 && found && cum > goal) token = at + i;
         }
     }
     // the lowest that passes, else the last that has a weight
-    if (tid == 0) s_count[0] = 0x7FFFFFFF;
-    __syncthreads();
-    if (token >= 0) atomicMin(&s_count[0], token);
-    if (last >= 0) atomicMax(&s_last, last);
+    const uint64_t passes = __ballot(token >= 0), has = __ballot(last >= 0);
+    if (passes) {
+        token = __builtin_amdgcn_readlane(token, __builtin_ctzll(passes));
+        if (lane == 0) atomicMin(&s_list_n, token);
+    }
+    if (has) {
+        last = __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(has));
+        if (lane == 0) atomicMax(&s_last, last);
+    }
     __syncthreads();
     if (tid == 0) {
-        a.tokens[seq] = s_count[0] != 0x7FFFFFFF ? s_count[0] : s_last;
+        a.tokens[seq] = s_list_n != 0x7FFFFFFF ? s_list_n : s_last;
         ws.cuts[seq].key = key;
         ws.cuts[seq].total = total;
     }
 }
 
-template <class T>
+// --------------------------------------------------------------- probs
+
+template <class T, int N>
 __global__ __launch_bounds__(SMP_WG) void k_sample_probs(const llapis_sample_args a, const SmpWs ws) {
-    const int seq = blockIdx.y, wave = threadIdx.x >> 6;
+    __shared__ float s_x[N][SMP_WG];                       // values, then probabilities
+    const int seq = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
     const SmpSet s = smp_settings(a, seq);
-    const SmpCut cut = ws.cuts[seq];
-    const int base = blockIdx.x * SMP_CHUNK + wave * SMP_SEG;
+    const int base = blockIdx.x * smp_chunk(N) + wave * smp_seg(N);
     if (base >= a.vocab) return;
-    float x[SMP_LANE];
-    smp_read((const T *)a.logits + seq * a.logits_stride, base, a.vocab, x);
-    T * out = (T *)a.probs + seq * a.probs_stride;
-    const double inv = 1.0 / cut.total;
-    const bool bins = s.by_k || s.by_p;
+    {
+        float x[N];
+        smp_read((const T *)a.logits + seq * a.logits_stride, base, a.vocab, x);
 #pragma unroll
-    for (int j = 0; j < SMP_LANE; ++j) {
+        for (int j = 0; j < N; ++j) s_x[j][tid] = x[j];
+    }
+    const SmpCut cut = ws.cuts[seq];
+    const double inv = 1.0 / cut.total;
+#pragma unroll 2
+    for (int j = 0; j < N; ++j) {
+        const float x = s_x[j][tid];
         const int i = smp_at<T>(base, j);
         float p = 0.0f;
         if (s.greedy) {
             p = i == cut.token ? 1.0f : 0.0f;
-        } else if (x[j] != SMP_NONE && cut.token >= 0) {
-            const int b = bins ? smp_bin(x[j], cut.top, s.per_bin) : 0;
-            if (b < cut.lo || ((b <= cut.hi || b == cut.last) && smp_key(x[j], i) >= cut.key)) {
-                const double w = smp_weight(x[j], cut.top, s.inv_t);
-                p = w >= s.min_p ? (float)(w * inv) : 0.0f;
-            }
+        } else if (x >= cut.x_sure || (x >= cut.x_end && !(x >= cut.x_mid && x < cut.x_cand) && smp_key(x, i) >= cut.key)) {
+            const double w = smp_weight(x, cut.top, s.octaves);
+            p = w >= s.min_p ? (float)(w * inv) : 0.0f;
         }
-        if (i < a.vocab) out[i] = (T)p;
+        s_x[j][tid] = p;
+    }
+    T * out = (T *)a.probs + seq * a.probs_stride;
+    constexpr int W = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < N / W; ++c) {
+        const int i = smp_at<T>(base, c * W);
+        typename SmpVec<T>::v w;
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j] = (T)s_x[c * W + j][tid];
+        if (i + W <= a.vocab) {
+            *(typename SmpVec<T>::v *)(out + i) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (i + j < a.vocab) out[i + j] = w[j];
+        }
     }
 }
 
@@ -596,36 +824,57 @@ int32_t refuse_sample(const char * why) noexcept {
 
 uint64_t round_up(uint64_t n) { return (n + 255) / 256 * 256; }
 
-// the workspace's parts; its size
-uint64_t sample_parts(int n_seq, int vocab, uint8_t * at, SmpWs & ws) {
-    ws.n_chunks = (vocab + SMP_CHUNK - 1) / SMP_CHUNK;
-    const uint64_t chunks = (uint64_t)n_seq * ws.n_chunks;
+// values of a lane: 8 where a call's rows leave most of the card without work at 32
+constexpr int64_t SMP_SHORT = 1 << 20;
+bool short_rows(int n_seq, int vocab) { return (int64_t)n_seq * vocab <= SMP_SHORT; }
+
+// the workspace's parts for `chunks` chunks of n_seq sequences; its size
+uint64_t sample_parts(uint64_t n_seq, uint64_t chunks, int lane_values, uint8_t * at, SmpWs & ws) {
     uint64_t n = 0;
     auto part = [&](uint64_t bytes) {
         uint8_t * p = at ? at + n : nullptr;
         n += round_up(bytes);
         return p;
     };
-    ws.cuts = (SmpCut *)part((uint64_t)n_seq * sizeof(SmpCut));
+    ws.cuts = (SmpCut *)part(n_seq * sizeof(SmpCut));
     ws.chunks = (SmpChunk *)part(chunks * sizeof(SmpChunk));
     ws.segs = (SmpSeg *)part(chunks * SMP_WAVES * sizeof(SmpSeg));
-    ws.hist = (uint64_t *)part(chunks * SMP_BINS * 8);
-    ws.keys = (uint64_t *)part(chunks * SMP_CHUNK * 8);
+    ws.hist = (uint32_t *)part(chunks * SMP_BINS * 4);
+    ws.keys = (uint64_t *)part(chunks * smp_chunk(lane_values) * 8);
     return n;
 }
 
-template <class T>
-hipError_t launch_sample(const llapis_sample_args & a, const SmpWs & ws, hipStream_t s) {
-    const dim3 grid(ws.n_chunks, a.n_seq), wg(SMP_WG);
-    hipLaunchKernelGGL((k_sample_scan<T>), grid, wg, 0, s, a, ws);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_sample_cut<T>), grid, wg, 0, s, a, ws);
+int chunks_of(int vocab, int lane_values) { return (vocab + smp_chunk(lane_values) - 1) / smp_chunk(lane_values); }
+
+// ... of the long chunks, and of the most short ones that a call of no more sequences and values has
+uint64_t sample_bytes(int n_seq, int vocab) {
+    SmpWs ws;
+    const uint64_t few = std::min<uint64_t>((uint64_t)n_seq * chunks_of(vocab, 8), SMP_SHORT / smp_chunk(8) + n_seq);
+    return std::max(sample_parts(n_seq, (uint64_t)n_seq * chunks_of(vocab, 32), 32, nullptr, ws), sample_parts(n_seq, few, 8, nullptr, ws));
+}
+
+template <class T, int N>
+hipError_t launch_sample(const llapis_sample_args & a, void * workspace, hipStream_t s) {
+    SmpWs ws;
+    ws.n_chunks = chunks_of(a.vocab, N);
+    sample_parts(a.n_seq, (uint64_t)a.n_seq * ws.n_chunks, N, (uint8_t *)workspace, ws);
+    const dim3 grid(ws.n_chunks, a.n_seq), wg(SMP_WG), each(a.n_seq), seq_wg(SMP_SEQ_WG);
+    hipError_t e;
+    hipLaunchKernelGGL((k_sample_scan<T, N>), grid, wg, 0, s, a, ws);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((k_sample_pick<T>), dim3(a.n_seq), wg, 0, s, a, ws);
+    hipLaunchKernelGGL(k_sample_find, each, seq_wg, 0, s, a, ws);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL((k_sample_split<T, N>), grid, wg, 0, s, a, ws);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL((k_sample_pick<T, N>), each, seq_wg, 0, s, a, ws);
     if ((e = hipGetLastError()) != hipSuccess || !a.probs) return e;
-    hipLaunchKernelGGL((k_sample_probs<T>), grid, wg, 0, s, a, ws);
+    hipLaunchKernelGGL((k_sample_probs<T, N>), grid, wg, 0, s, a, ws);
     return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_sample(const llapis_sample_args & a, void * workspace, hipStream_t s) {
+    return short_rows(a.n_seq, a.vocab) ? launch_sample<T, 8>(a, workspace, s) : launch_sample<T, 32>(a, workspace, s);
 }
 
 }  // namespace
@@ -636,8 +885,7 @@ using namespace llapis;
 extern "C" {
 
 uint64_t llapis_sample_workspace_size(int32_t n_seq, int32_t vocab) {
-    SmpWs ws;
-    return n_seq <= 0 || n_seq > SMP_MAX_SEQ || vocab <= 0 || vocab > SMP_MAX_VOCAB ? 0 : sample_parts(n_seq, vocab, nullptr, ws);
+    return n_seq <= 0 || n_seq > SMP_MAX_SEQ || vocab <= 0 || vocab > SMP_MAX_VOCAB ? 0 : sample_bytes(n_seq, vocab);
 }
 
 int32_t llapis_sample(const llapis_sample_args * a, void * workspace, uint64_t ws_bytes, void * stream) {
@@ -651,11 +899,9 @@ int32_t llapis_sample(const llapis_sample_args * a, void * workspace, uint64_t w
         return refuse_sample("rows shorter than vocab");
     if (!workspace || ((uintptr_t)workspace & 15) || ws_bytes < llapis_sample_workspace_size(a->n_seq, a->vocab))
         return refuse_sample("workspace too small or not 16-byte aligned");
-    SmpWs ws;
-    sample_parts(a->n_seq, a->vocab, (uint8_t *)workspace, ws);
     hipStream_t s = (hipStream_t)stream;
-    const hipError_t e = a->type == T_F32 ? launch_sample<float>(*a, ws, s) : a->type == T_F16 ? launch_sample<_Float16>(*a, ws, s)
-                                                                                           : launch_sample<__bf16>(*a, ws, s);
+    const hipError_t e = a->type == T_F32 ? launch_sample<float>(*a, workspace, s)
+                         : a->type == T_F16 ? launch_sample<_Float16>(*a, workspace, s) : launch_sample<__bf16>(*a, workspace, s);
     return e == hipSuccess ? 0 : refuse_sample(hipGetErrorString(e));
 }
 
