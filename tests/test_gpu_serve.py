@@ -7,6 +7,7 @@ import torch
 
 import llapis_amd as la
 import serve_ref as ref
+import step_ref
 from step_ref import DT, EPS
 
 pytestmark = pytest.mark.gpu
@@ -365,3 +366,182 @@ def test_sample_graphs_share_a_workspace(gpu):
             torch.cuda.synchronize()
             assert torch.equal(tok, la.sample(y, u, top_p=p))
         u.mul_(0.7)
+
+
+# ------------------------------------------------------------ together
+
+class Serve:
+    """A serving step of a two-layer model, from its tokens to the next ones: pages and
+    slots, norms and rotary positions, the cache, attention behind a shared prefix, sampling.  `check`
+    compares every stage with its 64-bit form on the stage's own inputs."""
+    V, H, N, D, P, WIDTH = 700, 2, 6, 64, 16, 12
+
+    def __init__(self, gpu, n_seq):
+        g = torch.Generator().manual_seed(901)
+        mat = lambda *s: (torch.randn(*s, generator=g) / math.sqrt(s[0])).to(gpu)
+        d = 96
+        self.gpu, self.n_seq, self.n_pages = gpu, n_seq, n_seq * self.WIDTH
+        self.emb, self.head = mat(self.V, d) * math.sqrt(self.V), 5 * mat(d, self.V)
+        self.layers = [dict(qkv=mat(d, (self.N + 2 * self.H) * self.D), o=mat(self.N * self.D, d),
+                            wq=(1 + 0.2 * torch.randn(self.D, generator=g)).to(gpu), wk=(1 + 0.2 * torch.randn(self.D, generator=g)).to(gpu),
+                            cache=la.KvCache.empty(self.n_pages, self.P, self.H, self.D, la.F16, gpu)) for _ in range(2)]
+        self.pages = la.KvPages([l["cache"] for l in self.layers])
+        self.freq, self.magnitude = la.rope_frequencies(self.D, 500000.0, la.ROPE_YARN, 8.0, 64.0, device=gpu)
+
+    def state(self):
+        S, dev = self.n_seq, self.gpu
+        return dict(table=torch.full((S, self.WIDTH), -1, dtype=torch.int32, device=dev), lens=i32([0] * S, dev),
+                    free=i32(list(range(self.n_pages)), dev), n_free=i32([self.n_pages], dev), tokens=i32([3 + 5 * i for i in range(S)], dev),
+                    probs=torch.zeros(S, self.V, device=dev), groups=i32([0, 0], dev), prefix=i32([0], dev), u=f32([0.0] * S, dev))
+
+    def step(self, s, tokens, n_new, T, max_new, check=False):
+        """tokens [T] of the new rows; their logits [T, V]"""
+        before = check and [s[k].tolist() for k in ("table", "lens")] + [n_new.tolist(), s["free"].tolist(), int(s["n_free"])]
+        start, pos, seq, slots = self.pages.extend(s["table"], s["lens"], n_new, s["free"], s["n_free"], T)
+        if check:
+            want = ref.extend(*before, T, self.P, self.n_pages)
+            assert [s["table"].tolist(), s["lens"].tolist(), int(s["n_free"]), start.tolist(), pos.tolist(), seq.tolist(), slots.tolist()] == list(want)
+        batch = la.KvBatch(s["table"], s["lens"], start, n_tokens=T, max_new=max_new)
+        x = self.emb[tokens.long()]
+        for l in self.layers:
+            qkv = (x @ l["qkv"]).view(T, self.N + 2 * self.H, self.D)
+            q, k, v = qkv[:, :self.N], qkv[:, self.N:self.N + self.H], qkv[:, self.N + self.H:]
+            q2, k2 = la.qk_rope(q, k, pos, self.freq, l["wq"], l["wk"], magnitude=self.magnitude)
+            l["cache"].append(batch, k2, v)
+            a = l["cache"].prefix_attention(batch, q2, s["groups"], s["prefix"], out=torch.zeros_like(q2))
+            if check:
+                rows = int(start[-1])
+                for raw, w, y in ((q, l["wq"], q2), (k, l["wk"], k2)):
+                    want, tol = ref.rope(raw.cpu(), pos.cpu(), self.freq.cpu(), w.cpu(), True, 1e-6, self.magnitude, True, la.F32)
+                    assert ((y.cpu().double() - want).abs() <= tol)[:rows].all()
+                flat = lambda t: t.transpose(1, 2).reshape(-1, self.H, self.D)
+                at = slots[:rows].long()
+                assert torch.equal(flat(l["cache"].k)[at], k2[:rows].half())
+                assert torch.equal(flat(l["cache"].v.transpose(2, 3))[at], v[:rows].half())
+                want, _, tol = step_ref.attention(l["cache"], s["table"].tolist(), s["lens"].tolist(), start.tolist(), q2.cpu(), self.D ** -0.5)
+                # (the prefix's sums are joined by their logarithms, which stays within twice the bound)
+                assert ((a.cpu().double() - want).abs() <= 2 * tol)[:rows].all()
+            x = x + a.reshape(T, -1) @ l["o"]
+        return start, x @ self.head
+
+    def sample(self, s, logits, check=False):
+        la.sample(logits, s["u"], s.get("temperature"), s.get("top_k"), s.get("top_p"), s.get("min_p"), tokens=s["tokens"], probs=s["probs"])
+        if check:
+            cpu = lambda k: s[k].tolist() if k in s else None
+            tokens, want = ref.sample(logits.cpu(), s["u"].cpu(), cpu("temperature"), cpu("top_k"), cpu("top_p"), cpu("min_p"))
+            assert s["tokens"].tolist() == tokens
+            assert ((s["probs"].cpu().double() - want).abs() <= want * (EPS[la.F32] + 1e-12) + 2 ** -63).all()
+
+
+def test_serving_steps_together(gpu):
+    """One user's prompt in chunks, forked for parallel samples and another user's beside it; decode
+    steps behind the shared prefix; a verify step whose refused draft leaves; and decode steps as a
+    graph, replay by replay against eager steps of a twin."""
+    S = 5
+    m = Serve(gpu, S)
+    s = m.state()
+    g = torch.Generator().manual_seed(902)
+    draw = lambda n: torch.randint(0, m.V, (n,), generator=g, dtype=torch.int32).to(gpu)
+    # 45 tokens of sequence 0 and 19 of sequence 4, 16 at most a call, a row of each call unused
+    for a, b in ((16, 16), (16, 3), (13, 0)):
+        m.step(s, draw(a + b + 1), i32([a, 0, 0, 0, b], gpu), a + b + 1, 16, True)
+    # rows 1 to 3 go on from sequence 0: its two full pages are theirs too
+    _, free, n_free = m.pages.refs(s["table"], s["lens"])
+    spare = free[:3].tolist()
+    m.pages.fork(s["table"], s["lens"], i32([[0, i + 1, spare[i]] for i in range(3)], gpu))
+    refs, s["free"], s["n_free"] = m.pages.refs(s["table"], s["lens"])
+    assert s["lens"].tolist() == [45] * 4 + [19] and refs.max() == 4 and int(s["n_free"]) == m.n_pages - (2 + 4 + 2)
+    s["groups"], s["prefix"] = i32([0, 4], gpu), i32([32], gpu)
+    s.update(temperature=f32([0.8, 1.0, 0.0, 1.5, 0.7], gpu), top_k=i32([0, 40, 0, 7, 0], gpu), top_p=f32([0.9, 1.0, 1.0, 0.8, 1.0], gpu),
+             min_p=f32([0.0, 0.05, 0.0, 0.0, 0.02], gpu))
+    one = i32([1] * S, gpu)
+    for _ in range(4):
+        s["u"] = torch.rand(S, generator=g).to(gpu)
+        _, logits = m.step(s, s["tokens"], one, S, 1, True)
+        m.sample(s, logits, True)
+    # two tokens a sequence, the second a draft, verified against the model's probabilities after the filters
+    last, lens = s["tokens"].clone(), s["lens"].clone()
+    drafts, u, u_next = s["tokens"][:, None].roll(1, 0).contiguous(), torch.rand(S, 1, generator=g).to(gpu), torch.rand(S, generator=g).to(gpu)
+    start, logits = m.step(s, torch.stack([last, drafts[:, 0]], 1).flatten(), i32([2] * S, gpu), 2 * S, 2, True)
+    probs = torch.empty(2 * S, m.V, device=gpu)
+    two = {k: s[k].repeat_interleave(2) for k in ("temperature", "top_k", "top_p", "min_p", "u")}
+    la.sample(logits, two["u"], two["temperature"], two["top_k"], two["top_p"], two["min_p"], probs=probs)
+    s["tokens"], accepted = la.verify_drafts(probs.view(S, 2, m.V), None, drafts, u, u_next)
+    want, taken = step_ref.verify(probs.view(S, 2, m.V).cpu(), None, drafts.cpu(), u.cpu(), u_next.cpu(), None)
+    assert s["tokens"].tolist() == want and accepted.tolist() == taken
+    s["tokens"] = s["tokens"].gather(1, accepted[:, None].long())[:, 0].contiguous()
+    s["lens"].copy_(lens + 1 + accepted)
+    _, s["free"], s["n_free"] = m.pages.refs(s["table"], s["lens"])
+    # the step as a graph, across page ends, and a twin of everything in eager steps
+    twin = Serve(gpu, S)
+    for x, y in zip(m.layers, twin.layers):
+        y["cache"].k.copy_(x["cache"].k)
+        y["cache"].v.copy_(x["cache"].v)
+    t = {k: v.clone() for k, v in s.items()}
+
+    def run(m, s):
+        _, logits = m.step(s, s["tokens"], one, S, 1)
+        m.sample(s, logits)
+
+    warm = {k: v.clone() for k, v in s.items()}
+    run(twin, warm)                     # (its pages' rows are written again by the first step, alike)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(m, s)
+    for i in range(20):
+        for x in (s, t):
+            x["u"].copy_(torch.rand(S, generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        run(twin, t)
+        for k in ("table", "lens", "n_free", "tokens", "probs"):
+            assert torch.equal(s[k], t[k]), (i, k)
+    assert s["lens"].tolist() == (lens + 1 + accepted + 20).tolist()
+    assert all(torch.equal(x["cache"].k, y["cache"].k) and torch.equal(x["cache"].v, y["cache"].v) for x, y in zip(m.layers, twin.layers))
+
+
+def test_threads_and_streams_at_once(gpu):
+    """Host threads with a stream and workspaces of their own run every operator at once: as
+    each does alone, bit for bit, and a refusal is its own thread's."""
+    import threading
+    S = 6
+    models = [Serve(gpu, S) for _ in range(2)]
+    logits = torch.randn(2, 3, 50001, generator=torch.Generator().manual_seed(903)).to(gpu)
+    u, k = f32([0.1, 0.5, 0.9], gpu), i32([50, 0, 3], gpu)
+
+    def work(i):
+        m = models[i]
+        s = m.state()
+        s["u"].fill_(0.3 + 0.2 * i)
+        one = i32([1] * S, gpu)
+        for _ in range(4):
+            _, x = m.step(s, s["tokens"], one, S, 1)
+            m.sample(s, x)
+        return [s["table"], s["lens"], s["tokens"], s["probs"], la.sample(logits[i], u, top_k=k)]
+
+    alone = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got = work(i)
+                    with pytest.raises((ValueError, la.LlapisError), match="layout" if i else "workspace"):
+                        if i:
+                            la.qk_rope(torch.zeros(1, 2, 64, device=gpu), pos=i32([0], gpu), freq=models[0].freq, layout=7)
+                        else:
+                            la.sample(logits[i], u, workspace=torch.zeros(8, dtype=torch.uint8, device=gpu))
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, alone[i]))
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
