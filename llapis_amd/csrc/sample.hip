@@ -100,22 +100,27 @@ __device__ __forceinline__ int smp_index(uint64_t key) { return (int)~(uint32_t)
 
 constexpr float SMP_NONE = -__builtin_inff();             // no value: it has no weight
 
-// 2^t for t <= 0: the whole part in the exponent, the rest r by sum (r ln 2)^k / k! to k = 11, whose
-// remainder is 2^-47 of it at r = 1/2.  (The library's exp took half as long again.)
+// 2^t for t <= 0: the whole part in the exponent, the rest r by the polynomial that agrees with 2^r at
+// the 11 Chebyshev nodes of |r| <= 1/2, to 2^-51 of it.  Its coefficients are kept in scalar
+// registers, where a multiply-add reads them: in vector registers each is first copied
 __device__ __forceinline__ double smp_exp2(double t) {
-    constexpr double c[12] = {1.0, 0.69314718055994530942, 0.24022650695910071233, 0.055504108664821579953,
-                              0.0096181291076284771619, 0.0013333558146428443423, 1.5403530393381609954e-4,
-                              1.5252733804059840280e-5, 1.3215486790144309488e-6, 1.0178086009239699728e-7,
-                              7.0549116208011233299e-9, 4.4455382718708114976e-10};
-    const double n = rint(fmax(t, -2000.0)), r = t - n;
-    double y = c[11];
+    constexpr double c[11] = {1.0, 0.69314718055995, 0.24022650695910097, 0.05550410866444772, 0.009618129107606888,
+                              0.0013333558230164974, 0.0001540353044173605, 1.5252657260200837e-05, 1.321544258792169e-06,
+                              1.0208690299958306e-07, 7.072585949269223e-09};
+    const double in = __builtin_fmax(t, -1100.0), n = __builtin_rint(in), r = in - n;
+    double y = c[10];
 #pragma unroll
-    for (int k = 10; k >= 0; --k) y = __builtin_fma(y, r, c[k]);
-    return t > -1100.0 ? __builtin_ldexp(y, (int)n) : 0.0;
+    for (int k = 9; k >= 0; --k) {
+        double ck = c[k];
+        asm("" : "+s"(ck));
+        y = __builtin_fma(y, r, ck);
+    }
+    return __builtin_ldexp(y, (int)n);
 }
+// (a difference with an infinite value, or times an infinite 1 / T, is -inf or NaN: weight 0 unless x is M)
 __device__ __forceinline__ double smp_weight(float x, float top, double octaves) {
-    // (the difference with an infinite M, or times an infinite 1 / T, says nothing)
-    return x == top ? 1.0 : x == SMP_NONE || top == __builtin_inff() ? 0.0 : smp_exp2(((double)x - (double)top) * octaves);
+    const double w = smp_exp2(((double)x - (double)top) * octaves);
+    return x == top ? 1.0 : w;
 }
 // A value's bin below the largest's, the same wherever it is asked for, and never less for a
 // smaller value.  What lies below all bins, or too far for fp32, is in SMP_OUT
@@ -148,6 +153,46 @@ __device__ __forceinline__ void smp_read(const T * row, int base, int n, float (
         for (int j = 0; j < N; ++j) {
             const int i = smp_at<T>(base, j);
             x[j] = i < n ? smp_clean((float)row[i]) : SMP_NONE;
+        }
+    }
+}
+
+// f(first value's index, values) of the segment's vectors one after the other, two of them under way.
+// (All of them at once, a loop over them unrolled: its code takes longer to fetch than to run.  Through
+// LDS: work waits for the last.)
+template <class T, int N, class F>
+__device__ __forceinline__ void smp_stream(const T * row, int base, int n, F f) {
+    constexpr int W = 16 / sizeof(T), C = N / W;
+    typedef typename SmpVec<T>::v V;
+    const bool whole = base + smp_seg(N) <= n;
+    auto fetch = [&](int c) {
+        const int i = smp_at<T>(base, min(c, C - 1) * W);
+        V w;
+        if (whole) {
+            w = *(const V *)(row + i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) w[j] = i + j < n ? row[i + j] : (T)SMP_NONE;
+        }
+        return w;
+    };
+    auto give = [&](int c, const V & w) {
+        float x[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[j] = smp_clean((float)w[j]);
+        f(smp_at<T>(base, c * W), x);
+    };
+    V a = fetch(0);
+    if constexpr (C == 1) {
+        give(0, a);
+    } else {
+        V b = fetch(1);
+#pragma unroll 1
+        for (int c = 0; c < C; c += 2) {
+            give(c, a);
+            a = fetch(c + 2);
+            give(c + 1, b);
+            b = fetch(c + 3);
         }
     }
 }
@@ -297,13 +342,23 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_
     int count = 0;
     uint64_t places = 0;
     const uint32_t * hist = ws.hist + (int64_t)seq * ws.n_chunks * SMP_BINS;
-#pragma unroll 8
-    for (int c = 0; c < ws.n_chunks; ++c) {
-        const float its = chunks[c].top;
-        const int b = tid - smp_bin(its, top, top_bin, s.bins);
-        const uint32_t v = its == SMP_NONE || b < 0 ? 0 : hist[(int64_t)c * SMP_BINS + b];
-        count += (int)(v >> SMP_COUNT_AT);
-        places += v & ((1u << SMP_COUNT_AT) - 1);
+    constexpr int MANY = 16;                               // loads under way, then their use: in the compiler's own order each is waited for
+    for (int c0 = 0; c0 < ws.n_chunks; c0 += MANY) {
+        int b[MANY];
+        uint32_t held[MANY];
+#pragma unroll
+        for (int i = 0; i < MANY; ++i) {
+            const int c = min(c0 + i, ws.n_chunks - 1);
+            b[i] = tid - smp_bin(chunks[c].top, top, top_bin, s.bins);
+            held[i] = hist[(int64_t)c * SMP_BINS + max(b[i], 0)];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < MANY; ++i) {
+            const uint32_t v = b[i] < 0 || c0 + i >= ws.n_chunks ? 0 : held[i];
+            count += (int)(v >> SMP_COUNT_AT);
+            places += v & ((1u << SMP_COUNT_AT) - 1);
+        }
     }
     // the bin's weight: 2^((place - top's place) / 16) lies between 1 + 0.0433 place and 1 + 0.0443
     // place times the bin's, a place between its 32nd and the next.  fp32 has each place to
@@ -346,11 +401,16 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_
     const int of = tid == 0 ? lo - 1 : tid == 1 ? hi : tid == 2 ? (s.by_k ? last - 1 : SMP_BINS - 1) : last;
     uint32_t below = (uint32_t)(smp_key(least, 0) >> 32) - 1, from = (uint32_t)(smp_key(top, 0) >> 32);
     if (tid < 4) {
-        while (from - below > 1) {
-            const uint32_t mid = below + (from - below) / 2;
-            if (smp_bin(smp_value((uint64_t)mid << 32), top, top_bin, s.bins) <= of) from = mid;
-            else below = mid;
-        }
+        auto try_at = [&](uint32_t at) {
+            if (smp_bin(smp_value((uint64_t)at << 32), top, top_bin, s.bins) <= of) from = at;
+            else below = at;
+        };
+        // the quotient is next to it: where it is, 5 steps remain of 32
+        const float near = (top_bin - (float)of) / s.bins;
+        const uint32_t at = (uint32_t)(smp_key(near, 0) >> 32);
+        if (near == near && at - 8 > below && at - 8 < from) try_at(at - 8);
+        if (near == near && at + 8 > below && at + 8 < from) try_at(at + 8);
+        while (from - below > 1) try_at(below + (from - below) / 2);
     }
     if (tid < 64) {
         const float x = of < 0 ? none : smp_value((uint64_t)from << 32);
@@ -367,47 +427,54 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_
 
 template <class T, int N>
 __global__ __launch_bounds__(SMP_WG) void k_sample_split(const llapis_sample_args a, const SmpWs ws) {
-    // the values, which a loop goes through: unrolled, its code takes longer to fetch than to run
-    __shared__ float s_x[N][SMP_WG];
     const int seq = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const SmpSet s = smp_settings(a, seq);
     if (s.greedy) return;
     const int base = blockIdx.x * smp_chunk(N) + wave * smp_seg(N);
-    {
-        float x[N];
-        smp_read((const T *)a.logits + seq * a.logits_stride, base, a.vocab, x);
-#pragma unroll
-        for (int j = 0; j < N; ++j) s_x[j][tid] = x[j];
-    }
     const SmpCut cut = ws.cuts[seq];
     if (cut.token < 0) return;
     SmpSeg g = {0.0, 0.0, 0.0, 0, 0, 0, 0};
     const int64_t seg = ((int64_t)seq * ws.n_chunks + blockIdx.x) * SMP_WAVES + wave;
     uint64_t * list = ws.keys + seg * smp_seg(N);
-#pragma unroll 2
-    for (int j = 0; j < N; ++j) {
-        const float x = s_x[j][tid];
-        const bool sure = x >= cut.x_sure, mid = x >= cut.x_mid && x < cut.x_cand;
-        const bool cand = !sure && x >= cut.x_end && !mid;
-        if (sure || mid) {
-            const double w = smp_weight(x, cut.top, s.octaves);
-            g.sure += sure ? w : 0.0;
-            g.draw += sure && w >= s.min_p ? w : 0.0;
-            g.mid += sure ? 0.0 : w;
-            g.n_sure += sure;
-            g.n_mid += !sure;
+    smp_stream<T, N>((const T *)a.logits + seq * a.logits_stride, base, a.vocab, [&](int at, const auto & x) {
+        constexpr int W = 16 / sizeof(T);
+#pragma unroll
+        for (int j0 = 0; j0 < W; j0 += 2) {                // (the two chains of multiply-adds overlap)
+            bool sure[2], mid[2], cand[2];
+            uint64_t any = 0;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float y = x[j0 + j];
+                sure[j] = y >= cut.x_sure;
+                mid[j] = !sure[j] && y >= cut.x_mid && y < cut.x_cand;
+                cand[j] = !sure[j] && y >= cut.x_end && !mid[j];
+                const uint64_t n_sure = __ballot(sure[j]), n_mid = __ballot(mid[j]);
+                g.n_sure += __popcll(n_sure);
+                g.n_mid += __popcll(n_mid);
+                any |= n_sure | n_mid;
+            }
+            if (any) {
+                double w[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) w[j] = smp_weight(x[j0 + j], cut.top, s.octaves);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    g.sure += sure[j] ? w[j] : 0.0;
+                    g.draw += sure[j] && w[j] >= s.min_p ? w[j] : 0.0;
+                    g.mid += mid[j] ? w[j] : 0.0;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint64_t votes = __ballot(cand[j]);
+                if (cand[j]) list[g.n_cand + __popcll(votes & ((1ull << lane) - 1))] = smp_key(x[j0 + j], at + j0 + j);
+                g.n_cand += __popcll(votes);
+            }
         }
-        const uint64_t votes = __ballot(cand);
-        if (votes) {
-            if (cand) list[g.n_cand + __popcll(votes & ((1ull << lane) - 1))] = smp_key(x, smp_at<T>(base, j));
-            g.n_cand += __popcll(votes);
-        }
-    }
+    });
     g.sure = smp_wave(g.sure, SmpAdd());
     g.draw = smp_wave(g.draw, SmpAdd());
     g.mid = smp_wave(g.mid, SmpAdd());
-    g.n_sure = smp_wave(g.n_sure, SmpAdd());
-    g.n_mid = smp_wave(g.n_mid, SmpAdd());
     if (lane == 63) ws.segs[seg] = g;
 }
 
@@ -421,7 +488,8 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_pick(const llapis_sample_
     __shared__ uint64_t s_mass[WAVES];
     __shared__ int s_first[SMP_HELD + 1], s_bucket_n[WG], s_list_n, s_found, s_last;
     __shared__ unsigned long long s_bucket[WG], s_kept[SMP_HELD], s_weigh[256], s_all_k;
-    __shared__ uint64_t s_list[SMP_LIST], s_key;
+    __shared__ uint64_t s_list[SMP_LIST], s_list_w[SMP_LIST], s_key;
+    __shared__ unsigned long long s_upto[SMP_LIST];
     __shared__ struct { int bucket, before, n; uint64_t mass; } s_sel;
     __shared__ double s_before;
     const int seq = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -561,27 +629,39 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_pick(const llapis_sample_
                     break;
                 }
 #pragma unroll
-                for (int e = 0; e < HOLD; ++e)
-                    if (bucket[e] == s_sel.bucket) s_list[atomicAdd(&s_list_n, 1)] = k[e];
+                for (int e = 0; e < HOLD; ++e) {
+                    if (bucket[e] == s_sel.bucket) {
+                        const int i = atomicAdd(&s_list_n, 1);
+                        s_list[i] = k[e];
+                        s_list_w[i] = w[e];
+                        s_upto[i] = 0;
+                    }
+                }
+                __syncthreads();
+                // a key's rank in the list, or the mass of it and those above it: the list in parts, as many as there are threads for
+                const int slots = (n + 63) & ~63, parts = WG / slots, part = tid / slots, at = tid - part * slots;
+                if (at < n && part < parts) {
+                    const uint64_t u = s_list[at];
+                    uint64_t upto = 0;
+                    if (pass == 0) {
+#pragma unroll 4
+                        for (int i = part; i < n; i += parts) upto += s_list[i] >= u;
+                    } else {
+#pragma unroll 4
+                        for (int i = part; i < n; i += parts) upto += s_list[i] >= u ? s_list_w[i] : 0;
+                    }
+                    atomicAdd(&s_upto[at], (unsigned long long)upto);
+                }
                 __syncthreads();
                 if (tid < n) {
-                    // the list's keys that are not below this thread's
-                    const uint64_t u = s_list[tid];
-                    int rank = 0;
-                    uint64_t upto = 0;
-                    const uint64_t own_mass = (uint64_t)(weight(u) * scale);
+                    const uint64_t mass = s_list_w[tid], upto = s_upto[tid];
                     if (pass == 0) {
-                        for (int i = 0; i < n; ++i) rank += s_list[i] >= u;
-                        if (s_sel.before + rank <= n_k) atomicAdd(&s_all_k, own_mass);
-                        if (s_sel.before + rank == n_k) s_key = u;
+                        const int rank = s_sel.before + (int)upto;
+                        if (rank <= n_k) atomicAdd(&s_all_k, (unsigned long long)mass);
+                        if (rank == n_k) s_key = s_list[tid];
                     } else {
-                        for (int i = 0; i < n; ++i) {
-                            const uint64_t v = s_list[i];
-                            // (equal values have equal weights: most buckets hold one)
-                            upto += v >= u ? (v >> 32 == u >> 32 ? own_mass : (uint64_t)(weight(v) * scale)) : 0;
-                        }
                         const uint64_t g = goal > s_sel.mass ? goal - s_sel.mass : 0;
-                        if (upto >= g && (upto - own_mass < g || upto == own_mass)) s_key = u;
+                        if (upto >= g && (upto - mass < g || upto == mass)) s_key = s_list[tid];
                     }
                 }
                 __syncthreads();
@@ -764,48 +844,41 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_pick(const llapis_sample_
 
 template <class T, int N>
 __global__ __launch_bounds__(SMP_WG) void k_sample_probs(const llapis_sample_args a, const SmpWs ws) {
-    __shared__ float s_x[N][SMP_WG];                       // values, then probabilities
     const int seq = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
     const SmpSet s = smp_settings(a, seq);
     const int base = blockIdx.x * smp_chunk(N) + wave * smp_seg(N);
     if (base >= a.vocab) return;
-    {
-        float x[N];
-        smp_read((const T *)a.logits + seq * a.logits_stride, base, a.vocab, x);
-#pragma unroll
-        for (int j = 0; j < N; ++j) s_x[j][tid] = x[j];
-    }
     const SmpCut cut = ws.cuts[seq];
     const double inv = 1.0 / cut.total;
-#pragma unroll 2
-    for (int j = 0; j < N; ++j) {
-        const float x = s_x[j][tid];
-        const int i = smp_at<T>(base, j);
-        float p = 0.0f;
-        if (s.greedy) {
-            p = i == cut.token ? 1.0f : 0.0f;
-        } else if (x >= cut.x_sure || (x >= cut.x_end && !(x >= cut.x_mid && x < cut.x_cand) && smp_key(x, i) >= cut.key)) {
-            const double w = smp_weight(x, cut.top, s.octaves);
-            p = w >= s.min_p ? (float)(w * inv) : 0.0f;
-        }
-        s_x[j][tid] = p;
-    }
     T * out = (T *)a.probs + seq * a.probs_stride;
-    constexpr int W = 16 / sizeof(T);
+    smp_stream<T, N>((const T *)a.logits + seq * a.logits_stride, base, a.vocab, [&](int at, const auto & x) {
+        constexpr int W = 16 / sizeof(T);
+        typename SmpVec<T>::v p;
 #pragma unroll
-    for (int c = 0; c < N / W; ++c) {
-        const int i = smp_at<T>(base, c * W);
-        typename SmpVec<T>::v w;
+        for (int j0 = 0; j0 < W; j0 += 2) {
+            bool keep[2];
 #pragma unroll
-        for (int j = 0; j < W; ++j) w[j] = (T)s_x[c * W + j][tid];
-        if (i + W <= a.vocab) {
-            *(typename SmpVec<T>::v *)(out + i) = w;
+            for (int j = 0; j < 2; ++j) {
+                const float y = x[j0 + j];
+                keep[j] = !s.greedy && (y >= cut.x_sure || (y >= cut.x_end && !(y >= cut.x_mid && y < cut.x_cand) && smp_key(y, at + j0 + j) >= cut.key));
+                p[j0 + j] = (T)(s.greedy && at + j0 + j == cut.token ? 1.0f : 0.0f);
+            }
+            if (__ballot(keep[0] || keep[1])) {
+                double w[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) w[j] = smp_weight(x[j0 + j], cut.top, s.octaves);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) p[j0 + j] = keep[j] && w[j] >= s.min_p ? (T)(float)(w[j] * inv) : p[j0 + j];
+            }
+        }
+        if (at + W <= a.vocab) {
+            *(typename SmpVec<T>::v *)(out + at) = p;
         } else {
 #pragma unroll
             for (int j = 0; j < W; ++j)
-                if (i + j < a.vocab) out[i + j] = w[j];
+                if (at + j < a.vocab) out[at + j] = p[j];
         }
-    }
+    });
 }
 
 }  // namespace dev
