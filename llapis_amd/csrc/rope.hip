@@ -18,7 +18,9 @@ namespace dev {
 // consecutive ones), reads them once, adds the squares over the head's L lanes and
 // writes them.
 //
-// Bound by memory for prompts, by the launch and one load's chain for a step.
+// Bound by memory for prompts (8192 tokens of 40 heads of 128 bf16: 168 MB in 40 us, 4.2 TB/s
+// where a large copy reaches 5.1), by the launch and one load's chain for a step (4 tokens of 24 heads of
+// 256: 3.7 us).
 constexpr int ROPE_WG = 256, ROPE_TABLE = 1024;      // pairs of a workgroup's tokens in LDS
 
 struct Rope {
@@ -169,10 +171,13 @@ hipError_t launch_rope_as(const llapis_qk_rope_args & a, hipStream_t s) {
     Rope p{a, 0, 0, 1};
     p.slots = (a.head_dim + 2 * V - 1) / (2 * V);
     while (p.lanes_log2 < 6 && (E << p.lanes_log2) < p.slots) ++p.lanes_log2;
-    // many tokens: four to a workgroup, whose heads fill its places; few: their heads over several
+    // Four tokens to a workgroup where their heads leave it places (8192 tokens of 6 heads of 64: 5.5 us, one token
+    // each 8.9) or the tokens are many; else a token's heads over several (2048 tokens of 40 heads of 128 bf16: 10.3 us, four
+    // tokens each 12.4; 4096: 16.8 and 16.7; 8192: 29.6 and 28.6)
     const int places = ROPE_WG >> p.lanes_log2, heads = a.n_head + a.n_kv, most = a.rot_dim ? ROPE_TABLE / (a.rot_dim / 2) : 4;
-    if (a.n_tokens >= 2048) p.each = std::min(4, most);
-    const int parts = a.n_tokens >= 2048 ? 1 : std::min((heads + places - 1) / places, 65535);
+    const bool four = 4 * heads <= places || a.n_tokens >= 4096;
+    if (four) p.each = std::min(4, most);
+    const int parts = four ? 1 : std::min((heads + places - 1) / places, 65535);
     hipLaunchKernelGGL((k_qk_rope<T, V, E>), dim3((a.n_tokens - 1) / p.each + 1, parts), dim3(ROPE_WG), 0, s, p);
     return hipGetLastError();
 }

@@ -897,9 +897,12 @@ int32_t refuse_sample(const char * why) noexcept {
 
 uint64_t round_up(uint64_t n) { return (n + 255) / 256 * 256; }
 
-// values of a lane: 8 where a call's rows leave most of the card without work at 32
-constexpr int64_t SMP_SHORT = 1 << 20;
-bool short_rows(int n_seq, int vocab) { return (int64_t)n_seq * vocab <= SMP_SHORT; }
+// Values of a lane: 8 where a call's rows leave most of the card without work at 32 (1 row of 32003: 23 us, at 32
+// values 32; 64 rows: 31 and 36), but k_sample_find adds four times the histograms then (16 rows of 128001: 37 us and
+// 34; 8 of 262144: 51 and 39)
+constexpr int SMP_SHORT = 1 << 16;
+constexpr int64_t SMP_SHORT_ALL = 1 << 21;
+bool short_rows(int n_seq, int vocab) { return vocab <= SMP_SHORT && (int64_t)n_seq * vocab <= SMP_SHORT_ALL; }
 
 // the workspace's parts for `chunks` chunks of n_seq sequences; its size
 uint64_t sample_parts(uint64_t n_seq, uint64_t chunks, int lane_values, uint8_t * at, SmpWs & ws) {
@@ -922,7 +925,7 @@ int chunks_of(int vocab, int lane_values) { return (vocab + smp_chunk(lane_value
 // ... of the long chunks, and of the most short ones that a call of no more sequences and values has
 uint64_t sample_bytes(int n_seq, int vocab) {
     SmpWs ws;
-    const uint64_t few = std::min<uint64_t>((uint64_t)n_seq * chunks_of(vocab, 8), SMP_SHORT / smp_chunk(8) + n_seq);
+    const uint64_t few = std::min<uint64_t>((uint64_t)n_seq * chunks_of(std::min(vocab, SMP_SHORT), 8), SMP_SHORT_ALL / smp_chunk(8) + n_seq);
     return std::max(sample_parts(n_seq, (uint64_t)n_seq * chunks_of(vocab, 32), 32, nullptr, ws), sample_parts(n_seq, few, 8, nullptr, ws));
 }
 

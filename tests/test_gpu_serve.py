@@ -78,7 +78,7 @@ def test_extend(gpu, S, width, P, new, spare, in_place):
         run_extend(gpu, P, table, lens, n_new, free, n, n_tokens, in_place)
 
 
-@pytest.mark.parametrize("n_tokens", [4095, 4096, 4097, 30000])
+@pytest.mark.parametrize("n_tokens", [1023, 1024, 1025, 4095, 4096, 4097, 30000])
 def test_extend_prompts(gpu, n_tokens):
     """Prompt chunks: many rows and pages a sequence, on either side of the rows that one workgroup fills."""
     want = run_extend(gpu, 16, [[-1] * 700 for _ in range(9)], [0, 5, 16, 17, 0, 300, 0, 1, 33][:9],
@@ -281,6 +281,13 @@ def test_sample(gpu, tag, V):
 def test_sample_large(gpu, S):
     x, u = logits_of(S, S, 262144, la.F32, 2.2)
     run_sample(gpu, x, u, [1.0] * S, [64 * (i % 3) for i in range(S)], [(0.9, 0.99, 1.0)[i % 3 - 1] for i in range(S)], None)
+
+
+@pytest.mark.parametrize("S,V", [(32, 65536), (33, 65536), (32, 65537), (1, 2097152), (2, 2100001)])
+def test_sample_borders(gpu, S, V):
+    """Either side of the rows that go to more workgroups, and of the segments that a thread has one of."""
+    x, u = logits_of(V + S, S, V, la.BF16, 2.2)
+    run_sample(gpu, x, u, None, [(50, 0, 1000)[i % 3] for i in range(S)], [(0.9, 0.99)[i % 2] for i in range(S)], [(0.0, 0.01)[i % 2] for i in range(S)])
 
 
 @pytest.mark.parametrize("V,k,p", [(20000, 7000, 1.0), (20000, 0, 0.4), (20000, 9000, 0.5), (5000, 4999, 0.999), (70000, 69999, 0.7),
