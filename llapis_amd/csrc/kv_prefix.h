@@ -11,15 +11,25 @@
 // rows from the prefix's end on.
 //
 // A unit's K and V are staged in LDS once for all rows, eight waves with 16 or 32 rows
-// each: loaded into registers while the unit before it is computed, written to the other
-// half of LDS behind it, one barrier a unit.  A wave forms S^T = K Q^T for its rows with
-// Q^T in registers, keeps maximum, sum and P in its lanes, and adds O^T += V^T P^T: K's rows lie in
-// LDS in the order that makes a lane's scores those of 8 consecutive keys, P's operand.
-// Rows of LDS are 16 bytes longer than their values, so that 16 rows' reads of a column
-// meet every bank once.
+// each (four of 16 at head size 512).  A wave forms S^T = K Q^T for its rows with Q^T in registers,
+// keeps maximum, sum and P in its lanes, and adds O^T += V^T P^T: K's rows lie in LDS in the order that
+// makes a lane's scores those of 8 consecutive keys, P's operand.  Rows of LDS are 16 bytes longer than their
+// values, so that 16 rows' reads of a column meet every bank once.
 //
-// Rounding is kv_attn.h's: fp32 scores, maxima and sums, 16-bit parts of q and p; q8_0
-// values are staged as an fp16 value and its exact remainder.
+// Bound by the issue of matrix and vector instructions, not by memory: 64 sequences of 32 heads of 128
+// behind 32768 tokens, bf16, are 34 GFLOP (52 with P in two parts) and 134 MB, and take 77 us, 446 TFLOP/s.  What
+// carries it, with what it measured there (the whole call):
+//  - the workgroup's two halves work half a unit apart, one at products while the other forms P and
+//    stages, so that a SIMD's matrix cores and VALU work at once: 142 to 119 us with the next two
+//  - sums are products with ones, P is split in two instructions a pair (split_p), and sums and output are scaled anew
+//    only when a row's maximum grows by more than P_SLACK
+//  - loads from memory stay in flight over barriers, and none is under a condition, which would have all of them waited for
+//  - a second tile of a wave's rows where the registers hold it: 64 sequences of 4 rows a kv head 91 us, with
+//    one tile 106; 16 sequences, whose 64 rows one tile holds, 61 us, with two 72
+// One part of P would take 10 us off and add 2^-9 to the error of its weights: it keeps kv_attn.h's instead.
+//
+// Rounding is kv_attn.h's: fp32 scores, maxima and sums, 16-bit parts of q and p (parts that are cut
+// off, not rounded, but for the last: the same sum); q8_0 values are staged as an fp16 value and its exact remainder.
 #pragma once
 
 #include "kv_attn.h"
@@ -625,7 +635,6 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
         barrier();
     }
     for (;; ++unit) {
-        if (TWO) __builtin_amdgcn_s_setprio(1);
         if (unit > 0 && busy) products(lds_v + ((unit - 1) % BUFS) * PARTS * VB);
         if (i == 0 && unit > 0) {
             write(past);
@@ -641,7 +650,6 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
 #pragma unroll
                 for (int j = 0; j < NK; ++j) sc[nt][j] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        if (TWO) __builtin_amdgcn_s_setprio(0);
         barrier();
         if (busy) {
             softmax(second ? missing[2] : missing[1]);

@@ -18,6 +18,11 @@
 // bins are looked at.  What decides is fp64 (and fixed point of 49 bits, where sums are
 // made by atomics): weights, their sums and products, in a fixed order, so that a draw next to a
 // border falls as the definition says.
+//
+// Bound, for few rows, by the four launches and a workgroup's barriers (1 row of 32003 fp32 values: 3.9, 6.5, 4.0 and
+// 9.1 us); for many by two passes over the logits (32 rows of 262144, 33.5 MB: 11.5 and 13.9 us, the sequences' kernels
+// 9.5 and 13.8), the second of which forms every kept value's weight in fp64: with top_p alone that is
+// most of them (64 rows of 128001 bf16: 10.1, 8.7, 18.4 and 13.4 us, probabilities 19.7).
 #include <algorithm>
 #include <cstdio>
 #include <type_traits>
