@@ -40,7 +40,7 @@ constexpr int smp_seg(int lane_values) { return 64 * lane_values; }
 constexpr int smp_chunk(int lane_values) { return SMP_WG * lane_values; }
 constexpr int SMP_BINS = 1024, SMP_OUT = SMP_BINS + 1;    // a value below all bins is in SMP_OUT
 constexpr float SMP_PER_OCTAVE = 16.0f;
-constexpr int SMP_FEW = 4096, SMP_HELD = 1024;            // candidates, and segments, that are held at once
+constexpr int SMP_FEW = 8192, SMP_HELD = 1024;            // candidates, and segments, that are held at once
 constexpr int SMP_LIST = 512;                             // candidates of a bucket that are ordered one by one
 // a histogram's word: the number of values above 18 bits of the sum of their places
 constexpr int SMP_COUNT_AT = 18;

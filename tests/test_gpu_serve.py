@@ -290,6 +290,13 @@ def test_sample_borders(gpu, S, V):
     run_sample(gpu, x, u, None, [(50, 0, 1000)[i % 3] for i in range(S)], [(0.9, 0.99)[i % 2] for i in range(S)], [(0.0, 0.01)[i % 2] for i in range(S)])
 
 
+@pytest.mark.parametrize("V", [700, 3001, 6000, 8192, 8193, 30000])
+def test_sample_flat(gpu, V):
+    """Values so near each other that all may be the last kept: candidates up to what is held at once, and more."""
+    x = 0.03 * torch.rand(4, V, generator=torch.Generator().manual_seed(V))
+    run_sample(gpu, x, [0.3, 0.999, 0.5, 0.0], None, [0, V // 3, V // 3, 1], [0.5, 1.0, 0.7, 0.5], [0.0, 0.0, 0.985, 0.0])
+
+
 @pytest.mark.parametrize("V,k,p", [(20000, 7000, 1.0), (20000, 0, 0.4), (20000, 9000, 0.5), (5000, 4999, 0.999), (70000, 69999, 0.7),
                                    (4096, 100, 0.5), (4097, 4000, 0.9)])
 def test_sample_ties(gpu, V, k, p):
