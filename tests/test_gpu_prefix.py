@@ -4,7 +4,8 @@ the plain 64-bit form of attention (step_ref.py), which reads every sequence's o
 The bound is step_ref.attention's.  What the prefix adds to its error: the weight of a
 sequence's own keys comes from the logarithm of their sum, rounded twice, 2^-23 |lse| of it, and |lse| is
 at most the largest score and the logarithm of their number: within the bound's 2^-22
-(|s| + |m|) and its 2^-21."""
+(|s| + |m|) and its 2^-21.  (Of a probability's two BF16 parts the first is cut off, not rounded: the sum is off by 2^-16
+of it at most where the bound counts 2^-17, and is held to that bound all the same.)"""
 import math
 
 import pytest
