@@ -976,6 +976,7 @@ int32_t llapis_sample(const llapis_sample_args * a, void * workspace, uint64_t w
         return refuse_sample("need 0 <= n_seq <= 65535, 0 < vocab <= 2^30");
     if (a->n_seq == 0) return 0;
     if (!a->logits || !a->u || !a->tokens) return refuse_sample("null logits, u or tokens");
+    if (a->probs == a->logits) return refuse_sample("probs may not be the logits");
     if (a->n_seq > 1 && (a->logits_stride < a->vocab || (a->probs && a->probs_stride < a->vocab)))
         return refuse_sample("rows shorter than vocab");
     if (!workspace || ((uintptr_t)workspace & 15) || ws_bytes < llapis_sample_workspace_size(a->n_seq, a->vocab))

@@ -260,6 +260,23 @@ def test_out_of_order(gpu):
     s.check(q.cpu())
 
 
+def test_beyond_32_bits(gpu):
+    """Pages past 4 GiB of a pool (strides apart, so that little memory is written)."""
+    D, H, P = 64, 1, 16
+    s = Shared(gpu, 27, la.F16, D, H, P, [(64, [(5, 1), (20, 2)])], la.F32, spare=0)
+    n_pages, gap = s.cache.n_pages, 1 << 28                       # values between pages: 512 MiB
+    pool = [torch.empty((n_pages - 1) * gap + H * P * D, dtype=torch.float16, device=gpu) for _ in range(2)]
+    k = pool[0].as_strided((n_pages, H, P, D), (gap, P * D, D, 1))
+    v = pool[1].as_strided((n_pages, H, D, P), (gap, P * D, P, 1))
+    for t, src in ((k, s.cache.k), (v, s.cache.v)):
+        for i in range(n_pages):
+            t[i] = src[i]
+    q = s.queries(28, 2).to(gpu)
+    assert torch.equal(la.KvCache(k, v).prefix_attention(s.batch, q, s.groups, s.prefix), s.cache.prefix_attention(s.batch, q, s.groups, s.prefix))
+    del pool, k, v
+    torch.cuda.empty_cache()
+
+
 def test_repeats_and_graphs(gpu):
     """Two captured graphs with one workspace, replayed in turn as the lengths and the prefix
     change, equal to eager calls bit for bit; a call on another stream."""

@@ -188,6 +188,19 @@ def test_rope_rows_left(gpu):
     assert torch.equal(dx[[0, 2, 4]], out[[0, 2, 4]]) and torch.isnan(dx[1]).all() and torch.isinf(dx[3]).all()
 
 
+@pytest.mark.parametrize("T", [3, 4097])
+@pytest.mark.parametrize("tag,D,rot,half", [(la.F32, 128, 128, True), (la.BF16, 128, 64, False), (la.F16, 80, 20, True), (la.BF16, 96, 24, False)])
+def test_rope_in_place(gpu, tag, D, rot, half, T):
+    """Queries and keys of a fused projection where they lie: as elsewhere bit for bit, values as they were."""
+    qkv = torch.randn(T, 3 + 2 + 2, D, generator=torch.Generator().manual_seed(D + T)).to(DT[tag]).to(gpu)
+    freq, _ = la.rope_frequencies(rot, device=gpu)
+    pos, layout = torch.arange(7, T + 7, dtype=torch.int32, device=gpu), la.ROPE_HALF if half else la.ROPE_PAIRS
+    q, k, v = qkv[:, :3], qkv[:, 3:5], qkv[:, 5:].clone()
+    want = la.qk_rope(q, k, pos, freq, layout=layout)
+    la.qk_rope(q, k, pos, freq, layout=layout, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(qkv[:, 5:], v)
+
+
 def test_rope_norms(gpu):
     """Without weights, rows of zeros, a large eps, values whose squares are small; norms alone without positions."""
     run_rope(gpu, 4, 4, 2, 1, 128, 128, True, la.F32, True, weights=False)

@@ -134,13 +134,13 @@ def test_rope_of_nothing():
 # -------------------------------------------------------------- sample
 
 def sample_args(**kw):
-    a = dict(type=la.F32, n_seq=2, vocab=100, logits=P, logits_stride=100, u=P, tokens=P, probs=P, probs_stride=100)
+    a = dict(type=la.F32, n_seq=2, vocab=100, logits=P, logits_stride=100, u=P, tokens=P, probs=2 * P, probs_stride=100)
     a.update(kw)
     return _lib.LlapisSampleArgs(**a)
 
 
 @pytest.mark.parametrize("bad", [dict(type=la.Q8_0), dict(n_seq=-1), dict(n_seq=65536), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(logits=None),
-                                 dict(u=None), dict(tokens=None), dict(logits_stride=99), dict(probs_stride=99)], ids=str)
+                                 dict(u=None), dict(tokens=None), dict(logits_stride=99), dict(probs_stride=99), dict(probs=P)], ids=str)
 def test_sample_refusals(bad):
     a = sample_args(**bad)
     refused(la.lib().llapis_sample(C.byref(a), P, 1 << 50, None), "llapis_sample")
