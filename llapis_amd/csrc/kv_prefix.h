@@ -17,7 +17,7 @@
 // values, so that 16 rows' reads of a column meet every bank once.
 //
 // Bound by the issue of matrix and vector instructions, not by memory: 64 sequences of 32 heads of 128
-// behind 32768 tokens, bf16, are 34 GFLOP (52 with P in two parts) and 134 MB, and take 77 us, 446 TFLOP/s.  What
+// behind 32768 tokens, bf16, are 34 GFLOP (52 with P in two parts) and 134 MB, and take 74 us, 465 TFLOP/s.  What
 // carries it, with what it measured there (the whole call):
 //  - the workgroup's two halves work half a unit apart, one at products while the other forms P and
 //    stages, so that a SIMD's matrix cores and VALU work at once: 142 to 119 us with the next two
@@ -95,6 +95,10 @@ struct KvpShape {
     static constexpr int UNIT = kvp_unit(Q8, HD), NB = UNIT / 32, NK = UNIT / 16, NC = HD / 32, NV = HD / 16;
     static constexpr int KP = 2 * HD + 16, VP = 2 * UNIT + 16;           // bytes from a row of LDS to the next
     static constexpr bool TWO = WAVES == 8;                              // groups of waves
+    // Where a unit's loads are issued: before its products, where these are the shorter half of its work (64 sequences
+    // behind 32768 tokens, bf16: 77.5 to 73.6 us; fp32 queries over fp16 1 to 2 % of a call), else behind the
+    // stores (Q8_0, 48 sequences: 122 us a call and 126; three parts of q at head size 256: 77 and 84)
+    static constexpr bool LATE = !Q8 && PQ <= 2;
     static constexpr int BUFS = TWO ? 2 : 1, PARTS = Q8 ? 2 : 1;         // units in LDS; q8_0: values and remainders
     static constexpr int KB = UNIT * KP, VB = HD * VP;                   // bytes of a part of K, of V
     static constexpr int LDS = BUFS * PARTS * (KB + VB);
@@ -424,6 +428,14 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
         k_ok = next_ok;
         v_page = next_v;
     };
+    constexpr bool LATE = Sh::LATE;
+    auto load = [&]() {
+        load_v(k_unit, v_page);
+        v_ok = has_page(v_page);
+        load_next_k();
+        ask();
+        if (LATE) __builtin_amdgcn_sched_barrier(0);
+    };
     auto stage = [&](bool with_v) {
         take_pages();
         __builtin_amdgcn_sched_barrier(0);
@@ -434,10 +446,7 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
             v_buf = (v_buf + 1) % BUFS;
         }
         __builtin_amdgcn_sched_barrier(0);
-        load_v(k_unit, v_page);
-        v_ok = has_page(v_page);
-        load_next_k();
-        ask();
+        if constexpr (!LATE) load();
     };
     // LDS is written and read as barriers order it; loads from memory stay in flight
     auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
@@ -631,10 +640,12 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     stage(false);
     barrier();
     if (second) {
+        if constexpr (LATE) load();
         stage(true);
         barrier();
     }
     for (;; ++unit) {
+        if constexpr (LATE) load();
         if (unit > 0 && busy) products(lds_v + ((unit - 1) % BUFS) * PARTS * VB);
         if (i == 0 && unit > 0) {
             write(past);
