@@ -40,8 +40,7 @@ constexpr int smp_seg(int lane_values) { return 64 * lane_values; }
 constexpr int smp_chunk(int lane_values) { return SMP_WG * lane_values; }
 constexpr int SMP_BINS = 1024, SMP_OUT = SMP_BINS + 1;    // a value below all bins is in SMP_OUT
 constexpr float SMP_PER_OCTAVE = 16.0f;
-constexpr int SMP_FEW = 8192, SMP_HELD = 1024;            // candidates, and segments, that are held at once
-constexpr int SMP_LIST = 512;                             // candidates of a bucket that are ordered one by one
+constexpr int SMP_HOLD = 8;                               // candidates of a thread, held at once
 // a histogram's word: the number of values above 18 bits of the sum of their places
 constexpr int SMP_COUNT_AT = 18;
 static_assert(smp_chunk(32) * 31 < 1 << SMP_COUNT_AT && smp_chunk(32) >> (32 - SMP_COUNT_AT) == 0, "a chunk's values fit in a word");
@@ -485,16 +484,19 @@ __global__ __launch_bounds__(SMP_WG) void k_sample_split(const llapis_sample_arg
 
 // ---------------------------------------------------------------- pick
 
+// short rows, whose barriers are what it costs, take fewer waves
+constexpr int smp_pick_wg(int lane_values) { return lane_values < 32 ? 256 : 1024; }
+
 template <class T, int N>
-__global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_pick(const llapis_sample_args a, const SmpWs ws) {
-    constexpr int WG = SMP_SEQ_WG, WAVES = SMP_SEQ_WAVES, SEG = smp_seg(N), HOLD = SMP_FEW / WG;
+__global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sample_args a, const SmpWs ws) {
+    constexpr int WG = smp_pick_wg(N), WAVES = WG / 64, SEG = smp_seg(N), HOLD = SMP_HOLD, FEW = HOLD * WG, LIST = WG;
     __shared__ double s_sure[WAVES], s_mid[WAVES], s_sum[2][WAVES];
     __shared__ int s_n[3][WAVES], s_count[WAVES], s_digit[256];
     __shared__ uint64_t s_mass[WAVES];
-    __shared__ int s_first[SMP_HELD + 1], s_bucket_n[WG], s_list_n, s_found, s_last;
-    __shared__ unsigned long long s_bucket[WG], s_kept[SMP_HELD], s_weigh[256], s_all_k;
-    __shared__ uint64_t s_list[SMP_LIST], s_list_w[SMP_LIST], s_key;
-    __shared__ unsigned long long s_upto[SMP_LIST];
+    __shared__ int s_first[WG + 1], s_bucket_n[WG], s_list_n, s_found, s_last;
+    __shared__ unsigned long long s_bucket[WG], s_kept[WG], s_weigh[256], s_all_k;
+    __shared__ uint64_t s_list[LIST], s_list_w[LIST], s_key;
+    __shared__ unsigned long long s_upto[LIST];
     __shared__ struct { int bucket, before, n; uint64_t mass; } s_sel;
     __shared__ double s_before;
     const int seq = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -547,7 +549,7 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_pick(const llapis_sample_
         mid = smp_all<WAVES>(s_mid, SmpAdd());
         // candidates within top_k, the first of them in order
         const int n_k = s.by_k ? max(min(s.k - n_sure - n_mid, n_cand), 0) : n_cand;
-        bool few = n_cand <= SMP_FEW && per == 1;
+        bool few = n_cand <= FEW && per == 1;
         if (few) {
             // ---- the candidates in registers, and in buckets by value, thread b's the b-th from above.
             // Weights are whole numbers of 2^-49 of the largest that a candidate may have
@@ -629,7 +631,7 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_pick(const llapis_sample_
                 __syncthreads();
                 if (s_sel.bucket < 0) break;               // the weight of all is not top_p's part by a rounding: all are kept
                 const int n = s_sel.n;
-                if (n > SMP_LIST) {
+                if (n > LIST) {
                     few = false;
                     break;
                 }
@@ -939,7 +941,7 @@ hipError_t launch_sample(const llapis_sample_args & a, void * workspace, hipStre
     SmpWs ws;
     ws.n_chunks = chunks_of(a.vocab, N);
     sample_parts(a.n_seq, (uint64_t)a.n_seq * ws.n_chunks, N, (uint8_t *)workspace, ws);
-    const dim3 grid(ws.n_chunks, a.n_seq), wg(SMP_WG), each(a.n_seq), seq_wg(SMP_SEQ_WG);
+    const dim3 grid(ws.n_chunks, a.n_seq), wg(SMP_WG), each(a.n_seq), seq_wg(SMP_SEQ_WG), pick_wg(smp_pick_wg(N));
     hipError_t e;
     hipLaunchKernelGGL((k_sample_scan<T, N>), grid, wg, 0, s, a, ws);
     if ((e = hipGetLastError()) != hipSuccess) return e;
@@ -947,7 +949,7 @@ hipError_t launch_sample(const llapis_sample_args & a, void * workspace, hipStre
     if ((e = hipGetLastError()) != hipSuccess) return e;
     hipLaunchKernelGGL((k_sample_split<T, N>), grid, wg, 0, s, a, ws);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((k_sample_pick<T, N>), each, seq_wg, 0, s, a, ws);
+    hipLaunchKernelGGL((k_sample_pick<T, N>), each, pick_wg, 0, s, a, ws);
     if ((e = hipGetLastError()) != hipSuccess || !a.probs) return e;
     hipLaunchKernelGGL((k_sample_probs<T, N>), grid, wg, 0, s, a, ws);
     return hipGetLastError();
