@@ -12,10 +12,11 @@
 //                   between only count towards top_p's whole (summed), the candidates are listed
 //   k_sample_pick   a workgroup a sequence ends both filters among the candidates exactly
 //                   and finds the token: its segment by the segments' sums, then the value
-// and k_sample_probs writes probabilities if they are wanted.  A histogram's word holds a
-// bin's number of values and the sum of their places in it, in 32nds: a weight is 2^(place / 16)
-// times the bin's, so that both bound the bin's weight to 0.3 %.  They only say which
-// bins are looked at.  What decides is fp64 (and fixed point of 49 bits, where sums are
+// and k_sample_probs writes probabilities if they are wanted.  A histogram's word holds the
+// sum of a bin's weights, in 2^-18 of the bin's least: all of it to 2^-15, and the number of its values
+// to 4 % (for top_k alone it holds their number).  They only say which bins are looked at: mostly one for
+// each filter.  (Words of numbers and of coarse weights, to 0.3 %, had ten times the candidates at a top_p of 0.99, where they
+// did not fit: 8 rows of 65536 230 us.)  What decides is fp64 (and fixed point of 49 bits, where sums are
 // made by atomics): weights, their sums and products, in a fixed order, so that a draw next to a
 // border falls as the definition says.
 //
@@ -41,9 +42,9 @@ constexpr int smp_chunk(int lane_values) { return SMP_WG * lane_values; }
 constexpr int SMP_BINS = 1024, SMP_OUT = SMP_BINS + 1;    // a value below all bins is in SMP_OUT
 constexpr float SMP_PER_OCTAVE = 16.0f;
 constexpr int SMP_HOLD = 8;                               // candidates of a thread, held at once
-// a histogram's word: the number of values above 18 bits of the sum of their places
-constexpr int SMP_COUNT_AT = 18;
-static_assert(smp_chunk(32) * 31 < 1 << SMP_COUNT_AT && smp_chunk(32) >> (32 - SMP_COUNT_AT) == 0, "a chunk's values fit in a word");
+// a weight in a histogram's word, the least and the most of a bin: 2^18 to 2^(18 + 1 / 16)
+constexpr uint32_t SMP_LEAST = 1 << 18, SMP_MOST = 273750;
+static_assert((uint64_t)smp_chunk(32) * SMP_MOST < 1ull << 32, "a chunk's values fit in a word");
 
 struct SmpChunk { float top; int32_t at; };               // a chunk's largest value and its lowest index
 struct SmpSeg { double sure, draw, mid; int32_t n_sure, n_mid, n_cand, pad; };
@@ -307,9 +308,10 @@ __global__ __launch_bounds__(SMP_WG) void k_sample_scan(const llapis_sample_args
     for (int j = 0; j < N; ++j) {
         const float at = x[j] * s.bins;
         const int b = smp_bin(x[j], top, top_bin, s.bins);
-        // (the place says nothing for what is out of fp32's range, as its bin does)
-        const uint32_t place = min((uint32_t)((at - floorf(at)) * 32.0f), 31u);
-        if (x[j] != SMP_NONE && b < SMP_BINS) atomicAdd(&s_hist[b], 1u << SMP_COUNT_AT | place);
+        // (its place in the bin says nothing for what is out of fp32's range, as its bin does)
+        const float w = __builtin_amdgcn_exp2f((at - floorf(at)) / SMP_PER_OCTAVE) * (float)SMP_LEAST;
+        const uint32_t v = s.by_p ? (uint32_t)fminf(fmaxf(w + 0.5f, (float)SMP_LEAST), (float)SMP_MOST) : 1;
+        if (x[j] != SMP_NONE && b < SMP_BINS) atomicAdd(&s_hist[b], v);
     }
     __syncthreads();
 #pragma unroll
@@ -320,8 +322,8 @@ __global__ __launch_bounds__(SMP_WG) void k_sample_scan(const llapis_sample_args
 
 __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_args a, const SmpWs ws) {
     __shared__ uint64_t s_best[SMP_SEQ_WAVES];
-    __shared__ int s_count[SMP_SEQ_WAVES], s_at[3];
-    __shared__ float s_low[SMP_SEQ_WAVES], s_high[SMP_SEQ_WAVES], s_mass[2];
+    __shared__ int s_few[SMP_SEQ_WAVES], s_many[SMP_SEQ_WAVES], s_at[4];
+    __shared__ float s_sum[SMP_SEQ_WAVES], s_mass[2];
     const int seq = blockIdx.x, tid = threadIdx.x;
     const SmpSet s = smp_settings(a, seq);
     const SmpChunk * chunks = ws.chunks + (int64_t)seq * ws.n_chunks;
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_
         best = key > best ? key : best;
     }
     smp_leave(smp_wave(best, SmpMax()), s_best);
-    if (tid == 0) s_at[0] = s_at[1] = s_at[2] = SMP_BINS - 1;
+    if (tid < 4) s_at[tid] = SMP_BINS - 1;
     __syncthreads();
     best = smp_all<SMP_SEQ_WAVES>(s_best, SmpMax());
     const float top = smp_value(best), none = __builtin_nanf(""), least = -3.40282347e38f;
@@ -343,8 +345,7 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_
     }
     // ---- a thread's bin over all chunks
     const float top_bin = floorf(top * s.bins);
-    int count = 0;
-    uint64_t places = 0;
+    uint64_t held_all = 0;
     const uint32_t * hist = ws.hist + (int64_t)seq * ws.n_chunks * SMP_BINS;
     constexpr int MANY = 16;                               // loads under way, then their use: in the compiler's own order each is waited for
     for (int c0 = 0; c0 < ws.n_chunks; c0 += MANY) {
@@ -359,50 +360,53 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < MANY; ++i) {
-            const uint32_t v = b[i] < 0 || c0 + i >= ws.n_chunks ? 0 : held[i];
-            count += (int)(v >> SMP_COUNT_AT);
-            places += v & ((1u << SMP_COUNT_AT) - 1);
+            held_all += b[i] < 0 || c0 + i >= ws.n_chunks ? 0 : held[i];
         }
     }
-    // the bin's weight: 2^((place - top's place) / 16) lies between 1 + 0.0433 place and 1 + 0.0443
-    // place times the bin's, a place between its 32nd and the next.  fp32 has each place to
-    // 2^-23 of its distance from 0
-    const float off = exp2f((fabsf(top * s.bins) + 2 * SMP_BINS) * 0x1p-22f / SMP_PER_OCTAVE) * (1.0f + 0x1p-14f);
-    const float unit = exp2f((top_bin - top * s.bins - (float)tid) / SMP_PER_OCTAVE);
-    const float low = unit * ((float)count + 0.0433f / 32 * (float)places);
-    const float high = unit * ((float)count + 0.0444f / 32 * ((float)places + (float)count));
-    const int count_w = smp_wave(count, SmpAdd());
-    const float low_w = smp_wave(low, SmpAdd()), high_w = smp_wave(high, SmpAdd());
-    smp_leave(count_w, s_count);
-    smp_leave(low_w, s_low);
-    smp_leave(high_w, s_high);
+    // the number of values, between two, and the sum of their weights.  fp32 has a value's place to 2^-23 of its
+    // distance from 0; the words' rounding and the sums' are less than the last factor
+    const int many = s.by_p ? (int)(held_all / SMP_LEAST) : (int)held_all;
+    const int few = s.by_p ? (int)((double)held_all * ((1.0 - 0x1p-40) / SMP_MOST)) : many;
+    const float off = exp2f((fabsf(top * s.bins) + 2 * SMP_BINS) * 0x1p-22f / SMP_PER_OCTAVE) * (1.0f + 0x1p-16f);
+    const float mass = exp2f((top_bin - top * s.bins - (float)tid) / SMP_PER_OCTAVE) * ((float)held_all / (float)SMP_LEAST);
+    const int few_w = smp_wave(few, SmpAdd()), many_w = smp_wave(many, SmpAdd());
+    const float mass_w = smp_wave(mass, SmpAdd());
+    smp_leave(few_w, s_few);
+    smp_leave(many_w, s_many);
+    smp_leave(mass_w, s_sum);
     __syncthreads();
-    int n_all;
-    float all_low, all_high;
-    const int n_upto = smp_before<SMP_SEQ_WAVES>(s_count, n_all) + count_w, n_before = n_upto - count;
-    const float low_upto = smp_before<SMP_SEQ_WAVES>(s_low, all_low) + low_w;
-    const float high_upto = smp_before<SMP_SEQ_WAVES>(s_high, all_high) + high_w;
-    const int k = s.by_k ? min(s.k, n_all) : n_all;
-    if (n_before < k && k <= n_upto) {                     // one bin: top_k ends here
-        s_at[2] = tid;
-        s_mass[0] = s.by_k ? low_upto - low : all_low;
-        s_mass[1] = s.by_k ? high_upto : all_high;
-    }
-    __syncthreads();
-    const int last = s_at[2];
-    int lo = last, hi = last;
-    if (s.by_p) {
-        // the first bin in which the sum may, and in which it must have reached top_p's part
-        const float p = (float)s.p;
-        smp_first(high_upto * off * off >= p * s_mass[0] * (1.0f - 0x1p-14f), &s_at[0]);
-        smp_first(low_upto >= p * s_mass[1] * off * off, &s_at[1]);
+    int few_all, many_all;
+    float mass_all;
+    const int few_upto = smp_before<SMP_SEQ_WAVES>(s_few, few_all) + few_w;
+    const int many_upto = smp_before<SMP_SEQ_WAVES>(s_many, many_all) + many_w;
+    const float mass_upto = smp_before<SMP_SEQ_WAVES>(s_sum, mass_all) + mass_w;
+    const bool spread = s.bins > 0.0f && fabsf(top * s.bins) < __builtin_inff();      // else the bins say nothing
+    // top_k ends in bins k_lo .. k_hi (in the last without one)
+    int k_lo = SMP_BINS - 1, k_hi = SMP_BINS - 1;
+    if (s.by_k) {
+        smp_first(many_upto >= s.k, &s_at[2]);
+        smp_first(few_upto >= s.k, &s_at[3]);
         __syncthreads();
-        lo = s.bins > 0.0f ? min(s_at[0], last) : 0;
-        hi = s.bins > 0.0f ? min(s_at[1], last) : last;
+        k_lo = spread ? s_at[2] : 0;
+        k_hi = spread ? s_at[3] : k_hi;
     }
-    // ---- the least value of bins lo - 1, hi and of those that top_k's end lies in, by bisection of the
+    int lo = k_lo, hi = k_hi;
+    if (s.by_p) {
+        // the first bin in which the sum may, and in which it must have reached top_p's part of what top_k leaves
+        if (tid == k_lo) s_mass[0] = s.by_k ? mass_upto - mass : mass_all;
+        if (tid == k_hi) s_mass[1] = s.by_k ? mass_upto : mass_all;
+        __syncthreads();
+        const float p = (float)s.p;
+        smp_first(mass_upto * off >= p * s_mass[0] / off, &s_at[0]);
+        smp_first(mass_upto / off >= p * s_mass[1] * off, &s_at[1]);
+        __syncthreads();
+        lo = spread ? min(s_at[0], k_lo) : 0;
+        hi = spread ? min(s_at[1], k_hi) : k_hi;
+        if (hi >= k_lo) hi = k_hi;                         // one window for both
+    }
+    // ---- the least value of bins lo - 1, hi, k_lo - 1 (without a top_k: k_hi) and k_hi, by bisection of the
     // values' order; a lane each
-    const int of = tid == 0 ? lo - 1 : tid == 1 ? hi : tid == 2 ? (s.by_k ? last - 1 : SMP_BINS - 1) : last;
+    const int of = tid == 0 ? lo - 1 : tid == 1 ? hi : tid == 2 ? (s.by_k ? k_lo - 1 : k_hi) : k_hi;
     uint32_t below = (uint32_t)(smp_key(least, 0) >> 32) - 1, from = (uint32_t)(smp_key(top, 0) >> 32);
     if (tid < 4) {
         auto try_at = [&](uint32_t at) {
@@ -420,9 +424,9 @@ __global__ __launch_bounds__(SMP_SEQ_WG) void k_sample_find(const llapis_sample_
         const float x = of < 0 ? none : smp_value((uint64_t)from << 32);
         cut.x_sure = smp_lane(x, 0);
         cut.x_cand = smp_lane(x, 1);
-        // (bins hi and last are one: no values between them)
-        cut.x_mid = s.by_k && last == hi ? cut.x_cand : smp_lane(x, 2);
-        cut.x_end = s.by_k && last > hi ? smp_lane(x, 3) : cut.x_mid;
+        // (in one window there are no values between)
+        cut.x_mid = hi == k_hi ? cut.x_cand : smp_lane(x, 2);
+        cut.x_end = hi == k_hi ? cut.x_cand : smp_lane(x, 3);
         if (tid == 0) ws.cuts[seq] = cut;
     }
 }
