@@ -310,6 +310,19 @@ def test_sample_flat(gpu, V):
     run_sample(gpu, x, [0.3, 0.999, 0.5, 0.0], None, [0, V // 3, V // 3, 1], [0.5, 1.0, 0.7, 0.5], [0.0, 0.0, 0.985, 0.0])
 
 
+@pytest.mark.parametrize("V", [300, 5000, 60000, 100000])
+def test_sample_many_ties(gpu, V):
+    """Hundreds and thousands of equal values where a filter ends: the first indices are kept, whichever filter it is."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randint(-40, 1, (6, V), generator=g) / 8.0
+    x[3] = torch.where(torch.arange(V) % 3 > 0, 1.0, -3.0)
+    x[4, V // 2:] = 0.25
+    k = [V // 3, 0, V // 2, V // 2, V // 5, 0]
+    p = [1.0, 0.6, 0.8, 0.7, 0.9, 0.35]
+    for tag in (la.F32, la.BF16):
+        run_sample(gpu, x.to(DT[tag]), [0.1, 0.999, 0.5, 0.7, 0.999, 0.3], [1.0, 1.0, 2.0, 1.0, 0.5, 3.0], k, p)
+
+
 @pytest.mark.parametrize("V,k,p", [(20000, 7000, 1.0), (20000, 0, 0.4), (20000, 9000, 0.5), (5000, 4999, 0.999), (70000, 69999, 0.7),
                                    (4096, 100, 0.5), (4097, 4000, 0.9)])
 def test_sample_ties(gpu, V, k, p):
