@@ -28,7 +28,6 @@
 // 262144 bf16 at top_p 0.9, a thousand ties: 79 us a call, at 0.99 without them 56).
 #include <algorithm>
 #include <cstdio>
-#include <type_traits>
 
 #include "kv.h"
 

@@ -358,7 +358,6 @@ class KvPages:
                   table_out.data_ptr(), refs.data_ptr(), n_live.data_ptr(), *scratch)
         return table_out, refs, n_live
 
-
     def extend_workspace(self, n_seq):
         """Scratch for extend with up to n_seq sequences, for a caller that keeps it: calls that share it must not overlap."""
         return _bytes("llapis_kv_extend_workspace_size", self.device, n_seq)
@@ -443,8 +442,9 @@ def qk_rope(q, k=None, pos=None, freq=None, q_weight=None, k_weight=None, norm=T
         _count(T, n_head, D)
 
     def heads(t, n, what):
-        s, stride = t.shape, t.stride()
-        if len(s) != 3 or s[0] != T or s[1] != n or s[2] != D or t.dtype != dtype or t.device != dev or (D > 1 and stride[2] != 1) or (n > 1 and stride[1] != D):
+        stride = t.stride()
+        if (t.shape != (T, n, D) or t.dtype != dtype or t.device != dev or (stride[2] != 1 and D > 1)
+                or (stride[1] != D and n > 1)):
             raise ValueError(f"{what} must be [{T}, {n}, {D}] of q's type and device, rows of consecutive values")
         return t.data_ptr(), stride[0]
 
@@ -459,8 +459,10 @@ def qk_rope(q, k=None, pos=None, freq=None, q_weight=None, k_weight=None, norm=T
         q_out = torch.empty(shape, dtype=dtype, device=dev)
     n_kv, k_in, k_to = 0, (None, 0), (None, 0)
     if k is not None:
-        _need(len(k.shape) == 3, "k must be [T, n_kv, head_dim]")
+        _need(k.dim() == 3, "k must be [T, n_kv, head_dim]")
         n_kv = k.shape[1]
+        if n_kv >> 31:
+            _count(n_kv)
         if k_out is None:
             k_out = torch.empty(k.shape, dtype=dtype, device=dev)
         k_in, k_to = heads(k, n_kv, "k"), heads(k_out, n_kv, "k_out")
