@@ -324,7 +324,8 @@ int32_t llapis_block_norm(const llapis_block_norm_args * a, void * stream);
  *   the token is the smallest v for which the kept w_0 + .. + w_v > u sum w.
  * A temperature that is not positive, and a min_p above 1, take the first value.
  * The settings are read on the device, one for each sequence; NULL: temperature 1,
- * the others off.  Weights and sums are fp64.  NaN and -infinity are no values (the
+ * the others off.  Weights are fp64, their sums fp64 or, next to where a filter ends, whole numbers of 2^-49 of the
+ * largest weight there.  NaN and -infinity are no values (the
  * token of a row without any is -1); where +infinity is the largest, the others have no
  * weight.  With top_k or top_p a value whose weight is below 2^-63 may not be kept.
  * probs [n_seq][vocab] of `type`, rows probs_stride apart, or NULL: the probabilities
