@@ -253,8 +253,9 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
                 p.lens[s] = len - min(eff, len);
                 p.seq_group[s] = eff > 0 ? g : -1;
             }
-            // entries to the end of the last unit, which its loads ask for
-            const int n = (min(len, cap) - min(eff, len) + kv_unit(HD)) / page + 1;
+            // entries to the end of the last unit that k_kv_attn asks for: it knows the table's end, but not
+            // that the table begins at the prefix's, so that the last `skip` entries have no page
+            const int n = (min(len - min(eff, len), cap) + kv_unit(HD)) / page + 1;
             for (int i = lane; i < min(n, p.b.max_pages); i += 64)
                 p.table[(int64_t)s * p.b.max_pages + i] = i + skip < p.b.max_pages ? from[i + skip] : -1;
         }

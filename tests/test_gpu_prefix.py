@@ -322,3 +322,46 @@ def test_refusals(gpu):
         call(workspace=torch.empty(64, dtype=torch.uint8, device=gpu))
     with pytest.raises(la.LlapisError, match="out may not be q"):
         call(out=q)
+
+
+def past_the_table(gpu, tag, io, D, P, max_new=None, huge=False):
+    """A batch whose table ends nine pages behind the prefix, among and before its sequences' ends"""
+    n, own = max(P, 64) * 3, 9 * P
+    members = [(own + over, k) for over, k in ((-5, 1), (0, 2), (1, 3), (P, 1), (129, 4), (2500, 2))]
+    s = Shared(gpu, 40 + D, tag, D, 2, P, [(n, members), (n + max(P, 64), [(own - max(P, 64) + 1, 1), (own + 700, 3)])], io, before=1)
+    width = (n + own) // P
+    s.table = [r[:width] for r in s.table]
+    if huge:
+        for i in (3, 6):
+            s.lens[i] = s.batch.lens[i] = 2 ** 31 - 1
+    s.batch = la.KvBatch(s.tb[:, :width], s.batch.lens, s.batch.new_start, n_tokens=s.T, max_new=max_new or 4)
+    # what an earlier call may have left: ids of pages that there are
+    room = s.cache.prefix_workspace
+    s.cache.prefix_workspace = lambda *a: room(*a).view(torch.int32).random_(0, s.cache.n_pages).view(torch.uint8)
+    return s
+
+
+@pytest.mark.parametrize("huge", [False, True])
+@pytest.mark.parametrize("tag,io,D,P", [(la.F16, la.F32, 64, 16), (la.BF16, la.BF16, 128, 16), (la.Q8_0, la.F16, 256, 64), (la.F16, la.F32, 512, 128)])
+def test_lengths_past_the_table(gpu, tag, io, D, P, huge):
+    """Keys past max_pages * page_size are not attended, whatever the workspace held: lengths of a token, a
+    page, a unit and thousands of tokens past it, and the largest that there is."""
+    s = past_the_table(gpu, tag, io, D, P, huge=huge)
+    q = s.queries(41, 4)
+    first = s.check(q)
+    assert torch.equal(s.check(q)[:s.T], first[:s.T])
+
+
+def test_cut_rows_past_the_table(gpu):
+    """... with new tokens past max_new, which are left out, the last ones of each sequence."""
+    s = past_the_table(gpu, la.F16, la.F32, 64, 16, max_new=2)
+    q = s.queries(42, 4)
+    out = torch.full(q.shape, 5.0, device=gpu)
+    s.cache.prefix_attention(s.batch, q.to(gpu), s.groups, s.prefix, out=out)
+    want, _, tol = ref.attention(s.cache, s.table, s.lens, s.start, q, 64 ** -0.5)
+    for i, k in enumerate(s.new):
+        rows = range(s.start[i], s.start[i + 1])
+        for r in rows[:2]:
+            assert ((out[r].cpu().double() - want[r]).abs() <= tol[r]).all(), (i, r)
+        for r in rows[2:]:
+            assert (out[r] == 5).all(), (i, r)
