@@ -16,16 +16,16 @@
 // sum of a bin's weights, in 2^-18 of the bin's least: all of it to 2^-15, and the number of its values
 // to 4 % (for top_k alone it holds their number).  They only say which bins are looked at: mostly one for
 // each filter.  (Words of numbers and of coarse weights, to 0.3 %, had ten times the candidates at a top_p of 0.99, where they
-// did not fit: 8 rows of 65536 230 us.)  What decides is fp64 (and fixed point of 49 bits, where sums are
-// made by atomics): weights, their sums and products, in a fixed order, so that a draw next to a
-// border falls as the definition says.
+// did not fit: 8 rows of 65536 230 us.)  What decides is fp64 (and fixed point, where sums are made by atomics: 49 bits
+// of the candidates' largest weight and more, and where the border may lie too far below that, twice as many): weights,
+// their sums and products, in a fixed order, so that a draw next to a border falls as the definition says.
 //
 // Bound, for few rows, by the four launches and a workgroup's barriers (1 row of 32003 fp32 values: 4.0, 6.9, 3.9 and
 // 8.9 us); for many by two passes over the logits (32 rows of 262144, 33.5 MB: 12.4 and 13.9 us, the sequences' kernels
 // 10.0 and 12.8), the second of which forms every kept value's weight in fp64: with top_p alone that is
 // most of them (64 rows of 128001 bf16: 11.7, 9.0, 18.5 and 13.0 us, probabilities 20.1).  Where more candidates than
 // SMP_HOLD a thread, or more ties than threads, are in the end's bin, k_sample_pick finds it digit by digit (32 rows of
-// 262144 bf16 at top_p 0.9, a thousand ties: 79 us a call, at 0.99 without them 56).
+// 262144 bf16 at top_p 0.9, a thousand ties: 80 us a call, at 0.99 without them 56; all values equal: 1.6 ms).
 #include <algorithm>
 #include <cstdio>
 
@@ -498,8 +498,9 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
     __shared__ double s_sure[WAVES], s_mid[WAVES], s_sum[2][WAVES];
     __shared__ int s_n[3][WAVES], s_count[WAVES], s_digit[256];
     __shared__ uint64_t s_mass[WAVES];
+    __shared__ int64_t s_parts[WAVES];
     __shared__ int s_first[WG + 1], s_bucket_n[WG], s_list_n, s_found, s_last;
-    __shared__ unsigned long long s_bucket[WG], s_kept[WG], s_weigh[256], s_all_k;
+    __shared__ unsigned long long s_bucket[WG], s_kept[WG], s_weigh[2][256], s_all_k;
     __shared__ uint64_t s_list[LIST], s_list_w[LIST], s_key;
     __shared__ unsigned long long s_upto[LIST];
     __shared__ struct { int bucket, before, n; uint64_t mass; } s_sel;
@@ -554,15 +555,21 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
         mid = smp_all<WAVES>(s_mid, SmpAdd());
         // candidates within top_k, the first of them in order
         const int n_k = s.by_k ? max(min(s.k - n_sure - n_mid, n_cand), 0) : n_cand;
-        bool few = n_cand <= FEW && per == 1;
+        // the largest weight that a candidate may have
+        const float upper = cut.x_sure == cut.x_sure ? cut.x_sure : cut.top;
+        const double upper_w = smp_weight(upper, cut.top, s.octaves);
+        const int sum_bits = n_cand > 1 ? 32 - __builtin_clz(n_cand - 1) : 0;      // 2^sum_bits candidates at most
+        // Held at once, weights are one word, cut off at 2^(sum_bits - 62) of the largest, which moves the border by at
+        // most n_cand^2 of that / (1 - top_p) of its values: 2^-5 here.  (All 8192 up to a top_p of 1 - 2^-17; 1 row of 131072
+        // at 0.999999 47 us, digit by digit 202)
+        bool few = n_cand <= FEW && per == 1 && (!s.by_p || (double)n_cand * n_cand * n_cand <= 0x1p56 * (1.0 - s.p));
         if (few) {
             // ---- the candidates in registers, and in buckets by value, thread b's the b-th from above.
-            // Weights are whole numbers of 2^-49 of the largest that a candidate may have
+            // Weights are whole numbers, of 2^-49 of the largest that a candidate may have, or less
+            const double scale = __builtin_ldexp(1.0, 62 - sum_bits) / upper_w;
             if (tid < n_segs) s_first[tid] = first;
             if (tid == 0) s_first[n_segs] = n_cand;
             __syncthreads();
-            const float upper = cut.x_sure == cut.x_sure ? cut.x_sure : cut.top;
-            const double scale = 0x1p49 / smp_weight(upper, cut.top, s.octaves);
             const bool two = cut.x_end < cut.x_mid;         // candidates of top_k's end apart
             const int n_upper = two ? WG / 2 : WG;
             const double per_upper = n_upper / fmax((double)upper - (double)cut.x_cand, 1e-300);
@@ -704,57 +711,97 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
         }
         if (!few) {
             // ---- too many at once: eight bits of the key at a time, the candidates counted (and
-            // weighed in fixed point) by them: the first key at which the number or the
-            // weight of what is not below it reaches the goal
+            // weighed) by them: the first key at which the number or the weight of what is not below
+            // it reaches the goal.  A weight is two whole numbers, of 2^-bits of the largest that a candidate may have and
+            // of 2^-2bits, as many bits as leave room for the sums (43 for 2^19 candidates): the border may
+            // lie far below the largest, and what one weight is cut by all of them are
+            const int bits = min(50, 62 - sum_bits);
+            const double one = __builtin_ldexp(1.0, bits), scale = one / upper_w;
+            // to nearest, the second of either sign (a number below 2^51 is in the low bits of its sum with 1.5 2^52)
+            auto parts = [&](double v, int64_t & hi, int64_t & lo) {
+                const double near = v + 0x1.8p52, rest = (v - (near - 0x1.8p52)) * one + 0x1.8p52;
+                hi = __builtin_bit_cast(int64_t, near) - __builtin_bit_cast(int64_t, 0x1.8p52);
+                lo = __builtin_bit_cast(int64_t, rest) - __builtin_bit_cast(int64_t, 0x1.8p52);
+            };
             auto each = [&](auto f) {                      // f(key) of each candidate, a wave a segment
                 for (int i = wave; i < n_segs; i += WAVES) {
                     const int n = segs[i].n_cand;
                     for (int c = lane; c < n; c += 64) f(keys[(int64_t)i * SEG + c]);
                 }
             };
-            int bits = 1;
-            while (bits < 31 && (1 << bits) < n_cand) ++bits;
-            const double scale = __builtin_ldexp(1.0, 61 - bits);
-            double goal = 0.0;
+            int64_t want_hi = 0, want_lo = 0;
             key = n_k > 0 ? 0 : ~0ull;
             for (int pass = n_k < n_cand ? 0 : 1; pass < (s.by_p ? 2 : 1) && n_k > 0; ++pass) {
                 const bool by_mass = pass == 1;
                 if (by_mass) {
-                    double within = 0.0, all_k;
-                    each([&](uint64_t u) { within += u >= key ? weight(u) : 0.0; });
+                    int64_t hi = 0, lo = 0, all_hi, all_lo;
+                    each([&](uint64_t u) {
+                        int64_t y, y_lo;
+                        parts(u >= key ? weight(u) * scale : 0.0, y, y_lo);
+                        hi += y;
+                        lo += y_lo;
+                    });
                     __syncthreads();
-                    smp_scan<WAVES>(within, s_sum[0], all_k);
-                    goal = s.p * (sure + mid + all_k) - sure;
+                    smp_scan<WAVES>(hi, s_parts, all_hi);
+                    __syncthreads();
+                    smp_scan<WAVES>(lo, s_parts, all_lo);
+                    const double all_k = ((double)all_hi + (double)all_lo / one) / scale;
+                    const double goal = fmax(s.p * (sure + mid + all_k) - sure, 0.0) * scale;
+                    want_hi = (int64_t)goal;
+                    want_lo = (int64_t)ceil((goal - (double)want_hi) * one);
                 }
                 uint64_t prefix = 0;
+                int64_t above_hi = 0, above_lo = 0;
                 int n_above = 0;
-                unsigned long long above = 0;
-                const unsigned long long want = by_mass ? (unsigned long long)ceil(fmax(goal, 0.0) * scale) : 0;
                 for (int shift = 56; shift >= 0; shift -= 8) {
                     __syncthreads();
                     if (tid < 256) {
                         s_digit[tid] = 0;
-                        s_weigh[tid] = 0;
+                        s_weigh[0][tid] = 0;
+                        s_weigh[1][tid] = 0;
                     }
                     __syncthreads();
+                    // (equal values have equal digits: a thread adds them up before it adds them to the others')
+                    int at = 0, n_at = 0;
+                    int64_t at_hi = 0, at_lo = 0;
+                    auto add = [&]() {
+                        if (n_at) atomicAdd(&s_digit[at], n_at);
+                        if (n_at && by_mass) {
+                            atomicAdd(&s_weigh[0][at], (unsigned long long)at_hi);
+                            atomicAdd(&s_weigh[1][at], (unsigned long long)at_lo);
+                        }
+                        n_at = 0;
+                        at_hi = at_lo = 0;
+                    };
                     each([&](uint64_t u) {
                         if (shift < 56 && (u >> (shift + 8)) != (prefix >> (shift + 8))) return;
                         const int d = (int)(u >> shift) & 255;
-                        atomicAdd(&s_digit[d], 1);
-                        if (by_mass) atomicAdd(&s_weigh[d], (unsigned long long)(weight(u) * scale));
+                        if (d != at) add();
+                        at = d;
+                        ++n_at;
+                        if (by_mass) {
+                            int64_t y, y_lo;
+                            parts(weight(u) * scale, y, y_lo);
+                            at_hi += y;
+                            at_lo += y_lo;
+                        }
                     });
+                    add();
                     __syncthreads();
-                    int d = 255, found = -1;
-                    for (; d >= 0; --d) {
-                        if (s_digit[d] == 0) continue;
+                    // the last digit that there is, if none reaches the goal
+                    int found = -1;
+                    for (int d = 255, n_before = 0; d >= 0; --d) {
+                        const int n = s_digit[d];
+                        if (n == 0) continue;
+                        if (found >= 0) {
+                            n_above += n_before;
+                            above_hi += s_weigh[0][found];
+                            above_lo += s_weigh[1][found];
+                        }
                         found = d;
-                        if (by_mass ? above + s_weigh[d] >= want : n_above + s_digit[d] >= n_k) break;
-                        n_above += s_digit[d];
-                        above += s_weigh[d];
-                    }
-                    if (d < 0) {                          // all of them: the last
-                        n_above -= s_digit[found];
-                        above -= s_weigh[found];
+                        n_before = n;
+                        const int64_t lo = above_lo + (int64_t)s_weigh[1][d], hi = above_hi + (int64_t)s_weigh[0][d] + (lo >> bits);
+                        if (by_mass ? hi > want_hi || (hi == want_hi && (lo & ((1ll << bits) - 1)) >= want_lo) : n_above + n >= n_k) break;
                     }
                     prefix |= (uint64_t)found << shift;
                 }

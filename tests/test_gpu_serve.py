@@ -585,3 +585,64 @@ def test_threads_and_streams_at_once(gpu):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+# ------------------------------------------------- borders far below the largest value
+
+def exact_kept(x, k, p):
+    """The indices that top_k and top_p keep of a row (float64, no NaN), their weights as whole numbers of 2^-200, and how
+    far the border is from another one, in weights of its value"""
+    z, order = torch.sort(x, descending=True, stable=True)
+    z, order = z[:k] if k else z, order[:k] if k else order
+    w = [int(math.ldexp(v, 200)) for v in (z - z[0]).exp().tolist()]
+    num, den = p.as_integer_ratio()
+    goal, n, upto = num * sum(w), 0, 0
+    while upto * den < goal:
+        upto += w[n]
+        n += 1
+    near = min(upto * den - goal, goal - (upto - w[n - 1]) * den) / (w[n - 1] * den)
+    return order[:n], w[:n], near
+
+
+def deep(kind, V, depth, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.full((V,), -float(depth))
+    if kind == "band":
+        x -= 0.02 * torch.rand(V, generator=g)
+    if kind == "few":
+        x[torch.randperm(V, generator=g)[8000:]] = -math.inf
+    if kind == "tail":
+        x = 2.5 * torch.randn(V, generator=g) - depth
+    x[V // 3] = 0.0
+    return x
+
+
+@pytest.mark.parametrize("kind,V,depth,k,p", [
+    ("equal", 1 << 18, 20.5, 0, 0.9999), ("equal", 1 << 20, 23.25, 0, 0.99995), ("equal", 1 << 18, 16, 0, 0.98), ("equal", 1 << 20, 24, 0, 0.99999),
+    ("equal", 1 << 18, 20.25, 200000, 0.9999), ("equal", 60000, 19, 0, 0.9999), ("equal", 2100001, 22, 0, 0.9999),
+    ("band", 1 << 18, 20.8, 0, 0.9999), ("band", 10 ** 6, 21, 0, 0.9997), ("band", 1 << 18, 18, 0, 0.999), ("band", 30000, 18, 0, 0.9999),
+    ("band", 10 ** 6, 22, 900001, 0.9999), ("band", 2100001, 24, 0, 0.99999), ("tail", 1 << 18, 12, 0, 0.9999999), ("tail", 10 ** 6, 20, 0, 0.999999),
+    ("tail", 2100001, 16, 0, 0.99999), ("few", 70000, 24.59375, 0, 1 - 2 ** -24), ("few", 70000, 24.90625, 0, 1 - 2 ** -24),
+    ("few", 70000, 24.21875, 0, 1 - 2 ** -22), ("few", 70000, 20.0, 0, 1 - 2 ** -17)])
+def test_sample_border_below_a_dominant_value(gpu, kind, V, depth, k, p):
+    """One value has nearly all of the weight and top_p ends among thousands to millions 16 to 25 below it, as many as
+    are held at once and more.  Their weights' sum decides to a small part of one of them (checked here), so the kept sets are equal."""
+    p = float(torch.tensor(p, dtype=torch.float32))
+    for tag in (la.F32, la.BF16) if kind == "equal" else (la.F32,):
+        x = deep(kind, V, depth, V).to(DT[tag])
+        want, w, near = exact_kept(x.double(), k, p)
+        assert 1 < len(want) < V and near > 1e-3
+        probs = torch.empty(1, V, dtype=DT[tag], device=gpu)
+        u = 1.0 - 2.0 ** -22
+        tok = la.sample(x[None].to(gpu), f32([u], gpu), top_k=i32([k], gpu), top_p=f32([p], gpu), probs=probs)
+        got = (probs[0] > 0).nonzero()[:, 0].cpu()
+        assert len(got) == len(want), (len(got), len(want))
+        assert torch.equal(got, want.sort().values)
+        # the first at which the sum passes u of the whole
+        num, den = u.as_integer_ratio()
+        goal, upto = num * sum(w), 0
+        for v, i in sorted(zip(want.tolist(), w)):
+            upto += i
+            if upto * den > goal:
+                break
+        assert int(tok) == v
