@@ -927,7 +927,7 @@ __global__ __launch_bounds__(SMP_WG) void k_sample_probs(const llapis_sample_arg
 #pragma unroll
                 for (int j = 0; j < 2; ++j) w[j] = smp_weight(x[j0 + j], cut.top, s.octaves);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) p[j0 + j] = keep[j] && w[j] >= s.min_p ? (T)(float)(w[j] * inv) : p[j0 + j];
+                for (int j = 0; j < 2; ++j) p[j0 + j] = keep[j] && w[j] >= s.min_p ? (T)(w[j] * inv) : p[j0 + j];
             }
         }
         if (at + W <= a.vocab) {

@@ -646,3 +646,25 @@ def test_sample_border_below_a_dominant_value(gpu, kind, V, depth, k, p):
             if upto * den > goal:
                 break
         assert int(tok) == v
+
+
+@pytest.mark.parametrize("tag", [la.F16, la.BF16])
+def test_sample_probabilities_are_rounded_once(gpu, tag):
+    """Probabilities next to the middle of two 16-bit numbers, nearer than fp32 tells: temperatures at which the first of
+    two values has one 2^-34 to 2^-26 above or below it."""
+    step, half = EPS[tag], 0.5
+    temps, want = [], []
+    for i in range(1, 60):
+        middle = half + (i + 0.5) * step                  # (numbers from 1/2 to 1 are EPS apart)
+        t0 = torch.tensor(half / math.log(middle / (1 - middle)), dtype=torch.float32)
+        for j in range(-40, 41):
+            t = float((t0.view(torch.int32) + j).view(torch.float32))
+            p = 1 / (1 + math.exp(-half / t))
+            if 2 ** -34 < abs(p - middle) < 2 ** -26:
+                temps.append(t)
+                want.append(half + (i + (p > middle)) * step)
+    assert len(temps) > 300
+    x = torch.tensor([[half, 0.0]], dtype=DT[tag]).expand(len(temps), 2).contiguous().to(gpu)
+    probs = torch.empty_like(x)
+    la.sample(x, f32([0.5] * len(temps), gpu), f32(temps, gpu), probs=probs)
+    assert probs[:, 0].double().tolist() == want
