@@ -768,9 +768,11 @@ const char * plan_prefix(const llapis_kv_cache * c, const llapis_kv_batch * b, i
     f.rows = 16 * wave_tiles * kvp_waves(hd);
     const int64_t tokens = b->n_tokens, tiles = (tokens * group + f.rows - 1) / f.rows + n_group;
     const int64_t units = (int64_t)b->max_pages * c->page_size / kvp_unit(c->type == LLAPIS_T_Q8_0, hd);
+    if (tokens > 1 << 24) return "more than 2^24 rows";
+    if (tokens * group >= (int64_t)1 << 31) return "2^31 query rows of a kv head or more";
     f.max_steps = tiles * c->n_kv * (2 * units + 1);
-    if (tokens > 1 << 24 || f.max_steps >= (int64_t)1 << 31) return "the groups' prefixes have 2^30 units of work or more";
-    // the join has a workgroup for each (sequence, kv head, tile)
+    if (f.max_steps >= (int64_t)1 << 31) return "the groups' prefixes have 2^30 units of work or more";
+    // the join, which every call has, has a workgroup for each (sequence, kv head, tile)
     if ((int64_t)b->n_seq * c->n_kv * attn_tiles >= KV_MAX_GRID) return "2^24 or more (sequence, kv head, 32 query rows)";
     f.slots = (int)(tiles * c->n_kv + KVP_RUNS);
     uint64_t at = own;
@@ -926,6 +928,7 @@ uint64_t llapis_kv_prefix_attention_workspace_size(const llapis_kv_cache * c, co
                                                    int32_t n_group) {
     const uint64_t own = llapis_kv_attention_workspace_size(c, b, n_head);
     if (!own || n_group < 0 || n_group > KVP_GROUPS || b->n_tokens < 0) return 0;
+    if (n_group == 0) return own;
     AttnPlan a;
     PrefixPlan one, two;
     plan_attention(c, b, n_head, a);
@@ -947,7 +950,8 @@ int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_ba
     PrefixPlan f{};
     // (how many rows a group has is the device's to know: the mean)
     const int tiles = bad ? 1 : kvp_tiles(c->type != T_BF16, q->type, c->head_dim, (int64_t)b->n_tokens * (q->n_head / c->n_kv) / std::max(x->n_group, 1));
-    if (!bad) bad = plan_prefix(c, b, q->n_head, x->n_group, tiles, a.tiles, a.bytes(), f);
+    f.bytes = a.bytes();
+    if (!bad && x->n_group > 0) bad = plan_prefix(c, b, q->n_head, x->n_group, tiles, a.tiles, a.bytes(), f);
     if (bad) return refuse_as(who, bad);
     const KvSeqs sq = seqs_of(b);
     if (sq.n_seq == 0 || sq.n_tokens == 0 || sq.max_new == 0) return 0;

@@ -272,3 +272,36 @@ def test_prefix_workspace_serves_less(head_dim, kind):
         for less in ((n_seq, new - 1, pages, groups), (max(n_seq - 1, 1), new, pages, groups), (n_seq, new, pages - 1, groups), (n_seq, new, pages, groups - 1),
                      (n_seq, new, pages, groups, 1), (1, 1, 1, 0)):
             assert 0 < size(*less) <= most, less
+
+
+def test_prefix_limits_and_their_names():
+    """Groups have limits of their own, each refused by its name; without groups the call is attention's."""
+    from test_step import batch, cache, query
+    lib, c, q = la.lib(), cache(n_kv=1, k_stride=1 << 20, v_stride=1 << 20), query(n_head=1)
+    new = lambda **kw: batch(**{**dict(n_seq=1 << 12, max_new=16, new_start=P, max_pages=4, table_stride=4), **kw})
+
+    def size(b, groups, heads=1):
+        return lib.llapis_kv_prefix_attention_workspace_size(C.byref(c), C.byref(b), heads, groups)
+
+    def call(b, groups, n, q=q):
+        x = _lib.LlapisKvPrefix(groups, P if groups else None, P if groups else None)
+        return lib.llapis_kv_prefix_attention(C.byref(c), C.byref(b), C.byref(q), C.byref(x), P, n, None)
+
+    many = new(n_tokens=(1 << 24) + 1)
+    assert size(many, 1) == 0 < size(many, 0) == lib.llapis_kv_attention_workspace_size(C.byref(c), C.byref(many), 1)
+    refused(call(many, 1, 1 << 40), "llapis_kv_prefix_attention", "2^24 rows")
+    refused(call(many, 0, 64), "llapis_kv_prefix_attention", "workspace")
+    assert size(new(n_tokens=1 << 24), 1) > 0
+    # query rows of a kv head past 31 bits
+    heads = query(n_head=256, q_stride=1 << 14, out_stride=1 << 14)
+    assert size(new(n_tokens=1 << 23), 1, 256) == 0
+    refused(call(new(n_tokens=1 << 23), 1, 1 << 40, heads), "2^31 query rows")
+    # a table of one unit needs no join of its own, one with a prefix does
+    short = batch(n_seq=1 << 24, n_tokens=1, max_pages=1, table_stride=1)
+    assert size(short, 1) == 0 < size(short, 0)
+    refused(call(short, 1, 1 << 40), "32 query rows")
+    refused(call(short, 0, 64), "workspace")
+    # prefixes of more units than 31 bits count
+    wide = batch(n_seq=64, n_tokens=1 << 22, max_new=16, new_start=P, max_pages=1 << 14, table_stride=1 << 14)
+    assert size(wide, 1, 16) == 0 < size(wide, 0, 16)
+    refused(call(wide, 1, 1 << 40, query(n_head=16, q_stride=1 << 10, out_stride=1 << 10)), "2^30 units")
