@@ -37,12 +37,14 @@ struct KvAttn {
     int n_kv, group;                 // query heads of a kv head
     int window, unit;
     float scale;
-    int type, out_type;              // of q, of out
+    int type;                        // of q and out
     const void * q;
     int64_t q_stride;
     void * out;
     int64_t out_stride;
     float * lse;
+    float * row_ml;                  // or null.  Rows that one run has all of stay parts: out is fp32 and
+                                     // unnormalised, here [n_tokens][heads][2] are their maxima and sums
     int32_t * base;                  // [n_seq + 1] first unit of each sequence, [n_seq] their number
     int nt;                          // 16-row tiles of a workgroup
     int runs, tiles;                 // runs (a multiple of 8) of `tiles` workgroups, one for each 16 nt query rows

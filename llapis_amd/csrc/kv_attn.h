@@ -776,14 +776,18 @@ __global__ __launch_bounds__(64 * kv_waves(HD), kv_wgs(HD, NT) * kv_waves(HD) / 
             if (whole) {
                 const int rr = tile * ROWS + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
                 const int64_t out_row = su.r.row0 + tok;
-                const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float norm = p.row_ml ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
                 for (int t = 0; t < NVW; ++t)
                     if (v_tile + t < NV)
-                        store4(p.out, WIDE ? (int)T_F32 : p.out_type, out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
-                if (p.lse && wave == 0 && lg == 0)
-                    p.lse[out_row * (p.group * p.n_kv) + hq] =
-                        sum == 0.0f ? -__builtin_inff() : (m[nt] + (__builtin_amdgcn_logf(sum) - P_SHIFT)) * KV_LN2;
+                        store4(p.out, p.row_ml ? (int)T_F32 : type, out_row * p.out_stride + (int64_t)hq * HD + 16 * (v_tile + t) + 4 * lg, acc[nt][t] * norm);
+                const int64_t at = out_row * (p.group * p.n_kv) + hq;
+                if (p.row_ml && wave == 0 && lg == 0) {
+                    p.row_ml[2 * at] = m[nt];
+                    p.row_ml[2 * at + 1] = sum;
+                } else if (p.lse && wave == 0 && lg == 0) {
+                    p.lse[at] = sum == 0.0f ? -__builtin_inff() : (m[nt] + (__builtin_amdgcn_logf(sum) - P_SHIFT)) * KV_LN2;
+                }
             } else {
                 float * a = p.acc + (slot * ROWS + r) * HD;
 #pragma unroll

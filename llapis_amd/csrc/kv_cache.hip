@@ -97,16 +97,15 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, f
     const int rr = tile * tile_rows + r, tok = rr / p.group, hq = head * p.group + rr - tok * p.group;
     const int64_t row = su.r.row0 + tok;
     const float inv = 1.0f / l;
-    store4(p.out, p.out_type, row * p.out_stride + (int64_t)hq * head_dim + d, l == 0.0f ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : a * inv);
+    store4(p.out, p.type, row * p.out_stride + (int64_t)hq * head_dim + d, l == 0.0f ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : a * inv);
     if (p.lse && d == 0)
         p.lse[row * (p.n_kv * p.group) + hq] = l == 0.0f ? -__builtin_inff() : (m + (__builtin_amdgcn_logf(l) - p_shift)) * KV_LN2;
 }
 
 // --------------------------------------------------- join with a prefix
 //
-// As k_kv_join, of the parts of a row's prefix (k_kv_prefix) and those of its own keys,
-// which are parts of k_kv_attn or, where one run had them all, its result with the
-// logarithm of its sum.  Bound by the parts' bytes: each of 256 runs leaves its rows' in fp32, 34 MB
+// As k_kv_join, of the parts of a row's prefix (k_kv_prefix) and those of its own keys, which
+// are k_kv_attn's: where one run had them all, in the row's place.  Bound by the parts' bytes: each of 256 runs leaves its rows' in fp32, 34 MB
 // for 256 rows of 128 values, 12 us.
 struct KvResult {
     void * out;
@@ -170,9 +169,10 @@ __global__ __launch_bounds__(256) void k_kv_prefix_join(const KvAttn p, const Kv
                 vm[j] = x.ml[2 * at_row];
                 vl[j] = x.ml[2 * at_row + 1];
             } else if (n_own == 1) {
-                v[j] = *(const f4v *)((const float *)p.out + row * p.out_stride + (int64_t)hq * head_dim + d) * __builtin_ldexpf(1.0f, (int)p_shift);
-                vm[j] = p.lse[row * (p.n_kv * p.group) + hq] * KV_LOG2E;
-                vl[j] = vm[j] == -__builtin_inff() ? 0.0f : __builtin_ldexpf(1.0f, (int)p_shift);
+                const int64_t at_row = row * (p.n_kv * p.group) + hq;
+                v[j] = *(const f4v *)((const float *)p.out + row * p.out_stride + (int64_t)hq * head_dim + d);
+                vm[j] = p.row_ml[2 * at_row];
+                vl[j] = p.row_ml[2 * at_row + 1];
             } else {
                 const int64_t at_row = (((int64_t)(w0 + i - n_pre) * p.tiles + tile) * 2 + (i == n_pre)) * tile_rows + r;
                 v[j] = *(const f4v *)(p.acc + at_row * head_dim + d);
@@ -731,7 +731,7 @@ KvAttn attn_of(const llapis_kv_cache * c, const llapis_kv_batch * b, const llapi
     p.window = std::min(q->window, 0x7FFFFF00);            // leaves room for sums with it
     p.unit = kv_unit(c->head_dim);
     p.scale = q->scale;
-    p.type = p.out_type = q->type;
+    p.type = q->type;
     p.q = q->q;
     p.q_stride = q->q_stride;
     p.out = q->out;
@@ -759,7 +759,7 @@ constexpr int KVP_RUNS = 256;                            // a workgroup a CU
 struct PrefixPlan {
     int rows, slots;
     int64_t max_steps;
-    uint64_t lens, table, seq_group, plan, total, out, lse, ml, acc, bytes;
+    uint64_t lens, table, seq_group, plan, total, out, row_ml, ml, acc, bytes;
 };
 
 const char * plan_prefix(const llapis_kv_cache * c, const llapis_kv_batch * b, int n_head, int n_group, int wave_tiles, int attn_tiles,
@@ -788,7 +788,7 @@ const char * plan_prefix(const llapis_kv_cache * c, const llapis_kv_batch * b, i
     part(f.plan, KVP_GROUPS * sizeof(KvGroup));
     part(f.total, 4);
     part(f.out, (uint64_t)b->n_tokens * width * 4);
-    part(f.lse, (uint64_t)b->n_tokens * n_head * 4);
+    part(f.row_ml, (uint64_t)b->n_tokens * n_head * 8);
     part(f.ml, (uint64_t)f.slots * f.rows * 8);
     part(f.acc, (uint64_t)f.slots * f.rows * hd * 4);
     f.bytes = at;
@@ -990,7 +990,7 @@ int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_ba
     hipStream_t s = (hipStream_t)stream;
     KV_TRY(c->type == T_F16 ? launch_kv_prefix_f16(p, c->head_dim, s)
                             : c->type == T_BF16 ? launch_kv_prefix_bf16(p, c->head_dim, s) : launch_kv_prefix_q8(p, c->head_dim, s));
-    // the sequences' own keys, with results in fp32
+    // the sequences' own keys
     llapis_kv_batch rest = *b;
     rest.page_table = p.table;
     rest.table_stride = b->max_pages;
@@ -998,9 +998,9 @@ int32_t llapis_kv_prefix_attention(const llapis_kv_cache * c, const llapis_kv_ba
     llapis_kv_query to = *q;
     to.out = ws + f.out;
     to.out_stride = (int64_t)q->n_head * c->head_dim;
-    to.lse = (float *)(ws + f.lse);
+    to.lse = nullptr;
     KvAttn k = attn_of(c, &rest, &to, a, ws);
-    k.out_type = T_F32;
+    k.row_ml = (float *)(ws + f.row_ml);
     KV_TRY(launch_attn(c, k, s));
     const KvResult o{q->out, q->out_stride, q->lse, q->type};
     const int64_t items = (int64_t)sq.n_seq * c->n_kv;

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
     constexpr int KPT = Sh::KPT, VPT = Sh::VPT, KL = Sh::KL;
     // log2 of p's scale, and how far a row's scores may pass the maximum that its sums are
     // taken against before these are scaled anew: p stays below 2^16, fp16's end
-    constexpr float KV_P_SHIFT = HALF ? 15.0f : 0.0f, P_SHIFT = HALF ? 12.0f : 0.0f, P_SLACK = HALF ? 3.0f : 16.0f;
+    constexpr float KV_P_SHIFT = HALF ? 15.0f : 0.0f, P_SHIFT = HALF ? 13.0f : 0.0f, P_SLACK = HALF ? 2.75f : 16.0f;
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int s_first[KVP_GROUPS + 1], s_eff[KVP_GROUPS], s_lead[KVP_GROUPS];
     __shared__ KvGroup s_plan[KVP_GROUPS];
@@ -550,7 +550,8 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[nt][j][i]);
             top = over_groups(top, [](float a, float b) { return fmaxf(a, b); }) * q_scale[nt];
             if (__any(top > m[nt] + P_SLACK)) {
-                const float now = fmaxf(m[nt], top);
+                // (a whole number: it and what it is added to are exact, and scaling by it is)
+                const float now = fmaxf(m[nt], ceilf(top));
                 const float f = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - now);
                 sum[nt] *= f;
 #pragma unroll

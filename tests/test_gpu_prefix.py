@@ -1,10 +1,9 @@
 """Attention of sequences that share a prefix (llapis_kv_prefix_attention) on the GPU against
 the plain 64-bit form of attention (step_ref.py), which reads every sequence's own row of the page table.
 
-The bound is step_ref.attention's.  What the prefix adds to its error: the weight of a
-sequence's own keys comes from the logarithm of their sum, rounded twice, 2^-23 |lse| of it, and |lse| is
-at most the largest score and the logarithm of their number: within the bound's 2^-22
-(|s| + |m|) and its 2^-21.  (Of a probability's two BF16 parts the first is cut off, not rounded: the sum is off by 2^-16
+The bound is step_ref.attention's.  What the prefix adds to its error: parts are joined by their
+maxima in base 2, whose difference is rounded once, 2^-24 (|s| + |m|), and 2^x of it, 2^-23: within the bound's
+2^-22 (|s| + |m|) and its 2^-21.  (Of a probability's two BF16 parts the first is cut off, not rounded: the sum is off by 2^-16
 of it at most where the bound counts 2^-17, and is held to that bound all the same.)"""
 import math
 
@@ -365,3 +364,51 @@ def test_cut_rows_past_the_table(gpu):
             assert ((out[r].cpu().double() - want[r]).abs() <= tol[r]).all(), (i, r)
         for r in rows[2:]:
             assert (out[r] == 5).all(), (i, r)
+
+
+def made(gpu, tag, heads, keys, values, own):
+    """Two sequences of one kv head of 64 values behind `heads` tokens of keys[:heads]; behind these each has the `own`
+    tokens that follow.  keys [heads + own]: a key's first two values; values: its V's first."""
+    P, n = 16, heads + own
+    held, rest = -(-heads // P), -(-own // P)
+    table = [list(range(held)) + [held + rest * i + j for j in range(rest)] for i in range(2)]
+    cache = poisoned(la.KvCache.empty(held + 2 * rest, P, 1, 64, tag, gpu))
+    k, v = torch.zeros(n, 1, 64), torch.zeros(n, 1, 64)
+    k[:, 0, :2], v[:, 0, 0] = keys, values
+    for row in table:
+        cache.append(la.KvBatch(i32([row], gpu), i32([n], gpu), i32([0, n], gpu), n_tokens=n, max_new=n), k.to(gpu), v.to(gpu))
+    batch = la.KvBatch(i32(table, gpu), i32([n, n], gpu))
+    return cache, batch, i32([0, 2], gpu), i32([heads], gpu)
+
+
+@pytest.mark.parametrize("tag", [la.F16, la.BF16])
+@pytest.mark.parametrize("far", [0, 416, 2912, 3616])
+def test_parts_join_exactly_far_from_zero(gpu, tag, far):
+    """Scores that are whole numbers in base 2, about `far`, in the prefix and behind it: every weight is a power of 2, so
+    that the result is off by what fp32 sums are, whatever the scores' size.
+
+    The scale is fp32's ln 2, which times fp32's log2 e is 1: scores, maxima and their differences are exact.
+    2^x of a whole number is off by 2^-23, a sum of n weights in fp32 by (n / 32 + 40) 2^-24 (the numerator and
+    the sum, of values up to 1), the quotient by 2^-23."""
+    g = torch.Generator().manual_seed(far)
+    heads, own = 128, 100
+    n = heads + own
+    near = torch.randint(0, 6, (n,), generator=g)
+    keys = torch.stack([torch.full((n,), far / 64.0), near.float()], 1)
+    values = torch.randint(0, 65, (n,), generator=g) / 64.0
+    values[:heads] *= -1                                  # either part's weight shows
+    cache, batch, groups, prefix = made(gpu, tag, heads, keys, values, own)
+    q = torch.zeros(2, 1, 64, device=gpu)
+    q[:, 0, 0], q[:, 0, 1] = 64, 1
+    lse = torch.empty(2, 1, device=gpu)
+    ln2 = float(torch.tensor(math.log(2), dtype=torch.float32))
+    out = cache.prefix_attention(batch, q, groups, prefix, scale=ln2, lse=lse)
+    w = 2.0 ** near.double()
+    want = float((w * values).sum() / w.sum())
+    tol = 2 * (n / 32 + 40) * 2 ** -24 + 2 * 2 ** -23 + 2 ** -23
+    off = (out[:, 0, 0].cpu().double() - want).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+    assert (out[:, 0, 1:] == 0).all()
+    # the logarithm: the sum's error, log2's and its product's roundings
+    want = math.log(2) * (far + math.log2(float(w.sum())))
+    assert (lse.cpu().double() - want).abs().max() <= tol + 3 * 2 ** -24 * max(want, 16)
