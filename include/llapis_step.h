@@ -121,9 +121,8 @@ int32_t  llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * 
  * are in order (as the rows of new_start are), sequences before the first and behind the
  * last share nothing.  A prefix is cut to what every sequence of its group with new tokens had before
  * them, and to a multiple of 64 tokens and of a page; what is cut off counts as each one's own.  Results are
- * llapis_kv_attention's but for the order of sums, and for the probabilities of 16-bit results over BF16 pages, which
- * are kept to 2^-16.  n_group is 256 at most; with none the call is attention's.  Refused:
- * what attention refuses, and with groups more than 2^24 rows (n_tokens), 2^31 query rows
+ * llapis_kv_attention's but for the order of sums, with its precision of every part.
+ * n_group is 256 at most; with none the call is attention's.  Refused: what attention refuses, and with groups more than 2^24 rows (n_tokens), 2^31 query rows
  * of a kv head and more, 2^24 and more (sequence, kv head, 32 query rows) however short the
  * table, and prefixes of 2^30 and more units of work (32 or 64 keys of a kv head for a tile
  * of rows).  The workspace serves every call of fewer sequences, rows, new tokens, pages and

@@ -28,8 +28,9 @@
 //    one tile 106; 16 sequences, whose 64 rows one tile holds, 61 us, with two 72
 // One part of P would take 10 us off and add 2^-9 to the error of its weights: it keeps kv_attn.h's instead.
 //
-// Rounding is kv_attn.h's: fp32 scores, maxima and sums, 16-bit parts of q and p (parts that are cut
-// off, not rounded, but for the last: the same sum); q8_0 values are staged as an fp16 value and its exact remainder.
+// Rounding is kv_attn.h's: fp32 scores, maxima and sums, 16-bit parts of q and p, a pair of p's bf16 parts good to 2^-17 (cut
+// off instead of rounded they took as long and were good to 2^-16); q8_0 values are staged as an fp16 value and its
+// exact remainder.  A row's maximum is rounded up to a whole number, in base 2: what it is taken from or scaled by is exact.
 #pragma once
 
 #include "kv_attn.h"
@@ -126,8 +127,8 @@ __device__ __forceinline__ int64_t kvp_scan(int64_t x, int64_t * s_part, int64_t
     return before + v - x;
 }
 
-// split8 with fewer instructions: the remainder of an fp16 part is taken and rounded in one,
-// bf16 parts but the last are cut off, not rounded
+// split8 with fewer instructions: the remainder of an fp16 part is taken and rounded in one, a pair of bf16 parts
+// rounded once
 template <bool HALF, int PARTS>
 __device__ __forceinline__ void split_p(const float (&x)[8], u4 (&out)[PARTS]) {
     if constexpr (HALF) {
@@ -146,15 +147,18 @@ __device__ __forceinline__ void split_p(const float (&x)[8], u4 (&out)[PARTS]) {
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t a = __builtin_bit_cast(uint32_t, x[2 * i]), b = __builtin_bit_cast(uint32_t, x[2 * i + 1]);
+            float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
-            for (int p = 0; p + 1 < PARTS; ++p) {
-                out[p][i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-                a = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) - __builtin_bit_cast(float, a & 0xFFFF0000u));
-                b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, b) - __builtin_bit_cast(float, b & 0xFFFF0000u));
+            for (int p = 0; p < PARTS; ++p) {
+                const b2v h = {(__bf16)a, (__bf16)b};
+                uint32_t w = __builtin_bit_cast(uint32_t, h);
+                out[p][i] = w;
+                if (p + 1 < PARTS) {
+                    asm("" : "+v"(w));                     // (else the low half is rounded once more, alone)
+                    a -= __builtin_bit_cast(float, w << 16);
+                    b -= __builtin_bit_cast(float, w & 0xFFFF0000u);
+                }
             }
-            const b2v h = {(__bf16)__builtin_bit_cast(float, a), (__bf16)__builtin_bit_cast(float, b)};
-            out[PARTS - 1][i] = __builtin_bit_cast(uint32_t, h);
         }
     }
 }

@@ -3,8 +3,7 @@ the plain 64-bit form of attention (step_ref.py), which reads every sequence's o
 
 The bound is step_ref.attention's.  What the prefix adds to its error: parts are joined by their
 maxima in base 2, whose difference is rounded once, 2^-24 (|s| + |m|), and 2^x of it, 2^-23: within the bound's
-2^-22 (|s| + |m|) and its 2^-21.  (Of a probability's two BF16 parts the first is cut off, not rounded: the sum is off by 2^-16
-of it at most where the bound counts 2^-17, and is held to that bound all the same.)"""
+2^-22 (|s| + |m|) and its 2^-21."""
 import math
 
 import pytest
@@ -412,3 +411,24 @@ def test_parts_join_exactly_far_from_zero(gpu, tag, far):
     # the logarithm: the sum's error, log2's and its product's roundings
     want = math.log(2) * (far + math.log2(float(w.sum())))
     assert (lse.cpu().double() - want).abs().max() <= tol + 3 * 2 ** -24 * max(want, 16)
+
+
+def test_probabilities_keep_17_bits_over_bf16_pages(gpu):
+    """Two kinds of keys, of weight 1 and x = e^-0.6809, whose two BF16 parts are off by 2^-20.4 of it if both are rounded and by
+    2^-16.05 if the first is cut off.  Their values are 1 and -1 and their sums nearly the same, so that the result is off by half of
+    what x is: by 2^-18 and by what scores (2^-22) and 2^x (2^-22) add, with fp16's half step of 2^-10."""
+    heads, own, scale = 192, 1, 2789 / 4096
+    # (both kinds in every unit: its largest weight is 1)
+    kind = torch.tensor([0, 1, 1]).repeat(heads // 3 + 1)[:heads + own]
+    kind[190:] = 2
+    keys = torch.stack([torch.zeros(heads + own), torch.tensor([0.0, -1.0, -60.0])[kind]], 1)
+    values = torch.tensor([1.0, -1.0, 0.0])[kind]
+    cache, batch, groups, prefix = made(gpu, la.BF16, heads, keys, values, own)
+    q = torch.zeros(2, 1, 64, dtype=torch.float16, device=gpu)
+    q[:, 0, 1] = 1
+    out = cache.prefix_attention(batch, q, groups, prefix, scale=scale)
+    x = math.exp(-scale)
+    n = [int((kind == i).sum()) for i in range(2)]
+    want = (n[0] - n[1] * x) / (n[0] + n[1] * x)
+    off = (out[:, 0, 0].cpu().double() - want).abs().max()
+    assert off <= 2 ** -18 + 2 * 2 ** -22 + 2 ** -11 * abs(want), float(off) * 2 ** 18
