@@ -668,3 +668,74 @@ def test_sample_probabilities_are_rounded_once(gpu, tag):
     probs = torch.empty_like(x)
     la.sample(x, f32([0.5] * len(temps), gpu), f32(temps, gpu), probs=probs)
     assert probs[:, 0].double().tolist() == want
+
+
+def test_serving_steps_behind_a_prefix_that_is_read_once(gpu):
+    """Parallel samples of one prompt of 140 tokens and another user beside them: the samples' first 128 are read once (two
+    units, where what is not a multiple of 64 is each one's own).  Every stage is held to its own bound, attention to that of
+    attention without a prefix; then the step as a graph against a twin's eager steps."""
+    S = 5
+    m = Serve(gpu, S)
+    s = m.state()
+    g = torch.Generator().manual_seed(904)
+    draw = lambda n: torch.randint(0, m.V, (n,), generator=g, dtype=torch.int32).to(gpu)
+    for n in [16] * 8 + [12]:
+        m.step(s, draw(n + 2), i32([n, 0, 0, 0, 2], gpu), n + 2, 16, True)
+    _, free, n_free = m.pages.refs(s["table"], s["lens"])
+    spare = free[:3].tolist()
+    m.pages.fork(s["table"], s["lens"], i32([[0, i + 1, spare[i]] for i in range(3)], gpu))
+    _, s["free"], s["n_free"] = m.pages.refs(s["table"], s["lens"])
+    s["groups"], s["prefix"] = i32([0, 4], gpu), i32([128], gpu)
+    s.update(temperature=f32([0.8, 1.0, 0.0, 1.5, 0.7], gpu), top_k=i32([0, 40, 0, 7, 0], gpu), top_p=f32([0.9, 1.0, 1.0, 0.8, 1.0], gpu))
+    one, seen = i32([1] * S, gpu), []
+
+    def within_the_bound(cache):
+        plain = cache.prefix_attention
+
+        def call(batch, q, groups, prefix, out):
+            a = plain(batch, q, groups, prefix, out=out)
+            rows = int(batch.new_start[-1])
+            want, _, tol = step_ref.attention(cache, s["table"].tolist(), s["lens"].tolist(), batch.new_start.tolist(), q.cpu(), m.D ** -0.5)
+            assert ((a.cpu().double() - want).abs() <= tol)[:rows].all()
+            # what the samples' rows of the table hold within the prefix is not looked at but in the first of them
+            other = s["table"].clone()
+            other[1:4, :8] = s["table"][4, 0]
+            held = la.KvBatch(other, s["lens"], batch.new_start, n_tokens=batch.n_tokens, max_new=batch.max_new)
+            assert torch.equal(plain(held, q, groups, prefix, out=torch.zeros_like(q)), a)
+            seen.append(rows)
+            return a
+
+        return call
+
+    for l in m.layers:
+        l["cache"].prefix_attention = within_the_bound(l["cache"])
+    for n_new, T in (([1] * S, S), ([1] * S, S), ([2, 1, 3, 0, 1], 8), ([1] * S, S)):
+        s["u"] = torch.rand(S, generator=g).to(gpu)
+        _, logits = m.step(s, s["tokens"] if T == S else draw(T), i32(n_new, gpu), T, max(n_new), True)
+        if T == S:
+            m.sample(s, logits, True)
+    assert seen == [5, 5, 5, 5, 7, 7, 5, 5]
+    twin = Serve(gpu, S)
+    for x, y in zip(m.layers, twin.layers):
+        del x["cache"].prefix_attention
+        y["cache"].k.copy_(x["cache"].k)
+        y["cache"].v.copy_(x["cache"].v)
+    t = {k: v.clone() for k, v in s.items()}
+
+    def run(m, s):
+        _, logits = m.step(s, s["tokens"], one, S, 1)
+        m.sample(s, logits)
+
+    run(twin, {k: v.clone() for k, v in s.items()})
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(m, s)
+    for i in range(12):
+        for x in (s, t):
+            x["u"].copy_(torch.rand(S, generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        run(twin, t)
+        for k in ("table", "lens", "n_free", "tokens", "probs"):
+            assert torch.equal(s[k], t[k]), (i, k)
