@@ -171,11 +171,13 @@ hipError_t launch_rope_as(const llapis_qk_rope_args & a, hipStream_t s) {
     Rope p{a, 0, 0, 1};
     p.slots = (a.head_dim + 2 * V - 1) / (2 * V);
     while (p.lanes_log2 < 6 && (E << p.lanes_log2) < p.slots) ++p.lanes_log2;
-    // Four tokens to a workgroup where their heads leave it places (8192 tokens of 6 heads of 64: 5.5 us, one token
-    // each 8.9) or the tokens are many; else a token's heads over several (2048 tokens of 40 heads of 128 bf16: 10.3 us, four
-    // tokens each 12.4; 4096: 16.8 and 16.7; 8192: 29.6 and 28.6)
+    // Four tokens to a workgroup where their heads leave it places (8192 tokens of 5 heads of 64 f16: 5.9 us, one token each
+    // 9.7), and for 16-bit values where that still fills the card with workgroups of 256, eight to a CU; else one token's heads,
+    // over several.  One and four, in us, on data that no cache holds: 40 heads of 128 bf16, 2048 tokens 13.9 and 17.8, 4096 22.8
+    // and 23.0, 8192 41.1 and 37.6; 72 heads 4096 tokens 36.1 and 38.7, 8192 67.6 and 66.5; fp32, 24 heads of 256, 4096 tokens
+    // 41.8 and 50.9, 8192 79.4 and 86.0
     const int places = ROPE_WG >> p.lanes_log2, heads = a.n_head + a.n_kv, most = a.rot_dim ? ROPE_TABLE / (a.rot_dim / 2) : 4;
-    const bool four = 4 * heads <= places || a.n_tokens >= 4096;
+    const bool four = 4 * heads <= places || (sizeof(T) == 2 && a.n_tokens >= 4 * 8 * 256);
     if (four) p.each = std::min(4, most);
     const int parts = four ? 1 : std::min((heads + places - 1) / places, 65535);
     hipLaunchKernelGGL((k_qk_rope<T, V, E>), dim3((a.n_tokens - 1) / p.each + 1, parts), dim3(ROPE_WG), 0, s, p);

@@ -739,3 +739,11 @@ def test_serving_steps_behind_a_prefix_that_is_read_once(gpu):
         run(twin, t)
         for k in ("table", "lens", "n_free", "tokens", "probs"):
             assert torch.equal(s[k], t[k]), (i, k)
+
+
+@pytest.mark.parametrize("T", [8191, 8192, 8195])
+@pytest.mark.parametrize("tag,D,rot,half", [(la.BF16, 128, 64, True), (la.F16, 80, 20, False), (la.F32, 128, 128, False)])
+def test_rope_many_tokens(gpu, tag, D, rot, half, T):
+    """Either side of the number of tokens from which a workgroup takes four, of more heads than it has places for."""
+    pos = torch.arange(T, dtype=torch.int32) * 3
+    run_rope(gpu, T + D, T, 7, 2, D, rot, half, tag, True, pos=pos)
