@@ -117,16 +117,18 @@ int32_t  llapis_kv_attention(const llapis_kv_cache * c, const llapis_kv_batch * 
  * sequences groups[g] .. groups[g + 1] - 1, in whose rows of the page table the first
  * prefix[g] tokens' entries are the same; they are read from the first of them with new
  * tokens, once for the whole group (in tiles of 64 to 256 query rows of a kv head),
- * and each sequence's other keys are attended as above.  Both arrays are read on the device; groups
- * are in order (as the rows of new_start are), sequences before the first and behind the
- * last share nothing.  A prefix is cut to what every sequence of its group with new tokens had before
- * them, and to a multiple of 64 tokens and of a page; what is cut off counts as each one's own.  Results are
- * llapis_kv_attention's but for the order of sums, with its precision of every part.
- * n_group is 256 at most; with none the call is attention's.  Refused: what attention refuses, and with groups more than 2^24 rows (n_tokens), 2^31 query rows
- * of a kv head and more, 2^24 and more (sequence, kv head, 32 query rows) however short the
- * table, and prefixes of 2^30 and more units of work (32 or 64 keys of a kv head for a tile
- * of rows).  The workspace serves every call of fewer sequences, rows, new tokens, pages and
- * groups too; its size reads b's n_tokens beside what attention's does. */
+ * and each sequence's other keys are attended as above.  Both arrays are read on the
+ * device; groups are in order (as the rows of new_start are), sequences before the first
+ * and behind the last share nothing.  A prefix is cut to what every sequence of its group
+ * with new tokens had before them, and to a multiple of 64 tokens and of a page; what is
+ * cut off counts as each one's own.  Results are llapis_kv_attention's but for the order
+ * of sums, with its precision of every part.  n_group is 256 at most; with none the call
+ * is attention's.  Refused: what attention refuses, and with groups more than 2^24 rows
+ * (n_tokens), 2^31 query rows of a kv head and more, 2^24 and more (sequence, kv head,
+ * 32 query rows) however short the table, and prefixes of 2^30 and more units of work (32
+ * or 64 keys of a kv head for a tile of rows).  The workspace serves every call of fewer
+ * sequences, rows, new tokens, pages and groups too; its size reads b's n_tokens beside
+ * what attention's does. */
 typedef struct llapis_kv_prefix {
     int32_t n_group;
     const int32_t * groups;        /* [n_group + 1] */

@@ -16,16 +16,18 @@
 // makes a lane's scores those of 8 consecutive keys, P's operand.  Rows of LDS are 16 bytes longer than their
 // values, so that 16 rows' reads of a column meet every bank once.
 //
-// Bound by the issue of matrix and vector instructions, not by memory: 64 sequences of 32 heads of 128
-// behind 32768 tokens, bf16, are 34 GFLOP (52 with P in two parts) and 134 MB, and take 74 us, 465 TFLOP/s.  What
-// carries it, with what it measured there (the whole call):
+// Bound by the issue of matrix and vector instructions, not by memory: 64 sequences of 32 heads of 128 (8 kv heads)
+// behind 32768 tokens, bf16, are 34 GFLOP (52 with P in two parts) and 134 MB, and take 74 us, 465 TFLOP/s.  The
+// VALU is busy for 52 % of the time and the matrix cores for 40; q8_0 (16 sequences behind each of three prefixes, 99 us)
+// 52 and 53.  A third of the waves' cycles wait for an instruction to be issued, a third for memory, LDS or a barrier.
+// What carries it, with what it measured there (the whole call):
 //  - the workgroup's two halves work half a unit apart, one at products while the other forms P and
 //    stages, so that a SIMD's matrix cores and VALU work at once: 142 to 119 us with the next two
 //  - sums are products with ones, P is split in two instructions a pair (split_p), and sums and output are scaled anew
 //    only when a row's maximum grows by more than P_SLACK
 //  - loads from memory stay in flight over barriers, and none is under a condition, which would have all of them waited for
-//  - a second tile of a wave's rows where the registers hold it: 64 sequences of 4 rows a kv head 91 us, with
-//    one tile 106; 16 sequences, whose 64 rows one tile holds, 61 us, with two 72
+//  - a second tile of a wave's rows where one leaves rows over: the same 64 sequences 114 us, with one tile 120, 33 of
+//    them 93 and 99 (q8_0 111 and 130); 32, whose 128 rows one tile of each wave holds, 91 with two and 76 with one
 // One part of P would take 10 us off and add 2^-9 to the error of its weights: it keeps kv_attn.h's instead.
 //
 // Rounding is kv_attn.h's: fp32 scores, maxima and sums, 16-bit parts of q and p, a pair of p's bf16 parts good to 2^-17 (cut
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(64 * kvp_waves(HD), kvp_waves(HD) / 4) void k_kv_pr
         if (blockIdx.x == 0) p.plan[tid] = mine;
     }
     __syncthreads();
-    // (row starts that are not in order may give groups more rows than there are: no prefix then)
+    // (row starts that are not in order may give groups more rows than there are: nothing is attended of them then)
     const int n_steps = same(n_steps_all <= p.max_steps ? (int)n_steps_all : 0), n_runs = runs_of(p.runs, n_steps);
     if (blockIdx.x == 0 && tid == 0) p.total[0] = n_steps;
     // ---- the sequences without their prefix, a wave each; last, when their loads hold up nothing

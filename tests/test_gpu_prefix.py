@@ -416,7 +416,7 @@ def test_parts_join_exactly_far_from_zero(gpu, tag, far):
 def test_probabilities_keep_17_bits_over_bf16_pages(gpu):
     """Two kinds of keys, of weight 1 and x = e^-0.6809, whose two BF16 parts are off by 2^-20.4 of it if both are rounded and by
     2^-16.05 if the first is cut off.  Their values are 1 and -1 and their sums nearly the same, so that the result is off by half of
-    what x is: by 2^-18 and by what scores (2^-22) and 2^x (2^-22) add, with fp16's half step of 2^-10."""
+    what x is: by 2^-18 and by what scores (2^-22) and 2^x (2^-22) add, with fp16's half step."""
     heads, own, scale = 192, 1, 2789 / 4096
     # (both kinds in every unit: its largest weight is 1)
     kind = torch.tensor([0, 1, 1]).repeat(heads // 3 + 1)[:heads + own]
