@@ -329,10 +329,10 @@ int32_t llapis_block_norm(const llapis_block_norm_args * a, void * stream);
  * The settings are read on the device, one for each sequence; NULL: temperature 1,
  * the others off.  Weights are fp64, their sums fp64 or, next to where a filter
  * ends, whole numbers of 2^-49 or less of the largest weight there: as little as lets
- * top_p end within a 32nd of a value's weight of its place.  NaN and -infinity are no
- * values (the token of a row without any is -1); where +infinity is the largest, the
- * others have no weight.  With top_k or top_p a value whose weight is below 2^-63 may
- * not be kept.
+ * top_p end within a 32nd of a value's weight of its place in rows of up to 2^20 values.
+ * NaN and -infinity are no values (the token of a row without any is -1); where
+ * +infinity is the largest, the others have no weight.  With top_k or top_p a value
+ * whose weight is below 2^-63 may not be kept.
  * probs [n_seq][vocab] of `type`, rows probs_stride apart, or NULL: the probabilities
  * that the token was drawn with, rounded once (what llapis_verify_drafts takes as a
  * draft's); not on logits.  n_seq is 65535 at most, vocab 2^30 (else the workspace size is 0). */

@@ -105,8 +105,8 @@ __global__ __launch_bounds__(256) void k_kv_join(const KvAttn p, int head_dim, f
 // --------------------------------------------------- join with a prefix
 //
 // As k_kv_join, of the parts of a row's prefix (k_kv_prefix) and those of its own keys, which
-// are k_kv_attn's: where one run had them all, in the row's place.  Bound by the parts' bytes: each of 256 runs leaves its rows' in fp32, 34 MB
-// for 256 rows of 128 values, 12 us.
+// are k_kv_attn's: where one run had them all, in the row's place.  Bound by the parts' bytes:
+// each of 256 runs leaves its rows' in fp32, 34 MB for 256 rows of 128 values, 12 us.
 struct KvResult {
     void * out;
     int64_t out_stride;

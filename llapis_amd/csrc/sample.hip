@@ -24,9 +24,10 @@
 // 8.9 us); for many by two passes over the logits (32 rows of 262144, 33.5 MB: 12.4 and 13.9 us, the sequences' kernels
 // 10.0 and 12.8), the second of which forms every kept value's weight in fp64: with top_p alone that is
 // most of them (64 rows of 128001 bf16: 11.7, 9.0, 18.5 and 13.0 us, probabilities 20.1; the VALU is busy for 68 % of the
-// split's time and 63 % of the probabilities').  All values kept, and the largest alone: 32 rows of 262144 34 and 14 us.  Where more candidates than
-// SMP_HOLD a thread, or more ties than threads, are in the end's bin, k_sample_pick finds it digit by digit (32 rows of
-// 262144 bf16 at top_p 0.9, a thousand ties: 80 us a call, at 0.99 without them 56; all values equal: 1.6 ms).
+// split's time and 63 % of the probabilities').  All values kept, and the largest alone: 32 rows of 262144 34 and 14 us.
+// Where more candidates than SMP_HOLD a thread, or more ties than threads, are in the end's bin, k_sample_pick finds it
+// digit by digit (32 rows of 262144 bf16 at top_p 0.9, a thousand ties: 80 us a call, at 0.99 without them 56; all
+// values equal: 1.6 ms).
 #include <algorithm>
 #include <cstdio>
 
@@ -720,6 +721,7 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
             const double one = __builtin_ldexp(1.0, bits), scale = one / upper_w;
             // to nearest, the second of either sign (a number below 2^51 is in the low bits of its sum with 1.5 2^52)
             auto parts = [&](double v, int64_t & hi, int64_t & lo) {
+#pragma clang fp contract(off)                             // (a weight is the same wherever it is added)
                 const double near = v + 0x1.8p52, rest = (v - (near - 0x1.8p52)) * one + 0x1.8p52;
                 hi = __builtin_bit_cast(int64_t, near) - __builtin_bit_cast(int64_t, 0x1.8p52);
                 lo = __builtin_bit_cast(int64_t, rest) - __builtin_bit_cast(int64_t, 0x1.8p52);
