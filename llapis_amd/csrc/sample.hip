@@ -25,9 +25,10 @@
 // 10.0 and 12.8), the second of which forms every kept value's weight in fp64: with top_p alone that is
 // most of them (64 rows of 128001 bf16: 11.7, 9.0, 18.5 and 13.0 us, probabilities 20.1; the VALU is busy for 68 % of the
 // split's time and 63 % of the probabilities').  All values kept, and the largest alone: 32 rows of 262144 34 and 14 us.
-// Where more candidates than SMP_HOLD a thread, or more ties than threads, are in the end's bin, k_sample_pick finds it
-// digit by digit (32 rows of 262144 bf16 at top_p 0.9, a thousand ties: 80 us a call, at 0.99 without them 56; all
-// values equal: 1.6 ms).
+// Where the end's bins hold more candidates than SMP_HOLD a thread, or a bucket of them more than there are threads,
+// k_sample_pick finds it digit by digit (8 rows of 262144 at top_p 0.9999999: 113 us a call; 32 rows all of whose values are
+// equal: 1.3 ms).  Hundreds of equal values there are compared each with each (32 rows of 262144 bf16 at 0.9, 480 ties:
+// 79 us, k_sample_pick 41 of them; at 0.99 with 90 56 and 19).
 #include <algorithm>
 #include <cstdio>
 
@@ -60,6 +61,8 @@ struct SmpCut {
     uint64_t key;                  // the last candidate that is kept, ~0 without one
     double total;                  // the kept weights' sum
 };
+
+struct SmpAbove { int32_t n; int64_t hi, lo; };            // number and weight of the candidates above a digit
 
 struct SmpWs {
     SmpCut * cuts;                 // [n_seq]
@@ -500,7 +503,8 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
     __shared__ double s_sure[WAVES], s_mid[WAVES], s_sum[2][WAVES];
     __shared__ int s_n[3][WAVES], s_count[WAVES], s_digit[256];
     __shared__ uint64_t s_mass[WAVES];
-    __shared__ int64_t s_parts[WAVES];
+    __shared__ int64_t s_parts[2][WAVES];
+    __shared__ SmpAbove s_above;
     __shared__ int s_first[WG + 1], s_bucket_n[WG], s_list_n, s_found, s_last;
     __shared__ unsigned long long s_bucket[WG], s_kept[WG], s_weigh[2][256], s_all_k;
     __shared__ uint64_t s_list[LIST], s_list_w[LIST], s_key;
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
         const int sum_bits = n_cand > 1 ? 32 - __builtin_clz(n_cand - 1) : 0;      // 2^sum_bits candidates at most
         // Held at once, weights are one word, cut off at 2^(sum_bits - 62) of the largest, which moves the border by at
         // most n_cand^2 of that / (1 - top_p) of its values: 2^-5 here.  (All 8192 up to a top_p of 1 - 2^-17; 1 row of 131072
-        // at 0.999999 47 us, digit by digit 202)
+        // at 0.999999 47 us, digit by digit 76)
         bool few = n_cand <= FEW && per == 1 && (!s.by_p || (double)n_cand * n_cand * n_cand <= 0x1p56 * (1.0 - s.p));
         if (few) {
             // ---- the candidates in registers, and in buckets by value, thread b's the b-th from above.
@@ -726,10 +730,16 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
                 hi = __builtin_bit_cast(int64_t, near) - __builtin_bit_cast(int64_t, 0x1.8p52);
                 lo = __builtin_bit_cast(int64_t, rest) - __builtin_bit_cast(int64_t, 0x1.8p52);
             };
-            auto each = [&](auto f) {                      // f(key) of each candidate, a wave a segment
-                for (int i = wave; i < n_segs; i += WAVES) {
-                    const int n = segs[i].n_cand;
-                    for (int c = lane; c < n; c += 64) f(keys[(int64_t)i * SEG + c]);
+            // f(key) of each candidate, a wave a segment; lane l knows the number of the wave's l-th segment from here
+            auto each = [&](auto f) {
+                for (int i0 = wave; i0 < n_segs; i0 += 64 * WAVES) {
+                    const int there = min((n_segs - i0 + WAVES - 1) / WAVES, 64);
+                    const int n_mine = lane < there ? segs[i0 + lane * WAVES].n_cand : 0;
+                    for (int l = 0; l < there; ++l) {
+                        const int n = smp_lane(n_mine, __builtin_amdgcn_readfirstlane(l));
+                        const uint64_t * list = keys + (int64_t)(i0 + l * WAVES) * SEG;
+                        for (int c = lane; c < n; c += 64) f(list[c]);
+                    }
                 }
             };
             int64_t want_hi = 0, want_lo = 0;
@@ -745,23 +755,25 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
                         lo += y_lo;
                     });
                     __syncthreads();
-                    smp_scan<WAVES>(hi, s_parts, all_hi);
-                    __syncthreads();
-                    smp_scan<WAVES>(lo, s_parts, all_lo);
+                    smp_scan<WAVES>(hi, s_parts[0], all_hi);
+                    smp_scan<WAVES>(lo, s_parts[1], all_lo);
                     const double all_k = ((double)all_hi + (double)all_lo / one) / scale;
                     const double goal = fmax(s.p * (sure + mid + all_k) - sure, 0.0) * scale;
                     want_hi = (int64_t)goal;
                     want_lo = (int64_t)ceil((goal - (double)want_hi) * one);
                 }
                 uint64_t prefix = 0;
-                int64_t above_hi = 0, above_lo = 0;
-                int n_above = 0;
+                SmpAbove above = {0, 0, 0};
                 for (int shift = 56; shift >= 0; shift -= 8) {
                     __syncthreads();
                     if (tid < 256) {
                         s_digit[tid] = 0;
                         s_weigh[0][tid] = 0;
                         s_weigh[1][tid] = 0;
+                    }
+                    if (tid == 0) {
+                        s_found = 0x7FFFFFFF;
+                        s_last = -1;
                     }
                     __syncthreads();
                     // (equal values have equal digits: a thread adds them up before it adds them to the others')
@@ -791,22 +803,31 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
                     });
                     add();
                     __syncthreads();
-                    // the last digit that there is, if none reaches the goal
-                    int found = -1;
-                    for (int d = 255, n_before = 0; d >= 0; --d) {
-                        const int n = s_digit[d];
-                        if (n == 0) continue;
-                        if (found >= 0) {
-                            n_above += n_before;
-                            above_hi += s_weigh[0][found];
-                            above_lo += s_weigh[1][found];
-                        }
-                        found = d;
-                        n_before = n;
-                        const int64_t lo = above_lo + (int64_t)s_weigh[1][d], hi = above_hi + (int64_t)s_weigh[0][d] + (lo >> bits);
-                        if (by_mass ? hi > want_hi || (hi == want_hi && (lo & ((1ll << bits) - 1)) >= want_lo) : n_above + n >= n_k) break;
-                    }
-                    prefix |= (uint64_t)found << shift;
+                    // thread t's digit is the t-th from above; the first that there is whose sum reaches the goal, else the last
+                    const int n_d = tid < 256 ? s_digit[255 - tid] : 0;
+                    const int64_t hi_d = tid < 256 ? (int64_t)s_weigh[0][255 - tid] : 0, lo_d = tid < 256 ? (int64_t)s_weigh[1][255 - tid] : 0;
+                    const int n_w = smp_wave(n_d, SmpAdd());
+                    const int64_t hi_w = smp_wave(hi_d, SmpAdd()), lo_w = smp_wave(lo_d, SmpAdd());
+                    smp_leave(n_w, s_n[0]);
+                    smp_leave(hi_w, s_parts[0]);
+                    smp_leave(lo_w, s_parts[1]);
+                    __syncthreads();
+                    int n_all;
+                    int64_t hi_all, lo_all;
+                    const int n_upto = above.n + smp_before<WAVES>(s_n[0], n_all) + n_w;
+                    const int64_t hi_upto = above.hi + smp_before<WAVES>(s_parts[0], hi_all) + hi_w;
+                    const int64_t lo_upto = above.lo + smp_before<WAVES>(s_parts[1], lo_all) + lo_w;
+                    const int64_t whole = hi_upto + (lo_upto >> bits), rest = lo_upto & ((1ll << bits) - 1);
+                    const bool reached = by_mass ? whole > want_hi || (whole == want_hi && rest >= want_lo) : n_upto >= n_k;
+                    smp_first(n_d > 0 && reached, &s_found);
+                    const uint64_t any = __ballot(n_d > 0);
+                    if (any && lane == 0) atomicMax(&s_last, tid + 63 - (int)__builtin_clzll(any));
+                    __syncthreads();
+                    const int who = s_found != 0x7FFFFFFF ? s_found : s_last;
+                    if (tid == who) s_above = {n_upto - n_d, hi_upto - hi_d, lo_upto - lo_d};
+                    __syncthreads();
+                    above = s_above;
+                    prefix |= (uint64_t)(255 - who) << shift;
                 }
                 key = prefix > key ? prefix : key;
             }
@@ -820,6 +841,10 @@ __global__ __launch_bounds__(smp_pick_wg(N)) void k_sample_pick(const llapis_sam
                 }
                 sum = smp_lane(smp_wave(sum, SmpAdd()), 63);
                 if (lane == 0) segs[i].draw += sum;
+            }
+            if (tid == 0) {
+                s_found = 0x7FFFFFFF;
+                s_last = -1;
             }
             __syncthreads();
             draw = 0.0;
